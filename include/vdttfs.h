@@ -410,6 +410,122 @@ int vdt_conv_layer_noalloc(const float* d_in, int tb_mode, const float* d_kernel
    on the legacy default stream and synchronises it. */
 int vdt_measure_peaks(int device, double* fma_per_s, double* l2_read_bytes_per_s);
 
+/* ------------------------------------------------------------------------
+ * Sequence operators (no counterpart in the reference): what a decoder next
+ * to a spiking encoder runs -- dense layers in 8-bit integers, the norm and
+ * position rotation of queries and keys, a paged cache held in 8 bits, and
+ * attention over it.  Sizes in values unless named bytes; strides too.
+ * ---------------------------------------------------------------------- */
+enum { VDT_F32 = 0, VDT_F16 = 1, VDT_BF16 = 2 };
+
+/* Codes of rows: scale[i] = max_k |x[i][k]| * (1/127) (32-bit product),
+   codes[i][k] = x / scale rounded to nearest even, in -127..127.  A row of
+   zeros has scale 0 and codes 0; one with an infinity or NaN a scale that is
+   not finite (its products are NaN).  type: VDT_F32 / VDT_F16 / VDT_BF16. */
+int vdt_quantize_rows(const void* d_x, int type, int64_t rows, int cols, int64_t x_stride, int8_t* d_codes,
+                      int64_t codes_stride, float* d_scale, vdt_stream stream);
+
+/* out[i][j] = a_scale[i] * w_scale[j] * sum_k a[i][k] w[j][k] + bias[j]
+   (d_bias may be NULL).  a [rows, inner] and w [cols, inner] are codes whose
+   rows start on 16-byte boundaries (strides multiples of 16) and whose last
+   row's storage reaches to the next multiple of 16 bytes; what lies between
+   `inner` and there does not matter.  inner <= 131072: the sums are exact
+   32-bit integers. */
+int vdt_int8_matmul(const int8_t* d_a, int64_t a_stride, const float* d_a_scale, const int8_t* d_w,
+                    int64_t w_stride, const float* d_w_scale, const float* d_bias, int64_t rows, int cols,
+                    int inner, int out_type, void* d_out, int64_t out_stride, vdt_stream stream);
+
+/* The two together for rows x [rows, inner] of `type`: each row's codes into
+   d_scratch (256-byte aligned, vdt_int8_linear_scratch_bytes; VDT_ERR_CAPACITY
+   when smaller), then the product. */
+size_t vdt_int8_linear_scratch_bytes(int64_t rows, int inner);
+int vdt_int8_linear(const void* d_x, int type, int64_t x_stride, const int8_t* d_w, int64_t w_stride,
+                    const float* d_w_scale, const float* d_bias, int64_t rows, int cols, int inner, int out_type,
+                    void* d_out, int64_t out_stride, void* d_scratch, size_t scratch_bytes, vdt_stream stream);
+
+/* The norm of every head of q [tokens, heads, dim] and k [tokens, kv_heads,
+   dim], times a weight [dim] of the same type (NULL: 1), and the rotation of
+   its first `rot` values by the row d_positions[token] of d_table
+   [positions, rot] (rot / 2 cosines, then rot / 2 sines), in one pass:
+   (a, b) -> (a cos - b sin, b cos + a sin).  VDT_ROPE_HALF pairs value i with
+   i + rot / 2, VDT_ROPE_PAIRS 2i with 2i + 1.  VDT_NORM_RMS divides by
+   sqrt(mean(x^2) + eps), VDT_NORM_L2 by sqrt(sum(x^2) + eps).  32-bit between
+   load and store.  Rows at a position outside the table become NaN.  The
+   outputs may be the inputs (same strides); heads or kv_heads may be 0. */
+enum { VDT_ROPE_HALF = 0, VDT_ROPE_PAIRS = 1 };
+enum { VDT_NORM_NONE = 0, VDT_NORM_RMS = 1, VDT_NORM_L2 = 2 };
+int vdt_qk_norm_rope(const void* d_q, int64_t q_token, int64_t q_head, const void* d_k, int64_t k_token,
+                     int64_t k_head, const void* d_q_weight, const void* d_k_weight, const int32_t* d_positions,
+                     const float* d_table, int positions, int rot, int layout, int norm, float eps, int64_t tokens,
+                     int heads, int kv_heads, int dim, int type, void* d_q_out, int64_t qo_token, int64_t qo_head,
+                     void* d_k_out, int64_t ko_token, int64_t ko_head, vdt_stream stream);
+
+/* The rotation's table for `positions` positions: row t has cos and sin of
+   t * f_i, i < rot / 2, times a magnitude, computed in 64 bits, with
+   f_i = base^(-2i / rot) and for contexts `factor` times as long as the
+   `trained` one:
+     VDT_SCALE_NONE    as it is (factor ignored);
+     VDT_SCALE_LINEAR  f_i / factor;
+     VDT_SCALE_BASE    base * factor^(rot / (rot - 2)) for base (rot > 2): the
+                       slowest frequency is divided by factor, the fastest kept;
+     VDT_SCALE_PARTS   frequencies that turn more than `fast` times over the
+                       trained length are kept, those under `slow` turns divided
+                       by factor, a linear ramp over i between (its ends rounded
+                       outwards); magnitude 0.1 ln(factor) + 1. */
+enum { VDT_SCALE_NONE = 0, VDT_SCALE_LINEAR = 1, VDT_SCALE_BASE = 2, VDT_SCALE_PARTS = 3 };
+int vdt_rope_table(int positions, int rot, double base, int scaling, double factor, int trained, double fast,
+                   double slow, float* d_table, vdt_stream stream);
+
+/* A paged cache of keys and values in 8 bits: a page holds `page` tokens (16,
+   32 or 64) of one sequence; k [pages, heads, page, dim], v [pages, heads,
+   dim, page] (16-byte aligned), and a scale for each page and head, k_scale
+   and v_scale [pages, heads].  dim: 32, 64, 96, 128, 192 or 256.  All memory
+   is the caller's.
+   A sequence's pages are d_pages[seq][0 .. width), its token t in page
+   t / page; packed rows of sequence s are d_starts[s] .. d_starts[s + 1] of
+   `total` rows, `most` the longest such run. */
+typedef struct {
+    int8_t* k;
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int pages, page, heads, dim;
+} vdt_cache8;
+
+/* The packed rows k, v [total, heads, dim] become tokens d_held[s] ... of
+   their sequences.  A page's scale is the largest magnitude in it / 127: a
+   page that tokens are in already keeps its scale or, when a new token is
+   larger, gets a larger one, and its old codes are rounded anew.  d_held is
+   not changed.  Two sequences of one call must not append to the same page;
+   tokens for which the table has no page of the cache are dropped. */
+int vdt_cache_append(const vdt_cache8* cache, const void* d_k, int64_t k_token, int64_t k_head, const void* d_v,
+                     int64_t v_token, int64_t v_head, int type, const int32_t* d_pages, int width,
+                     const int32_t* d_held, const int32_t* d_starts, int seqs, int64_t total, int most,
+                     vdt_stream stream);
+
+/* The sequences' d_kept[s] tokens as values of `type`, packed at d_starts[s]
+   into k, v [total, heads, dim] (contiguous).  Tokens of pages that are not
+   in the cache become NaN. */
+int vdt_cache_load(const vdt_cache8* cache, const int32_t* d_pages, int width, const int32_t* d_kept,
+                   const int32_t* d_starts, int seqs, int64_t total, int most, int type, void* d_k, void* d_v,
+                   vdt_stream stream);
+
+/* out = softmax(scale q k^T) v over the cache, for packed queries
+   q [total, heads, dim] (VDT_F16 or VDT_BF16; heads a multiple of the cache's,
+   consecutive heads share one).  causal: the queries are their sequence's last
+   tokens and see those up to themselves; else they see all d_kept[s] of them
+   (an encoder's states).  most_kept bounds d_kept.  A query that sees no token
+   gives 0.  A sequence with more tokens than most_kept or its table hold, and
+   rows that see a page that is not in the cache, give NaN.  d_scratch:
+   vdt_cache_attention_scratch_bytes (may be 0), 16-byte aligned. */
+size_t vdt_cache_attention_scratch_bytes(int64_t total, int heads, int kv_heads, int dim, int seqs, int most,
+                                         int most_kept);
+int vdt_cache_attention(const vdt_cache8* cache, const void* d_q, int64_t q_token, int64_t q_head, int heads,
+                        int type, const int32_t* d_pages, int width, const int32_t* d_kept, const int32_t* d_starts,
+                        int seqs, int64_t total, int most, int most_kept, int causal, float scale, void* d_out,
+                        int64_t out_token, int64_t out_head, void* d_scratch, size_t scratch_bytes,
+                        vdt_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,213 @@
+// seq_internal.h -- declarations shared by the sequence operators' kernel
+// files (k_int8.cu, k_rope.cu, k_cache.cu, k_attend.cu) and their entry
+// points (seq.cu); not part of the public ABI.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "vdt_internal.h"
+
+namespace vdt {
+
+constexpr int kSmCount = 148;
+// scale = largest magnitude * kCodeStep; the codes run from -127 to 127
+constexpr float kCodeStep = 1.0f / 127.0f;
+
+inline bool type_ok(int t) { return t == VDT_F32 || t == VDT_F16 || t == VDT_BF16; }
+inline int type_size(int t) { return t == VDT_F32 ? 4 : 2; }
+inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// 16 bytes of T as 32-bit values, and back
+template <typename T>
+struct Vec16 {
+    static constexpr int N = 16 / sizeof(T);
+    uint4 raw;
+    __device__ __forceinline__ void get(float* f) const {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                T lo, hi;
+                const unsigned short a = (unsigned short)(w[i] & 0xffffu), b = (unsigned short)(w[i] >> 16);
+                memcpy(&lo, &a, 2);
+                memcpy(&hi, &b, 2);
+                f[2 * i] = to_f32(lo);
+                f[2 * i + 1] = to_f32(hi);
+            }
+        }
+    }
+    __device__ __forceinline__ void set(const float* f) {
+        uint32_t w[4];
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const T lo = from_f32<T>(f[2 * i]), hi = from_f32<T>(f[2 * i + 1]);
+                unsigned short a, b;
+                memcpy(&a, &lo, 2);
+                memcpy(&b, &hi, 2);
+                w[i] = (uint32_t)a | ((uint32_t)b << 16);
+            }
+        }
+        raw = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+// The larger of two magnitudes; NaN wins, so that a row with a NaN gets a NaN scale
+__device__ __forceinline__ float max_nan(float a, float b) { return (a > b || a != a) ? a : b; }
+
+// One value's code: x / scale rounded to the nearest whole number, ties to
+// even (the division is the IEEE one: a host that restates it gets the same
+// codes).  A scale of 0 (nothing but zeros, or values below the smallest
+// scale) leaves the value undivided, which rounds to 0; NaN rounds to 0.
+__device__ __forceinline__ int code_of(float x, float scale) {
+    const float q = rintf(__fdiv_rn(x, scale > 0.0f ? scale : 1.0f));
+    return q != q ? 0 : (int)fminf(fmaxf(q, -127.0f), 127.0f);
+}
+
+// A launch that may start while the kernel before it on the stream ends; the
+// kernel calls chain_wait() before it reads what that one wrote.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_after(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                                Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// ------------------------------------------------- copies into shared memory
+// (mbarriers and bulk copies; the waits are bounded)
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t arrivals) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(arrivals) : "memory");
+}
+__device__ __forceinline__ void bar_init_done() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0;
+}
+// Every wait ends: after kWaitTries tries (each suspends for about a
+// microsecond at most) it gives up and returns false; the kernel then writes
+// NaN in the place of what it could not compute.
+constexpr int kWaitTries = 1 << 18;
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < kWaitTries; ++i)
+        if (bar_test(bar, parity)) return true;
+    return false;
+}
+// the same for a whole warp, which goes on or gives up together
+__device__ __forceinline__ bool bar_wait_all(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, bar_wait(bar, parity));
+}
+// size and both addresses multiples of 16 bytes
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+// ------------------------------------------------------ 8-bit integer product
+cudaError_t launch_quantize_rows(const void* x, int type, long long rows, int cols, long long x_stride,
+                                 int8_t* codes, long long codes_stride, float* scale, cudaStream_t s);
+
+struct Int8Params {
+    const int8_t* a;        // [rows, inner] codes, rows a_stride bytes apart
+    const float* a_scale;   // [rows]
+    const int8_t* w;        // [cols, inner] codes, rows w_stride bytes apart
+    const float* w_scale;   // [cols]
+    const float* bias;      // [cols] or null
+    void* out;              // [rows, cols], rows out_stride values apart
+    long long rows, a_stride, w_stride, out_stride;
+    int cols, inner, out_type;
+};
+// after_codes: the kernel before it on the stream is the one that writes `a`
+cudaError_t launch_int8_matmul(const Int8Params& p, bool after_codes, cudaStream_t s);
+
+// ---------------------------------------------------- head norms and rotation
+struct RopeParams {
+    const void *q, *k;                  // [tokens, heads, dim]
+    void *q_out, *k_out;
+    long long q_token, q_head, k_token, k_head;          // strides in values
+    long long qo_token, qo_head, ko_token, ko_head;
+    const void *wq, *wk;                // [dim] or null
+    const int32_t* at;                  // [tokens] positions
+    const float* table;                 // [positions, rot]: cosines, then sines
+    long long tokens;
+    int positions, rot, layout, norm, heads, kv_heads, dim, type;
+    float eps;
+};
+cudaError_t launch_qk_norm_rope(const RopeParams& p, cudaStream_t s);
+
+struct TableParams {
+    int positions, rot, scaling;
+    double base, factor;                // base: VDT_SCALE_BASE's factor is in it
+    double low, high;                   // VDT_SCALE_PARTS: the ramp's ends, in i
+    float* table;
+};
+cudaError_t launch_rope_table(const TableParams& p, cudaStream_t s);
+
+// ------------------------------------------------------------------ the cache
+struct CacheRows {
+    const int32_t* table;   // [seqs, width] page numbers
+    const int32_t* held;    // [seqs] tokens in the cache (before an append)
+    const int32_t* starts;  // [seqs + 1] first packed row of each sequence
+    int seqs, width;
+    long long total;        // packed rows
+    int most;               // longest run of packed rows
+};
+cudaError_t launch_cache_append(const vdt_cache8& c, const CacheRows& r, const void* k, const void* v, int type,
+                                long long k_token, long long k_head, long long v_token, long long v_head,
+                                cudaStream_t s);
+cudaError_t launch_cache_load(const vdt_cache8& c, const CacheRows& r, void* k, void* v, int type, cudaStream_t s);
+
+struct AttendParams {
+    vdt_cache8 c;
+    CacheRows r;            // r.held: tokens in the cache; r.most: longest run of queries
+    const void* q;          // [total, heads, dim]
+    void* out;              // [total, heads, dim]
+    long long q_token, q_head, out_token, out_head;
+    int heads, type, causal, most_kept;
+    float scale;            // of the scores, times log2(e)
+    float* scratch;
+};
+size_t attend_scratch_bytes(long long total, int heads, int kv_heads, int dim, int seqs, int most, int most_kept);
+bool attend_dim_ok(int dim);
+cudaError_t launch_cache_attention(const AttendParams& p, cudaStream_t s);
+
+}  // namespace vdt

@@ -44,8 +44,14 @@ class DvsDesc(C.Structure):
                 ("decay_fc", C.c_float), ("th_fc", C.c_float)]
 
 
+class Cache8Desc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pages", C.c_int), ("page", C.c_int), ("heads", C.c_int), ("dim", C.c_int)]
+
+
 # every function the header declares: name -> (restype, argtypes)
 _vp, _fp, _ip = C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_int)
+_i, _l, _cp = C.c_int, C.c_int64, C.POINTER(Cache8Desc)
 SIGNATURES = {
     "vdt_version": (C.c_char_p, []),
     "vdt_strerror": (C.c_char_p, [C.c_int]),
@@ -104,6 +110,19 @@ SIGNATURES = {
     "vdt_conv_layer_noalloc": (C.c_int, [_vp, C.c_int, _vp, _vp, _vp, _vp, C.c_int, C.c_int,
                                          C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                          C.c_int, C.c_int, C.c_int, C.POINTER(TimeCfg), _vp, _vp]),
+    # sequence operators
+    "vdt_quantize_rows": (_i, [_vp, _i, _l, _i, _l, _vp, _l, _vp, _vp]),
+    "vdt_int8_matmul": (_i, [_vp, _l, _vp, _vp, _l, _vp, _vp, _l, _i, _i, _i, _vp, _l, _vp]),
+    "vdt_int8_linear_scratch_bytes": (C.c_size_t, [_l, _i]),
+    "vdt_int8_linear": (_i, [_vp, _i, _l, _vp, _l, _vp, _vp, _l, _i, _i, _i, _vp, _l, _vp, C.c_size_t, _vp]),
+    "vdt_qk_norm_rope": (_i, [_vp, _l, _l, _vp, _l, _l, _vp, _vp, _vp, _vp, _i, _i, _i, _i, C.c_float, _l, _i, _i, _i,
+                              _i, _vp, _l, _l, _vp, _l, _l, _vp]),
+    "vdt_rope_table": (_i, [_i, _i, C.c_double, _i, C.c_double, _i, C.c_double, C.c_double, _vp, _vp]),
+    "vdt_cache_append": (_i, [_cp, _vp, _l, _l, _vp, _l, _l, _i, _vp, _i, _vp, _vp, _i, _l, _i, _vp]),
+    "vdt_cache_load": (_i, [_cp, _vp, _i, _vp, _vp, _i, _l, _i, _i, _vp, _vp, _vp]),
+    "vdt_cache_attention_scratch_bytes": (C.c_size_t, [_l, _i, _i, _i, _i, _i, _i]),
+    "vdt_cache_attention": (_i, [_cp, _vp, _l, _l, _i, _i, _vp, _i, _vp, _vp, _i, _l, _i, _i, _i, C.c_float, _vp, _l, _l,
+                                 _vp, C.c_size_t, _vp]),
 }
 
 _lib = None
