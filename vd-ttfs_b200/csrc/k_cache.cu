@@ -15,7 +15,6 @@ namespace vdt {
 namespace {
 
 constexpr int kCacheThreads = 128;
-constexpr int kMostPage = 64;
 
 // A sequence's part of a call: packed rows [first, first + rows), or none
 // where the caller's offsets do not fit the buffers.

@@ -82,6 +82,8 @@ __device__ __forceinline__ uint32_t keep_below(uint32_t v, int word, int inner) 
     return left >= 4 ? v : left <= 0 ? 0u : v & ((1u << (8 * left)) - 1u);
 }
 
+constexpr int kFewRows = 32;
+
 template <typename T, int NT>
 __global__ void __launch_bounds__(kRowsWarps * 32) k_int8_rows(Int8Params p) {
     __shared__ int part[kRowsWarps][16][8 * NT + 1];
@@ -149,6 +151,252 @@ cudaError_t rows_launch(const Int8Params& p, bool after, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+// --------------------------------------------------------------- many rows
+// Persistent CTAs over tiles of 128 rows x BN channels.  One thread keeps a
+// ring of stages (128 bytes of the inner dimension of both sides) full with
+// tile loads, one issues the products into the tensor memory, four warps turn
+// finished sums into outputs while the next tile's are made in the other half
+// of the tensor memory.  Loads past the rows, the channels and the inner size
+// give zeros.
+constexpr int kTileRows = 128, kStageBytes = 128;    // bytes of the inner dimension a stage
+constexpr int kGemmThreads = 192;
+
+template <int BN>
+struct GemmShape {
+    static constexpr int kStage = (kTileRows + BN) * kStageBytes;
+    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int kOut = 4 * 4096;                       // a 32-row, 128-byte block for each epilogue warp
+    static constexpr int kScales = 2 * 2 * BN * 4;              // channel scales and biases of two tiles
+    static constexpr int kBytes = 1024 + kStages * kStage + kOut + kScales;
+};
+
+struct GemmBars {
+    uint64_t full[8], empty[8], done[2], taken[2];
+    uint32_t tmem;
+};
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(kGemmThreads, 1) k_int8_tiles(const __grid_constant__ CUtensorMap map_a,
+                                                                const __grid_constant__ CUtensorMap map_w, Int8Params p,
+                                                                int tiles_m, int tiles) {
+    using Shape = GemmShape<BN>;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ GemmBars bars;
+    unsigned char* smem = smem_raw + ((1024 - (shared_address(smem_raw) & 1023)) & 1023);
+    const uint32_t stages = shared_address(smem);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int steps = (p.inner + kStageBytes - 1) / kStageBytes;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < Shape::kStages; ++i) {
+            bar_init(shared_address(&bars.full[i]), 1);
+            bar_init(shared_address(&bars.empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(shared_address(&bars.done[i]), 1);
+            bar_init(shared_address(&bars.taken[i]), 128);
+        }
+        bar_init_done();
+    }
+    if (warp == 1) tmem_alloc(shared_address(&bars.tmem), 2 * BN);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = bars.tmem;
+    chain_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int n = 0;
+            bool alive = true;
+            for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
+                const int y = tile % tiles_m * kTileRows, c = tile / tiles_m * BN;
+                for (int s = 0; s < steps; ++s, ++n) {
+                    const int slot = n % Shape::kStages;
+                    if (!(alive = bar_wait(shared_address(&bars.empty[slot]), (n / Shape::kStages & 1) ^ 1))) break;
+                    const uint32_t at = stages + slot * Shape::kStage, bar = shared_address(&bars.full[slot]);
+                    bar_expect(bar, Shape::kStage);
+                    tile_load(at, &map_a, s * kStageBytes, y, bar);
+                    tile_load(at + kTileRows * kStageBytes, &map_w, s * kStageBytes, c, bar);
+                }
+            }
+            // every load has landed before the CTA ends: the last ones' stages
+            for (int i = max(0, n - Shape::kStages); i < n; ++i)
+                bar_wait(shared_address(&bars.full[i % Shape::kStages]), i / Shape::kStages & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // 32-bit sums, signed 8-bit operands, both with the inner dimension consecutive
+            constexpr uint32_t shape = 2u << 4 | 1u << 7 | 1u << 10 | (BN >> 3) << 17 | (kTileRows >> 4) << 24;
+            int n = 0, i = 0;
+            bool alive = true;
+            for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x, ++i) {
+                const int half = i & 1;
+                if (!(alive = bar_wait(shared_address(&bars.taken[half]), (i / 2 & 1) ^ 1))) break;
+                tmem_fence_after();
+                for (int s = 0; s < steps; ++s, ++n) {
+                    const int slot = n % Shape::kStages;
+                    if (!(alive = bar_wait(shared_address(&bars.full[slot]), n / Shape::kStages & 1))) break;
+                    tmem_fence_after();
+                    const uint32_t at = stages + slot * Shape::kStage;
+                    const uint64_t a = tile_desc(at), w = tile_desc(at + kTileRows * kStageBytes);
+#pragma unroll
+                    for (int k = 0; k < kStageBytes / 32; ++k)
+                        mma_i8(tmem + half * BN, a + 2 * k, w + 2 * k, shape, s > 0 || k > 0);
+                    mma_commit(shared_address(&bars.empty[slot]));
+                }
+                if (alive) mma_commit(shared_address(&bars.done[half]));
+            }
+        }
+    } else {
+        const int quarter = warp % 4, thread = threadIdx.x - 64;     // a warp reads the rows of its quarter
+        unsigned char* stage = smem + Shape::kStages * Shape::kStage + (warp - 2) * 4096;
+        float* const scales = reinterpret_cast<float*>(smem + Shape::kStages * Shape::kStage + Shape::kOut);
+        T* const out = static_cast<T*>(p.out);
+        constexpr int kCols = 128 / sizeof(T), kPer = 16 / sizeof(T);   // columns of a block; of 16 bytes
+        const bool wide = p.out_stride * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+        bool alive = true;
+        int i = 0;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++i) {
+            const int half = i & 1;
+            const long long row0 = (long long)(tile % tiles_m) * kTileRows + quarter * 32;
+            const int col0 = tile / tiles_m * BN;
+            float* const ws = scales + half * 2 * BN;
+            // the scales of the tile before last are not in use any more: every
+            // warp has been past this barrier for the tile between
+            for (int c = thread; c < BN; c += 128) {
+                const int col = min(col0 + c, p.cols - 1);
+                ws[c] = p.w_scale[col];
+                ws[BN + c] = p.bias ? p.bias[col] : 0.0f;
+            }
+            const float as = p.a_scale[min(row0 + lane, p.rows - 1)];
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            alive = alive && bar_wait_all(shared_address(&bars.done[half]), i / 2 & 1);
+            tmem_fence_after();
+#pragma unroll
+            for (int b = 0; b < BN / kCols; ++b) {
+#pragma unroll
+                for (int part = 0; part < kCols / 32; ++part) {
+                    uint32_t r[32];
+                    tmem_load(tmem + half * BN + (quarter * 32 << 16) + b * kCols + part * 32, r);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int q = 0; q < 32 / kPer; ++q) {
+                        float f[kPer];
+                        const int c = b * kCols + part * 32 + q * kPer;
+#pragma unroll
+                        for (int j = 0; j < kPer; j += 4) {
+                            const float4 w = *reinterpret_cast<const float4*>(ws + c + j);
+                            const float4 d = *reinterpret_cast<const float4*>(ws + BN + c + j);
+                            f[j] = fmaf((float)(int)r[q * kPer + j] * as, w.x, d.x);
+                            f[j + 1] = fmaf((float)(int)r[q * kPer + j + 1] * as, w.y, d.y);
+                            f[j + 2] = fmaf((float)(int)r[q * kPer + j + 2] * as, w.z, d.z);
+                            f[j + 3] = fmaf((float)(int)r[q * kPer + j + 3] * as, w.w, d.w);
+                        }
+                        if (!alive)
+#pragma unroll
+                            for (int j = 0; j < kPer; ++j) f[j] = __int_as_float(0x7fffffff);
+                        Vec16<T> v;
+                        v.set(f);
+                        const int chunk = part * (32 / kPer) + q;
+                        *reinterpret_cast<uint4*>(stage + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = v.raw;
+                    }
+                }
+                __syncwarp();
+                // eight lanes write a row's 128 bytes
+                const int col = col0 + b * kCols + lane % 8 * kPer;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int r = k * 4 + lane / 8;
+                    const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((lane % 8 ^ (r & 7)) << 4));
+                    const long long row = row0 + r;
+                    if (row < p.rows && col < p.cols) {
+                        T* to = out + row * p.out_stride + col;
+                        if (wide && col + kPer <= p.cols) {
+                            *reinterpret_cast<uint4*>(to) = v;
+                        } else {
+                            T t[kPer];
+                            memcpy(t, &v, 16);
+#pragma unroll
+                            for (int j = 0; j < kPer; ++j)
+                                if (col + j < p.cols) to[j] = t[j];
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+            tmem_fence_before();
+            bar_arrive(shared_address(&bars.taken[half]));
+        }
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tmem_fence_after();
+        tmem_free(tmem, 2 * BN);
+    }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// cuTensorMapEncodeTiled, reached through the runtime (the library links the runtime only)
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q);
+        return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeTiled>(f) : nullptr;
+    }();
+    return fn;
+}
+
+bool byte_map(CUtensorMap* m, const int8_t* at, long long rows, int inner, long long stride, int box_rows) {
+    const EncodeTiled fn = encode_tiled();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {kStageBytes, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(at), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int BN>
+cudaError_t tiles_launch(const Int8Params& p, bool after, cudaStream_t s) {
+    using Shape = GemmShape<BN>;
+    CUtensorMap a, w;
+    if (!byte_map(&a, p.a, p.rows, p.inner, p.a_stride, kTileRows) || !byte_map(&w, p.w, p.cols, p.inner, p.w_stride, BN))
+        return cudaErrorInvalidValue;
+    const cudaError_t e = cudaFuncSetAttribute(k_int8_tiles<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kBytes);
+    if (e != cudaSuccess) return e;
+    const long long tiles_m = (p.rows + kTileRows - 1) / kTileRows, tiles = tiles_m * ((p.cols + BN - 1) / BN);
+    if (tiles > 0x7fffffff - 1024) return cudaErrorInvalidValue;
+    const dim3 grid((unsigned)(tiles < kSmCount ? tiles : kSmCount));
+    if (after)
+        return launch_after(k_int8_tiles<T, BN>, grid, dim3(kGemmThreads), Shape::kBytes, s, a, w, p, (int)tiles_m, (int)tiles);
+    k_int8_tiles<T, BN><<<grid, kGemmThreads, Shape::kBytes, s>>>(a, w, p, (int)tiles_m, (int)tiles);
+    return cudaGetLastError();
+}
+
+// The widest tile whose last round of CTAs is not much emptier than a narrower
+// one's: rounds times (channels + 64), the 64 for what a tile costs by itself.
+template <typename T>
+cudaError_t tiles_by_width(const Int8Params& p, bool after, cudaStream_t s) {
+    const long long tiles_m = (p.rows + kTileRows - 1) / kTileRows;
+    int best = 0;
+    long long cost = 0;
+    for (const int bn : {256, 128, 64}) {
+        const long long tiles = tiles_m * ((p.cols + bn - 1) / bn), c = (tiles + kSmCount - 1) / kSmCount * (bn + 64);
+        if (!best || c < cost) {
+            best = bn;
+            cost = c;
+        }
+    }
+    if (best == 256) return tiles_launch<T, 256>(p, after, s);
+    if (best == 128) return tiles_launch<T, 128>(p, after, s);
+    return tiles_launch<T, 64>(p, after, s);
+}
+
 template <typename T>
 cudaError_t quant_launch(const void* x, long long rows, int cols, long long x_stride, int8_t* codes,
                          long long codes_stride, float* scale, cudaStream_t s) {
@@ -171,9 +419,10 @@ cudaError_t launch_quantize_rows(const void* x, int type, long long rows, int co
 }
 
 cudaError_t launch_int8_matmul(const Int8Params& p, bool after_codes, cudaStream_t s) {
-    if (p.out_type == VDT_F32) return rows_launch<float>(p, after_codes, s);
-    if (p.out_type == VDT_F16) return rows_launch<__half>(p, after_codes, s);
-    return rows_launch<__nv_bfloat16>(p, after_codes, s);
+    const bool few = p.rows <= kFewRows;
+    if (p.out_type == VDT_F32) return few ? rows_launch<float>(p, after_codes, s) : tiles_by_width<float>(p, after_codes, s);
+    if (p.out_type == VDT_F16) return few ? rows_launch<__half>(p, after_codes, s) : tiles_by_width<__half>(p, after_codes, s);
+    return few ? rows_launch<__nv_bfloat16>(p, after_codes, s) : tiles_by_width<__nv_bfloat16>(p, after_codes, s);
 }
 
 }  // namespace vdt
