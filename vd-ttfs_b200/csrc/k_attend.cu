@@ -458,7 +458,7 @@ cudaError_t rows_launch(const AttendParams& p, cudaStream_t s) {
     const long long tiles = ((long long)p.r.most * (p.heads / p.c.heads) + 15) / 16;
     const dim3 grid(c.count, (unsigned)(tiles * p.c.heads), p.r.seqs);
     if (tiles * p.c.heads > 65535) return cudaErrorInvalidValue;
-    cudaError_t e = cudaFuncSetAttribute(k_attend_rows<D, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lay.bytes);
+    cudaError_t e = allow_shared<k_attend_rows<D, P>>((int)rows_layout(D, kMostChunk, P).bytes);
     if (e != cudaSuccess) return e;
     k_attend_rows<D, P><<<grid, kRowsWarps * 32, lay.bytes, s>>>(p, c.tokens);
     if ((e = cudaGetLastError()) != cudaSuccess || c.count == 1) return e;

@@ -367,7 +367,7 @@ cudaError_t tiles_launch(const Int8Params& p, bool after, cudaStream_t s) {
     CUtensorMap a, w;
     if (!byte_map(&a, p.a, p.rows, p.inner, p.a_stride, kTileRows) || !byte_map(&w, p.w, p.cols, p.inner, p.w_stride, BN))
         return cudaErrorInvalidValue;
-    const cudaError_t e = cudaFuncSetAttribute(k_int8_tiles<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kBytes);
+    const cudaError_t e = allow_shared<k_int8_tiles<T, BN>>(Shape::kBytes);
     if (e != cudaSuccess) return e;
     const long long tiles_m = (p.rows + kTileRows - 1) / kTileRows, tiles = tiles_m * ((p.cols + BN - 1) / BN);
     if (tiles > 0x7fffffff - 1024) return cudaErrorInvalidValue;
