@@ -504,7 +504,7 @@ int vdt_cache_append(const vdt_cache8* cache, const void* d_k, int64_t k_token, 
                      vdt_stream stream);
 
 /* The sequences' d_kept[s] tokens as values of `type`, packed at d_starts[s]
-   into k, v [total, heads, dim] (contiguous).  Tokens of pages that are not
+   into k, v [total, heads, dim] (contiguous, 16-byte aligned).  Tokens of pages that are not
    in the cache become NaN. */
 int vdt_cache_load(const vdt_cache8* cache, const int32_t* d_pages, int width, const int32_t* d_kept,
                    const int32_t* d_starts, int seqs, int64_t total, int most, int type, void* d_k, void* d_v,

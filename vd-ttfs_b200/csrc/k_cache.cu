@@ -9,6 +9,8 @@
 //   scale' = max(scale, m / 127) if tokens are in the page already, else m / 127
 //   old codes: round(code * (scale / scale')),  new codes: round(x / scale')
 // An old code moves only where a new token is larger than all before it.
+#include <type_traits>
+
 #include "seq_internal.h"
 
 namespace vdt {
@@ -50,80 +52,225 @@ __device__ __forceinline__ float block_max(float m) {
     return m;
 }
 
-// One CTA for each (page touched, head, sequence).
-template <typename T>
-__global__ void __launch_bounds__(kCacheThreads) k_cache_append(vdt_cache8 c, CacheRows r, const T* __restrict__ k,
-                                                                const T* __restrict__ v, long long k_token,
-                                                                long long k_head, long long v_token, long long v_head) {
-    const int b = blockIdx.z, h = blockIdx.y;
+// The tokens of a call that fall into one page of one head
+struct Place {
+    int n, old;             // new tokens; tokens before them in the page
+    long long first, slot;  // the first one's packed row; page number * heads + head
+};
+__device__ __forceinline__ bool place_of(const vdt_cache8& c, const CacheRows& r, Place& o) {
+    const int b = blockIdx.z;
     const Part p = part_of(r, b);
-    if (!p.rows) return;
+    if (!p.rows) return false;
     const int j = p.held / c.page + blockIdx.x;
     const int lo = max(p.held, j * c.page), hi = min(p.held + p.rows, (j + 1) * c.page);
-    if (lo >= hi) return;
+    if (lo >= hi) return false;
     const int no = page_of(r, b, j, c.pages);
-    if (no < 0) return;
-    const int n = hi - lo, old = lo - j * c.page, dim = c.dim;      // new tokens, tokens before them in the page
-    const long long first = p.first + (lo - p.held), at = ((long long)no * c.heads + h) * c.page * dim;
+    if (no < 0) return false;
+    o.n = hi - lo;
+    o.old = lo - j * c.page;
+    o.first = p.first + (lo - p.held);
+    o.slot = (long long)no * c.heads + blockIdx.y;
+    return true;
+}
+
+// The scale after the new tokens' largest magnitude m; old codes rounded anew
+// where it grew.  All threads of the CTA.
+__device__ __forceinline__ float grow(const vdt_cache8& c, const Place& o, bool values, float m) {
+    float* scale = (values ? c.v_scale : c.k_scale) + o.slot;
+    int8_t* codes = (values ? c.v : c.k) + o.slot * c.page * c.dim;
+    float to = m * kCodeStep;
+    const float was = o.old ? *scale : 0.0f;
+    if (o.old) to = max_nan(to, was);
+    __syncthreads();
+    if (threadIdx.x == 0) *scale = to;
+    const float ratio = o.old && to > 0.0f ? __fdiv_rn(was, to) : 1.0f;
+    if (ratio != 1.0f)
+        for (int i = threadIdx.x; i < o.old * c.dim; i += kCacheThreads) {
+            int8_t* q = codes + (values ? (long long)(i / o.old) * c.page + i % o.old : (long long)i);
+            *q = (int8_t)rintf((float)*q * ratio);
+        }
+    return to;
+}
+
+// Any stride and alignment: one CTA for each (page touched, head, sequence).
+template <typename T>
+__global__ void __launch_bounds__(kCacheThreads) k_cache_append_any(vdt_cache8 c, CacheRows r, const T* __restrict__ k,
+                                                                    const T* __restrict__ v, long long k_token, long long k_head,
+                                                                    long long v_token, long long v_head) {
+    Place o;
+    if (!place_of(c, r, o)) return;
+    const int h = blockIdx.y, dim = c.dim;
     for (int side = 0; side < 2; ++side) {
-        const T* x = side ? v + first * v_token + h * v_head : k + first * k_token + h * k_head;
+        const T* x = side ? v + o.first * v_token + h * v_head : k + o.first * k_token + h * k_head;
         const long long step = side ? v_token : k_token;
-        int8_t* codes = (side ? c.v : c.k) + at;
-        float* scale = (side ? c.v_scale : c.k_scale) + (long long)no * c.heads + h;
+        int8_t* codes = (side ? c.v : c.k) + o.slot * c.page * dim;
         float m = 0.0f;
-        for (int i = threadIdx.x; i < n * dim; i += kCacheThreads) m = max_nan(fabsf(to_f32(x[i / dim * step + i % dim])), m);
-        m = block_max(m);
-        float to = m * kCodeStep;
-        const float was = old ? *scale : 0.0f;
-        if (old) to = max_nan(to, was);
-        __syncthreads();
-        if (threadIdx.x == 0) *scale = to;
-        const float ratio = old && to > 0.0f ? __fdiv_rn(was, to) : 1.0f;
-        if (old && ratio != 1.0f)
-            for (int i = threadIdx.x; i < old * dim; i += kCacheThreads) {
-                int8_t* q = codes + (side ? (long long)(i % dim) * c.page + i / dim : (long long)i);
-                *q = (int8_t)rintf((float)*q * ratio);
-            }
-        for (int i = threadIdx.x; i < n * dim; i += kCacheThreads) {
+        for (int i = threadIdx.x; i < o.n * dim; i += kCacheThreads) m = max_nan(fabsf(to_f32(x[i / dim * step + i % dim])), m);
+        const float to = grow(c, o, side, block_max(m));
+        for (int i = threadIdx.x; i < o.n * dim; i += kCacheThreads) {
             const int t = i / dim, d = i % dim;
-            codes[side ? (long long)d * c.page + old + t : (long long)(old + t) * dim + d] =
-                (int8_t)code_of(to_f32(x[t * step + d]), to);
+            codes[side ? (long long)d * c.page + o.old + t : (long long)(o.old + t) * dim + d] = (int8_t)code_of(to_f32(x[t * step + d]), to);
         }
     }
 }
 
-// One CTA for each (page, head, sequence): its tokens as values, packed.
-template <typename T>
+// A value tile in shared memory, [dim][page] bytes; a row's pad keeps lanes
+// that write eight rows apart on few banks.
+template <int P>
+constexpr int kTileRow = P + 4;
+
+// Rows of whole 16-byte vectors.  The page's new vectors are read once and
+// stay in registers (at most 64 tokens x 256 values over 128 threads); keys go
+// out as they are, values through shared memory, where their tokens come to
+// lie side by side.
+template <typename T, int D, int P>
+__global__ void __launch_bounds__(kCacheThreads) k_cache_append_rows(vdt_cache8 c, CacheRows r, const T* __restrict__ k,
+                                                                     const T* __restrict__ v, long long k_token, long long k_head,
+                                                                     long long v_token, long long v_head) {
+    constexpr int N = Vec16<T>::N, kRow = D / N, kHeld = (P * kRow + kCacheThreads - 1) / kCacheThreads;
+    __shared__ __align__(16) unsigned char tile[D * kTileRow<P>];
+    Place o;
+    if (!place_of(c, r, o)) return;
+    const int h = blockIdx.y;
+    for (int side = 0; side < 2; ++side) {
+        const T* x = side ? v + o.first * v_token + h * v_head : k + o.first * k_token + h * k_head;
+        const long long step = side ? v_token : k_token;
+        int8_t* codes = (side ? c.v : c.k) + o.slot * (P * D);
+        Vec16<T> held[kHeld];
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int at = threadIdx.x + i * kCacheThreads, t = at / kRow, e = at % kRow;
+            held[i].raw = t < o.n ? *reinterpret_cast<const uint4*>(x + t * step + e * N) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            float f[N];
+            held[i].get(f);
+#pragma unroll
+            for (int j = 0; j < N; ++j) m = max_nan(fabsf(f[j]), m);
+        }
+        const Coder coder(grow(c, o, side, block_max(m)));
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int at = threadIdx.x + i * kCacheThreads, t = at / kRow, e = at % kRow;
+            if (t >= o.n) continue;
+            float f[N];
+            uint32_t w[N / 4];
+            held[i].get(f);
+            coder.words<N>(f, w);
+            if (!side) {
+                int8_t* to = codes + (o.old + t) * D + e * N;
+                if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint32_t*>(to) = w[0];
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) tile[(e * N + j) * kTileRow<P> + o.old + t] = (unsigned char)(w[j / 4] >> (8 * (j % 4)));
+            }
+        }
+        if (!side) continue;
+        __syncthreads();
+        if (o.n == P) {
+            for (int i = threadIdx.x; i < D * P / 16; i += kCacheThreads) {
+                const uint32_t* from = reinterpret_cast<const uint32_t*>(tile + i / (P / 16) * kTileRow<P> + i % (P / 16) * 16);
+                *reinterpret_cast<uint4*>(codes + i * 16) = make_uint4(from[0], from[1], from[2], from[3]);
+            }
+        } else {
+            for (int i = threadIdx.x; i < D * o.n; i += kCacheThreads) {
+                const int d = i / o.n, t = o.old + i % o.n;
+                codes[d * P + t] = (int8_t)tile[d * kTileRow<P> + t];
+            }
+        }
+    }
+}
+
+// Any size: one CTA for each (page, head, sequence), its tokens as values,
+// packed.  A page's value codes go through shared memory.
+template <typename T, int D, int P>
 __global__ void __launch_bounds__(kCacheThreads) k_cache_load(vdt_cache8 c, CacheRows r, T* __restrict__ k, T* __restrict__ v) {
+    constexpr int N = Vec16<T>::N, kRow = D / N;
+    __shared__ __align__(16) unsigned char tile[D * kTileRow<P>];
     const int b = blockIdx.z, h = blockIdx.y, j = blockIdx.x;
     const long long start = r.starts[b], rows = (long long)r.starts[b + 1] - start;
     const int kept = r.held[b];
-    const int n = min(kept - j * c.page, c.page);
+    const int n = min(kept - j * P, P);
     if (n <= 0 || kept > rows || start < 0 || start + rows > r.total) return;
     const int no = page_of(r, b, j, c.pages);
     const float nan = __int_as_float(0x7fffffff);        // a page that is not in the cache
-    const long long slot = (long long)max(no, 0) * c.heads + h, at = slot * c.page * c.dim;
+    const long long slot = (long long)max(no, 0) * c.heads + h, at = slot * (P * D);
     const float ks = no < 0 ? nan : c.k_scale[slot], vs = no < 0 ? nan : c.v_scale[slot];
-    for (int i = threadIdx.x; i < n * c.dim; i += kCacheThreads) {
-        const int t = i / c.dim, d = i % c.dim;
-        const long long to = ((start + j * c.page + t) * c.heads + h) * c.dim + d;
-        k[to] = from_f32<T>((float)c.k[at + i] * ks);
-        v[to] = from_f32<T>((float)c.v[at + (long long)d * c.page + t] * vs);
+    const uint4* vc = reinterpret_cast<const uint4*>(c.v + at);
+    for (int i = threadIdx.x; i < D * P / 16; i += kCacheThreads) {
+        const uint4 w = vc[i];
+        uint32_t* to = reinterpret_cast<uint32_t*>(tile + i / (P / 16) * kTileRow<P> + i % (P / 16) * 16);
+        to[0] = w.x; to[1] = w.y; to[2] = w.z; to[3] = w.w;
+    }
+    const long long out = ((start + (long long)j * P) * c.heads + h) * D, step = (long long)c.heads * D;
+    for (int i = threadIdx.x; i < n * kRow; i += kCacheThreads) {
+        const int t = i / kRow, e = i % kRow;
+        float f[N];
+#pragma unroll
+        for (int q = 0; q < N; q += 4) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(c.k + at + t * D + e * N + q);
+#pragma unroll
+            for (int a = 0; a < 4; ++a) f[q + a] = (float)(int8_t)(w >> (8 * a)) * ks;
+        }
+        Vec16<T> y;
+        y.set(f);
+        *reinterpret_cast<uint4*>(k + out + t * step + e * N) = y.raw;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * kRow; i += kCacheThreads) {
+        const int t = i / kRow, e = i % kRow;
+        float f[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) f[q] = (float)(int8_t)tile[(e * N + q) * kTileRow<P> + t] * vs;
+        Vec16<T> y;
+        y.set(f);
+        *reinterpret_cast<uint4*>(v + out + t * step + e * N) = y.raw;
+    }
+}
+
+// calls go(dim, page) with both as compile-time constants
+template <typename Go>
+cudaError_t by_shape(const vdt_cache8& c, Go go) {
+    auto by_page = [&](auto dim) {
+        if (c.page == 16) return go(dim, std::integral_constant<int, 16>{});
+        if (c.page == 32) return go(dim, std::integral_constant<int, 32>{});
+        return go(dim, std::integral_constant<int, 64>{});
+    };
+    switch (c.dim) {
+        case 32: return by_page(std::integral_constant<int, 32>{});
+        case 64: return by_page(std::integral_constant<int, 64>{});
+        case 96: return by_page(std::integral_constant<int, 96>{});
+        case 128: return by_page(std::integral_constant<int, 128>{});
+        case 192: return by_page(std::integral_constant<int, 192>{});
+        default: return by_page(std::integral_constant<int, 256>{});
     }
 }
 
 template <typename T>
 cudaError_t append(const vdt_cache8& c, const CacheRows& r, const void* k, const void* v, long long kt, long long kh,
                    long long vt, long long vh, cudaStream_t s) {
-    const dim3 grid((r.most + c.page - 1) / c.page + 1, c.heads, r.seqs);
-    k_cache_append<T><<<grid, kCacheThreads, 0, s>>>(c, r, static_cast<const T*>(k), static_cast<const T*>(v), kt, kh, vt, vh);
-    return cudaGetLastError();
+    const dim3 grid((r.most + c.page - 2) / c.page + 1, c.heads, r.seqs);
+    const T *kp = static_cast<const T*>(k), *vp = static_cast<const T*>(v);
+    constexpr int N = Vec16<T>::N;
+    if (!aligned(k, 16) || !aligned(v, 16) || kt % N || kh % N || vt % N || vh % N) {
+        k_cache_append_any<T><<<grid, kCacheThreads, 0, s>>>(c, r, kp, vp, kt, kh, vt, vh);
+        return cudaGetLastError();
+    }
+    return by_shape(c, [&](auto dim, auto page) {
+        k_cache_append_rows<T, dim(), page()><<<grid, kCacheThreads, 0, s>>>(c, r, kp, vp, kt, kh, vt, vh);
+        return cudaGetLastError();
+    });
 }
 template <typename T>
 cudaError_t load(const vdt_cache8& c, const CacheRows& r, void* k, void* v, cudaStream_t s) {
     const dim3 grid((r.most + c.page - 1) / c.page, c.heads, r.seqs);
-    k_cache_load<T><<<grid, kCacheThreads, 0, s>>>(c, r, static_cast<T*>(k), static_cast<T*>(v));
-    return cudaGetLastError();
+    return by_shape(c, [&](auto dim, auto page) {
+        k_cache_load<T, dim(), page()><<<grid, kCacheThreads, 0, s>>>(c, r, static_cast<T*>(k), static_cast<T*>(v));
+        return cudaGetLastError();
+    });
 }
 
 }  // namespace

@@ -15,9 +15,11 @@ namespace {
 // ------------------------------------------------------------------ quantise
 constexpr int kQuantThreads = 256;
 
-// One CTA a row: the largest magnitude (a first pass), then the codes (a
-// second, from L1 / L2).  16-byte loads where the row allows them.
-template <typename T, bool VEC>
+// One CTA a row: the largest magnitude, then the codes.  Rows of up to HELD
+// vectors a thread are read once and stay in registers; longer ones, and rows
+// that are not on 16 bytes (HELD 0), are read twice, the second time from L1
+// and L2.
+template <typename T, int HELD>
 __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T* __restrict__ x, int cols,
                                                                  long long x_stride, int8_t* __restrict__ codes,
                                                                  long long codes_stride, float* __restrict__ scale) {
@@ -26,9 +28,16 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T* __rest
     chain_release();
     const T* row = x + (long long)blockIdx.x * x_stride;
     int8_t* out = codes + (long long)blockIdx.x * codes_stride;
-    const int vecs = VEC ? cols / N : 0;
+    const int vecs = HELD ? cols / N : 0;
     float m = 0.0f;
-    for (int i = threadIdx.x; i < vecs; i += kQuantThreads) {
+    Vec16<T> held[HELD ? HELD : 1];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const int at = threadIdx.x + i * kQuantThreads;
+        held[i].raw = at < vecs ? *reinterpret_cast<const uint4*>(row + (long long)at * N) : make_uint4(0, 0, 0, 0);
+    }
+    for (int i = vecs * N + threadIdx.x; i < cols; i += kQuantThreads) m = max_nan(fabsf(to_f32(row[i])), m);
+    for (int i = threadIdx.x + HELD * kQuantThreads; i < vecs; i += kQuantThreads) {
         Vec16<T> v;
         v.raw = *reinterpret_cast<const uint4*>(row + (long long)i * N);
         float f[N];
@@ -36,29 +45,38 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T* __rest
 #pragma unroll
         for (int j = 0; j < N; ++j) m = max_nan(fabsf(f[j]), m);
     }
-    for (int i = vecs * N + threadIdx.x; i < cols; i += kQuantThreads) m = max_nan(fabsf(to_f32(row[i])), m);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        float f[N];
+        held[i].get(f);
+#pragma unroll
+        for (int j = 0; j < N; ++j) m = max_nan(fabsf(f[j]), m);
+    }
 #pragma unroll
     for (int d = 16; d; d >>= 1) m = max_nan(__shfl_xor_sync(0xffffffffu, m, d), m);
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = m;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kQuantThreads / 32; ++i) m = max_nan(part[i], m);
-    const float sc = m * kCodeStep;
-    if (threadIdx.x == 0) scale[blockIdx.x] = sc;
-    for (int i = threadIdx.x; i < vecs; i += kQuantThreads) {
+    const Coder coder(m * kCodeStep);
+    if (threadIdx.x == 0) scale[blockIdx.x] = coder.scale;
+    auto store = [&](const Vec16<T>& v, int at) {
+        float f[N];
+        uint32_t w[N / 4];
+        v.get(f);
+        coder.words<N>(f, w);
+        if constexpr (N == 8) *reinterpret_cast<uint2*>(out + (long long)at * N) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(out + (long long)at * N) = w[0];
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+        if ((int)threadIdx.x + i * kQuantThreads < vecs) store(held[i], threadIdx.x + i * kQuantThreads);
+    for (int i = threadIdx.x + HELD * kQuantThreads; i < vecs; i += kQuantThreads) {
         Vec16<T> v;
         v.raw = *reinterpret_cast<const uint4*>(row + (long long)i * N);
-        float f[N];
-        v.get(f);
-        uint32_t w[N / 4];
-#pragma unroll
-        for (int j = 0; j < N / 4; ++j)
-            w[j] = (code_of(f[4 * j], sc) & 255) | (code_of(f[4 * j + 1], sc) & 255) << 8 |
-                   (code_of(f[4 * j + 2], sc) & 255) << 16 | (uint32_t)code_of(f[4 * j + 3], sc) << 24;
-        if constexpr (N == 8) *reinterpret_cast<uint2*>(out + (long long)i * N) = make_uint2(w[0], w[1]);
-        else *reinterpret_cast<uint32_t*>(out + (long long)i * N) = w[0];
+        store(v, i);
     }
-    for (int i = vecs * N + threadIdx.x; i < cols; i += kQuantThreads) out[i] = (int8_t)code_of(to_f32(row[i]), sc);
+    for (int i = vecs * N + threadIdx.x; i < cols; i += kQuantThreads) out[i] = (int8_t)code_of(to_f32(row[i]), coder.scale);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -404,8 +422,9 @@ cudaError_t quant_launch(const void* x, long long rows, int cols, long long x_st
     const bool vec = aligned(x, 16) && (x_stride * (long long)sizeof(T)) % 16 == 0 && aligned(codes, N) &&
                      codes_stride % N == 0;
     const T* in = static_cast<const T*>(x);
-    if (vec) k_quantize_rows<T, true><<<(unsigned)rows, kQuantThreads, 0, s>>>(in, cols, x_stride, codes, codes_stride, scale);
-    else k_quantize_rows<T, false><<<(unsigned)rows, kQuantThreads, 0, s>>>(in, cols, x_stride, codes, codes_stride, scale);
+    const int each = (cols / N + kQuantThreads - 1) / kQuantThreads;       // vectors a thread
+    auto kern = !vec ? k_quantize_rows<T, 0> : each <= 1 ? k_quantize_rows<T, 1> : each <= 2 ? k_quantize_rows<T, 2> : k_quantize_rows<T, 4>;
+    kern<<<(unsigned)rows, kQuantThreads, 0, s>>>(in, cols, x_stride, codes, codes_stride, scale);
     return cudaGetLastError();
 }
 

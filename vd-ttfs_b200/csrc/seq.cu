@@ -203,7 +203,7 @@ extern "C" int vdt_cache_load(const vdt_cache8* cache, const int32_t* d_pages, i
     if (int s = check_rows(d_pages, width, d_kept, d_starts, seqs, total, most)) return s;
     if (!seqs || !total || !most) return VDT_OK;
     SEQ_REQUIRE(d_k && d_v, "NULL buffer");
-    SEQ_REQUIRE(aligned(d_k, type_size(type)) && aligned(d_v, type_size(type)), "alignment");
+    SEQ_REQUIRE(aligned(d_k, 16) && aligned(d_v, 16), "outputs must start on 16-byte boundaries");
     if (int s = api_check_buffers(-1, {cache->k, cache->v, cache->k_scale, cache->v_scale, d_k, d_v, d_pages, d_kept, d_starts})) return s;
     return launched(launch_cache_load(*cache, cache_rows(d_pages, width, d_kept, d_starts, seqs, total, most), d_k, d_v, type,
                                       static_cast<cudaStream_t>(stream)), "cache_load");

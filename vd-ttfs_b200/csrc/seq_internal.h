@@ -87,6 +87,39 @@ __device__ __forceinline__ int code_of(float x, float scale) {
     return q != q ? 0 : (int)fminf(fmaxf(q, -127.0f), 127.0f);
 }
 
+// The codes of values under one scale.  x / scale and x * (1 / scale) differ by
+// less than 2^-15 (three roundings of numbers up to 128), so they round to the
+// same code unless the product is that near to the middle between two; then,
+// and for scales whose reciprocal is not a normal number, the division decides.
+struct Coder {
+    float scale, inverse;
+    bool exact;          // 1 / scale is of use
+    __device__ __forceinline__ explicit Coder(float s) : scale(s), inverse(1.0f / s), exact(s > 1e-37f && s < 1e37f) {}
+    template <int N>
+    __device__ __forceinline__ void words(const float* f, uint32_t* w) const {
+        // 1.5 * 2^23 added: the nearest whole number, ties to even, in the low bits
+        constexpr float kRound = 12582912.0f;
+        float near = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            uint32_t c[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float q = f[j + i] * inverse, r = q + kRound;
+                near = fmaxf(near, fabsf(q - (r - kRound)));
+                c[i] = __float_as_uint(r);
+            }
+            w[j / 4] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+        }
+        if (!exact || near > 0.5f - 1.0f / 32768) {
+#pragma unroll
+            for (int j = 0; j < N; j += 4)
+                w[j / 4] = (code_of(f[j], scale) & 255) | (code_of(f[j + 1], scale) & 255) << 8 | (code_of(f[j + 2], scale) & 255) << 16 |
+                           (uint32_t)code_of(f[j + 3], scale) << 24;
+        }
+    }
+};
+
 // A launch that may start while the kernel before it on the stream ends; the
 // kernel calls chain_wait() before it reads what that one wrote.
 template <typename... KArgs, typename... Args>
