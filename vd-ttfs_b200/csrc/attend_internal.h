@@ -1,0 +1,68 @@
+// attend_internal.h -- what the two attention kernels (k_attend.cu for few
+// query rows, k_attend_tiles.cu for many) share.
+#pragma once
+
+#include "seq_internal.h"
+
+namespace vdt {
+
+// How the cached tokens are divided among CTAs
+struct Chunks {
+    int tokens, count;             // of one chunk; chunks
+};
+
+// A sequence's queries; none where the caller's offsets do not fit the buffers.
+struct Queries {
+    long long first;
+    int rows;            // queries
+    int kept;            // tokens in the cache; -1: more than the table or most_kept allow
+};
+__device__ __forceinline__ Queries queries_of(const AttendParams& p, int b) {
+    Queries s;
+    s.first = p.r.starts[b];
+    const long long rows = (long long)p.r.starts[b + 1] - s.first;
+    s.rows = rows > 0 && rows <= p.r.most && s.first >= 0 && s.first + rows <= p.r.total ? (int)rows : 0;
+    const int kept = p.r.held[b];
+    s.kept = kept > p.most_kept || (long long)kept > (long long)p.r.width * p.c.page ? -1 : max(kept, 0);
+    return s;
+}
+
+// Four codes as two pairs of 16-bit floats: code + 128 in the low bits of
+// 1024's significand, less 1152.
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    w ^= 0x80808080u;
+    const __half2 bias = __half2half2(__ushort_as_half(0x6480));   // 1152
+    uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    __half2 x, y;
+    memcpy(&x, &a, 4);
+    memcpy(&y, &b, 4);
+    x = __hsub2(x, bias);
+    y = __hsub2(y, bias);
+    memcpy(&lo, &x, 4);
+    memcpy(&hi, &y, 4);
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    uint32_t u;
+    memcpy(&u, &h, 4);
+    return u;
+}
+__device__ __forceinline__ float nan_f() { return __int_as_float(0x7fffffff); }
+__device__ __forceinline__ float inf_f() { return __int_as_float(0x7f800000); }
+
+// values of the queries' and the output's type (f16 or bf16)
+__device__ __forceinline__ float load_value(const void* p, long long i, int type) {
+    return type == VDT_F16 ? __half2float(static_cast<const __half*>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_value(void* p, long long i, int type, float x) {
+    if (type == VDT_F16) static_cast<__half*>(p)[i] = __float2half_rn(x);
+    else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+}
+
+// many query rows: one CTA for up to 256 rows (k_attend_tiles.cu)
+bool attend_tiles_dim(int dim);
+Chunks plan_tiles(int heads, int kv_heads, int seqs, int most, int most_kept);
+int tile_rows(long long rows);          // rows of a CTA
+cudaError_t launch_attend_tiles(const AttendParams& p, const Chunks& c, cudaStream_t s);
+
+}  // namespace vdt

@@ -14,7 +14,7 @@
 // the largest vs so far, and into the sums' rescaling when that grows.  Their
 // rounding to 16 bits is at most 2^-11: that of an f16 output, an eighth of a
 // bf16 one's, and it averages over the tokens.
-#include "seq_internal.h"
+#include "attend_internal.h"
 
 namespace vdt {
 namespace {
@@ -32,10 +32,6 @@ constexpr int kRowsWarps = 4;
 constexpr int kRing = 3;           // entries of a warp's ring; a unit's keys are one, its values one
 constexpr int kMostChunk = 4096;   // tokens of a chunk: bounds the page lists in shared memory
 
-struct Chunks {
-    int tokens, count;             // of one chunk; chunks
-};
-
 // Chunks so that the grid has a few CTAs for each SM, none under 64 tokens a
 // warp.  With one chunk the CTAs write the output themselves.
 Chunks plan_chunks(int heads, int kv_heads, int seqs, int most, int most_kept) {
@@ -51,50 +47,11 @@ Chunks plan_chunks(int heads, int kv_heads, int seqs, int most, int most_kept) {
     return {(int)tokens, (int)(count < 1 ? 1 : count)};
 }
 
-// A sequence's queries; none where the caller's offsets do not fit the buffers.
-struct Queries {
-    long long first;
-    int rows;            // queries
-    int kept;            // tokens in the cache; -1: more than the table or most_kept allow
-};
-__device__ __forceinline__ Queries queries_of(const AttendParams& p, int b) {
-    Queries s;
-    s.first = p.r.starts[b];
-    const long long rows = (long long)p.r.starts[b + 1] - s.first;
-    s.rows = rows > 0 && rows <= p.r.most && s.first >= 0 && s.first + rows <= p.r.total ? (int)rows : 0;
-    const int kept = p.r.held[b];
-    s.kept = kept > p.most_kept || (long long)kept > (long long)p.r.width * p.c.page ? -1 : max(kept, 0);
-    return s;
-}
-
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// Four codes as two pairs of 16-bit floats: code + 128 in the low bits of
-// 1024's significand, less 1152.
-__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    w ^= 0x80808080u;
-    const __half2 bias = __half2half2(__ushort_as_half(0x6480));   // 1152
-    uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
-    __half2 x, y;
-    memcpy(&x, &a, 4);
-    memcpy(&y, &b, 4);
-    x = __hsub2(x, bias);
-    y = __hsub2(y, bias);
-    memcpy(&lo, &x, 4);
-    memcpy(&hi, &y, 4);
-}
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    uint32_t u;
-    memcpy(&u, &h, 4);
-    return u;
-}
-__device__ __forceinline__ float nan_f() { return __int_as_float(0x7fffffff); }
-__device__ __forceinline__ float inf_f() { return __int_as_float(0x7f800000); }
 
 struct RowsLayout {
     uint32_t ring, q, bars, pages, bytes;
@@ -109,15 +66,6 @@ __host__ __device__ inline RowsLayout rows_layout(int dim, int chunk, int page) 
     l.pages = l.bars + kRowsWarps * kRing * 8;
     l.bytes = l.pages + chunk / page * 12;
     return l;
-}
-
-// values of the queries' and the output's type (f16 or bf16)
-__device__ __forceinline__ float load_value(const void* p, long long i, int type) {
-    return type == VDT_F16 ? __half2float(static_cast<const __half*>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-__device__ __forceinline__ void store_value(void* p, long long i, int type, float x) {
-    if (type == VDT_F16) static_cast<__half*>(p)[i] = __float2half_rn(x);
-    else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
 }
 
 template <int D, int P>
@@ -413,7 +361,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
 }
 
 // One warp for each row and head: its chunks' sums, joined.
-__global__ void __launch_bounds__(128) k_attend_join(AttendParams p, int chunk, int count) {
+__global__ void __launch_bounds__(128) k_attend_join(AttendParams p, int chunk, int count, int tile) {
     const int lane = threadIdx.x % 32, group = p.heads / p.c.heads, dim = p.c.dim;
     const long long i = (long long)blockIdx.x * 4 + threadIdx.x / 32;
     chain_wait();
@@ -434,8 +382,8 @@ __global__ void __launch_bounds__(128) k_attend_join(AttendParams p, int chunk, 
         for (int d = lane; d < dim; d += 32) store_value(p.out, out + d, p.type, nan_f());
         return;
     }
-    // the chunks that the row's tile of 16 has: up to the tokens its last row sees
-    const int row = at * group + head % group, last = min(row / 16 * 16 + 15, s.rows * group - 1) / group;
+    // the chunks that the row's tile has: up to the tokens its last row sees
+    const int row = at * group + head % group, last = min(row / tile * tile + tile - 1, s.rows * group - 1) / group;
     const int sees = p.causal ? max(0, s.kept - s.rows + last + 1) : s.kept;
     const int n = min((sees + chunk - 1) / chunk, count);
     const float* from = p.scratch + i * count * (dim + 2);
@@ -452,37 +400,33 @@ __global__ void __launch_bounds__(128) k_attend_join(AttendParams p, int chunk, 
 }
 
 template <int D, int P>
-cudaError_t rows_launch(const AttendParams& p, cudaStream_t s) {
-    const Chunks c = plan_chunks(p.heads, p.c.heads, p.r.seqs, p.r.most, p.most_kept);
+cudaError_t rows_launch(const AttendParams& p, const Chunks& c, cudaStream_t s) {
     const RowsLayout lay = rows_layout(D, c.tokens, P);
     const long long tiles = ((long long)p.r.most * (p.heads / p.c.heads) + 15) / 16;
     const dim3 grid(c.count, (unsigned)(tiles * p.c.heads), p.r.seqs);
-    if (tiles * p.c.heads > 65535) return cudaErrorInvalidValue;
     cudaError_t e = allow_shared<k_attend_rows<D, P>>((int)rows_layout(D, kMostChunk, P).bytes);
     if (e != cudaSuccess) return e;
     k_attend_rows<D, P><<<grid, kRowsWarps * 32, lay.bytes, s>>>(p, c.tokens);
-    if ((e = cudaGetLastError()) != cudaSuccess || c.count == 1) return e;
-    const long long n = p.r.total * p.heads;
-    return launch_after(k_attend_join, dim3((unsigned)((n + 3) / 4)), dim3(128), 0, s, p, c.tokens, c.count);
+    return cudaGetLastError();
 }
 
 template <int D>
-cudaError_t by_page(const AttendParams& p, cudaStream_t s) {
+cudaError_t by_page(const AttendParams& p, const Chunks& c, cudaStream_t s) {
     switch (p.c.page) {
-        case 16: return rows_launch<D, 16>(p, s);
-        case 32: return rows_launch<D, 32>(p, s);
-        default: return rows_launch<D, 64>(p, s);
+        case 16: return rows_launch<D, 16>(p, c, s);
+        case 32: return rows_launch<D, 32>(p, c, s);
+        default: return rows_launch<D, 64>(p, c, s);
     }
 }
 
-cudaError_t by_dim(const AttendParams& p, cudaStream_t s) {
+cudaError_t by_dim(const AttendParams& p, const Chunks& c, cudaStream_t s) {
     switch (p.c.dim) {
-        case 32: return by_page<32>(p, s);
-        case 64: return by_page<64>(p, s);
-        case 96: return by_page<96>(p, s);
-        case 128: return by_page<128>(p, s);
-        case 192: return by_page<192>(p, s);
-        default: return by_page<256>(p, s);
+        case 32: return by_page<32>(p, c, s);
+        case 64: return by_page<64>(p, c, s);
+        case 96: return by_page<96>(p, c, s);
+        case 128: return by_page<128>(p, c, s);
+        case 192: return by_page<192>(p, c, s);
+        default: return by_page<256>(p, c, s);
     }
 }
 
@@ -490,13 +434,35 @@ cudaError_t by_dim(const AttendParams& p, cudaStream_t s) {
 
 bool attend_dim_ok(int dim) { return dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256; }
 
+// Many rows go to the tile kernel where it has the head's size; up to 16 rows
+// fill one tile of this file's kernel, which reads the cache as fast.
+bool use_tiles(int dim, int heads, int kv_heads, int most) {
+    return attend_tiles_dim(dim) && (long long)most * (heads / kv_heads) > 16;
+}
+
+Chunks plan(int dim, int heads, int kv_heads, int seqs, int most, int most_kept) {
+    return use_tiles(dim, heads, kv_heads, most) ? plan_tiles(heads, kv_heads, seqs, most, most_kept)
+                                                 : plan_chunks(heads, kv_heads, seqs, most, most_kept);
+}
+
+// the grid's y counts tiles of 16 rows
+bool attend_fits(int dim, int heads, int kv_heads, int most) {
+    return use_tiles(dim, heads, kv_heads, most) || ((long long)most * (heads / kv_heads) + 15) / 16 * kv_heads <= 65535;
+}
+
 size_t attend_scratch_bytes(long long total, int heads, int kv_heads, int dim, int seqs, int most, int most_kept) {
-    const Chunks c = plan_chunks(heads, kv_heads, seqs, most, most_kept);
+    const Chunks c = plan(dim, heads, kv_heads, seqs, most, most_kept);
     return c.count == 1 ? 0 : (size_t)total * heads * c.count * (dim + 2) * sizeof(float);
 }
 
 cudaError_t launch_cache_attention(const AttendParams& p, cudaStream_t s) {
-    return by_dim(p, s);
+    const bool tiles = use_tiles(p.c.dim, p.heads, p.c.heads, p.r.most);
+    const Chunks c = plan(p.c.dim, p.heads, p.c.heads, p.r.seqs, p.r.most, p.most_kept);
+    const cudaError_t e = tiles ? launch_attend_tiles(p, c, s) : by_dim(p, c, s);
+    if (e != cudaSuccess || c.count == 1) return e;
+    const long long n = p.r.total * p.heads;
+    const int rows = tiles ? tile_rows((long long)p.r.most * (p.heads / p.c.heads)) : 16;
+    return launch_after(k_attend_join, dim3((unsigned)((n + 3) / 4)), dim3(128), 0, s, p, c.tokens, c.count, rows);
 }
 
 }  // namespace vdt

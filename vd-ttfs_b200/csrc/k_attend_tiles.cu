@@ -1,0 +1,545 @@
+// k_attend_tiles.cu -- attention over the paged 8-bit cache for many query
+// rows, on the fifth-generation tensor cores (mathematics: k_attend.cu).
+//
+// One CTA: a sequence, a head of the cache, one or two tiles of 128 of the
+// rows (query, head of the group) that share it.  For 128 tokens at a time,
+//   S = Q K^T    128 x 128 x dim   from shared memory into tensor memory
+//   P = exp2(S c - m)              tensor memory -> registers -> tensor memory
+//   O += P V     128 x dim x 128   P from tensor memory, V from shared memory
+// and every part has its own warps, joined by barriers:
+//   - four warps for each tile: a thread has a row, so the softmax needs no
+//     exchange; P takes the place of S;
+//   - four warps turn the codes of the next keys and values into 16-bit floats
+//     in shared memory (both are rows of 128 bytes, swizzled, with what the
+//     product sums over side by side: a value row's tokens are so in the
+//     cache already);
+//   - one thread issues the products: with two tiles, one tile's run while the
+//     other's softmax does;
+//   - one warp reads the page table and the pages' scales ahead.
+// O is not divided or rescaled on the way unless a row's maximum grows by more
+// than 2^8 over what its weights are relative to (the weights are 16-bit
+// floats, which have room for that: at most 2^8 x 2^4 below), or a page's value
+// scale by more than 2^4.
+#include "attend_internal.h"
+
+namespace vdt {
+namespace {
+
+constexpr int kTile = 128;        // query rows of a tile; tokens of a step
+constexpr int kAhead = 4;         // steps that the page lists are ahead
+constexpr float kSlack = 8.0f;    // by how much (a power of two) a weight may pass 1
+constexpr float kValueSlack = 16.0f;
+
+template <int D, int NT, int P>
+struct Shape {
+    static constexpr int kSub = (D + 63) / 64;                     // 64-wide blocks of a head
+    static constexpr int kQ = kSub * kTile * 128, kK = kQ, kV = 2 * D * 128;
+    static constexpr int kPages = kTile / P;
+    static constexpr int kSoft = 4 * NT, kCode = kSoft, kIssue = kSoft + 4;   // first warps of each part; the lists' is the last
+    static constexpr int kThreads = (kSoft + 6) * 32;
+    static constexpr int kTmem = NT * (kTile + D) <= 256 ? 256 : 512;
+    static constexpr int kBytes = 1024 + NT * kQ + 2 * kK + 2 * kV;
+};
+
+template <int NT, int PAGES>
+struct State {
+    uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[NT], p_full[NT], o_done[NT], list_full[kAhead], list_free[kAhead];
+    uint32_t tmem;
+    int page[kAhead][PAGES];
+    float k_scale[kAhead][PAGES], v_scale[kAhead][PAGES], v_most[kAhead];
+};
+
+// d (128 x N, 32-bit) (+)= a b^T for 16 columns of 16-bit floats
+__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32]) {
+    uint32_t a[16], b[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        a[i] = r[i];
+        b[i] = r[16 + i];
+    }
+    tmem_store16(at, a);
+    tmem_store16(at + 16, b);
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// what this thread wrote to shared memory is there for the tensor cores
+__device__ __forceinline__ void fence_shared_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 16 codes to two 16-byte pieces `chunk` and `chunk + 1` of a swizzled row;
+// `flip` writes the second first (lanes that would meet on one bank)
+__device__ __forceinline__ void store_codes(unsigned char* rows, int row, int chunk, const uint4& w, bool flip) {
+    uint4 a, b;
+    codes_to_f16(w.x, a.x, a.y);
+    codes_to_f16(w.y, a.z, a.w);
+    codes_to_f16(w.z, b.x, b.y);
+    codes_to_f16(w.w, b.z, b.w);
+    unsigned char* at = rows + row * 128;
+    *reinterpret_cast<uint4*>(at + (((chunk + flip) ^ (row & 7)) << 4)) = flip ? b : a;
+    *reinterpret_cast<uint4*>(at + (((chunk + !flip) ^ (row & 7)) << 4)) = flip ? a : b;
+}
+
+template <int D, int NT, int P>
+__global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, NT == 1 && D <= 64 ? 2 : 1) k_attend_tiles(AttendParams p, int chunk, int count) {
+    using Sh = Shape<D, NT, P>;
+    constexpr int kPages = Sh::kPages;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ State<NT, kPages> st;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int b = blockIdx.z, h = blockIdx.y, group = p.heads / p.c.heads;
+    // the longest rows first: they see the most tokens
+    const int part = blockIdx.x % count, row0 = (gridDim.x / count - 1 - blockIdx.x / count) * (NT * kTile);
+    const Queries s = queries_of(p, b);
+    const int rows = s.rows * group;
+    if (row0 >= rows) return;
+    auto sees = [&](int r) {                       // tokens that row r of the sequence sees
+        if (r >= rows || s.kept < 0) return 0;
+        return p.causal ? max(0, s.kept - s.rows + r / group + 1) : s.kept;
+    };
+    const int begin = part * chunk;
+    // steps that each tile takes, and the longer of them
+    int steps[NT], most = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int last = min(row0 + (t + 1) * kTile, rows) - 1;
+        const int end = row0 + t * kTile < rows ? min(begin + chunk, sees(last)) : 0;
+        steps[t] = max(0, (end - begin + kTile - 1) / kTile);
+        most = max(most, steps[t]);
+    }
+    if (count > 1 && begin >= max(1, sees(min(row0 + NT * kTile, rows) - 1))) return;     // the join knows as well
+
+    unsigned char* smem = smem_raw + ((1024 - (shared_address(smem_raw) & 1023)) & 1023);
+    unsigned char* const kt = smem + NT * Sh::kQ;
+    unsigned char* const vt = kt + 2 * Sh::kK;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            bar_init(shared_address(&st.k_full[i]), 4);
+            bar_init(shared_address(&st.k_free[i]), 1);
+            bar_init(shared_address(&st.v_full[i]), 4);
+            bar_init(shared_address(&st.v_free[i]), 1);
+        }
+        for (int i = 0; i < NT; ++i) {
+            bar_init(shared_address(&st.s_full[i]), 1);
+            bar_init(shared_address(&st.p_full[i]), kTile);
+            bar_init(shared_address(&st.o_done[i]), 1);
+        }
+        for (int i = 0; i < kAhead; ++i) {
+            bar_init(shared_address(&st.list_full[i]), 1);
+            bar_init(shared_address(&st.list_free[i]), 4 + 4 * NT);
+        }
+        bar_init_done();
+    }
+    if (warp == Sh::kIssue) tmem_alloc(shared_address(&st.tmem), Sh::kTmem);
+
+    // a softmax thread's row: its queries into shared memory, scaled by a power of two
+    float q_scale = 0.0f;
+    long long token = 0;
+    int head = 0, limit = 0;
+    const int mine = row0 + threadIdx.x;           // softmax threads are the first NT * 128
+    if (warp < Sh::kSoft) {
+        limit = sees(mine);
+        token = s.first + mine / group;
+        head = h * group + mine % group;
+        unsigned char* const to = smem + warp / 4 * Sh::kQ;
+        const int r = threadIdx.x % kTile;
+        const long long from = token * p.q_token + (long long)head * p.q_head;
+        const bool in = mine < rows, wide = p.q_token % 8 == 0 && p.q_head % 8 == 0 && reinterpret_cast<uintptr_t>(p.q) % 16 == 0;
+        auto eight = [&](int d, float (&f)[8]) {
+            if (!in) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = 0.0f;
+            } else if (wide) {
+                const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) + from + d);
+                if (p.type == VDT_F16) {
+                    Vec16<__half> v{raw};
+                    v.get(f);
+                } else {
+                    Vec16<__nv_bfloat16> v{raw};
+                    v.get(f);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = load_value(p.q, from + d + j, p.type);
+            }
+        };
+        float m = 0.0f;
+        for (int d = 0; d < D; d += 8) {
+            float f[8];
+            eight(d, f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[j]));
+        }
+        const int e = m > 0.0f && m < inf_f() ? max(-126, min(126, ilogbf(m))) : 0;
+        q_scale = scalbnf(fabsf(p.scale), e);
+        const float f1 = copysignf(scalbnf(1.0f, -e), p.scale);        // a negative scale goes into the queries
+        for (int d = 0; d < D; d += 8) {
+            float f[8];
+            eight(d, f);
+            uint4 w;
+            w.x = pack_f16(f[0] * f1, f[1] * f1);
+            w.y = pack_f16(f[2] * f1, f[3] * f1);
+            w.z = pack_f16(f[4] * f1, f[5] * f1);
+            w.w = pack_f16(f[6] * f1, f[7] * f1);
+            *reinterpret_cast<uint4*>(to + d / 64 * (kTile * 128) + r * 128 + ((d % 64 / 8 ^ (r & 7)) << 4)) = w;
+        }
+        fence_shared_async();
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = st.tmem, tmem_o = tmem + NT * kTile;
+    bool alive = true;
+
+    if (warp < Sh::kSoft) {
+        // ------------------------------------------------------------ softmax
+        const int t = warp / 4;
+        const uint32_t lanes = (uint32_t)(warp % 4) << 21;             // this warp's rows of the tensor memory
+        const uint32_t at_s = tmem + t * kTile + lanes, at_o = tmem_o + t * D + lanes;
+        int my_steps = 0;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) my_steps = i == t ? steps[i] : my_steps;
+        float ref = -inf_f(), vref = 0.0f, sum = 0.0f;                 // what the weights and O are relative to
+        for (int j = 0; j < most; ++j) {
+            const int slot = j % kAhead;
+            alive = bar_wait_all(shared_address(&st.list_full[slot]), j / kAhead & 1);
+            if (!alive) break;
+            if (j < my_steps) {
+                float c[kPages];
+#pragma unroll
+                for (int i = 0; i < kPages; ++i) c[i] = st.k_scale[slot][i] * q_scale;
+                const int left = limit - (begin + j * kTile);          // tokens of the step that the row sees
+                const bool partial = __any_sync(0xffffffffu, left < kTile);
+                alive = bar_wait_all(shared_address(&st.s_full[t]), j & 1);
+                if (!alive) break;
+                tmem_fence_after();
+                float top = -inf_f();
+#pragma unroll
+                for (int i = 0; i < kTile; i += 32) {
+                    uint32_t r[32];
+                    tmem_load(at_s + i, r);
+                    tmem_load_wait();
+                    if (partial)
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) r[q] = i + q < left ? r[q] : 0xff800000u;
+#pragma unroll
+                    for (int g = 0; g < 32; g += 16) {
+                        float m = __uint_as_float(r[g]);
+#pragma unroll
+                        for (int q = 1; q < 16; ++q) m = fmaxf(m, __uint_as_float(r[g + q]));
+                        top = fmaxf(top, m * c[(i + g) / P]);
+                    }
+                }
+                const float v_most = st.v_most[slot];
+                const bool up = top > ref + kSlack || (ref == -inf_f() && top > ref), v_up = v_most > kValueSlack * vref;
+                if (v_up || __any_sync(0xffffffffu, up)) {
+                    const float to = up ? top : ref, by = ref == -inf_f() ? 0.0f : exp2_fast(ref - to);
+                    const float v_by = v_up ? vref / v_most : 1.0f;
+                    sum *= by;
+                    if (j > 0) {
+                        alive = bar_wait_all(shared_address(&st.o_done[t]), (j - 1) & 1);
+                        if (!alive) break;
+                        tmem_fence_after();
+#pragma unroll
+                        for (int i = 0; i < D; i += 32) {
+                            uint32_t r[32];
+                            tmem_load(at_o + i, r);
+                            tmem_load_wait();
+#pragma unroll
+                            for (int q = 0; q < 32; ++q) r[q] = __float_as_uint(__uint_as_float(r[q]) * (by * v_by));
+                            tmem_store32(at_o + i, r);
+                        }
+                    }
+                    ref = to;
+                    if (v_up) vref = v_most;
+                }
+                const float shift = ref == -inf_f() ? 0.0f : -ref;
+                float f[kPages];
+#pragma unroll
+                for (int i = 0; i < kPages; ++i) f[i] = vref > 0.0f ? st.v_scale[slot][i] / vref : st.v_scale[slot][i];
+                float l[4] = {};
+#pragma unroll
+                for (int i = 0; i < kTile; i += 32) {
+                    uint32_t r[32], w[16];
+                    tmem_load(at_s + i, r);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int q = 0; q < 32; q += 2) {
+                        float x = exp2_fast(fmaf(__uint_as_float(r[q]), c[(i + q) / P], shift));
+                        float y = exp2_fast(fmaf(__uint_as_float(r[q + 1]), c[(i + q) / P], shift));
+                        if (partial) {
+                            x = i + q < left ? x : 0.0f;
+                            y = i + q + 1 < left ? y : 0.0f;
+                        }
+                        l[q / 2 % 2 * 2] += x;
+                        l[q / 2 % 2 * 2 + 1] += y;
+                        x *= f[(i + q) / P];
+                        y *= f[(i + q) / P];
+                        if (partial) {                                 // a scale that is not a number stays with those who see it
+                            x = i + q < left ? x : 0.0f;
+                            y = i + q + 1 < left ? y : 0.0f;
+                        }
+                        w[q / 2] = pack_f16(x, y);
+                    }
+                    tmem_store16(at_s + i / 2, w);
+                }
+                sum += (l[0] + l[1]) + (l[2] + l[3]);
+                tmem_store_wait();
+                tmem_fence_before();
+                bar_arrive(shared_address(&st.p_full[t]));
+            }
+            __syncwarp();
+            if (lane == 0) bar_arrive(shared_address(&st.list_free[slot]));
+        }
+        // ------------------------------------------------------------- output
+        if (alive && my_steps) alive = bar_wait_all(shared_address(&st.o_done[t]), (my_steps - 1) & 1);
+        tmem_fence_after();
+        const bool bad = !alive || s.kept < 0;
+        const float scale = bad ? nan_f() : count > 1 ? vref : sum == 0.0f ? 0.0f : vref / sum;
+        const bool nothing = !bad && sum == 0.0f;                       // no token seen (O may not have been written)
+        const long long out = token * p.out_token + (long long)head * p.out_head;
+        float* const rest = p.scratch + ((token * p.heads + head) * count + part) * (D + 2);
+        const bool wide = p.out_token % 8 == 0 && p.out_head % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+        if (count > 1 && mine < rows) {
+            rest[0] = ref;
+            rest[1] = bad ? nan_f() : sum;
+        }
+#pragma unroll
+        for (int i = 0; i < D; i += 32) {
+            uint32_t r[32];
+            __syncwarp();
+            tmem_load(at_o + i, r);
+            tmem_load_wait();
+            if (mine >= rows) continue;
+            if (count > 1) {
+#pragma unroll
+                for (int q = 0; q < 32; ++q) rest[2 + i + q] = nothing ? 0.0f : __uint_as_float(r[q]) * scale;
+            } else if (wide) {
+#pragma unroll
+                for (int q = 0; q < 32; q += 8) {
+                    float f[8];
+#pragma unroll
+                    for (int a = 0; a < 8; ++a) f[a] = nothing ? 0.0f : __uint_as_float(r[q + a]) * scale;
+                    uint4* to = reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + out + i + q);
+                    if (p.type == VDT_F16) {
+                        Vec16<__half> v;
+                        v.set(f);
+                        *to = v.raw;
+                    } else {
+                        Vec16<__nv_bfloat16> v;
+                        v.set(f);
+                        *to = v.raw;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < 32; ++q) store_value(p.out, out + i + q, p.type, nothing ? 0.0f : __uint_as_float(r[q]) * scale);
+            }
+        }
+    } else if (warp < Sh::kIssue) {
+        // ------------------------------------------------- codes to 16 bits
+        const int thread = threadIdx.x - Sh::kCode * 32;
+        constexpr int kPer = D / 16;                                   // 16-byte pieces of a thread, keys or values
+        constexpr int kBlock = P * D / 16;                             // of a page
+        uint4 kw[kPer], vw[kPer];
+        auto load = [&](const int8_t* from, int slot, uint4 (&w)[kPer]) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int at = thread + i * 128, no = st.page[slot][at / kBlock];
+                w[i] = no < 0 ? make_uint4(0, 0, 0, 0)
+                              : __ldg(reinterpret_cast<const uint4*>(from + ((long long)no * p.c.heads + h) * (P * D)) + at % kBlock);
+            }
+        };
+        auto list = [&](int j) { return bar_wait_all(shared_address(&st.list_full[j % kAhead]), j / kAhead & 1); };
+        if (most && (alive = list(0))) load(p.c.k, 0, kw);
+        for (int j = 0; j < most && alive; ++j) {
+            load(p.c.v, j % kAhead, vw);
+            const int slot = j & 1, phase = (j / 2 & 1) ^ 1;
+            if (!(alive = bar_wait_all(shared_address(&st.k_free[slot]), phase))) break;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int at = thread + i * 128, row = at / kPer, e = at % kPer;
+                store_codes(kt + slot * Sh::kK + e / 4 * (kTile * 128), row, e % 4 * 2, kw[i], e & 4);
+            }
+            fence_shared_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(shared_address(&st.k_full[slot]));
+            if (j + 1 < most) {
+                if (!(alive = list(j + 1))) break;
+                load(p.c.k, (j + 1) % kAhead, kw);
+            }
+            __syncwarp();
+            if (lane == 0) bar_arrive(shared_address(&st.list_free[j % kAhead]));
+            if (!(alive = bar_wait_all(shared_address(&st.v_free[slot]), phase))) break;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int at = thread + i * 128, pg = at / kBlock, rest = at % kBlock, row = rest / (P / 16);
+                const int block = pg * (P / 16) + rest % (P / 16);     // 16 tokens of the step's 128
+                store_codes(vt + slot * Sh::kV + block / 4 * (D * 128), row, block % 4 * 2, vw[i], false);
+            }
+            fence_shared_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(shared_address(&st.v_full[slot]));
+        }
+    } else if (warp == Sh::kIssue) {
+        // ---------------------------------------------------------- products
+        if (lane == 0) {
+            constexpr uint32_t shape = 1u << 4 | (kTile >> 4) << 24;   // 32-bit sums of 16-bit floats
+            constexpr uint32_t shape_s = shape | (kTile >> 3) << 17, shape_o = shape | (D >> 3) << 17;
+            const uint32_t q_at = shared_address(smem), k_at = shared_address(kt), v_at = shared_address(vt);
+            auto scores = [&](int t, int slot) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    mma_shared(tmem + t * kTile, tile_desc(q_at + t * Sh::kQ + k / 4 * (kTile * 128)) + k % 4 * 2,
+                               tile_desc(k_at + slot * Sh::kK + k / 4 * (kTile * 128)) + k % 4 * 2, shape_s, k > 0);
+                mma_commit(shared_address(&st.s_full[t]));
+            };
+            auto outputs = [&](int t, int slot, bool add) {
+#pragma unroll
+                for (int k = 0; k < kTile / 16; ++k)
+                    mma_tensor(tmem_o + t * D, tmem + t * kTile + k * 8, tile_desc(v_at + slot * Sh::kV + k / 4 * (D * 128)) + k % 4 * 2,
+                               shape_o, add || k > 0);
+                mma_commit(shared_address(&st.o_done[t]));
+            };
+            if (most && (alive = bar_wait(shared_address(&st.k_full[0]), 0))) {
+                tmem_fence_after();
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    if (steps[t]) scores(t, 0);
+                mma_commit(shared_address(&st.k_free[0]));
+            }
+            for (int j = 0; j < most && alive; ++j) {
+                const int slot = j & 1, next = slot ^ 1;
+                if (!(alive = bar_wait(shared_address(&st.v_full[slot]), j / 2 & 1))) break;
+                if (j + 1 < most && !(alive = bar_wait(shared_address(&st.k_full[next]), (j + 1) / 2 & 1))) break;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if (j >= steps[t]) continue;
+                    if (!(alive = bar_wait(shared_address(&st.p_full[t]), j & 1))) break;
+                    tmem_fence_after();
+                    outputs(t, slot, j > 0);
+                    if (j + 1 < steps[t]) scores(t, next);             // behind the product that reads P in S's place
+                }
+                mma_commit(shared_address(&st.v_free[slot]));
+                if (j + 1 < most) mma_commit(shared_address(&st.k_free[next]));
+            }
+            // the last commit has arrived before the CTA ends
+            if (most && alive) bar_wait(shared_address(&st.v_free[(most - 1) & 1]), (most - 1) / 2 & 1);
+        }
+    } else {
+        // -------------------------------------------------------- page lists
+        for (int j = 0; j < most; ++j) {
+            const int slot = j % kAhead;
+            alive = bar_wait_all(shared_address(&st.list_free[slot]), (j / kAhead & 1) ^ 1);
+            if (!alive) break;
+            float vs = 0.0f;
+            if (lane < kPages) {
+                const int first = begin + j * kTile + lane * P;
+                int no = -1;
+                float ks = 0.0f;
+                if (first < min(begin + chunk, s.kept)) {
+                    no = p.r.table[(long long)b * p.r.width + first / P];
+                    const bool known = no >= 0 && no < p.c.pages;      // else page 0 under scales that are not numbers
+                    if (!known) no = 0;
+                    ks = known ? p.c.k_scale[(long long)no * p.c.heads + h] : nan_f();
+                    vs = known ? p.c.v_scale[(long long)no * p.c.heads + h] : nan_f();
+                }
+                st.page[slot][lane] = no;
+                st.k_scale[slot][lane] = ks;
+                st.v_scale[slot][lane] = vs;
+            }
+            float m = fmaxf(vs, 0.0f);
+#pragma unroll
+            for (int d = 1; d < kPages; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            if (lane == 0) st.v_most[slot] = m;
+            __syncwarp();
+            if (lane == 0) bar_arrive(shared_address(&st.list_full[slot]));
+        }
+    }
+    // the products are done: every tile's last commit has been waited for
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == Sh::kIssue) {
+        __syncwarp();
+        tmem_fence_after();
+        tmem_free(tmem, Sh::kTmem);
+    }
+}
+
+template <int D, int NT, int P>
+cudaError_t tiles_launch(const AttendParams& p, const Chunks& c, cudaStream_t s) {
+    using Sh = Shape<D, NT, P>;
+    const cudaError_t e = allow_shared<k_attend_tiles<D, NT, P>>(Sh::kBytes);
+    if (e != cudaSuccess) return e;
+    const long long rows = (long long)p.r.most * (p.heads / p.c.heads), x = (rows + NT * kTile - 1) / (NT * kTile) * c.count;
+    if (x > 0x7fffffff) return cudaErrorInvalidValue;
+    k_attend_tiles<D, NT, P><<<dim3((unsigned)x, p.c.heads, p.r.seqs), Sh::kThreads, Sh::kBytes, s>>>(p, c.tokens, c.count);
+    return cudaGetLastError();
+}
+
+template <int D, int NT>
+cudaError_t by_page(const AttendParams& p, const Chunks& c, cudaStream_t s) {
+    switch (p.c.page) {
+        case 16: return tiles_launch<D, NT, 16>(p, c, s);
+        case 32: return tiles_launch<D, NT, 32>(p, c, s);
+        default: return tiles_launch<D, NT, 64>(p, c, s);
+    }
+}
+
+template <int NT>
+cudaError_t by_dim(const AttendParams& p, const Chunks& c, cudaStream_t s) {
+    switch (p.c.dim) {
+        case 32: return by_page<32, NT>(p, c, s);
+        case 64: return by_page<64, NT>(p, c, s);
+        case 96: return by_page<96, NT>(p, c, s);
+        default: return by_page<128, NT>(p, c, s);
+    }
+}
+
+}  // namespace
+
+// the tensor memory holds two tiles' scores and sums up to 128 values a head
+bool attend_tiles_dim(int dim) { return dim <= 128; }
+
+int tile_rows(long long rows) { return rows <= kTile ? kTile : 2 * kTile; }
+
+// The tokens divided where the tiles alone leave SMs idle, 512 of them at least
+// to a CTA.
+Chunks plan_tiles(int heads, int kv_heads, int seqs, int most, int most_kept) {
+    const long long rows = (long long)most * (heads / kv_heads);
+    const long long ctas = (long long)kv_heads * seqs * ((rows + tile_rows(rows) - 1) / tile_rows(rows));
+    const long long want = kSmCount / ctas;
+    if (want <= 1) return {(most_kept + kTile - 1) / kTile * kTile, 1};
+    long long tokens = ((long long)most_kept + want - 1) / want;
+    tokens = (tokens + kTile - 1) / kTile * kTile;
+    if (tokens < 4 * kTile) tokens = 4 * kTile;
+    const long long count = ((long long)most_kept + tokens - 1) / tokens;
+    return {(int)tokens, (int)(count < 1 ? 1 : count)};
+}
+
+cudaError_t launch_attend_tiles(const AttendParams& p, const Chunks& c, cudaStream_t s) {
+    return tile_rows((long long)p.r.most * (p.heads / p.c.heads)) == kTile ? by_dim<1>(p, c, s) : by_dim<2>(p, c, s);
+}
+
+}  // namespace vdt

@@ -235,7 +235,7 @@ extern "C" int vdt_cache_attention(const vdt_cache8* cache, const void* d_q, int
     if (need > scratch_bytes || (need && !d_scratch))
         return api_fail(VDT_ERR_CAPACITY, "scratch smaller than vdt_cache_attention_scratch_bytes");
     SEQ_REQUIRE(aligned(d_scratch, 16), "scratch alignment");
-    if ((((int64_t)most * (heads / cache->heads) + 15) / 16) * cache->heads > 65535)
+    if (!attend_fits(cache->dim, heads, cache->heads, most))
         return api_fail(VDT_ERR_UNSUPPORTED, "too many query rows in one sequence: give them in parts");
     if (int s = api_check_buffers(-1, {cache->k, cache->v, cache->k_scale, cache->v_scale, d_q, d_out, d_pages, d_kept, d_starts, d_scratch})) return s;
     AttendParams p{};

@@ -304,6 +304,7 @@ struct AttendParams {
 };
 size_t attend_scratch_bytes(long long total, int heads, int kv_heads, int dim, int seqs, int most, int most_kept);
 bool attend_dim_ok(int dim);
+bool attend_fits(int dim, int heads, int kv_heads, int most);
 cudaError_t launch_cache_attention(const AttendParams& p, cudaStream_t s);
 
 }  // namespace vdt
