@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
             if (!known) no = 0;
             ks = known ? p.c.k_scale[(long long)no * p.c.heads + h] : nan_f();
             vs = known ? p.c.v_scale[(long long)no * p.c.heads + h] : nan_f();
+            if (vs == inf_f()) vs = nan_f();      // it would be what all other weights are relative to
         }
         pages[i] = no;
         k_scale[i] = ks;

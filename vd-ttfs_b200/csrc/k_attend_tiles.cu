@@ -9,13 +9,13 @@
 // and every part has its own warps, joined by barriers:
 //   - four warps for each tile: a thread has a row, so the softmax needs no
 //     exchange; P takes the place of S;
-//   - four warps turn the codes of the next keys and values into 16-bit floats
-//     in shared memory (both are rows of 128 bytes, swizzled, with what the
-//     product sums over side by side: a value row's tokens are so in the
-//     cache already);
+//   - one warp reads the page table and the pages' scales ahead and copies the
+//     pages' codes into shared memory;
+//   - four warps turn those into 16-bit floats, again in shared memory (rows of
+//     128 bytes, swizzled, with what the product sums over side by side: a
+//     value row's tokens are so in the cache already);
 //   - one thread issues the products: with two tiles, one tile's run while the
-//     other's softmax does;
-//   - one warp reads the page table and the pages' scales ahead.
+//     other's softmax does.
 // O is not divided or rescaled on the way unless a row's maximum grows by more
 // than 2^8 over what its weights are relative to (the weights are 16-bit
 // floats, which have room for that: at most 2^8 x 2^4 below), or a page's value
@@ -28,25 +28,39 @@ namespace {
 constexpr int kTile = 128;        // query rows of a tile; tokens of a step
 constexpr int kAhead = 4;         // steps that the page lists are ahead
 constexpr float kSlack = 8.0f;    // by how much (a power of two) a weight may pass 1
-constexpr float kValueSlack = 16.0f;
+constexpr float kValueSlack = 4.0f;
 
 template <int D, int NT, int P>
 struct Shape {
     static constexpr int kSub = (D + 63) / 64;                     // 64-wide blocks of a head
     static constexpr int kQ = kSub * kTile * 128, kK = kQ, kV = 2 * D * 128;
     static constexpr int kPages = kTile / P;
-    static constexpr int kSoft = 4 * NT, kCode = kSoft, kIssue = kSoft + 4;   // first warps of each part; the lists' is the last
-    static constexpr int kThreads = (kSoft + 6) * 32;
+    static constexpr int kRaw = kTile * D;                         // the codes of a step's keys, or values
+    static constexpr int kSoft = 4 * NT, kCode = kSoft, kIssue = kSoft + 4, kList = kSoft + 5;   // first warps of each part
+    static constexpr int kThreads = (kSoft + 8) * 32;              // whole groups of four warps: two have nothing to do
     static constexpr int kTmem = NT * (kTile + D) <= 256 ? 256 : 512;
-    static constexpr int kBytes = 1024 + NT * kQ + 2 * kK + 2 * kV;
+    static constexpr int kBytes = 1024 + NT * kQ + 2 * kK + 2 * kV + 2 * kRaw;
 };
+// registers a thread with two tiles: at launch, and how the four groups of
+// warps share them out
+constexpr int kRegs = 128, kSoftRegs = 200, kCodeRegs = 64, kIssueRegs = 48;
+static_assert(2 * kSoftRegs + kCodeRegs + kIssueRegs == 4 * kRegs, "registers");
+
+template <int N>
+__device__ __forceinline__ void take_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void give_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 template <int NT, int PAGES>
 struct State {
-    uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[NT], p_full[NT], o_done[NT], list_full[kAhead], list_free[kAhead];
+    uint64_t k_full[2], k_free[2], v_full[2], v_free[2], raw_full[2], raw_free[2], s_full[NT], p_full[NT], o_done[NT];
+    uint64_t list_full[kAhead], list_free[kAhead];
     uint32_t tmem;
-    int page[kAhead][PAGES];
-    float k_scale[kAhead][PAGES], v_scale[kAhead][PAGES], v_most[kAhead];
+    float k_scale[kAhead][PAGES], v_log[kAhead][PAGES], v_most[kAhead];    // of the values' scales, the logarithm
 };
 
 // d (128 x N, 32-bit) (+)= a b^T for 16 columns of 16-bit floats
@@ -68,6 +82,13 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16
         "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at));
 }
 __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32]) {
     uint32_t a[16], b[16];
@@ -102,7 +123,7 @@ __device__ __forceinline__ void store_codes(unsigned char* rows, int row, int ch
 }
 
 template <int D, int NT, int P>
-__global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, NT == 1 && D <= 64 ? 2 : 1) k_attend_tiles(AttendParams p, int chunk, int count) {
+__global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(AttendParams p, int chunk, int count) {
     using Sh = Shape<D, NT, P>;
     constexpr int kPages = Sh::kPages;
     extern __shared__ unsigned char smem_raw[];
@@ -133,12 +154,15 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, NT == 1 && D <= 64 
     unsigned char* smem = smem_raw + ((1024 - (shared_address(smem_raw) & 1023)) & 1023);
     unsigned char* const kt = smem + NT * Sh::kQ;
     unsigned char* const vt = kt + 2 * Sh::kK;
+    unsigned char* const raw = vt + 2 * Sh::kV;    // keys' codes, then values'
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             bar_init(shared_address(&st.k_full[i]), 4);
             bar_init(shared_address(&st.k_free[i]), 1);
             bar_init(shared_address(&st.v_full[i]), 4);
             bar_init(shared_address(&st.v_free[i]), 1);
+            bar_init(shared_address(&st.raw_full[i]), 1);
+            bar_init(shared_address(&st.raw_free[i]), 4);
         }
         for (int i = 0; i < NT; ++i) {
             bar_init(shared_address(&st.s_full[i]), 1);
@@ -147,7 +171,7 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, NT == 1 && D <= 64 
         }
         for (int i = 0; i < kAhead; ++i) {
             bar_init(shared_address(&st.list_full[i]), 1);
-            bar_init(shared_address(&st.list_free[i]), 4 + 4 * NT);
+            bar_init(shared_address(&st.list_free[i]), 4 * NT);
         }
         bar_init_done();
     }
@@ -214,97 +238,92 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, NT == 1 && D <= 64 
 
     if (warp < Sh::kSoft) {
         // ------------------------------------------------------------ softmax
+        if constexpr (NT == 2) take_registers<kSoftRegs>();
         const int t = warp / 4;
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;             // this warp's rows of the tensor memory
         const uint32_t at_s = tmem + t * kTile + lanes, at_o = tmem_o + t * D + lanes;
         int my_steps = 0;
 #pragma unroll
         for (int i = 0; i < NT; ++i) my_steps = i == t ? steps[i] : my_steps;
-        float ref = -inf_f(), vref = 0.0f, sum = 0.0f;                 // what the weights and O are relative to
+        // what the weights and O are relative to: 2^ref, 2^vref
+        float ref = -inf_f(), vref = -inf_f(), sum = 0.0f;
         for (int j = 0; j < most; ++j) {
             const int slot = j % kAhead;
             alive = bar_wait_all(shared_address(&st.list_full[slot]), j / kAhead & 1);
             if (!alive) break;
             if (j < my_steps) {
-                float c[kPages];
-#pragma unroll
-                for (int i = 0; i < kPages; ++i) c[i] = st.k_scale[slot][i] * q_scale;
                 const int left = limit - (begin + j * kTile);          // tokens of the step that the row sees
                 const bool partial = __any_sync(0xffffffffu, left < kTile);
                 alive = bar_wait_all(shared_address(&st.s_full[t]), j & 1);
                 if (!alive) break;
                 tmem_fence_after();
+                uint32_t r[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_load(at_s + i * 32, r[i]);
+                float c[kPages];
+#pragma unroll
+                for (int i = 0; i < kPages; ++i) c[i] = st.k_scale[slot][i] * q_scale;
+                tmem_load_wait();
                 float top = -inf_f();
+                if (partial)
 #pragma unroll
-                for (int i = 0; i < kTile; i += 32) {
-                    uint32_t r[32];
-                    tmem_load(at_s + i, r);
-                    tmem_load_wait();
-                    if (partial)
+                    for (int i = 0; i < kTile; ++i) r[i / 32][i % 32] = i < left ? r[i / 32][i % 32] : 0xff800000u;
 #pragma unroll
-                        for (int q = 0; q < 32; ++q) r[q] = i + q < left ? r[q] : 0xff800000u;
+                for (int i = 0; i < kTile; i += P < 32 ? P : 32) {
+                    float m = __uint_as_float(r[i / 32][i % 32]);
 #pragma unroll
-                    for (int g = 0; g < 32; g += 16) {
-                        float m = __uint_as_float(r[g]);
-#pragma unroll
-                        for (int q = 1; q < 16; ++q) m = fmaxf(m, __uint_as_float(r[g + q]));
-                        top = fmaxf(top, m * c[(i + g) / P]);
-                    }
+                    for (int q = 1; q < (P < 32 ? P : 32); ++q) m = fmaxf(m, __uint_as_float(r[i / 32][i % 32 + q]));
+                    top = fmaxf(top, m * c[i / P]);
                 }
                 const float v_most = st.v_most[slot];
-                const bool up = top > ref + kSlack || (ref == -inf_f() && top > ref), v_up = v_most > kValueSlack * vref;
+                const bool up = top > ref + kSlack || (ref == -inf_f() && top > ref), v_up = v_most > vref + kValueSlack || (vref == -inf_f() && v_most > vref);
                 if (v_up || __any_sync(0xffffffffu, up)) {
                     const float to = up ? top : ref, by = ref == -inf_f() ? 0.0f : exp2_fast(ref - to);
-                    const float v_by = v_up ? vref / v_most : 1.0f;
+                    const float v_by = !v_up ? 1.0f : vref == -inf_f() ? 0.0f : exp2_fast(vref - v_most);
                     sum *= by;
                     if (j > 0) {
                         alive = bar_wait_all(shared_address(&st.o_done[t]), (j - 1) & 1);
                         if (!alive) break;
                         tmem_fence_after();
-#pragma unroll
-                        for (int i = 0; i < D; i += 32) {
-                            uint32_t r[32];
-                            tmem_load(at_o + i, r);
+                        for (int i = 0; i < D; i += 16) {
+                            uint32_t o[16];
+                            tmem_load16(at_o + i, o);
                             tmem_load_wait();
 #pragma unroll
-                            for (int q = 0; q < 32; ++q) r[q] = __float_as_uint(__uint_as_float(r[q]) * (by * v_by));
-                            tmem_store32(at_o + i, r);
+                            for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * (by * v_by));
+                            tmem_store16(at_o + i, o);
                         }
                     }
                     ref = to;
                     if (v_up) vref = v_most;
                 }
-                const float shift = ref == -inf_f() ? 0.0f : -ref;
-                float f[kPages];
+                // a weight times its page's scale over 2^vref is one power of
+                // two; the sum of the weights takes the scale out again.  Not
+                // under 2^-100: a page of zeros still has weights.
+                const float shift = ref == -inf_f() ? 0.0f : -ref, v_shift = vref == -inf_f() ? 0.0f : vref;
 #pragma unroll
-                for (int i = 0; i < kPages; ++i) f[i] = vref > 0.0f ? st.v_scale[slot][i] / vref : st.v_scale[slot][i];
-                float l[4] = {};
+                for (int i = 0; i < kPages; ++i) {
+                    float f = st.v_log[slot][i] - v_shift;
+                    f = f < -100.0f ? -100.0f : f;
+                    const float d = shift + f;
+                    float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
-                for (int i = 0; i < kTile; i += 32) {
-                    uint32_t r[32], w[16];
-                    tmem_load(at_s + i, r);
-                    tmem_load_wait();
-#pragma unroll
-                    for (int q = 0; q < 32; q += 2) {
-                        float x = exp2_fast(fmaf(__uint_as_float(r[q]), c[(i + q) / P], shift));
-                        float y = exp2_fast(fmaf(__uint_as_float(r[q + 1]), c[(i + q) / P], shift));
-                        if (partial) {
-                            x = i + q < left ? x : 0.0f;
-                            y = i + q + 1 < left ? y : 0.0f;
+                    for (int q = i * P; q < (i + 1) * P; q += 2) {
+                        float x = exp2_fast(fmaf(__uint_as_float(r[q / 32][q % 32]), c[i], d));
+                        float y = exp2_fast(fmaf(__uint_as_float(r[q / 32][q % 32 + 1]), c[i], d));
+                        if (partial) {                                 // also for scales that are not numbers
+                            x = q < left ? x : 0.0f;
+                            y = q + 1 < left ? y : 0.0f;
                         }
-                        l[q / 2 % 2 * 2] += x;
-                        l[q / 2 % 2 * 2 + 1] += y;
-                        x *= f[(i + q) / P];
-                        y *= f[(i + q) / P];
-                        if (partial) {                                 // a scale that is not a number stays with those who see it
-                            x = i + q < left ? x : 0.0f;
-                            y = i + q + 1 < left ? y : 0.0f;
-                        }
-                        w[q / 2] = pack_f16(x, y);
+                        l0 += x;
+                        l1 += y;
+                        r[q / 64][q / 2 % 32] = pack_f16(x, y);
                     }
-                    tmem_store16(at_s + i / 2, w);
+                    l0 += l1;
+                    sum = partial && i * P >= left ? sum : fmaf(l0, exp2_fast(-f), sum);
                 }
-                sum += (l[0] + l[1]) + (l[2] + l[3]);
+                tmem_store32(at_s, r[0]);
+                tmem_store32(at_s + 32, r[1]);
                 tmem_store_wait();
                 tmem_fence_before();
                 bar_arrive(shared_address(&st.p_full[t]));
@@ -316,7 +335,7 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, NT == 1 && D <= 64 
         if (alive && my_steps) alive = bar_wait_all(shared_address(&st.o_done[t]), (my_steps - 1) & 1);
         tmem_fence_after();
         const bool bad = !alive || s.kept < 0;
-        const float scale = bad ? nan_f() : count > 1 ? vref : sum == 0.0f ? 0.0f : vref / sum;
+        const float scale = bad ? nan_f() : count > 1 ? exp2f(vref) : sum == 0.0f ? 0.0f : exp2f(vref) / sum;
         const bool nothing = !bad && sum == 0.0f;                       // no token seen (O may not have been written)
         const long long out = token * p.out_token + (long long)head * p.out_head;
         float* const rest = p.scratch + ((token * p.heads + head) * count + part) * (D + 2);
@@ -359,51 +378,44 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, NT == 1 && D <= 64 
         }
     } else if (warp < Sh::kIssue) {
         // ------------------------------------------------- codes to 16 bits
+        if constexpr (NT == 2) give_registers<kCodeRegs>();
         const int thread = threadIdx.x - Sh::kCode * 32;
         constexpr int kPer = D / 16;                                   // 16-byte pieces of a thread, keys or values
         constexpr int kBlock = P * D / 16;                             // of a page
-        uint4 kw[kPer], vw[kPer];
-        auto load = [&](const int8_t* from, int slot, uint4 (&w)[kPer]) {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int at = thread + i * 128, no = st.page[slot][at / kBlock];
-                w[i] = no < 0 ? make_uint4(0, 0, 0, 0)
-                              : __ldg(reinterpret_cast<const uint4*>(from + ((long long)no * p.c.heads + h) * (P * D)) + at % kBlock);
-            }
-        };
-        auto list = [&](int j) { return bar_wait_all(shared_address(&st.list_full[j % kAhead]), j / kAhead & 1); };
-        if (most && (alive = list(0))) load(p.c.k, 0, kw);
-        for (int j = 0; j < most && alive; ++j) {
-            load(p.c.v, j % kAhead, vw);
+        for (int j = 0; j < most; ++j) {
             const int slot = j & 1, phase = (j / 2 & 1) ^ 1;
-            if (!(alive = bar_wait_all(shared_address(&st.k_free[slot]), phase))) break;
+            alive = bar_wait_all(shared_address(&st.raw_full[0]), j & 1) && bar_wait_all(shared_address(&st.k_free[slot]), phase);
+            if (!alive) break;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int at = thread + i * 128, row = at / kPer, e = at % kPer;
-                store_codes(kt + slot * Sh::kK + e / 4 * (kTile * 128), row, e % 4 * 2, kw[i], e & 4);
+                store_codes(kt + slot * Sh::kK + e / 4 * (kTile * 128), row, e % 4 * 2, *reinterpret_cast<const uint4*>(raw + at * 16), e & 4);
             }
             fence_shared_async();
             __syncwarp();
-            if (lane == 0) bar_arrive(shared_address(&st.k_full[slot]));
-            if (j + 1 < most) {
-                if (!(alive = list(j + 1))) break;
-                load(p.c.k, (j + 1) % kAhead, kw);
+            if (lane == 0) {
+                bar_arrive(shared_address(&st.raw_free[0]));
+                bar_arrive(shared_address(&st.k_full[slot]));
             }
-            __syncwarp();
-            if (lane == 0) bar_arrive(shared_address(&st.list_free[j % kAhead]));
-            if (!(alive = bar_wait_all(shared_address(&st.v_free[slot]), phase))) break;
+            alive = bar_wait_all(shared_address(&st.raw_full[1]), j & 1) && bar_wait_all(shared_address(&st.v_free[slot]), phase);
+            if (!alive) break;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int at = thread + i * 128, pg = at / kBlock, rest = at % kBlock, row = rest / (P / 16);
                 const int block = pg * (P / 16) + rest % (P / 16);     // 16 tokens of the step's 128
-                store_codes(vt + slot * Sh::kV + block / 4 * (D * 128), row, block % 4 * 2, vw[i], false);
+                store_codes(vt + slot * Sh::kV + block / 4 * (D * 128), row, block % 4 * 2,
+                            *reinterpret_cast<const uint4*>(raw + Sh::kRaw + at * 16), false);
             }
             fence_shared_async();
             __syncwarp();
-            if (lane == 0) bar_arrive(shared_address(&st.v_full[slot]));
+            if (lane == 0) {
+                bar_arrive(shared_address(&st.raw_free[1]));
+                bar_arrive(shared_address(&st.v_full[slot]));
+            }
         }
     } else if (warp == Sh::kIssue) {
         // ---------------------------------------------------------- products
+        if constexpr (NT == 2) give_registers<kIssueRegs>();
         if (lane == 0) {
             constexpr uint32_t shape = 1u << 4 | (kTile >> 4) << 24;   // 32-bit sums of 16-bit floats
             constexpr uint32_t shape_s = shape | (kTile >> 3) << 17, shape_o = shape | (D >> 3) << 17;
@@ -447,35 +459,64 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, NT == 1 && D <= 64 
             // the last commit has arrived before the CTA ends
             if (most && alive) bar_wait(shared_address(&st.v_free[(most - 1) & 1]), (most - 1) / 2 & 1);
         }
-    } else {
-        // -------------------------------------------------------- page lists
-        for (int j = 0; j < most; ++j) {
+    } else if (warp == Sh::kList) {
+        // ----------------------------------------------- page lists and codes
+        if constexpr (NT == 2) give_registers<kIssueRegs>();
+        const int end = min(begin + chunk, s.kept);
+        const bool on = lane < kPages;
+        // step j's page: -1 past the end, -2 if it is not in the cache
+        auto page = [&](int j) {
+            const int first = begin + j * kTile + lane * P;
+            if (!on || first >= end) return -1;
+            const int no = p.r.table[(long long)b * p.r.width + first / P];
+            return no >= 0 && no < p.c.pages ? no : -2;
+        };
+        auto scale = [&](const float* of, int no) {                    // one that is not in the cache, or is infinite: not a number
+            const float x = no >= 0 ? of[(long long)no * p.c.heads + h] : 0.0f;
+            return no == -2 || x == inf_f() ? nan_f() : x;
+        };
+        constexpr uint32_t kBlock = P * D;
+        auto copy = [&](int side, int j, int no) {
+            const uint32_t bar = shared_address(&st.raw_full[side]);
+            if (!bar_wait_all(shared_address(&st.raw_free[side]), (j & 1) ^ 1)) return false;
+            const int n = __popc(__ballot_sync(0xffffffffu, no != -1));
+            if (lane == 0) bar_expect(bar, n * kBlock);
+            __syncwarp();
+            if (no != -1)
+                bulk_load(shared_address(raw + side * Sh::kRaw) + lane * kBlock,
+                          (side ? p.c.v : p.c.k) + ((long long)max(no, 0) * p.c.heads + h) * kBlock, kBlock, bar);
+            return true;
+        };
+        int no = most ? page(0) : -1, next = most > 1 ? page(1) : -1;
+        float ks = scale(p.c.k_scale, no), vs = scale(p.c.v_scale, no);
+        int j = 0;
+        for (; j < most; ++j) {
             const int slot = j % kAhead;
             alive = bar_wait_all(shared_address(&st.list_free[slot]), (j / kAhead & 1) ^ 1);
             if (!alive) break;
-            float vs = 0.0f;
-            if (lane < kPages) {
-                const int first = begin + j * kTile + lane * P;
-                int no = -1;
-                float ks = 0.0f;
-                if (first < min(begin + chunk, s.kept)) {
-                    no = p.r.table[(long long)b * p.r.width + first / P];
-                    const bool known = no >= 0 && no < p.c.pages;      // else page 0 under scales that are not numbers
-                    if (!known) no = 0;
-                    ks = known ? p.c.k_scale[(long long)no * p.c.heads + h] : nan_f();
-                    vs = known ? p.c.v_scale[(long long)no * p.c.heads + h] : nan_f();
-                }
-                st.page[slot][lane] = no;
+            float m = vs > 0.0f ? log2f(vs) : vs == 0.0f || no == -1 ? -inf_f() : nan_f();
+            if (on) {
                 st.k_scale[slot][lane] = ks;
-                st.v_scale[slot][lane] = vs;
+                st.v_log[slot][lane] = m;
             }
-            float m = fmaxf(vs, 0.0f);
+            m = m == m && on ? m : -inf_f();
 #pragma unroll
             for (int d = 1; d < kPages; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
             if (lane == 0) st.v_most[slot] = m;
             __syncwarp();
             if (lane == 0) bar_arrive(shared_address(&st.list_full[slot]));
+            const int now = no;
+            no = next;
+            ks = scale(p.c.k_scale, no);
+            vs = scale(p.c.v_scale, no);
+            next = j + 2 < most ? page(j + 2) : -1;
+            if (!(alive = copy(0, j, now) && copy(1, j, now))) break;
         }
+        if (!alive)                                                    // what is in flight gets as long again to land
+            for (int side = 0; side < 2; ++side)
+                for (int ph = 0; ph < 2; ++ph) bar_wait(shared_address(&st.raw_full[side]), ph);
+    } else {
+        if constexpr (NT == 2) give_registers<kIssueRegs>();
     }
     // the products are done: every tile's last commit has been waited for
     tmem_fence_before();
@@ -490,8 +531,17 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, NT == 1 && D <= 64 
 template <int D, int NT, int P>
 cudaError_t tiles_launch(const AttendParams& p, const Chunks& c, cudaStream_t s) {
     using Sh = Shape<D, NT, P>;
-    const cudaError_t e = allow_shared<k_attend_tiles<D, NT, P>>(Sh::kBytes);
+    cudaError_t e = allow_shared<k_attend_tiles<D, NT, P>>(Sh::kBytes);
     if (e != cudaSuccess) return e;
+    if constexpr (NT == 2) {
+        // the groups share out exactly what the block is launched with; with
+        // less they would wait for ever
+        static const int regs = [] {
+            cudaFuncAttributes a{};
+            return cudaFuncGetAttributes(&a, k_attend_tiles<D, NT, P>) == cudaSuccess ? a.numRegs : 0;
+        }();
+        if (regs < kRegs) return cudaErrorInvalidKernelImage;
+    }
     const long long rows = (long long)p.r.most * (p.heads / p.c.heads), x = (rows + NT * kTile - 1) / (NT * kTile) * c.count;
     if (x > 0x7fffffff) return cudaErrorInvalidValue;
     k_attend_tiles<D, NT, P><<<dim3((unsigned)x, p.c.heads, p.r.seqs), Sh::kThreads, Sh::kBytes, s>>>(p, c.tokens, c.count);
