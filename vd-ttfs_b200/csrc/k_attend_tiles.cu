@@ -416,49 +416,55 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
     } else if (warp == Sh::kIssue) {
         // ---------------------------------------------------------- products
         if constexpr (NT == 2) give_registers<kIssueRegs>();
-        if (lane == 0) {
-            constexpr uint32_t shape = 1u << 4 | (kTile >> 4) << 24;   // 32-bit sums of 16-bit floats
-            constexpr uint32_t shape_s = shape | (kTile >> 3) << 17, shape_o = shape | (D >> 3) << 17;
-            const uint32_t q_at = shared_address(smem), k_at = shared_address(kt), v_at = shared_address(vt);
-            auto scores = [&](int t, int slot) {
+        constexpr uint32_t shape = 1u << 4 | (kTile >> 4) << 24;       // 32-bit sums of 16-bit floats
+        constexpr uint32_t shape_s = shape | (kTile >> 3) << 17, shape_o = shape | (D >> 3) << 17;
+        const uint32_t at = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t q_at = tile_desc(shared_address(smem)), k_at = tile_desc(shared_address(kt)), v_at = tile_desc(shared_address(vt));
+        const bool one = elected();
+        auto scores = [&](int t, int slot) {
+            if (one) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_shared(tmem + t * kTile, tile_desc(q_at + t * Sh::kQ + k / 4 * (kTile * 128)) + k % 4 * 2,
-                               tile_desc(k_at + slot * Sh::kK + k / 4 * (kTile * 128)) + k % 4 * 2, shape_s, k > 0);
+                    mma_shared(at + t * kTile, q_at + (t * Sh::kQ + k / 4 * (kTile * 128) + k % 4 * 32) / 16,
+                               k_at + (slot * Sh::kK + k / 4 * (kTile * 128) + k % 4 * 32) / 16, shape_s, k > 0);
                 mma_commit(shared_address(&st.s_full[t]));
-            };
-            auto outputs = [&](int t, int slot, bool add) {
+            }
+        };
+        auto outputs = [&](int t, int slot, bool add) {
+            if (one) {
 #pragma unroll
                 for (int k = 0; k < kTile / 16; ++k)
-                    mma_tensor(tmem_o + t * D, tmem + t * kTile + k * 8, tile_desc(v_at + slot * Sh::kV + k / 4 * (D * 128)) + k % 4 * 2,
+                    mma_tensor(at + NT * kTile + t * D, at + t * kTile + k * 8, v_at + (slot * Sh::kV + k / 4 * (D * 128) + k % 4 * 32) / 16,
                                shape_o, add || k > 0);
                 mma_commit(shared_address(&st.o_done[t]));
-            };
-            if (most && (alive = bar_wait(shared_address(&st.k_full[0]), 0))) {
-                tmem_fence_after();
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    if (steps[t]) scores(t, 0);
-                mma_commit(shared_address(&st.k_free[0]));
             }
-            for (int j = 0; j < most && alive; ++j) {
-                const int slot = j & 1, next = slot ^ 1;
-                if (!(alive = bar_wait(shared_address(&st.v_full[slot]), j / 2 & 1))) break;
-                if (j + 1 < most && !(alive = bar_wait(shared_address(&st.k_full[next]), (j + 1) / 2 & 1))) break;
+        };
+        if (most && (alive = bar_wait_all(shared_address(&st.k_full[0]), 0))) {
+            tmem_fence_after();
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    if (j >= steps[t]) continue;
-                    if (!(alive = bar_wait(shared_address(&st.p_full[t]), j & 1))) break;
-                    tmem_fence_after();
-                    outputs(t, slot, j > 0);
-                    if (j + 1 < steps[t]) scores(t, next);             // behind the product that reads P in S's place
-                }
+            for (int t = 0; t < NT; ++t)
+                if (steps[t]) scores(t, 0);
+            if (one) mma_commit(shared_address(&st.k_free[0]));
+        }
+        for (int j = 0; j < most && alive; ++j) {
+            const int slot = j & 1, next = slot ^ 1;
+            if (!(alive = bar_wait_all(shared_address(&st.v_full[slot]), j / 2 & 1))) break;
+            if (j + 1 < most && !(alive = bar_wait_all(shared_address(&st.k_full[next]), (j + 1) / 2 & 1))) break;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if (j >= steps[t] || !alive) continue;
+                if (!(alive = bar_wait_all(shared_address(&st.p_full[t]), j & 1))) continue;
+                tmem_fence_after();
+                outputs(t, slot, j > 0);
+                if (j + 1 < steps[t]) scores(t, next);                 // behind the product that reads P in S's place
+            }
+            if (one) {
                 mma_commit(shared_address(&st.v_free[slot]));
                 if (j + 1 < most) mma_commit(shared_address(&st.k_free[next]));
             }
-            // the last commit has arrived before the CTA ends
-            if (most && alive) bar_wait(shared_address(&st.v_free[(most - 1) & 1]), (most - 1) / 2 & 1);
         }
+        // the last commit has arrived before the CTA ends
+        if (most && alive) bar_wait_all(shared_address(&st.v_free[(most - 1) & 1]), (most - 1) / 2 & 1);
     } else if (warp == Sh::kList) {
         // ----------------------------------------------- page lists and codes
         if constexpr (NT == 2) give_registers<kIssueRegs>();

@@ -242,28 +242,30 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_int8_tiles(const __grid_con
                 bar_wait(shared_address(&bars.full[i % Shape::kStages]), i / Shape::kStages & 1);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // 32-bit sums, signed 8-bit operands, both with the inner dimension consecutive
-            constexpr uint32_t shape = 2u << 4 | 1u << 7 | 1u << 10 | (BN >> 3) << 17 | (kTileRows >> 4) << 24;
-            int n = 0, i = 0;
-            bool alive = true;
-            for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x, ++i) {
-                const int half = i & 1;
-                if (!(alive = bar_wait(shared_address(&bars.taken[half]), (i / 2 & 1) ^ 1))) break;
+        // 32-bit sums, signed 8-bit operands, both with the inner dimension consecutive
+        constexpr uint32_t shape = 2u << 4 | 1u << 7 | 1u << 10 | (BN >> 3) << 17 | (kTileRows >> 4) << 24;
+        const uint32_t sums = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t a = tile_desc(stages), w = tile_desc(stages + kTileRows * kStageBytes);
+        const bool one = elected();
+        int n = 0, i = 0;
+        bool alive = true;
+        for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x, ++i) {
+            const int half = i & 1;
+            if (!(alive = bar_wait_all(shared_address(&bars.taken[half]), (i / 2 & 1) ^ 1))) break;
+            tmem_fence_after();
+            for (int s = 0; s < steps; ++s, ++n) {
+                const int slot = n % Shape::kStages;
+                if (!(alive = bar_wait_all(shared_address(&bars.full[slot]), n / Shape::kStages & 1))) break;
                 tmem_fence_after();
-                for (int s = 0; s < steps; ++s, ++n) {
-                    const int slot = n % Shape::kStages;
-                    if (!(alive = bar_wait(shared_address(&bars.full[slot]), n / Shape::kStages & 1))) break;
-                    tmem_fence_after();
-                    const uint32_t at = stages + slot * Shape::kStage;
-                    const uint64_t a = tile_desc(at), w = tile_desc(at + kTileRows * kStageBytes);
+                if (one) {
 #pragma unroll
                     for (int k = 0; k < kStageBytes / 32; ++k)
-                        mma_i8(tmem + half * BN, a + 2 * k, w + 2 * k, shape, s > 0 || k > 0);
+                        mma_i8(sums + half * BN, a + (slot * Shape::kStage + k * 32) / 16, w + (slot * Shape::kStage + k * 32) / 16, shape,
+                               s > 0 || k > 0);
                     mma_commit(shared_address(&bars.empty[slot]));
                 }
-                if (alive) mma_commit(shared_address(&bars.done[half]));
             }
+            if (alive && one) mma_commit(shared_address(&bars.done[half]));
         }
     } else {
         const int quarter = warp % 4, thread = threadIdx.x - 64;     // a warp reads the rows of its quarter

@@ -215,6 +215,14 @@ __device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {
 }
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// True in one lane of the warp.  The products are issued under it, in loops
+// that the whole warp runs: their operands then stay in uniform registers
+// (issued under `lane == 0`, a product took some 190 cycles to issue).
+__device__ __forceinline__ bool elected() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
 // arrives on the barrier once every product issued by this thread is done
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
