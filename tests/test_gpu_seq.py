@@ -533,10 +533,10 @@ def test_attention_broken_pages_reach_only_those_who_see_them(S, new):
     q = normal(1, new, heads, dim, kind=torch.bfloat16).cuda()
     args = (ints(table), ints([kept]), ints([0, new]), new, kept)
     good = S.cache_attention(q, cache, *args)
-    for broken in range(2):
+    for broken, value in ((0, math.nan), (1, math.nan), (0, INF), (1, INF)):
         last = table[0][-1]
         c = S.Cache8(*(t.clone() for t in cache))
-        c[2 + broken][last] = math.nan
+        c[2 + broken][last] = value
         got = S.cache_attention(q, c, *args)
         blind = max(0, new - page)
         assert torch.equal(got[:blind], good[:blind])

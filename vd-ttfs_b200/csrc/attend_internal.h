@@ -59,10 +59,35 @@ __device__ __forceinline__ void store_value(void* p, long long i, int type, floa
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
 }
 
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Where the tokens are divided, a row and head's chunk leaves its maximum and
+// sum and its unscaled output: first all rows' and chunks' pairs, then (on 16
+// bytes) all outputs.
+struct Partial {
+    float2* stats;
+    float* sums;
+};
+__host__ __device__ inline long long partial_pairs(long long rows, int count) { return (rows * count + 1) / 2 * 4; }
+__host__ __device__ inline long long partial_floats(long long rows, int count, int dim) {
+    return partial_pairs(rows, count) + rows * count * dim;
+}
+__device__ __forceinline__ Partial partial_of(const AttendParams& p, long long row, int count, int chunk) {
+    const long long i = row * count + chunk;
+    return {reinterpret_cast<float2*>(p.scratch) + i, p.scratch + partial_pairs(p.r.total * p.heads, count) + i * p.c.dim};
+}
+
+// By how much (powers of two) a weight may pass 1, and a page's value scale what
+// the sums are relative to, before both are taken anew
+constexpr float kSlack = 8.0f, kValueSlack = 4.0f;
+
 // many query rows: one CTA for up to 256 rows (k_attend_tiles.cu)
-bool attend_tiles_dim(int dim);
-Chunks plan_tiles(int heads, int kv_heads, int seqs, int most, int most_kept);
-int tile_rows(long long rows);          // rows of a CTA
+Chunks plan_tiles(int dim, int heads, int kv_heads, int seqs, int most, int most_kept);
+int tile_rows(int dim, long long rows);          // rows of a CTA
 cudaError_t launch_attend_tiles(const AttendParams& p, const Chunks& c, cudaStream_t s);
 
 }  // namespace vdt

@@ -10,10 +10,15 @@
 // The queries' rounding: q is scaled by a power of two for each row so that
 // its largest magnitude is in [1, 2); a 16-bit float then holds every bf16 or
 // f16 value whole down to 2^-14 of that (below, to 2^-24 of it).  The weights
-// exp(s - max) are in [0, 1]; vs is a page's, so it goes into them relative to
-// the largest vs so far, and into the sums' rescaling when that grows.  Their
-// rounding to 16 bits is at most 2^-11: that of an f16 output, an eighth of a
-// bf16 one's, and it averages over the tokens.
+// exp(s - max) take their page's vs with them, relative to the largest vs so
+// far: exp2(s - m + log2(vs) - log2(vs_max)), and the sum of a page's weights
+// takes it out again.  Their rounding to 16 bits is at most 2^-11: that of an
+// f16 output, an eighth of a bf16 one's, and it averages over the tokens.
+//
+// m is not the running maximum itself: it moves only when a score passes it by
+// more than 2^8 (as a factor), and vs_max when a scale passes it by more than
+// 2^4; 16-bit floats have room for that, and the sums are rescaled a few times
+// instead of at every step.
 #include "attend_internal.h"
 
 namespace vdt {
@@ -22,23 +27,39 @@ namespace {
 constexpr int kUnit = 64;          // tokens that a warp takes at a time
 
 // ------------------------------------------------------------ few query rows
-// One CTA: a sequence, a head of the cache, 16 of the rows (query, head of
-// the group) that share it, and a chunk of the tokens.  Its warps take units
-// of 64 tokens in turn; each warp has its own ring of shared memory, into
+// One CTA: a sequence, a head of the cache, up to 8 x NR of the rows (query,
+// head of the group) that share it, and a chunk of the tokens.  Its warps take
+// units of 64 tokens in turn; each warp has its own ring of shared memory, into
 // which the units' codes are copied in bulk (a page's codes of one head are
 // consecutive).  The warps' sums are joined in shared memory, the chunks' by
 // k_attend_join.
+//
+// Tokens are the rows of the first product (S^T = K Q^T) and values' dimensions
+// those of the second (O^T = V^T P^T), the queries the columns, eight at a time:
+// the codes, turned into 16-bit floats once, serve all the queries, and one
+// query costs half of what 16 would.  A lane ends up with tokens that lie side
+// by side in a value row: row m of 16 is token (m % 8 / 2) (P / 4) + 4 j + (m /
+// 8) 2 + m % 2 of its page, j counting the page's groups of 16.
 constexpr int kRowsWarps = 4;
-constexpr int kRing = 3;           // entries of a warp's ring; a unit's keys are one, its values one
+constexpr int kRing = 2;           // entries of a warp's ring; a unit's keys are one, its values one
 constexpr int kMostChunk = 4096;   // tokens of a chunk: bounds the page lists in shared memory
 
-// Chunks so that the grid has a few CTAs for each SM, none under 64 tokens a
-// warp.  With one chunk the CTAs write the output themselves.
+// groups of eight rows of a CTA
+int row_groups(long long rows) { return rows <= 8 ? 1 : 2; }
+
+// Fewer tiles than the SMs have room for (three CTAs each): as many chunks as
+// fill it once (a second round of a few CTAs costs as much as the first: 100,000
+// tokens in 66 chunks of 8 heads took 63 us, in 49 50 us).  More tiles: chunks
+// of about 2048 tokens, which even out sequences of different lengths (64 of
+// 1,000 to 8,191 tokens: 121 us with 1536 or 2048, 127 with 2816).  None under
+// 64 tokens a warp.  With one chunk the CTAs write the output themselves.
+constexpr int kEvenChunk = 2048;
+
 Chunks plan_chunks(int heads, int kv_heads, int seqs, int most, int most_kept) {
-    const long long tiles = (long long)kv_heads * seqs * (((long long)most * (heads / kv_heads) + 15) / 16);
-    const long long target = 8 * kSmCount;
-    const long long want = (target + tiles - 1) / tiles;
-    long long tokens = ((long long)most_kept + want - 1) / want;
+    const long long rows = (long long)most * (heads / kv_heads), each = 8 * row_groups(rows);
+    const long long tiles = kv_heads * seqs * ((rows + each - 1) / each), slots = 3 * kSmCount;
+    const long long want = tiles < slots ? slots / tiles : ((long long)most_kept + kEvenChunk - 1) / kEvenChunk;
+    long long tokens = ((long long)most_kept + want - 1) / (want ? want : 1);
     constexpr int step = kUnit * kRowsWarps;
     tokens = (tokens + step - 1) / step * step;
     if (tokens < step) tokens = step;
@@ -52,56 +73,83 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// an 8 x 8 block of 16-bit values, a row's pair a lane, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(const unsigned char* at, uint32_t (&w)[N]) {
+    if constexpr (N == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(at);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(at);
+        w[0] = v.x; w[1] = v.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(at);
+    }
+}
 
 struct RowsLayout {
-    uint32_t ring, q, bars, pages, bytes;
+    uint32_t q, bars, pages, bytes;          // the ring is first
 };
-__host__ __device__ inline RowsLayout rows_layout(int dim, int chunk, int page) {
+__host__ __device__ inline RowsLayout rows_layout(int dim, int groups, int chunk, int page) {
     RowsLayout l;
     const uint32_t ring = (uint32_t)(kRowsWarps * kRing * kUnit * dim);
-    const uint32_t sums = (uint32_t)(kRowsWarps * 16 * (dim + 2) * 4);     // reuses the ring
-    l.ring = 0;
+    const uint32_t sums = (uint32_t)(kRowsWarps * 8 * groups * (dim + 2) * 4);     // reuses the ring
     l.q = ring > sums ? ring : sums;
-    l.bars = l.q + dim * 32 + 64;
+    l.bars = l.q + dim * 16 * groups + 32 * groups;
     l.pages = l.bars + kRowsWarps * kRing * 8;
     l.bytes = l.pages + chunk / page * 12;
     return l;
 }
 
-template <int D, int P>
+template <int D, int P, int NR>
 __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p, int chunk) {
     extern __shared__ __align__(128) unsigned char smem[];
+    chain_release();
     constexpr int kGroups = P / 16;              // 16-token groups of a page
     constexpr int kPages = kUnit / P;            // pages of a unit
-    const RowsLayout lay = rows_layout(D, chunk, P);
+    constexpr int kRows = 8 * NR;
+    constexpr int kPart = kUnit / 16;            // 16-token groups of a unit
+    const RowsLayout lay = rows_layout(D, NR, chunk, P);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const int b = blockIdx.z, group = p.heads / p.c.heads;
     const int tile = blockIdx.y / p.c.heads, h = blockIdx.y % p.c.heads;
     const Queries s = queries_of(p, b);
-    const int rows = s.rows * group - tile * 16;              // rows of this tile
+    const int rows = s.rows * group - tile * kRows;           // rows of this tile
     if (rows <= 0) return;
     const bool split = gridDim.x > 1;
     // tokens that a row sees: all, or up to its own place at the sequence's end
     auto sees = [&](int r) {
         if (r >= rows || s.kept < 0) return 0;
-        return p.causal ? max(0, s.kept - s.rows + (tile * 16 + r) / group + 1) : s.kept;
+        return p.causal ? max(0, s.kept - s.rows + (tile * kRows + r) / group + 1) : s.kept;
     };
-    const int lim0 = sees(g), lim1 = sees(g + 8);
-    const int begin = blockIdx.x * chunk, end = min(begin + chunk, sees(min(rows, 16) - 1));
+    const int begin = blockIdx.x * chunk, end = min(begin + chunk, sees(min(rows, kRows) - 1));
     if (begin >= end && split) return;                        // the join knows as well
     const int units = max(0, (end - begin + kUnit - 1) / kUnit);
+    int limit[NR][2], least = 0x7fffffff;                     // of the lane's columns; of all rows there are
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) limit[n][i] = sees(8 * n + 2 * t + i);
+    least = sees(0);
 
-    float* q_scale = reinterpret_cast<float*>(smem + lay.q + D * 32);
-    uint4* q_frag = reinterpret_cast<uint4*>(smem + lay.q);
+    float* q_scale = reinterpret_cast<float*>(smem + lay.q + D * 16 * NR);
+    uint2* q_frag = reinterpret_cast<uint2*>(smem + lay.q);
     int* pages = reinterpret_cast<int*>(smem + lay.pages);
     float* k_scale = reinterpret_cast<float*>(pages + chunk / P);
-    float* v_scale = k_scale + chunk / P;
+    float* v_log = k_scale + chunk / P;
     const uint32_t bars = shared_address(smem + lay.bars) + warp * kRing * 8;
-    const uint32_t ring = shared_address(smem + lay.ring) + warp * kRing * kUnit * D;
+    const uint32_t ring = shared_address(smem) + warp * kRing * kUnit * D;
 
     if (lane < kRing) bar_init(bars + lane * 8, 1);
-    // the chunk's pages: number and scales; one that is not in the cache is
-    // read as page 0 under NaN scales, one past the end is not read at all
+    // the chunk's pages: number, scale, logarithm of the values' scale; one
+    // that is not in the cache is read as page 0 under scales that are not
+    // numbers, one past the end is not read at all
     for (int i = threadIdx.x; i < units * kPages; i += kRowsWarps * 32) {
         const int j = begin / P + i;
         int no = -1;
@@ -116,13 +164,13 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
         }
         pages[i] = no;
         k_scale[i] = ks;
-        v_scale[i] = vs;
+        v_log[i] = vs > 0.0f ? log2f(vs) : vs == 0.0f ? -inf_f() : nan_f();
     }
     // the queries, each row scaled by a power of two
-    for (int r = warp; r < 16; r += kRowsWarps) {
+    for (int r = warp; r < kRows; r += kRowsWarps) {
         float x[D / 32], m = 0.0f;
         const bool in = r < rows;
-        const int row = tile * 16 + r;
+        const int row = tile * kRows + r;
         const long long q = (s.first + row / group) * p.q_token + (long long)(h * group + row % group) * p.q_head;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -132,8 +180,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
 #pragma unroll
         for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
         const int e = m > 0.0f && m < inf_f() ? max(-126, min(126, ilogbf(m))) : 0;
-        if (lane == 0) q_scale[r] = scalbnf(1.0f, e);
-        const float f = scalbnf(1.0f, -e);
+        if (lane == 0) q_scale[r] = scalbnf(fabsf(p.scale), e);
+        const float f = copysignf(scalbnf(1.0f, -e), p.scale);        // a negative scale goes into the queries
         // value d of row r sits where the lane that multiplies it looks
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -141,8 +189,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
             const bool wide = d < D / 64 * 64;               // 64-wide blocks, then one of 32
             const int in64 = wide ? d % 64 : d % 32, tt = wide ? in64 / 16 : in64 / 8, byte = wide ? in64 % 16 : in64 % 8;
             const int step = (wide ? d / 64 * 4 : D / 64 * 4) + byte / 4;
-            const int reg = (byte % 4) / 2 * 2 + r / 8;
-            __half* at = reinterpret_cast<__half*>(q_frag + step * 32 + (r % 8) * 4 + tt) + reg * 2 + byte % 2;
+            __half* at = reinterpret_cast<__half*>(q_frag + (step * NR + r / 8) * 32 + (r % 8) * 4 + tt) + byte % 4;
             *at = __float2half_rn(x[i] * f);
         }
     }
@@ -166,137 +213,172 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
     if (lane == 0)
         for (int e = 0; e < kRing; ++e) fetch(e);
 
-    const float f0 = q_scale[g] * p.scale, f1 = q_scale[g + 8] * p.scale;
-    float o[D / 8][4] = {}, m0 = -inf_f(), m1 = -inf_f(), l0 = 0.0f, l1 = 0.0f, vref = 0.0f;
+    float f[NR][2], ref[NR][2], sum[NR][2], vref = -inf_f();     // the lane's columns: factor, what the weights are relative to, their sum
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f[n][i] = q_scale[8 * n + 2 * t + i];
+            ref[n][i] = -inf_f();
+            sum[n][i] = 0.0f;
+        }
+    float o[D / 16][NR][4] = {};
     bool alive = true;
     for (int i = 0, u = warp; u < units; ++i, u += kRowsWarps) {
-        // scores of 64 tokens: tile n's column c is token (c / 2) * (P / 4) +
-        // 4 * group + 2 * half + c % 2 of its page, so that a lane ends up
-        // with tokens that lie side by side in a value row
-        float sc[kUnit / 8][4] = {};
-        const int ek = 2 * i, ev = 2 * i + 1;
+        const int ek = 2 * i, ev = 2 * i + 1, base = begin + u * kUnit;
+        const bool partial = base + kUnit > least;
+        const unsigned char* kt = smem + (warp * kRing + ek % kRing) * (kUnit * D);
+        const unsigned char* vt = smem + (warp * kRing + ev % kRing) * (kUnit * D);
+        // pages' value scales that pass what the sums are relative to
+        float v_most = -inf_f();
+#pragma unroll
+        for (int pg = 0; pg < kPages; ++pg) v_most = fmaxf(v_most, v_log[u * kPages + pg]);
+        if (v_most > vref + kValueSlack || (vref == -inf_f() && v_most > vref)) {
+            const float by = exp2f(vref - v_most);
+#pragma unroll
+            for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[m][n][e] *= by;
+            vref = v_most;
+        }
+        const float v_shift = vref == -inf_f() ? 0.0f : vref;
         alive = bar_wait_all(bars + (ek % kRing) * 8, (ek / kRing) & 1);
         if (!alive) break;
-        const unsigned char* kt = smem + lay.ring + (warp * kRing + ek % kRing) * (kUnit * D);
+        {
+            float sc[kPart][NR][4] = {};
 #pragma unroll
-        for (int c = 0; c < (D + 63) / 64; ++c) {
-            constexpr int kWide = D / 64;
-            const bool wide = c < kWide;
-            uint32_t a[4][4];
+            for (int c = 0; c < (D + 63) / 64; ++c) {
+                constexpr int kWide = D / 64;
+                const bool wide = c < kWide;
+                uint32_t x[kPart][4], y[kPart][4];           // of tokens m and m + 8 of 16
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (wide || j < 2) {
-                    const uint4 v = q_frag[(c * 4 + j) * 32 + lane];
-                    a[j][0] = v.x; a[j][1] = v.y; a[j][2] = v.z; a[j][3] = v.w;
+                for (int m = 0; m < kPart; ++m) {
+                    const int pg = m / kGroups, j16 = m % kGroups;
+                    const unsigned char* at = kt + (pg * P + (g / 2) * (P / 4) + 4 * j16 + g % 2) * D + c * 64 + t * (wide ? 16 : 8);
+                    if (wide) {
+                        const uint4 a = *reinterpret_cast<const uint4*>(at), d = *reinterpret_cast<const uint4*>(at + 2 * D);
+                        x[m][0] = a.x; x[m][1] = a.y; x[m][2] = a.z; x[m][3] = a.w;
+                        y[m][0] = d.x; y[m][1] = d.y; y[m][2] = d.z; y[m][3] = d.w;
+                    } else {
+                        const uint2 a = *reinterpret_cast<const uint2*>(at), d = *reinterpret_cast<const uint2*>(at + 2 * D);
+                        x[m][0] = a.x; x[m][1] = a.y;
+                        y[m][0] = d.x; y[m][1] = d.y;
+                    }
                 }
 #pragma unroll
-            for (int n = 0; n < kUnit / 8; ++n) {
-                const int pg = n / (2 * kGroups), j16 = n / 2 % kGroups, hf = n % 2;
-                const int token = pg * P + (g / 2) * (P / 4) + 4 * j16 + 2 * hf + g % 2;
-                const unsigned char* at = kt + token * D + c * 64 + t * (wide ? 16 : 8);
-                uint32_t w[4], lo, hi;
-                if (wide) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(at);
-                    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-                } else {
-                    const uint2 v = *reinterpret_cast<const uint2*>(at);
-                    w[0] = v.x; w[1] = v.y; w[2] = w[3] = 0;
-                }
+                for (int w = 0; w < 4; ++w) {
+                    if (!wide && w >= 2) continue;
+                    uint2 q[NR];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (wide || j < 2) {
-                        codes_to_f16(w[j], lo, hi);
-                        mma_f16(sc[n], a[j], lo, hi);
+                    for (int n = 0; n < NR; ++n) q[n] = q_frag[((c * 4 + w) * NR + n) * 32 + lane];
+#pragma unroll
+                    for (int m = 0; m < kPart; ++m) {
+                        uint32_t a[4];
+                        codes_to_f16(x[m][w], a[0], a[2]);
+                        codes_to_f16(y[m][w], a[1], a[3]);
+#pragma unroll
+                        for (int n = 0; n < NR; ++n) mma_f16(sc[m][n], a, q[n].x, q[n].y);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) fetch(ek + kRing);
+            // scores, in powers of two; the lane's tokens are base + page + t' (P / 4) + ... of rows g and g + 8
+            bool over = false;
+            float top[NR][2];
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) top[n][e] = -inf_f();
+#pragma unroll
+            for (int m = 0; m < kPart; ++m) {
+                const int pg = m / kGroups, j16 = m % kGroups;
+                const float ks = k_scale[u * kPages + pg];
+                const int token = base + pg * P + (g / 2) * (P / 4) + 4 * j16 + g % 2;
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float v = sc[m][n][e] * (f[n][e % 2] * ks);
+                        if (partial) v = token + e / 2 * 2 < limit[n][e % 2] ? v : -inf_f();
+                        sc[m][n][e] = v;
+                        top[n][e % 2] = fmaxf(top[n][e % 2], v);
                     }
             }
-        }
-        __syncwarp();
-        if (lane == 0) fetch(ek + kRing);
-        // softmax: a lane has columns 2t and 2t + 1 of rows g and g + 8
-        const int base = begin + u * kUnit;
-        float vnew = vref;
 #pragma unroll
-        for (int pg = 0; pg < kPages; ++pg) vnew = fmaxf(vnew, v_scale[u * kPages + pg]);
-        float t0 = m0, t1 = m1;
-        const bool partial = base + kUnit > min(lim0, lim1);
+            for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int n = 0; n < kUnit / 8; ++n) {
-            const int pg = n / (2 * kGroups), j16 = n / 2 % kGroups, hf = n % 2;
-            const float ks = k_scale[u * kPages + pg];
-            const int token = base + pg * P + t * (P / 4) + 4 * j16 + 2 * hf;
-            sc[n][0] *= f0 * ks;
-            sc[n][1] *= f0 * ks;
-            sc[n][2] *= f1 * ks;
-            sc[n][3] *= f1 * ks;
-            if (partial) {
-                if (token >= lim0) sc[n][0] = -inf_f();
-                if (token + 1 >= lim0) sc[n][1] = -inf_f();
-                if (token >= lim1) sc[n][2] = -inf_f();
-                if (token + 1 >= lim1) sc[n][3] = -inf_f();
+                for (int e = 0; e < 2; ++e) over = over || top[n][e] > ref[n][e] + kSlack || (ref[n][e] == -inf_f() && top[n][e] > ref[n][e]);
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = top[n][e];
+#pragma unroll
+                        for (int d = 4; d <= 16; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                        const float old = ref[n][e], to = fmaxf(x, old), by = to == -inf_f() ? 1.0f : exp2f(old - to);
+                        ref[n][e] = to;
+                        sum[n][e] *= by;
+#pragma unroll
+                        for (int m = 0; m < D / 16; ++m) {
+                            o[m][n][e] *= by;
+                            o[m][n][e + 2] *= by;
+                        }
+                    }
             }
-            t0 = fmaxf(t0, fmaxf(sc[n][0], sc[n][1]));
-            t1 = fmaxf(t1, fmaxf(sc[n][2], sc[n][3]));
-        }
+            alive = bar_wait_all(bars + (ev % kRing) * 8, (ev / kRing) & 1);
+            if (!alive) break;
+            uint32_t w[kPart][NR][2];
 #pragma unroll
-        for (int d = 1; d <= 2; d <<= 1) {
-            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, d));
-            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, d));
-        }
-        const float r0 = t0 == -inf_f() ? 0.0f : t0, r1 = t1 == -inf_f() ? 0.0f : t1;   // nothing seen yet
-        const float e0 = exp2f(m0 - r0), e1 = exp2f(m1 - r1);
-        const float grow = vnew > 0.0f ? vref / vnew : 1.0f;
-        m0 = t0;
-        m1 = t1;
-        l0 *= e0;
-        l1 *= e1;
+            for (int m = 0; m < kPart; ++m) {
+                const int pg = m / kGroups, j16 = m % kGroups;
+                const int token = base + pg * P + (g / 2) * (P / 4) + 4 * j16 + g % 2;
+                // the page's scale, over what the sums are relative to; not
+                // under 2^-100: a page of zeros still has weights
+                float d = v_log[u * kPages + pg] - v_shift;
+                d = d < -100.0f ? -100.0f : d;
+                const float back = exp2_fast(-d);
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-            o[n][0] *= e0 * grow;
-            o[n][1] *= e0 * grow;
-            o[n][2] *= e1 * grow;
-            o[n][3] *= e1 * grow;
-        }
-        vref = vnew;
-        uint32_t w[kUnit / 8][2];
+                for (int n = 0; n < NR; ++n) {
+                    float x[4];
 #pragma unroll
-        for (int n = 0; n < kUnit / 8; ++n) {
-            const int pg = n / (2 * kGroups);
-            const float vs = v_scale[u * kPages + pg], f = vnew > 0.0f ? vs / vnew : vs;
-            float x[4] = {exp2f(sc[n][0] - r0), exp2f(sc[n][1] - r0), exp2f(sc[n][2] - r1), exp2f(sc[n][3] - r1)};
-            l0 += x[0] + x[1];
-            l1 += x[2] + x[3];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = partial && x[j] == 0.0f ? 0.0f : x[j] * f;   // a scale that is not a number stays with those who see it
-            w[n][0] = pack_f16(x[0], x[1]);
-            w[n][1] = pack_f16(x[2], x[3]);
-        }
-        alive = bar_wait_all(bars + (ev % kRing) * 8, (ev / kRing) & 1);
-        if (!alive) break;
-        const unsigned char* vt = smem + lay.ring + (warp * kRing + ev % kRing) * (kUnit * D);
-#pragma unroll
-        for (int pg = 0; pg < kPages; ++pg)
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n) {
-                const unsigned char* at = vt + pg * P * D + (n * 8 + g) * P + t * (P / 4);
-                uint32_t c[4];
-                if constexpr (P == 64) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(at);
-                    c[0] = v.x; c[1] = v.y; c[2] = v.z; c[3] = v.w;
-                } else if constexpr (P == 32) {
-                    const uint2 v = *reinterpret_cast<const uint2*>(at);
-                    c[0] = v.x; c[1] = v.y;
-                } else {
-                    c[0] = *reinterpret_cast<const uint32_t*>(at);
-                }
-#pragma unroll
-                for (int j = 0; j < kGroups; ++j) {
-                    const int s0 = pg * 2 * kGroups + 2 * j;
-                    const uint32_t a[4] = {w[s0][0], w[s0][1], w[s0 + 1][0], w[s0 + 1][1]};
-                    uint32_t lo, hi;
-                    codes_to_f16(c[j], lo, hi);
-                    mma_f16(o[n], a, lo, hi);
+                    for (int e = 0; e < 4; ++e) {
+                        const float r = ref[n][e % 2] == -inf_f() ? 0.0f : ref[n][e % 2];
+                        x[e] = exp2_fast(sc[m][n][e] - r + d);
+                        if (partial) x[e] = token + e / 2 * 2 < limit[n][e % 2] ? x[e] : 0.0f;     // also for scales that are not numbers
+                    }
+                    const float a = x[0] + x[2], c = x[1] + x[3];
+                    sum[n][0] = partial && a == 0.0f ? sum[n][0] : fmaf(a, back, sum[n][0]);
+                    sum[n][1] = partial && c == 0.0f ? sum[n][1] : fmaf(c, back, sum[n][1]);
+                    w[m][n][0] = transposed(pack_f16(x[0], x[1]));
+                    w[m][n][1] = transposed(pack_f16(x[2], x[3]));
                 }
             }
+            // a value row's tokens of kRun groups lie side by side
+            constexpr int kRun = kGroups < kPart ? kGroups : kPart;
+#pragma unroll
+            for (int m0 = 0; m0 < kPart; m0 += kRun) {
+                const int pg = m0 / kGroups, j16 = m0 % kGroups;
+                const unsigned char* at = vt + pg * P * D + g * P + t * (P / 4) + 4 * j16;
+#pragma unroll
+                for (int q = 0; q < D / 16; ++q) {
+                    uint32_t x[kRun], y[kRun];               // of dimensions m and m + 8 of 16
+                    load_words<kRun>(at + q * 16 * P, x);
+                    load_words<kRun>(at + (q * 16 + 8) * P, y);
+#pragma unroll
+                    for (int m = 0; m < kRun; ++m) {
+                        uint32_t a[4];
+                        codes_to_f16(x[m], a[0], a[2]);
+                        codes_to_f16(y[m], a[1], a[3]);
+#pragma unroll
+                        for (int n = 0; n < NR; ++n) mma_f16(o[q][n], a, w[m0 + m][n][0], w[m0 + m][n][1]);
+                    }
+                }
+            }
+        }
         __syncwarp();
         if (lane == 0) fetch(ev + kRing);
     }
@@ -307,116 +389,228 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
     // join the warps (every copy that was begun has been waited for)
     const bool dead = __syncthreads_or(!alive);
     float* sums = reinterpret_cast<float*>(smem);            // [warp][row][D], then [warp][row][2]
-    float* tops = sums + kRowsWarps * 16 * D;
+    float* tops = sums + kRowsWarps * kRows * D;
+    const float v_scale = exp2f(vref);
 #pragma unroll
-    for (int d = 1; d <= 2; d <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
-    }
-    if (!dead) {
-        float* to = sums + (warp * 16 + g) * D + 2 * t;
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-            to[n * 8] = o[n][0] * vref;
-            to[n * 8 + 1] = o[n][1] * vref;
-            to[n * 8 + 8 * D] = o[n][2] * vref;
-            to[n * 8 + 8 * D + 1] = o[n][3] * vref;
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int d = 4; d <= 16; d <<= 1) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], d);
+            const int row = warp * kRows + 8 * n + 2 * t + e;
+            if (!dead) {
+#pragma unroll
+                for (int m = 0; m < D / 16; ++m) {
+                    sums[row * D + m * 16 + g] = o[m][n][e] * v_scale;
+                    sums[row * D + m * 16 + g + 8] = o[m][n][e + 2] * v_scale;
+                }
+                if (g == 0) {
+                    tops[row * 2] = ref[n][e];
+                    tops[row * 2 + 1] = sum[n][e];
+                }
+            }
         }
-        if (t == 0) {
-            tops[(warp * 16 + g) * 2] = m0;
-            tops[(warp * 16 + g) * 2 + 1] = l0;
-            tops[(warp * 16 + g + 8) * 2] = m1;
-            tops[(warp * 16 + g + 8) * 2 + 1] = l1;
-        }
-    }
     __syncthreads();
-    for (int i = threadIdx.x; i < min(rows, 16) * D; i += kRowsWarps * 32) {
-        const int r = i / D, d = i % D, row = tile * 16 + r;
+    for (int i = threadIdx.x; i < min(rows, kRows) * D; i += kRowsWarps * 32) {
+        const int r = i / D, d = i % D, row = tile * kRows + r;
         float top = -inf_f(), sum = 0.0f, l = 0.0f;
         if (dead || s.kept < 0) {
             sum = l = nan_f();
         } else {
 #pragma unroll
-            for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, tops[(w * 16 + r) * 2]);
-            const float ref = top == -inf_f() ? 0.0f : top;
+            for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, tops[(w * kRows + r) * 2]);
+            const float to = top == -inf_f() ? 0.0f : top;
 #pragma unroll
             for (int w = 0; w < kRowsWarps; ++w) {
-                const float e = exp2f(tops[(w * 16 + r) * 2] - ref);
-                sum += e * sums[(w * 16 + r) * D + d];
-                l += e * tops[(w * 16 + r) * 2 + 1];
+                const float e = exp2f(tops[(w * kRows + r) * 2] - to);
+                sum += e * sums[(w * kRows + r) * D + d];
+                l += e * tops[(w * kRows + r) * 2 + 1];
             }
         }
         const long long token = s.first + row / group;
         const int head = h * group + row % group;
         if (split) {
-            float* to = p.scratch + ((token * p.heads + head) * gridDim.x + blockIdx.x) * (D + 2);
-            to[2 + d] = sum;
-            if (d == 0) {
-                to[0] = top;
-                to[1] = l;
-            }
+            const Partial to = partial_of(p, token * p.heads + head, gridDim.x, blockIdx.x);
+            to.sums[d] = sum;
+            if (d == 0) *to.stats = make_float2(top, l);
         } else {
             store_value(p.out, token * p.out_token + head * p.out_head + d, p.type, l == 0.0f ? 0.0f : sum / l);
         }
     }
 }
 
-// One warp for each row and head: its chunks' sums, joined.
-__global__ void __launch_bounds__(128) k_attend_join(AttendParams p, int chunk, int count, int tile) {
-    const int lane = threadIdx.x % 32, group = p.heads / p.c.heads, dim = p.c.dim;
-    const long long i = (long long)blockIdx.x * 4 + threadIdx.x / 32;
-    chain_wait();
-    if (i >= p.r.total * p.heads) return;
-    const long long token = i / p.heads;
-    const int head = (int)(i % p.heads);
-    // the row's sequence: the last whose first row is not past it
-    int lo = 0, hi = p.r.seqs - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (p.r.starts[mid] <= token) lo = mid; else hi = mid - 1;
+// A packed row and head whose chunks are to be joined
+struct JoinRow {
+    long long out;          // where its output starts
+    int chunks;             // -1: no such row; -2: more tokens than the table or most_kept allow
+};
+__device__ __forceinline__ JoinRow join_row(const AttendParams& p, long long token, int head, int chunk, int count, int tile) {
+    const int lane = threadIdx.x % 32, group = p.heads / p.c.heads;
+    // its sequence: the last whose first row is not past it (the lanes look at 32 at a time)
+    int seq = -1;
+    for (int j = 0; j < p.r.seqs; j += 32) {
+        const unsigned not_past = __ballot_sync(0xffffffffu, j + lane < p.r.seqs && p.r.starts[j + lane] <= token);
+        if (not_past) seq = j + 31 - __clz(not_past);
+        if (not_past != 0xffffffffu) break;
     }
-    const Queries s = queries_of(p, lo);
-    if (token < s.first || token >= s.first + s.rows) return;
-    const int at = (int)(token - s.first);
-    const long long out = token * p.out_token + head * p.out_head;
-    if (s.kept < 0) {
-        for (int d = lane; d < dim; d += 32) store_value(p.out, out + d, p.type, nan_f());
-        return;
-    }
+    if (seq < 0) return {0, -1};
+    const Queries s = queries_of(p, seq);
+    if (token < s.first || token >= s.first + s.rows) return {0, -1};
     // the chunks that the row's tile has: up to the tokens its last row sees
-    const int row = at * group + head % group, last = min(row / tile * tile + tile - 1, s.rows * group - 1) / group;
+    const int row = (int)(token - s.first) * group + head % group, last = min(row / tile * tile + tile - 1, s.rows * group - 1) / group;
     const int sees = p.causal ? max(0, s.kept - s.rows + last + 1) : s.kept;
-    const int n = min((sees + chunk - 1) / chunk, count);
-    const float* from = p.scratch + i * count * (dim + 2);
-    float top = -inf_f(), l = 0.0f;
-    for (int c = 0; c < n; ++c) top = fmaxf(top, from[(long long)c * (dim + 2)]);
-    const float ref = top == -inf_f() ? 0.0f : top;
-    for (int c = 0; c < n; ++c) l += exp2f(from[(long long)c * (dim + 2)] - ref) * from[(long long)c * (dim + 2) + 1];
-    for (int d = lane; d < dim; d += 32) {
-        float sum = 0.0f;
-        for (int c = 0; c < n; ++c)
-            sum += exp2f(from[(long long)c * (dim + 2)] - ref) * from[(long long)c * (dim + 2) + 2 + d];
-        store_value(p.out, out + d, p.type, l == 0.0f ? 0.0f : sum / l);
+    return {token * p.out_token + head * p.out_head, s.kept < 0 ? -2 : min((sees + chunk - 1) / chunk, count)};
+}
+
+// Four of a lane's values; lane + 32 i counts groups of four
+__device__ __forceinline__ void add_four(float (&sum)[4], const float4& v, float f) {
+    sum[0] = fmaf(f, v.x, sum[0]);
+    sum[1] = fmaf(f, v.y, sum[1]);
+    sum[2] = fmaf(f, v.z, sum[2]);
+    sum[3] = fmaf(f, v.w, sum[3]);
+}
+
+// Up to 32 chunks: a warp a row, a lane a chunk's maximum and sum.
+__global__ void __launch_bounds__(128) k_attend_join_few(AttendParams p, int chunk, int count, int tile) {
+    const int lane = threadIdx.x % 32, four = p.c.dim / 4;
+    const long long i = (long long)blockIdx.x * 4 + threadIdx.x / 32;
+    if (i >= p.r.total * p.heads) return;
+    const JoinRow r = join_row(p, i / p.heads, (int)(i % p.heads), chunk, count, tile);
+    if (r.chunks == -1) return;
+    chain_wait();
+    const Partial from = partial_of(p, i, count, 0);
+    const float2 own = lane < r.chunks ? from.stats[lane] : make_float2(-inf_f(), 0.0f);
+    float top = own.x;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float factor = exp2f(own.x - (top == -inf_f() ? 0.0f : top));
+    float l = factor * own.y, sum[2][4] = {};
+#pragma unroll
+    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    for (int c0 = 0; c0 < r.chunks; c0 += 4) {
+        float4 v[4][2];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                v[c][j] = c0 + c < r.chunks && lane + 32 * j < four
+                              ? reinterpret_cast<const float4*>(from.sums + (long long)(c0 + c) * p.c.dim)[lane + 32 * j]
+                              : make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float f = __shfl_sync(0xffffffffu, factor, c0 + c);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) add_four(sum[j], v[c][j], f);
+        }
+    }
+    if (r.chunks == -2) l = nan_f();
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        if (lane + 32 * j < four)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                store_value(p.out, r.out + (lane + 32 * j) * 4 + e, p.type, l == 0.0f ? 0.0f : sum[j][e] / l);
+}
+
+// More chunks: a CTA a row.  The chunks' factors are made by all threads and
+// kept in shared memory; then each warp adds up every fourth chunk, eight of
+// them in flight.
+constexpr int kJoinThreads = 128, kJoinChunks = 512;
+
+__global__ void __launch_bounds__(kJoinThreads) k_attend_join(AttendParams p, int chunk, int count, int tile) {
+    __shared__ float factor[kJoinChunks], part[4][256], side[2][4];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, four = p.c.dim / 4;
+    const JoinRow r = join_row(p, blockIdx.x / p.heads, blockIdx.x % p.heads, chunk, count, tile);
+    if (r.chunks == -1) return;
+    chain_wait();
+    float top = -inf_f(), l = 0.0f, sum[2][4] = {};
+    for (int first = 0; first < r.chunks; first += kJoinChunks) {
+        const int here = min(r.chunks - first, kJoinChunks);
+        const Partial from = partial_of(p, blockIdx.x, count, first);
+        constexpr int kEach = kJoinChunks / kJoinThreads;
+        float2 v[kEach];
+        float most = top;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int c = threadIdx.x + i * kJoinThreads;
+            v[i] = c < here ? from.stats[c] : make_float2(-inf_f(), 0.0f);
+            most = fmaxf(most, v[i].x);
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        __syncthreads();
+        if (lane == 0) side[0][warp] = most;
+        __syncthreads();
+        most = fmaxf(fmaxf(side[0][0], side[0][1]), fmaxf(side[0][2], side[0][3]));
+        const float ref = most == -inf_f() ? 0.0f : most, by = exp2f(top - ref);
+        top = most;
+        l *= by;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[j][e] *= by;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const float f = exp2f(v[i].x - ref);
+            factor[threadIdx.x + i * kJoinThreads] = f;       // 0 past the last
+            l += f * v[i].y;
+        }
+        __syncthreads();
+        for (int c0 = warp; c0 < here; c0 += 32) {
+            float4 x[8][2];
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    x[c][j] = c0 + 4 * c < here && lane + 32 * j < four
+                                  ? reinterpret_cast<const float4*>(from.sums + (long long)(c0 + 4 * c) * p.c.dim)[lane + 32 * j]
+                                  : make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const float f = c0 + 4 * c < here ? factor[c0 + 4 * c] : 0.0f;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) add_four(sum[j], x[c][j], f);
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    if (lane == 0) side[1][warp] = l;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[warp][(lane + 32 * j) * 4 + e] = sum[j][e];
+    __syncthreads();
+    l = (side[1][0] + side[1][1]) + (side[1][2] + side[1][3]);
+    if (r.chunks == -2) l = nan_f();
+    for (int d = threadIdx.x; d < p.c.dim; d += kJoinThreads) {
+        const float x = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
+        store_value(p.out, r.out + d, p.type, l == 0.0f ? 0.0f : x / l);
     }
 }
 
-template <int D, int P>
+template <int D, int P, int NR>
 cudaError_t rows_launch(const AttendParams& p, const Chunks& c, cudaStream_t s) {
-    const RowsLayout lay = rows_layout(D, c.tokens, P);
-    const long long tiles = ((long long)p.r.most * (p.heads / p.c.heads) + 15) / 16;
+    const RowsLayout lay = rows_layout(D, NR, c.tokens, P);
+    const long long rows = (long long)p.r.most * (p.heads / p.c.heads), tiles = (rows + 8 * NR - 1) / (8 * NR);
     const dim3 grid(c.count, (unsigned)(tiles * p.c.heads), p.r.seqs);
-    cudaError_t e = allow_shared<k_attend_rows<D, P>>((int)rows_layout(D, kMostChunk, P).bytes);
+    const cudaError_t e = allow_shared<k_attend_rows<D, P, NR>>((int)rows_layout(D, NR, kMostChunk, P).bytes);
     if (e != cudaSuccess) return e;
-    k_attend_rows<D, P><<<grid, kRowsWarps * 32, lay.bytes, s>>>(p, c.tokens);
+    k_attend_rows<D, P, NR><<<grid, kRowsWarps * 32, lay.bytes, s>>>(p, c.tokens);
     return cudaGetLastError();
+}
+
+template <int D, int P>
+cudaError_t by_rows(const AttendParams& p, const Chunks& c, cudaStream_t s) {
+    return row_groups((long long)p.r.most * (p.heads / p.c.heads)) == 1 ? rows_launch<D, P, 1>(p, c, s) : rows_launch<D, P, 2>(p, c, s);
 }
 
 template <int D>
 cudaError_t by_page(const AttendParams& p, const Chunks& c, cudaStream_t s) {
     switch (p.c.page) {
-        case 16: return rows_launch<D, 16>(p, c, s);
-        case 32: return rows_launch<D, 32>(p, c, s);
-        default: return rows_launch<D, 64>(p, c, s);
+        case 16: return by_rows<D, 16>(p, c, s);
+        case 32: return by_rows<D, 32>(p, c, s);
+        default: return by_rows<D, 64>(p, c, s);
     }
 }
 
@@ -435,35 +629,37 @@ cudaError_t by_dim(const AttendParams& p, const Chunks& c, cudaStream_t s) {
 
 bool attend_dim_ok(int dim) { return dim == 32 || dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256; }
 
-// Many rows go to the tile kernel where it has the head's size; up to 16 rows
-// fill one tile of this file's kernel, which reads the cache as fast.
-bool use_tiles(int dim, int heads, int kv_heads, int most) {
-    return attend_tiles_dim(dim) && (long long)most * (heads / kv_heads) > 16;
-}
+// Up to 16 rows go to this file's kernel, more to the tile kernel: with 32 rows
+// of 16 heads of 64 over 16 caches of up to 1500 tokens this one (made for four
+// groups of eight rows) took 45 us, with 32 of 128 over 2000 tokens 28 us; the
+// tile kernel 27 and 26.
+bool use_tiles(int heads, int kv_heads, int most) { return (long long)most * (heads / kv_heads) > 16; }
 
 Chunks plan(int dim, int heads, int kv_heads, int seqs, int most, int most_kept) {
-    return use_tiles(dim, heads, kv_heads, most) ? plan_tiles(heads, kv_heads, seqs, most, most_kept)
+    return use_tiles(heads, kv_heads, most) ? plan_tiles(dim, heads, kv_heads, seqs, most, most_kept)
                                                  : plan_chunks(heads, kv_heads, seqs, most, most_kept);
 }
 
-// the grid's y counts tiles of 16 rows
+// the grid's y counts tiles of rows
 bool attend_fits(int dim, int heads, int kv_heads, int most) {
-    return use_tiles(dim, heads, kv_heads, most) || ((long long)most * (heads / kv_heads) + 15) / 16 * kv_heads <= 65535;
+    const long long rows = (long long)most * (heads / kv_heads), each = 8 * row_groups(rows);
+    return use_tiles(heads, kv_heads, most) || (rows + each - 1) / each * kv_heads <= 65535;
 }
 
 size_t attend_scratch_bytes(long long total, int heads, int kv_heads, int dim, int seqs, int most, int most_kept) {
     const Chunks c = plan(dim, heads, kv_heads, seqs, most, most_kept);
-    return c.count == 1 ? 0 : (size_t)total * heads * c.count * (dim + 2) * sizeof(float);
+    return c.count == 1 ? 0 : (size_t)partial_floats((long long)total * heads, c.count, dim) * sizeof(float);
 }
 
 cudaError_t launch_cache_attention(const AttendParams& p, cudaStream_t s) {
-    const bool tiles = use_tiles(p.c.dim, p.heads, p.c.heads, p.r.most);
+    const bool tiles = use_tiles(p.heads, p.c.heads, p.r.most);
     const Chunks c = plan(p.c.dim, p.heads, p.c.heads, p.r.seqs, p.r.most, p.most_kept);
     const cudaError_t e = tiles ? launch_attend_tiles(p, c, s) : by_dim(p, c, s);
     if (e != cudaSuccess || c.count == 1) return e;
-    const long long n = p.r.total * p.heads;
-    const int rows = tiles ? tile_rows((long long)p.r.most * (p.heads / p.c.heads)) : 16;
-    return launch_after(k_attend_join, dim3((unsigned)((n + 3) / 4)), dim3(128), 0, s, p, c.tokens, c.count, rows);
+    const long long n = p.r.total * p.heads, rows = (long long)p.r.most * (p.heads / p.c.heads);
+    const int tile = tiles ? tile_rows(p.c.dim, rows) : 8 * row_groups(rows);
+    if (c.count <= 32) return launch_after(k_attend_join_few, dim3((unsigned)((n + 3) / 4)), dim3(128), 0, s, p, c.tokens, c.count, tile);
+    return launch_after(k_attend_join, dim3((unsigned)n), dim3(kJoinThreads), 0, s, p, c.tokens, c.count, tile);
 }
 
 }  // namespace vdt

@@ -25,21 +25,23 @@
 namespace vdt {
 namespace {
 
-constexpr int kTile = 128;        // query rows of a tile; tokens of a step
+constexpr int kTile = 128;        // query rows of a tile
 constexpr int kAhead = 4;         // steps that the page lists are ahead
-constexpr float kSlack = 8.0f;    // by how much (a power of two) a weight may pass 1
-constexpr float kValueSlack = 4.0f;
-
 template <int D, int NT, int P>
 struct Shape {
+    static constexpr int kStep = D <= 128 ? 128 : 64;              // tokens of a step
     static constexpr int kSub = (D + 63) / 64;                     // 64-wide blocks of a head
-    static constexpr int kQ = kSub * kTile * 128, kK = kQ, kV = 2 * D * 128;
-    static constexpr int kPages = kTile / P;
-    static constexpr int kRaw = kTile * D;                         // the codes of a step's keys, or values
+    static constexpr int kQ = kSub * kTile * 128, kK = kSub * kStep * 128, kV = kStep / 64 * D * 128;
+    static constexpr int kPages = kStep / P;
+    static constexpr int kRaw = kStep * D;                         // the codes of a step's keys, or values
     static constexpr int kSoft = 4 * NT, kCode = kSoft, kIssue = kSoft + 4, kList = kSoft + 5;   // first warps of each part
-    static constexpr int kThreads = (kSoft + 8) * 32;              // whole groups of four warps: two have nothing to do
-    static constexpr int kTmem = NT * (kTile + D) <= 256 ? 256 : 512;
+    // two tiles share out registers by groups of four warps: two have nothing to do
+    static constexpr int kThreads = (NT == 2 ? kSoft + 8 : kSoft + 6) * 32;
+    static constexpr int kTmem = NT * (kStep + D) <= 256 ? 256 : 512;
     static constexpr int kBytes = 1024 + NT * kQ + 2 * kK + 2 * kV + 2 * kRaw;
+    // one tile of a small head leaves room for a second CTA on the SM; its
+    // softmax then holds half of the scores at a time
+    static constexpr int kPerSm = NT == 1 && D <= 64 ? 2 : 1, kHold = kPerSm == 2 ? 64 : kStep;
 };
 // registers a thread with two tiles: at launch, and how the four groups of
 // warps share them out
@@ -103,12 +105,6 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // what this thread wrote to shared memory is there for the tensor cores
 __device__ __forceinline__ void fence_shared_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // 16 codes to two 16-byte pieces `chunk` and `chunk + 1` of a swizzled row;
 // `flip` writes the second first (lanes that would meet on one bank)
 __device__ __forceinline__ void store_codes(unsigned char* rows, int row, int chunk, const uint4& w, bool flip) {
@@ -123,11 +119,12 @@ __device__ __forceinline__ void store_codes(unsigned char* rows, int row, int ch
 }
 
 template <int D, int NT, int P>
-__global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(AttendParams p, int chunk, int count) {
+__global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kPerSm) k_attend_tiles(AttendParams p, int chunk, int count) {
     using Sh = Shape<D, NT, P>;
-    constexpr int kPages = Sh::kPages;
+    constexpr int kPages = Sh::kPages, kStep = Sh::kStep;
     extern __shared__ unsigned char smem_raw[];
     __shared__ State<NT, kPages> st;
+    chain_release();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int b = blockIdx.z, h = blockIdx.y, group = p.heads / p.c.heads;
     // the longest rows first: they see the most tokens
@@ -146,7 +143,7 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
     for (int t = 0; t < NT; ++t) {
         const int last = min(row0 + (t + 1) * kTile, rows) - 1;
         const int end = row0 + t * kTile < rows ? min(begin + chunk, sees(last)) : 0;
-        steps[t] = max(0, (end - begin + kTile - 1) / kTile);
+        steps[t] = max(0, (end - begin + kStep - 1) / kStep);
         most = max(most, steps[t]);
     }
     if (count > 1 && begin >= max(1, sees(min(row0 + NT * kTile, rows) - 1))) return;     // the join knows as well
@@ -190,50 +187,57 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
         const int r = threadIdx.x % kTile;
         const long long from = token * p.q_token + (long long)head * p.q_head;
         const bool in = mine < rows, wide = p.q_token % 8 == 0 && p.q_head % 8 == 0 && reinterpret_cast<uintptr_t>(p.q) % 16 == 0;
-        auto eight = [&](int d, float (&f)[8]) {
-            if (!in) {
+        // the row as it is: all its loads are in flight together
+        uint4 raw_q[D / 8];
+        const __half* const q = static_cast<const __half*>(p.q) + from;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) f[j] = 0.0f;
-            } else if (wide) {
-                const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) + from + d);
-                if (p.type == VDT_F16) {
-                    Vec16<__half> v{raw};
-                    v.get(f);
-                } else {
-                    Vec16<__nv_bfloat16> v{raw};
-                    v.get(f);
-                }
+        for (int i = 0; i < D / 8; ++i) raw_q[i] = in && wide ? *reinterpret_cast<const uint4*>(q + i * 8) : make_uint4(0, 0, 0, 0);
+        if (in && !wide) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                __half v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = q[i * 8 + j];
+                memcpy(&raw_q[i], v, 16);
+            }
+        }
+        auto eight = [&](int i, float (&f)[8]) {
+            if (p.type == VDT_F16) {
+                Vec16<__half> v{raw_q[i]};
+                v.get(f);
             } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) f[j] = load_value(p.q, from + d + j, p.type);
+                Vec16<__nv_bfloat16> v{raw_q[i]};
+                v.get(f);
             }
         };
         float m = 0.0f;
-        for (int d = 0; d < D; d += 8) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
             float f[8];
-            eight(d, f);
+            eight(i, f);
 #pragma unroll
             for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[j]));
         }
         const int e = m > 0.0f && m < inf_f() ? max(-126, min(126, ilogbf(m))) : 0;
         q_scale = scalbnf(fabsf(p.scale), e);
         const float f1 = copysignf(scalbnf(1.0f, -e), p.scale);        // a negative scale goes into the queries
-        for (int d = 0; d < D; d += 8) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
             float f[8];
-            eight(d, f);
+            eight(i, f);
             uint4 w;
             w.x = pack_f16(f[0] * f1, f[1] * f1);
             w.y = pack_f16(f[2] * f1, f[3] * f1);
             w.z = pack_f16(f[4] * f1, f[5] * f1);
             w.w = pack_f16(f[6] * f1, f[7] * f1);
-            *reinterpret_cast<uint4*>(to + d / 64 * (kTile * 128) + r * 128 + ((d % 64 / 8 ^ (r & 7)) << 4)) = w;
+            *reinterpret_cast<uint4*>(to + i / 8 * (kTile * 128) + r * 128 + ((i % 8 ^ (r & 7)) << 4)) = w;
         }
         fence_shared_async();
     }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = st.tmem, tmem_o = tmem + NT * kTile;
+    const uint32_t tmem = st.tmem, tmem_o = tmem + NT * kStep;
     bool alive = true;
 
     if (warp < Sh::kSoft) {
@@ -241,39 +245,53 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
         if constexpr (NT == 2) take_registers<kSoftRegs>();
         const int t = warp / 4;
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;             // this warp's rows of the tensor memory
-        const uint32_t at_s = tmem + t * kTile + lanes, at_o = tmem_o + t * D + lanes;
+        const uint32_t at_s = tmem + t * kStep + lanes, at_o = tmem_o + t * D + lanes;
         int my_steps = 0;
 #pragma unroll
         for (int i = 0; i < NT; ++i) my_steps = i == t ? steps[i] : my_steps;
         // what the weights and O are relative to: 2^ref, 2^vref
         float ref = -inf_f(), vref = -inf_f(), sum = 0.0f;
+        const bool busy = __any_sync(0xffffffffu, mine < rows);
         for (int j = 0; j < most; ++j) {
             const int slot = j % kAhead;
             alive = bar_wait_all(shared_address(&st.list_full[slot]), j / kAhead & 1);
             if (!alive) break;
             if (j < my_steps) {
-                const int left = limit - (begin + j * kTile);          // tokens of the step that the row sees
-                const bool partial = __any_sync(0xffffffffu, left < kTile);
+                const int left = limit - (begin + j * kStep);          // tokens of the step that the row sees
+                const bool partial = __any_sync(0xffffffffu, left < kStep);
                 alive = bar_wait_all(shared_address(&st.s_full[t]), j & 1);
                 if (!alive) break;
                 tmem_fence_after();
-                uint32_t r[4][32];
+                if (!busy) {                                           // rows past the last: whatever stands there
+                    tmem_fence_before();
+                    bar_arrive(shared_address(&st.p_full[t]));
+                    if (lane == 0) bar_arrive(shared_address(&st.list_free[slot]));
+                    continue;
+                }
+                constexpr int kHold = Sh::kHold;
+                uint32_t r[kHold / 32][32];
+                auto load = [&](int from) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tmem_load(at_s + i * 32, r[i]);
-                float c[kPages];
+                    for (int i = 0; i < kHold / 32; ++i) tmem_load(at_s + from + i * 32, r[i]);
+                };
+                float c[kPages], top = -inf_f();
 #pragma unroll
-                for (int i = 0; i < kPages; ++i) c[i] = st.k_scale[slot][i] * q_scale;
-                tmem_load_wait();
-                float top = -inf_f();
-                if (partial)
+                for (int from = kStep - kHold; from >= 0; from -= kHold) {
+                    load(from);
+                    if (from == kStep - kHold)
 #pragma unroll
-                    for (int i = 0; i < kTile; ++i) r[i / 32][i % 32] = i < left ? r[i / 32][i % 32] : 0xff800000u;
+                        for (int i = 0; i < kPages; ++i) c[i] = st.k_scale[slot][i] * q_scale;
+                    tmem_load_wait();
+                    if (partial)
 #pragma unroll
-                for (int i = 0; i < kTile; i += P < 32 ? P : 32) {
-                    float m = __uint_as_float(r[i / 32][i % 32]);
+                        for (int i = 0; i < kHold; ++i) r[i / 32][i % 32] = from + i < left ? r[i / 32][i % 32] : 0xff800000u;
 #pragma unroll
-                    for (int q = 1; q < (P < 32 ? P : 32); ++q) m = fmaxf(m, __uint_as_float(r[i / 32][i % 32 + q]));
-                    top = fmaxf(top, m * c[i / P]);
+                    for (int i = 0; i < kHold; i += P < 32 ? P : 32) {
+                        float m = __uint_as_float(r[i / 32][i % 32]);
+#pragma unroll
+                        for (int q = 1; q < (P < 32 ? P : 32); ++q) m = fmaxf(m, __uint_as_float(r[i / 32][i % 32 + q]));
+                        top = fmaxf(top, m * c[(from + i) / P]);
+                    }
                 }
                 const float v_most = st.v_most[slot];
                 const bool up = top > ref + kSlack || (ref == -inf_f() && top > ref), v_up = v_most > vref + kValueSlack || (vref == -inf_f() && v_most > vref);
@@ -302,28 +320,36 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
                 // under 2^-100: a page of zeros still has weights.
                 const float shift = ref == -inf_f() ? 0.0f : -ref, v_shift = vref == -inf_f() ? 0.0f : vref;
 #pragma unroll
-                for (int i = 0; i < kPages; ++i) {
-                    float f = st.v_log[slot][i] - v_shift;
-                    f = f < -100.0f ? -100.0f : f;
-                    const float d = shift + f;
-                    float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll
-                    for (int q = i * P; q < (i + 1) * P; q += 2) {
-                        float x = exp2_fast(fmaf(__uint_as_float(r[q / 32][q % 32]), c[i], d));
-                        float y = exp2_fast(fmaf(__uint_as_float(r[q / 32][q % 32 + 1]), c[i], d));
-                        if (partial) {                                 // also for scales that are not numbers
-                            x = q < left ? x : 0.0f;
-                            y = q + 1 < left ? y : 0.0f;
-                        }
-                        l0 += x;
-                        l1 += y;
-                        r[q / 64][q / 2 % 32] = pack_f16(x, y);
+                for (int from = 0; from < kStep; from += kHold) {
+                    if (from) {
+                        load(from);
+                        tmem_load_wait();
                     }
-                    l0 += l1;
-                    sum = partial && i * P >= left ? sum : fmaf(l0, exp2_fast(-f), sum);
+#pragma unroll
+                    for (int i = from / P; i < (from + kHold) / P; ++i) {
+                        float f = st.v_log[slot][i] - v_shift;
+                        f = f < -100.0f ? -100.0f : f;
+                        const float d = shift + f;
+                        float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+                        for (int a = i * P; a < (i + 1) * P; a += 2) {
+                            const int q = a - from;
+                            float x = exp2_fast(fmaf(__uint_as_float(r[q / 32][q % 32]), c[i], d));
+                            float y = exp2_fast(fmaf(__uint_as_float(r[q / 32][q % 32 + 1]), c[i], d));
+                            if (partial) {                             // also for scales that are not numbers
+                                x = a < left ? x : 0.0f;
+                                y = a + 1 < left ? y : 0.0f;
+                            }
+                            l0 += x;
+                            l1 += y;
+                            r[q / 64][q / 2 % 32] = pack_f16(x, y);
+                        }
+                        l0 += l1;
+                        sum = partial && i * P >= left ? sum : fmaf(l0, exp2_fast(-f), sum);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kHold / 64; ++i) tmem_store32(at_s + from / 2 + i * 32, r[i]);
                 }
-                tmem_store32(at_s, r[0]);
-                tmem_store32(at_s + 32, r[1]);
                 tmem_store_wait();
                 tmem_fence_before();
                 bar_arrive(shared_address(&st.p_full[t]));
@@ -338,12 +364,9 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
         const float scale = bad ? nan_f() : count > 1 ? exp2f(vref) : sum == 0.0f ? 0.0f : exp2f(vref) / sum;
         const bool nothing = !bad && sum == 0.0f;                       // no token seen (O may not have been written)
         const long long out = token * p.out_token + (long long)head * p.out_head;
-        float* const rest = p.scratch + ((token * p.heads + head) * count + part) * (D + 2);
+        const Partial rest = partial_of(p, token * p.heads + head, count, part);
         const bool wide = p.out_token % 8 == 0 && p.out_head % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
-        if (count > 1 && mine < rows) {
-            rest[0] = ref;
-            rest[1] = bad ? nan_f() : sum;
-        }
+        if (count > 1 && mine < rows) *rest.stats = make_float2(ref, bad ? nan_f() : sum);
 #pragma unroll
         for (int i = 0; i < D; i += 32) {
             uint32_t r[32];
@@ -353,7 +376,12 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
             if (mine >= rows) continue;
             if (count > 1) {
 #pragma unroll
-                for (int q = 0; q < 32; ++q) rest[2 + i + q] = nothing ? 0.0f : __uint_as_float(r[q]) * scale;
+                for (int q = 0; q < 32; q += 4) {
+                    float f[4];
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) f[a] = nothing ? 0.0f : __uint_as_float(r[q + a]) * scale;
+                    *reinterpret_cast<float4*>(rest.sums + i + q) = make_float4(f[0], f[1], f[2], f[3]);
+                }
             } else if (wide) {
 #pragma unroll
                 for (int q = 0; q < 32; q += 8) {
@@ -380,16 +408,16 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
         // ------------------------------------------------- codes to 16 bits
         if constexpr (NT == 2) give_registers<kCodeRegs>();
         const int thread = threadIdx.x - Sh::kCode * 32;
-        constexpr int kPer = D / 16;                                   // 16-byte pieces of a thread, keys or values
-        constexpr int kBlock = P * D / 16;                             // of a page
+        constexpr int kPer = kStep * D / 16 / 128;                     // 16-byte pieces of a thread, keys or values
+        constexpr int kRow = D / 16, kBlock = P * D / 16;              // of a token's keys, of a page
         for (int j = 0; j < most; ++j) {
             const int slot = j & 1, phase = (j / 2 & 1) ^ 1;
             alive = bar_wait_all(shared_address(&st.raw_full[0]), j & 1) && bar_wait_all(shared_address(&st.k_free[slot]), phase);
             if (!alive) break;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                const int at = thread + i * 128, row = at / kPer, e = at % kPer;
-                store_codes(kt + slot * Sh::kK + e / 4 * (kTile * 128), row, e % 4 * 2, *reinterpret_cast<const uint4*>(raw + at * 16), e & 4);
+                const int at = thread + i * 128, row = at / kRow, e = at % kRow;
+                store_codes(kt + slot * Sh::kK + e / 4 * (kStep * 128), row, e % 4 * 2, *reinterpret_cast<const uint4*>(raw + at * 16), e & 4);
             }
             fence_shared_async();
             __syncwarp();
@@ -402,7 +430,7 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int at = thread + i * 128, pg = at / kBlock, rest = at % kBlock, row = rest / (P / 16);
-                const int block = pg * (P / 16) + rest % (P / 16);     // 16 tokens of the step's 128
+                const int block = pg * (P / 16) + rest % (P / 16);     // 16 tokens of the step
                 store_codes(vt + slot * Sh::kV + block / 4 * (D * 128), row, block % 4 * 2,
                             *reinterpret_cast<const uint4*>(raw + Sh::kRaw + at * 16), false);
             }
@@ -417,7 +445,7 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
         // ---------------------------------------------------------- products
         if constexpr (NT == 2) give_registers<kIssueRegs>();
         constexpr uint32_t shape = 1u << 4 | (kTile >> 4) << 24;       // 32-bit sums of 16-bit floats
-        constexpr uint32_t shape_s = shape | (kTile >> 3) << 17, shape_o = shape | (D >> 3) << 17;
+        constexpr uint32_t shape_s = shape | (kStep >> 3) << 17, shape_o = shape | (D >> 3) << 17;
         const uint32_t at = __shfl_sync(0xffffffffu, tmem, 0);
         const uint64_t q_at = tile_desc(shared_address(smem)), k_at = tile_desc(shared_address(kt)), v_at = tile_desc(shared_address(vt));
         const bool one = elected();
@@ -425,16 +453,16 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
             if (one) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_shared(at + t * kTile, q_at + (t * Sh::kQ + k / 4 * (kTile * 128) + k % 4 * 32) / 16,
-                               k_at + (slot * Sh::kK + k / 4 * (kTile * 128) + k % 4 * 32) / 16, shape_s, k > 0);
+                    mma_shared(at + t * kStep, q_at + (t * Sh::kQ + k / 4 * (kTile * 128) + k % 4 * 32) / 16,
+                               k_at + (slot * Sh::kK + k / 4 * (kStep * 128) + k % 4 * 32) / 16, shape_s, k > 0);
                 mma_commit(shared_address(&st.s_full[t]));
             }
         };
         auto outputs = [&](int t, int slot, bool add) {
             if (one) {
 #pragma unroll
-                for (int k = 0; k < kTile / 16; ++k)
-                    mma_tensor(at + NT * kTile + t * D, at + t * kTile + k * 8, v_at + (slot * Sh::kV + k / 4 * (D * 128) + k % 4 * 32) / 16,
+                for (int k = 0; k < kStep / 16; ++k)
+                    mma_tensor(at + NT * kStep + t * D, at + t * kStep + k * 8, v_at + (slot * Sh::kV + k / 4 * (D * 128) + k % 4 * 32) / 16,
                                shape_o, add || k > 0);
                 mma_commit(shared_address(&st.o_done[t]));
             }
@@ -472,7 +500,7 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
         const bool on = lane < kPages;
         // step j's page: -1 past the end, -2 if it is not in the cache
         auto page = [&](int j) {
-            const int first = begin + j * kTile + lane * P;
+            const int first = begin + j * kStep + lane * P;
             if (!on || first >= end) return -1;
             const int no = p.r.table[(long long)b * p.r.width + first / P];
             return no >= 0 && no < p.c.pages ? no : -2;
@@ -521,8 +549,8 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, 1) k_attend_tiles(A
         if (!alive)                                                    // what is in flight gets as long again to land
             for (int side = 0; side < 2; ++side)
                 for (int ph = 0; ph < 2; ++ph) bar_wait(shared_address(&st.raw_full[side]), ph);
-    } else {
-        if constexpr (NT == 2) give_registers<kIssueRegs>();
+    } else if constexpr (NT == 2) {
+        give_registers<kIssueRegs>();
     }
     // the products are done: every tile's last commit has been waited for
     tmem_fence_before();
@@ -569,22 +597,23 @@ cudaError_t by_dim(const AttendParams& p, const Chunks& c, cudaStream_t s) {
         case 32: return by_page<32, NT>(p, c, s);
         case 64: return by_page<64, NT>(p, c, s);
         case 96: return by_page<96, NT>(p, c, s);
-        default: return by_page<128, NT>(p, c, s);
+        case 128: return by_page<128, NT>(p, c, s);
+        case 192: return by_page<192, 1>(p, c, s);
+        default: return by_page<256, 1>(p, c, s);
     }
 }
 
 }  // namespace
 
-// the tensor memory holds two tiles' scores and sums up to 128 values a head
-bool attend_tiles_dim(int dim) { return dim <= 128; }
-
-int tile_rows(long long rows) { return rows <= kTile ? kTile : 2 * kTile; }
+// Two tiles share the turned codes where there are the rows, and where the
+// tensor memory holds both tiles' scores and sums: up to 128 values a head.
+int tile_rows(int dim, long long rows) { return rows <= kTile || dim > 128 ? kTile : 2 * kTile; }
 
 // The tokens divided where the tiles alone leave SMs idle, 512 of them at least
 // to a CTA.
-Chunks plan_tiles(int heads, int kv_heads, int seqs, int most, int most_kept) {
-    const long long rows = (long long)most * (heads / kv_heads);
-    const long long ctas = (long long)kv_heads * seqs * ((rows + tile_rows(rows) - 1) / tile_rows(rows));
+Chunks plan_tiles(int dim, int heads, int kv_heads, int seqs, int most, int most_kept) {
+    const long long rows = (long long)most * (heads / kv_heads), each = tile_rows(dim, rows);
+    const long long ctas = (long long)kv_heads * seqs * ((rows + each - 1) / each);
     const long long want = kSmCount / ctas;
     if (want <= 1) return {(most_kept + kTile - 1) / kTile * kTile, 1};
     long long tokens = ((long long)most_kept + want - 1) / want;
@@ -595,7 +624,7 @@ Chunks plan_tiles(int heads, int kv_heads, int seqs, int most, int most_kept) {
 }
 
 cudaError_t launch_attend_tiles(const AttendParams& p, const Chunks& c, cudaStream_t s) {
-    return tile_rows((long long)p.r.most * (p.heads / p.c.heads)) == kTile ? by_dim<1>(p, c, s) : by_dim<2>(p, c, s);
+    return tile_rows(p.c.dim, (long long)p.r.most * (p.heads / p.c.heads)) == kTile ? by_dim<1>(p, c, s) : by_dim<2>(p, c, s);
 }
 
 }  // namespace vdt

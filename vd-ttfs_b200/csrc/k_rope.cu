@@ -213,12 +213,20 @@ cudaError_t rows_launch(const RopeParams& p, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-// four rows a lane group where there are enough of them to fill the GPU
+// Several rows a lane group where there are enough of them to fill the GPU: as
+// many as leave the fewest places empty at a token's end (40 heads in groups of
+// 4: five rows, twice), of those the most.
 template <typename T, int LANES>
 cudaError_t by_rows(const RopeParams& p, cudaStream_t s) {
-    const long long rows = p.tokens * (p.heads + p.kv_heads);
-    return rows * LANES >= 4LL * 32 * 16 * kSmCount && p.heads + p.kv_heads > 32 / LANES ? rows_launch<T, LANES, 4>(p, s)
-                                                                                         : rows_launch<T, LANES, 1>(p, s);
+    const int all = p.heads + p.kv_heads, each = 32 / LANES, turns = (all + each - 1) / each;
+    if (p.tokens * all * LANES < 4LL * 32 * 16 * kSmCount || turns < 2) return rows_launch<T, LANES, 1>(p, s);
+    int best = 2;
+    for (const int n : {3, 4, 5})
+        if ((turns + n - 1) / n * n <= (turns + best - 1) / best * best) best = n;
+    if (best == 2) return rows_launch<T, LANES, 2>(p, s);
+    if (best == 3) return rows_launch<T, LANES, 3>(p, s);
+    if (best == 4) return rows_launch<T, LANES, 4>(p, s);
+    return rows_launch<T, LANES, 5>(p, s);
 }
 
 template <typename T>
