@@ -57,7 +57,7 @@ struct Place {
     int n, old;             // new tokens; tokens before them in the page
     long long first, slot;  // the first one's packed row; page number * heads + head
 };
-__device__ __forceinline__ bool place_of(const vdt_cache8& c, const CacheRows& r, Place& o) {
+__device__ __forceinline__ bool place_of(const vdt_cache8& c, const CacheRows& r, int h, Place& o) {
     const int b = blockIdx.z;
     const Part p = part_of(r, b);
     if (!p.rows) return false;
@@ -69,7 +69,7 @@ __device__ __forceinline__ bool place_of(const vdt_cache8& c, const CacheRows& r
     o.n = hi - lo;
     o.old = lo - j * c.page;
     o.first = p.first + (lo - p.held);
-    o.slot = (long long)no * c.heads + blockIdx.y;
+    o.slot = (long long)no * c.heads + h;
     return true;
 }
 
@@ -98,8 +98,8 @@ __global__ void __launch_bounds__(kCacheThreads) k_cache_append_any(vdt_cache8 c
                                                                     const T* __restrict__ v, long long k_token, long long k_head,
                                                                     long long v_token, long long v_head) {
     Place o;
-    if (!place_of(c, r, o)) return;
     const int h = blockIdx.y, dim = c.dim;
+    if (!place_of(c, r, h, o)) return;
     for (int side = 0; side < 2; ++side) {
         const T* x = side ? v + o.first * v_token + h * v_head : k + o.first * k_token + h * k_head;
         const long long step = side ? v_token : k_token;
@@ -114,120 +114,126 @@ __global__ void __launch_bounds__(kCacheThreads) k_cache_append_any(vdt_cache8 c
     }
 }
 
-// A value tile in shared memory, [dim][page] bytes; a row's pad keeps lanes
-// that write eight rows apart on few banks.
+// A value tile in shared memory: byte (d, t) of [dim][page].  The words of a
+// row are permuted by the row's group of eight, so that lanes that hold eight
+// dimensions each of one token meet on as few banks as there are words.
 template <int P>
-constexpr int kTileRow = P + 4;
+__device__ __forceinline__ int tile_byte(int d, int t) {
+    return d * P + ((t / 4 ^ (d / 8 & (P / 4 - 1))) * 4) + t % 4;
+}
 
-// Rows of whole 16-byte vectors.  The page's new vectors are read once and
-// stay in registers (at most 64 tokens x 256 values over 128 threads); keys go
-// out as they are, values through shared memory, where their tokens come to
-// lie side by side.
+// Rows of whole 16-byte vectors: one CTA for each (page touched, head, sequence)
+// and for keys and values apart.  The page's new vectors are read once and stay
+// in registers (at most 64 tokens x 256 values over 128 threads); keys go out as
+// they are, values through shared memory, where their tokens come to lie side
+// by side.
 template <typename T, int D, int P>
 __global__ void __launch_bounds__(kCacheThreads) k_cache_append_rows(vdt_cache8 c, CacheRows r, const T* __restrict__ k,
                                                                      const T* __restrict__ v, long long k_token, long long k_head,
                                                                      long long v_token, long long v_head) {
     constexpr int N = Vec16<T>::N, kRow = D / N, kHeld = (P * kRow + kCacheThreads - 1) / kCacheThreads;
-    __shared__ __align__(16) unsigned char tile[D * kTileRow<P>];
+    __shared__ __align__(16) unsigned char tile[D * P];
     Place o;
-    if (!place_of(c, r, o)) return;
-    const int h = blockIdx.y;
-    for (int side = 0; side < 2; ++side) {
-        const T* x = side ? v + o.first * v_token + h * v_head : k + o.first * k_token + h * k_head;
-        const long long step = side ? v_token : k_token;
-        int8_t* codes = (side ? c.v : c.k) + o.slot * (P * D);
-        Vec16<T> held[kHeld];
-        float m = 0.0f;
+    const bool side = (int)blockIdx.y >= c.heads;
+    const int h = blockIdx.y - (side ? c.heads : 0);
+    if (!place_of(c, r, h, o)) return;
+    const T* x = side ? v + o.first * v_token + h * v_head : k + o.first * k_token + h * k_head;
+    const long long step = side ? v_token : k_token;
+    int8_t* codes = (side ? c.v : c.k) + o.slot * (P * D);
+    Vec16<T> held[kHeld];
+    float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            const int at = threadIdx.x + i * kCacheThreads, t = at / kRow, e = at % kRow;
-            held[i].raw = t < o.n ? *reinterpret_cast<const uint4*>(x + t * step + e * N) : make_uint4(0, 0, 0, 0);
-        }
+    for (int i = 0; i < kHeld; ++i) {
+        const int at = threadIdx.x + i * kCacheThreads, t = at / kRow, e = at % kRow;
+        held[i].raw = t < o.n ? *reinterpret_cast<const uint4*>(x + t * step + e * N) : make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            float f[N];
-            held[i].get(f);
+    for (int i = 0; i < kHeld; ++i) {
+        float f[N];
+        held[i].get(f);
 #pragma unroll
-            for (int j = 0; j < N; ++j) m = max_nan(fabsf(f[j]), m);
-        }
-        const Coder coder(grow(c, o, side, block_max(m)));
+        for (int j = 0; j < N; ++j) m = max_nan(fabsf(f[j]), m);
+    }
+    const Coder coder(grow(c, o, side, block_max(m)));
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
-            const int at = threadIdx.x + i * kCacheThreads, t = at / kRow, e = at % kRow;
-            if (t >= o.n) continue;
-            float f[N];
-            uint32_t w[N / 4];
-            held[i].get(f);
-            coder.words<N>(f, w);
-            if (!side) {
-                int8_t* to = codes + (o.old + t) * D + e * N;
-                if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-                else *reinterpret_cast<uint32_t*>(to) = w[0];
-            } else {
-#pragma unroll
-                for (int j = 0; j < N; ++j) tile[(e * N + j) * kTileRow<P> + o.old + t] = (unsigned char)(w[j / 4] >> (8 * (j % 4)));
-            }
-        }
-        if (!side) continue;
-        __syncthreads();
-        if (o.n == P) {
-            for (int i = threadIdx.x; i < D * P / 16; i += kCacheThreads) {
-                const uint32_t* from = reinterpret_cast<const uint32_t*>(tile + i / (P / 16) * kTileRow<P> + i % (P / 16) * 16);
-                *reinterpret_cast<uint4*>(codes + i * 16) = make_uint4(from[0], from[1], from[2], from[3]);
-            }
+    for (int i = 0; i < kHeld; ++i) {
+        const int at = threadIdx.x + i * kCacheThreads, t = at / kRow, e = at % kRow;
+        if (t >= o.n) continue;
+        float f[N];
+        uint32_t w[N / 4];
+        held[i].get(f);
+        coder.words<N>(f, w);
+        if (!side) {
+            int8_t* to = codes + (o.old + t) * D + e * N;
+            if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+            else *reinterpret_cast<uint32_t*>(to) = w[0];
         } else {
-            for (int i = threadIdx.x; i < D * o.n; i += kCacheThreads) {
-                const int d = i / o.n, t = o.old + i % o.n;
-                codes[d * P + t] = (int8_t)tile[d * kTileRow<P> + t];
-            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) tile[tile_byte<P>(e * N + j, o.old + t)] = (unsigned char)(w[j / 4] >> (8 * (j % 4)));
+        }
+    }
+    if (!side) return;
+    __syncthreads();
+    if (o.n == P) {
+        for (int i = threadIdx.x; i < D * P / 16; i += kCacheThreads) {
+            const int d = i / (P / 16), t = i % (P / 16) * 16;
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint32_t*>(tile + tile_byte<P>(d, t + 4 * j));
+            *reinterpret_cast<uint4*>(codes + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    } else {
+        for (int i = threadIdx.x; i < D * o.n; i += kCacheThreads) {
+            const int d = i / o.n, t = o.old + i % o.n;
+            codes[d * P + t] = (int8_t)tile[tile_byte<P>(d, t)];
         }
     }
 }
 
-// Any size: one CTA for each (page, head, sequence), its tokens as values,
-// packed.  A page's value codes go through shared memory.
+// One CTA for each (page, head, sequence), for keys and values apart: its
+// tokens as values, packed.  Value codes go through shared memory.
 template <typename T, int D, int P>
 __global__ void __launch_bounds__(kCacheThreads) k_cache_load(vdt_cache8 c, CacheRows r, T* __restrict__ k, T* __restrict__ v) {
     constexpr int N = Vec16<T>::N, kRow = D / N;
-    __shared__ __align__(16) unsigned char tile[D * kTileRow<P>];
-    const int b = blockIdx.z, h = blockIdx.y, j = blockIdx.x;
+    __shared__ __align__(16) unsigned char tile[D * P];
+    const bool side = (int)blockIdx.y >= c.heads;
+    const int b = blockIdx.z, h = blockIdx.y - (side ? c.heads : 0), j = blockIdx.x;
     const long long start = r.starts[b], rows = (long long)r.starts[b + 1] - start;
     const int kept = r.held[b];
     const int n = min(kept - j * P, P);
     if (n <= 0 || kept > rows || start < 0 || start + rows > r.total) return;
     const int no = page_of(r, b, j, c.pages);
-    const float nan = __int_as_float(0x7fffffff);        // a page that is not in the cache
     const long long slot = (long long)max(no, 0) * c.heads + h, at = slot * (P * D);
-    const float ks = no < 0 ? nan : c.k_scale[slot], vs = no < 0 ? nan : c.v_scale[slot];
-    const uint4* vc = reinterpret_cast<const uint4*>(c.v + at);
-    for (int i = threadIdx.x; i < D * P / 16; i += kCacheThreads) {
-        const uint4 w = vc[i];
-        uint32_t* to = reinterpret_cast<uint32_t*>(tile + i / (P / 16) * kTileRow<P> + i % (P / 16) * 16);
-        to[0] = w.x; to[1] = w.y; to[2] = w.z; to[3] = w.w;
-    }
+    const float scale = no < 0 ? __int_as_float(0x7fffffff) : (side ? c.v_scale : c.k_scale)[slot];   // a page that is not in the cache: NaN
     const long long out = ((start + (long long)j * P) * c.heads + h) * D, step = (long long)c.heads * D;
+    if (side) {
+        const uint4* from = reinterpret_cast<const uint4*>(c.v + at);
+        for (int i = threadIdx.x; i < D * P / 16; i += kCacheThreads) {
+            const uint4 x = from[i];
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            const int d = i / (P / 16), t = i % (P / 16) * 16;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *reinterpret_cast<uint32_t*>(tile + tile_byte<P>(d, t + 4 * q)) = w[q];
+        }
+        __syncthreads();
+    }
     for (int i = threadIdx.x; i < n * kRow; i += kCacheThreads) {
         const int t = i / kRow, e = i % kRow;
         float f[N];
+        if (side) {
 #pragma unroll
-        for (int q = 0; q < N; q += 4) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(c.k + at + t * D + e * N + q);
+            for (int q = 0; q < N; ++q) f[q] = (float)(int8_t)tile[tile_byte<P>(e * N + q, t)] * scale;
+        } else {
 #pragma unroll
-            for (int a = 0; a < 4; ++a) f[q + a] = (float)(int8_t)(w >> (8 * a)) * ks;
+            for (int q = 0; q < N; q += 4) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(c.k + at + t * D + e * N + q);
+#pragma unroll
+                for (int a = 0; a < 4; ++a) f[q + a] = (float)(int8_t)(w >> (8 * a)) * scale;
+            }
         }
         Vec16<T> y;
         y.set(f);
-        *reinterpret_cast<uint4*>(k + out + t * step + e * N) = y.raw;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n * kRow; i += kCacheThreads) {
-        const int t = i / kRow, e = i % kRow;
-        float f[N];
-#pragma unroll
-        for (int q = 0; q < N; ++q) f[q] = (float)(int8_t)tile[(e * N + q) * kTileRow<P> + t] * vs;
-        Vec16<T> y;
-        y.set(f);
-        *reinterpret_cast<uint4*>(v + out + t * step + e * N) = y.raw;
+        *reinterpret_cast<uint4*>((side ? v : k) + out + t * step + e * N) = y.raw;
     }
 }
 
@@ -260,13 +266,13 @@ cudaError_t append(const vdt_cache8& c, const CacheRows& r, const void* k, const
         return cudaGetLastError();
     }
     return by_shape(c, [&](auto dim, auto page) {
-        k_cache_append_rows<T, dim(), page()><<<grid, kCacheThreads, 0, s>>>(c, r, kp, vp, kt, kh, vt, vh);
+        k_cache_append_rows<T, dim(), page()><<<dim3(grid.x, 2 * grid.y, grid.z), kCacheThreads, 0, s>>>(c, r, kp, vp, kt, kh, vt, vh);
         return cudaGetLastError();
     });
 }
 template <typename T>
 cudaError_t load(const vdt_cache8& c, const CacheRows& r, void* k, void* v, cudaStream_t s) {
-    const dim3 grid((r.most + c.page - 1) / c.page, c.heads, r.seqs);
+    const dim3 grid((r.most + c.page - 1) / c.page, 2 * c.heads, r.seqs);
     return by_shape(c, [&](auto dim, auto page) {
         k_cache_load<T, dim(), page()><<<grid, kCacheThreads, 0, s>>>(c, r, static_cast<T*>(k), static_cast<T*>(v));
         return cudaGetLastError();

@@ -108,7 +108,6 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_int8_rows(Int8Params p) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const int col0 = blockIdx.x * 16;
     const long long row0 = (long long)blockIdx.y * (8 * NT);
-    chain_wait();
     int acc[NT][4] = {};
     // rows past the end read the last one; their products are not stored
     const int8_t* w0 = p.w + (long long)min(col0 + g, p.cols - 1) * p.w_stride;
@@ -118,22 +117,42 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_int8_rows(Int8Params p) {
     for (int n = 0; n < NT; ++n) a[n] = p.a + min(row0 + 8 * n + g, p.rows - 1) * p.a_stride;
     const int steps = (p.inner + 63) / 64;
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int s = warp; s < steps; s += kRowsWarps) {
-        const int k = s * 64 + t * 16;
-        const bool in = k < p.inner;     // a row's storage reaches to the next multiple of 16
-        const uint4 u0 = in ? __ldg(reinterpret_cast<const uint4*>(w0 + k)) : zero;
-        const uint4 u1 = in ? __ldg(reinterpret_cast<const uint4*>(w1 + k)) : zero;
+    constexpr int kDeep = NT == 4 ? 2 : 4;                   // steps in flight
+    // a row's storage reaches to the next multiple of 16
+    auto weights = [&](int s, uint4 (&u)[2]) {
+        const bool in = s < steps && s * 64 + t * 16 < p.inner;
+        u[0] = in ? __ldg(reinterpret_cast<const uint4*>(w0 + s * 64 + t * 16)) : zero;
+        u[1] = in ? __ldg(reinterpret_cast<const uint4*>(w1 + s * 64 + t * 16)) : zero;
+    };
+    auto rows = [&](int s, uint4 (&b)[NT]) {
+        const bool in = s < steps && s * 64 + t * 16 < p.inner;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            uint4 b = in ? *reinterpret_cast<const uint4*>(a[n] + k) : zero;
-            if (k + 16 > p.inner) {
-                b.x = keep_below(b.x, k / 4, p.inner);
-                b.y = keep_below(b.y, k / 4 + 1, p.inner);
-                b.z = keep_below(b.z, k / 4 + 2, p.inner);
-                b.w = keep_below(b.w, k / 4 + 3, p.inner);
+        for (int n = 0; n < NT; ++n) b[n] = in ? *reinterpret_cast<const uint4*>(a[n] + s * 64 + t * 16) : zero;
+    };
+    uint4 u[kDeep][2], x[kDeep][NT];
+    // the weights are the caller's: their first loads need not wait for the codes
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) weights(warp + d * kRowsWarps, u[d]);
+    chain_wait();
+    for (int s0 = warp; s0 < steps; s0 += kDeep * kRowsWarps) {
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) rows(s0 + d * kRowsWarps, x[d]);
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            const int s = s0 + d * kRowsWarps, k = s * 64 + t * 16;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                uint4 b = x[d][n];
+                if (k + 16 > p.inner) {
+                    b.x = keep_below(b.x, k / 4, p.inner);
+                    b.y = keep_below(b.y, k / 4 + 1, p.inner);
+                    b.z = keep_below(b.z, k / 4 + 2, p.inner);
+                    b.w = keep_below(b.w, k / 4 + 3, p.inner);
+                }
+                mma_s8(acc[n], u[d][0].x, u[d][1].x, u[d][0].y, u[d][1].y, b.x, b.y);
+                mma_s8(acc[n], u[d][0].z, u[d][1].z, u[d][0].w, u[d][1].w, b.z, b.w);
             }
-            mma_s8(acc[n], u0.x, u1.x, u0.y, u1.y, b.x, b.y);
-            mma_s8(acc[n], u0.z, u1.z, u0.w, u1.w, b.z, b.w);
+            weights(s + kDeep * kRowsWarps, u[d]);
         }
     }
 #pragma unroll

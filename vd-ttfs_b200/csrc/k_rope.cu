@@ -39,7 +39,7 @@ __device__ __forceinline__ RopeRow rope_row(const RopeParams& p, long long token
 
 __device__ __forceinline__ float norm_factor(float squares, const RopeParams& p) {
     if (p.norm == VDT_NORM_NONE) return 1.0f;
-    return rsqrtf((p.norm == VDT_NORM_RMS ? squares / (float)p.dim : squares) + p.eps);
+    return rsqrtf(fmaf(squares, p.share, p.eps));
 }
 
 // Any size, stride and alignment: a warp a row, a lane a pair at a time.
@@ -79,124 +79,148 @@ __global__ void __launch_bounds__(kRopeWarps * 32) k_rope_any(RopeParams p) {
     }
 }
 
+// Two independent 32-bit multiplications, or multiply-adds
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
 // Rows of whole 16-byte vectors: LANES lanes a row, a lane two vectors that
 // hold each other's partners (half a rotation apart, or neighbours), so the
-// rotation stays in the lane.  A warp takes one token and ITER rows for each
-// of its lane groups: the angles are read once for all of them, and ITER rows'
-// loads are in flight together.
-template <typename T, int LANES, int ITER>
-__global__ void __launch_bounds__(kRopeWarps * 32) k_rope_rows(RopeParams p, long long items, int parts) {
-    constexpr int N = Vec16<T>::N;
+// rotation stays in the lane.  A warp takes one token and up to ITER heads of
+// the queries, or of the keys, for each of its lane groups, all loads in
+// flight together.  The weights times the angles are made once for them:
+//   a' = f (a w_a cos - b w_b sin),  b' = f (b w_b cos + a w_a sin)
+// is then four products and a factor for two values, two values to an
+// instruction.  What bounds this is memory: with the products made for each
+// row it was the instructions (280 a row and lane against 90).
+template <typename T, int LANES, int ITER, bool PAIRS>
+__global__ void __launch_bounds__(kRopeWarps * 32) k_rope_rows(RopeParams p, int q_parts) {
+    constexpr int N = Vec16<T>::N, kGroups = 32 / LANES;
     const int lane = threadIdx.x % LANES, group = threadIdx.x % 32 / LANES;
-    constexpr int kGroups = 32 / LANES;
-    const long long item = (long long)blockIdx.x * kRopeWarps + threadIdx.x / 32;
-    if (item >= items) return;
-    const long long token = item / parts;
-    const int first = (int)(item - token * parts) * (kGroups * ITER) + group, all = p.heads + p.kv_heads;
-    const bool pairs = p.layout == VDT_ROPE_PAIRS, in = lane < p.dim / (2 * N);
-    const int turned = p.rot / (2 * N);                    // VDT_ROPE_HALF: lanes that rotate
-    int v0 = 2 * lane, v1 = v0 + 1;                        // the lane's vectors
-    if (!pairs && lane < turned) {
-        v0 = lane;
-        v1 = lane + turned;
-    }
-    const bool t0 = in && v0 * N < p.rot, t1 = in && v1 * N < p.rot;
+    const long long token = (long long)blockIdx.x * kRopeWarps + threadIdx.x / 32;
+    if (token >= p.tokens) return;
+    const bool keys = (int)blockIdx.y >= q_parts;
+    const int first = (blockIdx.y - (keys ? q_parts : 0)) * (kGroups * ITER), all = keys ? p.kv_heads : p.heads;
+    const long long in_step = keys ? p.k_head : p.q_head, out_step = keys ? p.ko_head : p.qo_head;
+    const bool on = lane < p.dim / (2 * N), turned = lane < p.rot / (2 * N);
+    const int v0 = PAIRS || !turned ? 2 * lane : lane, v1 = PAIRS || !turned ? v0 + 1 : lane + p.rot / (2 * N);   // the lane's vectors
+    const T* const in = (keys ? static_cast<const T*>(p.k) + token * p.k_token : static_cast<const T*>(p.q) + token * p.q_token) +
+                        (first + group) * in_step;
+    T* const out = (keys ? static_cast<T*>(p.k_out) + token * p.ko_token : static_cast<T*>(p.q_out) + token * p.qo_token) +
+                   (first + group) * out_step;
     Vec16<T> x[ITER][2];
-    T* to[ITER];
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-        const int h = first + i * kGroups;
-        const RopeRow r = rope_row<T>(p, token, min(h, all - 1));
-        to[i] = h < all ? static_cast<T*>(r.out) : nullptr;
-        const T* from = static_cast<const T*>(r.in);
         x[i][0].raw = x[i][1].raw = make_uint4(0, 0, 0, 0);
-        if (in && h < all) {
+        if (on && first + group + i * kGroups < all) {
+            const T* const from = in + i * kGroups * in_step;
             x[i][0].raw = *reinterpret_cast<const uint4*>(from + v0 * N);
             x[i][1].raw = *reinterpret_cast<const uint4*>(from + v1 * N);
         }
     }
-    // the angles: N of them; with neighbours paired half of them are v0's, half v1's
+    // factors of a and b in a' (the second negative) and of b and a in b'; of
+    // the lanes that do not rotate the first and third are the weights
+    float2 fa[2][N / 2], fb[2][N / 2];
     const int at = p.rot ? p.at[token] : 0;
     const bool known = !p.rot || (at >= 0 && at < p.positions);
-    float c[N], s[N];
     {
-        const float* row = p.table + (long long)(known ? at : 0) * p.rot + lane * N;
+        float w[2][N];
+        const void* const weight = keys ? p.wk : p.wq;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (weight && on) {
+                Vec16<T> v;
+                v.raw = __ldg(reinterpret_cast<const uint4*>(weight) + (e ? v1 : v0));
+                v.get(w[e]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) w[e][j] = 1.0f;
+            }
+        }
+        float c[N], s[N];
+        const float* const row = p.table + (long long)(known ? at : 0) * p.rot + lane * N;
 #pragma unroll
         for (int j = 0; j < N; j += 4) {
-            const bool on = pairs && j >= N / 2 && N > 4 ? t1 : t0;
-            const float4 a = on ? __ldg(reinterpret_cast<const float4*>(row + j)) : make_float4(1, 1, 1, 1);
-            const float4 b = on ? __ldg(reinterpret_cast<const float4*>(row + p.rot / 2 + j)) : make_float4(0, 0, 0, 0);
+            const float4 a = turned ? __ldg(reinterpret_cast<const float4*>(row + j)) : make_float4(1, 1, 1, 1);
+            const float4 b = turned ? __ldg(reinterpret_cast<const float4*>(row + p.rot / 2 + j)) : make_float4(0, 0, 0, 0);
             c[j] = a.x; c[j + 1] = a.y; c[j + 2] = a.z; c[j + 3] = a.w;
             s[j] = b.x; s[j + 1] = b.y; s[j + 2] = b.z; s[j + 3] = b.w;
+        }
+        if (PAIRS) {
+            // a vector's pair (x, y): (x, y) (w_x cos, w_y cos) + (y, x) (-w_y sin, w_x sin)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j) {
+                    const float cj = c[e * N / 2 + j], sj = s[e * N / 2 + j];
+                    fa[e][j] = make_float2(w[e][2 * j] * cj, w[e][2 * j + 1] * cj);
+                    fb[e][j] = make_float2(-w[e][2 * j + 1] * sj, w[e][2 * j] * sj);
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N / 2; ++j) {
+                fa[0][j] = make_float2(w[0][2 * j] * c[2 * j], w[0][2 * j + 1] * c[2 * j + 1]);
+                fb[0][j] = make_float2(-w[1][2 * j] * s[2 * j], -w[1][2 * j + 1] * s[2 * j + 1]);
+                fa[1][j] = make_float2(w[1][2 * j] * c[2 * j], w[1][2 * j + 1] * c[2 * j + 1]);
+                fb[1][j] = make_float2(w[0][2 * j] * s[2 * j], w[0][2 * j + 1] * s[2 * j + 1]);
+            }
         }
     }
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-        float a[N], b[N];
-        x[i][0].get(a);
-        x[i][1].get(b);
-        float sq = 0.0f;
+        if (first + i * kGroups >= all) break;               // of the whole warp
+        float2 a[N / 2], b[N / 2];
+        x[i][0].get(reinterpret_cast<float*>(a));
+        x[i][1].get(reinterpret_cast<float*>(b));
+        float2 sq = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int j = 0; j < N; ++j) sq = fmaf(a[j], a[j], fmaf(b[j], b[j], sq));
+        for (int j = 0; j < N / 2; ++j) sq = fma2(a[j], a[j], fma2(b[j], b[j], sq));
+        float squares = sq.x + sq.y;
 #pragma unroll
-        for (int d = LANES / 2; d; d >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, d);
-        float f = norm_factor(sq, p);
-        if (!known) f = __int_as_float(0x7fffffff);
-        const void* weight = first + i * kGroups < p.heads ? p.wq : p.wk;
-        if (weight && in) {
-            Vec16<T> w;
-            float g[N];
-            w.raw = __ldg(reinterpret_cast<const uint4*>(weight) + v0);
-            w.get(g);
+        for (int d = LANES / 2; d; d >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, d);
+        const float f1 = known ? norm_factor(squares, p) : __int_as_float(0x7fffffff);
+        const float2 f = make_float2(f1, f1);
+        float2 ya[N / 2], yb[N / 2];
+        if (turned) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) a[j] *= f * g[j];
-            w.raw = __ldg(reinterpret_cast<const uint4*>(weight) + v1);
-            w.get(g);
-#pragma unroll
-            for (int j = 0; j < N; ++j) b[j] *= f * g[j];
+            for (int j = 0; j < N / 2; ++j) {
+                const float2 pa = PAIRS ? make_float2(a[j].y, a[j].x) : b[j], pb = PAIRS ? make_float2(b[j].y, b[j].x) : a[j];
+                ya[j] = mul2(f, fma2(pa, fb[0][j], mul2(a[j], fa[0][j])));
+                yb[j] = mul2(f, fma2(pb, fb[1][j], mul2(b[j], fa[1][j])));
+            }
         } else {
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                a[j] *= f;
-                b[j] *= f;
+            for (int j = 0; j < N / 2; ++j) {
+                ya[j] = mul2(f, mul2(a[j], fa[0][j]));
+                yb[j] = mul2(f, mul2(b[j], fa[1][j]));
             }
         }
-        if (pairs) {
-#pragma unroll
-            for (int j = 0; j < N; j += 2) {
-                const float ca = c[j / 2], sa = s[j / 2], cb = c[N / 2 + j / 2], sb = s[N / 2 + j / 2];
-                const float a0 = a[j], b0 = b[j];
-                if (t0) {
-                    a[j] = a0 * ca - a[j + 1] * sa;
-                    a[j + 1] = a[j + 1] * ca + a0 * sa;
-                }
-                if (t1) {
-                    b[j] = b0 * cb - b[j + 1] * sb;
-                    b[j + 1] = b[j + 1] * cb + b0 * sb;
-                }
-            }
-        } else if (t0) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const float a0 = a[j];
-                a[j] = a0 * c[j] - b[j] * s[j];
-                b[j] = b[j] * c[j] + a0 * s[j];
-            }
-        }
-        if (to[i] && in) {
+        if (on && first + group + i * kGroups < all) {
+            T* const to = out + i * kGroups * out_step;
             Vec16<T> y;
-            y.set(a);
-            *reinterpret_cast<uint4*>(to[i] + v0 * N) = y.raw;
-            y.set(b);
-            *reinterpret_cast<uint4*>(to[i] + v1 * N) = y.raw;
+            y.set(reinterpret_cast<const float*>(ya));
+            *reinterpret_cast<uint4*>(to + v0 * N) = y.raw;
+            y.set(reinterpret_cast<const float*>(yb));
+            *reinterpret_cast<uint4*>(to + v1 * N) = y.raw;
         }
     }
 }
 
-// whether every row and weight starts on 16 bytes, and the rotation keeps to whole vectors
+// whether every row and weight starts on 16 bytes, and a lane's two vectors
+// rotate both or neither
 bool whole_vectors(const RopeParams& p) {
     const int n = 16 / type_size(p.type);
-    if (p.dim % (2 * n) || p.dim > 64 * n || p.rot % (p.layout == VDT_ROPE_PAIRS && n == 4 ? 8 : 2 * n)) return false;
+    if (p.dim % (2 * n) || p.dim > 64 * n || p.rot % (2 * n)) return false;
     for (const long long s : {p.q_token, p.q_head, p.k_token, p.k_head, p.qo_token, p.qo_head, p.ko_token, p.ko_head})
         if (s % n) return false;
     for (const void* a : {p.q, p.k, (const void*)p.q_out, (const void*)p.k_out, p.wq, p.wk, (const void*)p.table})
@@ -206,27 +230,19 @@ bool whole_vectors(const RopeParams& p) {
 
 template <typename T, int LANES, int ITER>
 cudaError_t rows_launch(const RopeParams& p, cudaStream_t s) {
-    const int parts = (p.heads + p.kv_heads + 32 / LANES * ITER - 1) / (32 / LANES * ITER);
-    const long long items = p.tokens * parts, grid = (items + kRopeWarps - 1) / kRopeWarps;
-    if (grid > 0x7fffffff) return cudaErrorInvalidValue;
-    k_rope_rows<T, LANES, ITER><<<(unsigned)grid, kRopeWarps * 32, 0, s>>>(p, items, parts);
+    constexpr int kEach = 32 / LANES * ITER;
+    const int q_parts = (p.heads + kEach - 1) / kEach, k_parts = (p.kv_heads + kEach - 1) / kEach;
+    const dim3 grid((unsigned)((p.tokens + kRopeWarps - 1) / kRopeWarps), q_parts + k_parts);
+    if (p.layout == VDT_ROPE_PAIRS) k_rope_rows<T, LANES, ITER, true><<<grid, kRopeWarps * 32, 0, s>>>(p, q_parts);
+    else k_rope_rows<T, LANES, ITER, false><<<grid, kRopeWarps * 32, 0, s>>>(p, q_parts);
     return cudaGetLastError();
 }
 
-// Several rows a lane group where there are enough of them to fill the GPU: as
-// many as leave the fewest places empty at a token's end (40 heads in groups of
-// 4: five rows, twice), of those the most.
+// Four rows a lane group where there are enough of them to fill the GPU
 template <typename T, int LANES>
 cudaError_t by_rows(const RopeParams& p, cudaStream_t s) {
-    const int all = p.heads + p.kv_heads, each = 32 / LANES, turns = (all + each - 1) / each;
-    if (p.tokens * all * LANES < 4LL * 32 * 16 * kSmCount || turns < 2) return rows_launch<T, LANES, 1>(p, s);
-    int best = 2;
-    for (const int n : {3, 4, 5})
-        if ((turns + n - 1) / n * n <= (turns + best - 1) / best * best) best = n;
-    if (best == 2) return rows_launch<T, LANES, 2>(p, s);
-    if (best == 3) return rows_launch<T, LANES, 3>(p, s);
-    if (best == 4) return rows_launch<T, LANES, 4>(p, s);
-    return rows_launch<T, LANES, 5>(p, s);
+    const long long rows = p.tokens * (p.heads + p.kv_heads);
+    return rows * LANES >= 4LL * 32 * 16 * kSmCount ? rows_launch<T, LANES, 4>(p, s) : rows_launch<T, LANES, 1>(p, s);
 }
 
 template <typename T>

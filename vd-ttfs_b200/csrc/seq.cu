@@ -150,6 +150,7 @@ extern "C" int vdt_qk_norm_rope(const void* d_q, int64_t q_token, int64_t q_head
     p.wq = d_q_weight; p.wk = d_k_weight; p.at = d_positions; p.table = d_table;
     p.tokens = tokens; p.positions = positions; p.rot = rot; p.layout = layout; p.norm = norm;
     p.heads = heads; p.kv_heads = kv_heads; p.dim = dim; p.type = type; p.eps = eps;
+    p.share = norm == VDT_NORM_RMS ? 1.0f / (float)dim : 1.0f;
     return launched(launch_qk_norm_rope(p, static_cast<cudaStream_t>(stream)), "qk_norm_rope");
 }
 

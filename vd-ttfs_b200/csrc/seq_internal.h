@@ -9,6 +9,8 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cstring>
+#include <type_traits>
 
 #include "vdt_internal.h"
 
@@ -34,6 +36,33 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// Two 16-bit values of a word as 32-bit ones, and back
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        lo = __uint_as_float(w << 16);
+        hi = __uint_as_float(w & 0xffff0000u);
+    } else {
+        __half2 h;
+        memcpy(&h, &w, 4);
+        const float2 f = __half22float2(h);
+        lo = f.x;
+        hi = f.y;
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t w;
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        memcpy(&w, &h, 4);
+    } else {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        memcpy(&w, &h, 4);
+    }
+    return w;
+}
+
 // 16 bytes of T as 32-bit values, and back
 template <typename T>
 struct Vec16 {
@@ -41,35 +70,18 @@ struct Vec16 {
     uint4 raw;
     __device__ __forceinline__ void get(float* f) const {
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                T lo, hi;
-                const unsigned short a = (unsigned short)(w[i] & 0xffffu), b = (unsigned short)(w[i] >> 16);
-                memcpy(&lo, &a, 2);
-                memcpy(&hi, &b, 2);
-                f[2 * i] = to_f32(lo);
-                f[2 * i + 1] = to_f32(hi);
-            }
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) f[i] = __uint_as_float(w[i]);
+            else unpack2<T>(w[i], f[2 * i], f[2 * i + 1]);
         }
     }
     __device__ __forceinline__ void set(const float* f) {
         uint32_t w[4];
-        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const T lo = from_f32<T>(f[2 * i]), hi = from_f32<T>(f[2 * i + 1]);
-                unsigned short a, b;
-                memcpy(&a, &lo, 2);
-                memcpy(&b, &hi, 2);
-                w[i] = (uint32_t)a | ((uint32_t)b << 16);
-            }
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+            else w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
         }
         raw = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -274,7 +286,7 @@ struct RopeParams {
     const float* table;                 // [positions, rot]: cosines, then sines
     long long tokens;
     int positions, rot, layout, norm, heads, kv_heads, dim, type;
-    float eps;
+    float eps, share;                   // share: 1 / dim for the mean of the squares, 1 for their sum
 };
 cudaError_t launch_qk_norm_rope(const RopeParams& p, cudaStream_t s);
 
