@@ -140,36 +140,73 @@ __global__ void __launch_bounds__(kCacheThreads) k_cache_append_rows(vdt_cache8 
     const T* x = side ? v + o.first * v_token + h * v_head : k + o.first * k_token + h * k_head;
     const long long step = side ? v_token : k_token;
     int8_t* codes = (side ? c.v : c.k) + o.slot * (P * D);
+    // a thread has vector e of tokens t; of values that start a page, four
+    // tokens side by side, whose codes make whole words
+    constexpr bool kFours = kHeld % 4 == 0 && kCacheThreads % kRow == 0;
+    const bool fours = kFours && side && o.old == 0;
+    auto place = [&](int i, int& t, int& e) {
+        const int at = threadIdx.x + i * kCacheThreads;
+        t = at / kRow;
+        e = at % kRow;
+        if (fours) {
+            t = 4 * (threadIdx.x / kRow + i / 4 * (kCacheThreads / kRow)) + i % 4;
+            e = threadIdx.x % kRow;
+        }
+    };
     Vec16<T> held[kHeld];
-    float m = 0.0f;
+    Largest<T> most;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
-        const int at = threadIdx.x + i * kCacheThreads, t = at / kRow, e = at % kRow;
+        int t, e;
+        place(i, t, e);
         held[i].raw = t < o.n ? *reinterpret_cast<const uint4*>(x + t * step + e * N) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        float f[N];
-        held[i].get(f);
+    for (int i = 0; i < kHeld; ++i) most.add(held[i]);
+    const Coder coder(grow(c, o, side, block_max(most.value())));
+    if (fours) {
+        if constexpr (kFours) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) m = max_nan(fabsf(f[j]), m);
-    }
-    const Coder coder(grow(c, o, side, block_max(m)));
+            for (int i = 0; i < kHeld; i += 4) {
+                int t, e;
+                place(i, t, e);
+                uint32_t w[4][N / 4];
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        const int at = threadIdx.x + i * kCacheThreads, t = at / kRow, e = at % kRow;
-        if (t >= o.n) continue;
-        float f[N];
-        uint32_t w[N / 4];
-        held[i].get(f);
-        coder.words<N>(f, w);
-        if (!side) {
-            int8_t* to = codes + (o.old + t) * D + e * N;
-            if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-            else *reinterpret_cast<uint32_t*>(to) = w[0];
-        } else {
+                for (int a = 0; a < 4; ++a) {
+                    float f[N];
+                    held[i + a].get(f);
+                    coder.words<N>(f, w[a]);
+                }
 #pragma unroll
-            for (int j = 0; j < N; ++j) tile[tile_byte<P>(e * N + j, o.old + t)] = (unsigned char)(w[j / 4] >> (8 * (j % 4)));
+                for (int j = 0; j < N; j += 4) {
+                    const uint32_t x0 = w[0][j / 4], x1 = w[1][j / 4], x2 = w[2][j / 4], x3 = w[3][j / 4];
+                    const uint32_t a = __byte_perm(x0, x1, 0x5140), b = __byte_perm(x2, x3, 0x5140);     // dimensions j, j + 1
+                    const uint32_t d = __byte_perm(x0, x1, 0x7362), g = __byte_perm(x2, x3, 0x7362);     // j + 2, j + 3
+                    const uint32_t y[4] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(d, g, 0x5410),
+                                           __byte_perm(d, g, 0x7632)};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) *reinterpret_cast<uint32_t*>(tile + tile_byte<P>(e * N + j + q, t)) = y[q];
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            int t, e;
+            place(i, t, e);
+            if (t >= o.n) continue;
+            float f[N];
+            uint32_t w[N / 4];
+            held[i].get(f);
+            coder.words<N>(f, w);
+            if (!side) {
+                int8_t* to = codes + (o.old + t) * D + e * N;
+                if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint32_t*>(to) = w[0];
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) tile[tile_byte<P>(e * N + j, o.old + t)] = (unsigned char)(w[j / 4] >> (8 * (j % 4)));
+            }
         }
     }
     if (!side) return;
@@ -217,23 +254,38 @@ __global__ void __launch_bounds__(kCacheThreads) k_cache_load(vdt_cache8 c, Cach
         }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < n * kRow; i += kCacheThreads) {
-        const int t = i / kRow, e = i % kRow;
-        float f[N];
-        if (side) {
+    if (side) {
+        // a word is four tokens of a dimension: N of them make four rows' vectors
+        for (int i = threadIdx.x; i < (n + 3) / 4 * kRow; i += kCacheThreads) {
+            const int t = i / kRow * 4, e = i % kRow;
+            uint32_t w[N];
 #pragma unroll
-            for (int q = 0; q < N; ++q) f[q] = (float)(int8_t)tile[tile_byte<P>(e * N + q, t)] * scale;
-        } else {
+            for (int q = 0; q < N; ++q) w[q] = *reinterpret_cast<const uint32_t*>(tile + tile_byte<P>(e * N + q, t)) ^ 0x80808080u;
 #pragma unroll
-            for (int q = 0; q < N; q += 4) {
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(c.k + at + t * D + e * N + q);
+            for (int a = 0; a < 4; ++a) {
+                if (t + a >= n) break;
+                float2 f[N / 2];
 #pragma unroll
-                for (int a = 0; a < 4; ++a) f[q + a] = (float)(int8_t)(w >> (8 * a)) * scale;
+                for (int q = 0; q < N; q += 2) f[q / 2] = code_pair(code_byte(w[q], a), code_byte(w[q + 1], a), scale);
+                Vec16<T> y;
+                y.set(reinterpret_cast<const float*>(f));
+                *reinterpret_cast<uint4*>(v + out + (t + a) * step + e * N) = y.raw;
             }
         }
+        return;
+    }
+    for (int i = threadIdx.x; i < n * kRow; i += kCacheThreads) {
+        const int t = i / kRow, e = i % kRow;
+        float2 f[N / 2];
+#pragma unroll
+        for (int q = 0; q < N; q += 4) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(c.k + at + t * D + e * N + q) ^ 0x80808080u;
+            f[q / 2] = code_pair(code_byte(w, 0), code_byte(w, 1), scale);
+            f[q / 2 + 1] = code_pair(code_byte(w, 2), code_byte(w, 3), scale);
+        }
         Vec16<T> y;
-        y.set(f);
-        *reinterpret_cast<uint4*>((side ? v : k) + out + t * step + e * N) = y.raw;
+        y.set(reinterpret_cast<const float*>(f));
+        *reinterpret_cast<uint4*>(k + out + t * step + e * N) = y.raw;
     }
 }
 

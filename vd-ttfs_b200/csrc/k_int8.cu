@@ -13,53 +13,47 @@ namespace vdt {
 namespace {
 
 // ------------------------------------------------------------------ quantise
-constexpr int kQuantThreads = 256;
-
 // One CTA a row: the largest magnitude, then the codes.  Rows of up to HELD
 // vectors a thread are read once and stay in registers; longer ones, and rows
 // that are not on 16 bytes (HELD 0), are read twice, the second time from L1
-// and L2.
-template <typename T, int HELD>
-__global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T* __restrict__ x, int cols,
+// and L2.  (A warp a row, without barriers, took 46 us for 8192 x 4096 bf16.)
+template <typename T, int HELD, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_quantize_rows(const T* __restrict__ x, int cols,
                                                                  long long x_stride, int8_t* __restrict__ codes,
                                                                  long long codes_stride, float* __restrict__ scale) {
     constexpr int N = Vec16<T>::N;
-    __shared__ float part[kQuantThreads / 32];
+    __shared__ float part[THREADS / 32];
     chain_release();
-    const T* row = x + (long long)blockIdx.x * x_stride;
-    int8_t* out = codes + (long long)blockIdx.x * codes_stride;
+    const long long r = blockIdx.x;
+    const int thread = threadIdx.x;
+    const T* row = x + r * x_stride;
+    int8_t* out = codes + r * codes_stride;
     const int vecs = HELD ? cols / N : 0;
     float m = 0.0f;
+    Largest<T> most;
     Vec16<T> held[HELD ? HELD : 1];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
-        const int at = threadIdx.x + i * kQuantThreads;
+        const int at = thread + i * THREADS;
         held[i].raw = at < vecs ? *reinterpret_cast<const uint4*>(row + (long long)at * N) : make_uint4(0, 0, 0, 0);
     }
-    for (int i = vecs * N + threadIdx.x; i < cols; i += kQuantThreads) m = max_nan(fabsf(to_f32(row[i])), m);
-    for (int i = threadIdx.x + HELD * kQuantThreads; i < vecs; i += kQuantThreads) {
+    for (int i = vecs * N + thread; i < cols; i += THREADS) m = max_nan(fabsf(to_f32(row[i])), m);
+    for (int i = thread + HELD * THREADS; i < vecs; i += THREADS) {
         Vec16<T> v;
         v.raw = *reinterpret_cast<const uint4*>(row + (long long)i * N);
-        float f[N];
-        v.get(f);
-#pragma unroll
-        for (int j = 0; j < N; ++j) m = max_nan(fabsf(f[j]), m);
+        most.add(v);
     }
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        float f[N];
-        held[i].get(f);
-#pragma unroll
-        for (int j = 0; j < N; ++j) m = max_nan(fabsf(f[j]), m);
-    }
+    for (int i = 0; i < HELD; ++i) most.add(held[i]);
+    m = max_nan(most.value(), m);
 #pragma unroll
     for (int d = 16; d; d >>= 1) m = max_nan(__shfl_xor_sync(0xffffffffu, m, d), m);
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = m;
+    if (thread % 32 == 0) part[thread / 32] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kQuantThreads / 32; ++i) m = max_nan(part[i], m);
+    for (int i = 0; i < THREADS / 32; ++i) m = max_nan(part[i], m);
     const Coder coder(m * kCodeStep);
-    if (threadIdx.x == 0) scale[blockIdx.x] = coder.scale;
+    if (thread == 0) scale[r] = coder.scale;
     auto store = [&](const Vec16<T>& v, int at) {
         float f[N];
         uint32_t w[N / 4];
@@ -70,13 +64,13 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantize_rows(const T* __rest
     };
 #pragma unroll
     for (int i = 0; i < HELD; ++i)
-        if ((int)threadIdx.x + i * kQuantThreads < vecs) store(held[i], threadIdx.x + i * kQuantThreads);
-    for (int i = threadIdx.x + HELD * kQuantThreads; i < vecs; i += kQuantThreads) {
+        if (thread + i * THREADS < vecs) store(held[i], thread + i * THREADS);
+    for (int i = thread + HELD * THREADS; i < vecs; i += THREADS) {
         Vec16<T> v;
         v.raw = *reinterpret_cast<const uint4*>(row + (long long)i * N);
         store(v, i);
     }
-    for (int i = vecs * N + threadIdx.x; i < cols; i += kQuantThreads) out[i] = (int8_t)code_of(to_f32(row[i]), coder.scale);
+    for (int i = vecs * N + thread; i < cols; i += THREADS) out[i] = (int8_t)code_of(to_f32(row[i]), coder.scale);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -443,9 +437,20 @@ cudaError_t quant_launch(const void* x, long long rows, int cols, long long x_st
     const bool vec = aligned(x, 16) && (x_stride * (long long)sizeof(T)) % 16 == 0 && aligned(codes, N) &&
                      codes_stride % N == 0;
     const T* in = static_cast<const T*>(x);
-    const int each = (cols / N + kQuantThreads - 1) / kQuantThreads;       // vectors a thread
-    auto kern = !vec ? k_quantize_rows<T, 0> : each <= 1 ? k_quantize_rows<T, 1> : each <= 2 ? k_quantize_rows<T, 2> : k_quantize_rows<T, 4>;
-    kern<<<(unsigned)rows, kQuantThreads, 0, s>>>(in, cols, x_stride, codes, codes_stride, scale);
+    // many rows: 128 threads each, so that more rows are under way (8192 x 4096
+    // bf16: 29 us against 33 with 256); few: 256, for the latency
+    auto go = [&](auto threads) {
+        constexpr int kThreads = threads();
+        const int each = (cols / N + kThreads - 1) / kThreads;             // vectors a thread
+        auto kern = !vec        ? k_quantize_rows<T, 0, kThreads>
+                    : each <= 1 ? k_quantize_rows<T, 1, kThreads>
+                    : each <= 2 ? k_quantize_rows<T, 2, kThreads>
+                    : each <= 4 ? k_quantize_rows<T, 4, kThreads>
+                                : k_quantize_rows<T, 8, kThreads>;
+        kern<<<(unsigned)rows, kThreads, 0, s>>>(in, cols, x_stride, codes, codes_stride, scale);
+    };
+    if (rows >= 8 * kSmCount) go(std::integral_constant<int, 128>{});
+    else go(std::integral_constant<int, 256>{});
     return cudaGetLastError();
 }
 

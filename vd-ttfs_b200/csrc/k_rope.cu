@@ -79,21 +79,6 @@ __global__ void __launch_bounds__(kRopeWarps * 32) k_rope_any(RopeParams p) {
     }
 }
 
-// Two independent 32-bit multiplications, or multiply-adds
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
-        "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-
 // Rows of whole 16-byte vectors: LANES lanes a row, a lane two vectors that
 // hold each other's partners (half a rotation apart, or neighbours), so the
 // rotation stays in the lane.  A warp takes one token and up to ITER heads of
@@ -112,8 +97,10 @@ __global__ void __launch_bounds__(kRopeWarps * 32) k_rope_rows(RopeParams p, int
     const bool keys = (int)blockIdx.y >= q_parts;
     const int first = (blockIdx.y - (keys ? q_parts : 0)) * (kGroups * ITER), all = keys ? p.kv_heads : p.heads;
     const long long in_step = keys ? p.k_head : p.q_head, out_step = keys ? p.ko_head : p.qo_head;
-    const bool on = lane < p.dim / (2 * N), turned = lane < p.rot / (2 * N);
-    const int v0 = PAIRS || !turned ? 2 * lane : lane, v1 = PAIRS || !turned ? v0 + 1 : lane + p.rot / (2 * N);   // the lane's vectors
+    // the lane's vectors: lanes side by side take vectors side by side
+    const int half = p.rot / (2 * N), rest = p.dim / (2 * N) - half;
+    const bool on = lane < half + rest, turned = lane < half;
+    const int v0 = turned ? lane : half + lane, v1 = v0 + (turned ? half : rest);
     const T* const in = (keys ? static_cast<const T*>(p.k) + token * p.k_token : static_cast<const T*>(p.q) + token * p.q_token) +
                         (first + group) * in_step;
     T* const out = (keys ? static_cast<T*>(p.k_out) + token * p.ko_token : static_cast<T*>(p.q_out) + token * p.qo_token) +
@@ -147,14 +134,30 @@ __global__ void __launch_bounds__(kRopeWarps * 32) k_rope_rows(RopeParams p, int
                 for (int j = 0; j < N; ++j) w[e][j] = 1.0f;
             }
         }
+        // the angles: N, of values 0..N - 1 of a; with neighbours paired N / 2 of
+        // a's pairs and N / 2 of b's
         float c[N], s[N];
-        const float* const row = p.table + (long long)(known ? at : 0) * p.rot + lane * N;
+        const float* const row = p.table + (long long)(known ? at : 0) * p.rot;
+        constexpr int kRun = PAIRS && N == 4 ? 2 : 4;
 #pragma unroll
-        for (int j = 0; j < N; j += 4) {
-            const float4 a = turned ? __ldg(reinterpret_cast<const float4*>(row + j)) : make_float4(1, 1, 1, 1);
-            const float4 b = turned ? __ldg(reinterpret_cast<const float4*>(row + p.rot / 2 + j)) : make_float4(0, 0, 0, 0);
-            c[j] = a.x; c[j + 1] = a.y; c[j + 2] = a.z; c[j + 3] = a.w;
-            s[j] = b.x; s[j + 1] = b.y; s[j + 2] = b.z; s[j + 3] = b.w;
+        for (int j = 0; j < N; j += kRun) {
+            const int from = !PAIRS ? lane * N + j : j < N / 2 ? v0 * (N / 2) + j : v1 * (N / 2) + j - N / 2;
+#pragma unroll
+            for (int q = 0; q < kRun; ++q) {
+                c[j + q] = 1.0f;
+                s[j + q] = 0.0f;
+            }
+            if (turned) {
+                if constexpr (kRun == 4) {
+                    const float4 a = __ldg(reinterpret_cast<const float4*>(row + from)), b = __ldg(reinterpret_cast<const float4*>(row + p.rot / 2 + from));
+                    c[j] = a.x; c[j + 1] = a.y; c[j + 2] = a.z; c[j + 3] = a.w;
+                    s[j] = b.x; s[j + 1] = b.y; s[j + 2] = b.z; s[j + 3] = b.w;
+                } else {
+                    const float2 a = __ldg(reinterpret_cast<const float2*>(row + from)), b = __ldg(reinterpret_cast<const float2*>(row + p.rot / 2 + from));
+                    c[j] = a.x; c[j + 1] = a.y;
+                    s[j] = b.x; s[j + 1] = b.y;
+                }
+            }
         }
         if (PAIRS) {
             // a vector's pair (x, y): (x, y) (w_x cos, w_y cos) + (y, x) (-w_y sin, w_x sin)

@@ -87,14 +87,60 @@ struct Vec16 {
     }
 };
 
+// Two independent 32-bit multiplications, or multiply-adds
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 // The larger of two magnitudes; NaN wins, so that a row with a NaN gets a NaN scale
 __device__ __forceinline__ float max_nan(float a, float b) { return (a > b || a != a) ? a : b; }
+
+// The largest magnitude of many values: magnitudes order as their bits do, NaN
+// above infinity.  16-bit values two to a word.
+template <typename T>
+struct Largest {
+    uint32_t bits = 0;
+    __device__ __forceinline__ void add(const Vec16<T>& v) {
+        const uint32_t w[4] = {v.raw.x, v.raw.y, v.raw.z, v.raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) bits = max(bits, w[i] & 0x7fffffffu);
+            else bits = __vmaxu2(bits, w[i] & 0x7fff7fffu);
+        }
+    }
+    __device__ __forceinline__ float value() const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(bits);
+        } else {
+            float lo, hi;
+            unpack2<T>(bits, lo, hi);
+            return max_nan(lo, hi);
+        }
+    }
+};
 
 // One value's code: x / scale rounded to the nearest whole number, ties to
 // even (the division is the IEEE one: a host that restates it gets the same
 // codes).  A scale of 0 (nothing but zeros, or values below the smallest
 // scale) leaves the value undivided, which rounds to 0; NaN rounds to 0.
-__device__ __forceinline__ int code_of(float x, float scale) {
+static __device__ __noinline__ int code_of(float x, float scale) {
     const float q = rintf(__fdiv_rn(x, scale > 0.0f ? scale : 1.0f));
     return q != q ? 0 : (int)fminf(fmaxf(q, -127.0f), 127.0f);
 }
@@ -110,27 +156,39 @@ struct Coder {
     template <int N>
     __device__ __forceinline__ void words(const float* f, uint32_t* w) const {
         // 1.5 * 2^23 added: the nearest whole number, ties to even, in the low bits
-        constexpr float kRound = 12582912.0f;
+        const float2 round = make_float2(12582912.0f, 12582912.0f), by = make_float2(inverse, inverse);
         float near = 0.0f;
 #pragma unroll
         for (int j = 0; j < N; j += 4) {
             uint32_t c[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float q = f[j + i] * inverse, r = q + kRound;
-                near = fmaxf(near, fabsf(q - (r - kRound)));
-                c[i] = __float_as_uint(r);
+            for (int i = 0; i < 4; i += 2) {
+                const float2 x = make_float2(f[j + i], f[j + i + 1]), r = fma2(x, by, round);
+                const float2 n = add2(r, make_float2(-round.x, -round.y)), off = fma2(x, by, make_float2(-n.x, -n.y));
+                near = fmaxf(near, fmaxf(fabsf(off.x), fabsf(off.y)));
+                c[i] = __float_as_uint(r.x);
+                c[i + 1] = __float_as_uint(r.y);
             }
             w[j / 4] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
         }
         if (!exact || near > 0.5f - 1.0f / 32768) {
 #pragma unroll
-            for (int j = 0; j < N; j += 4)
-                w[j / 4] = (code_of(f[j], scale) & 255) | (code_of(f[j + 1], scale) & 255) << 8 | (code_of(f[j + 2], scale) & 255) << 16 |
-                           (uint32_t)code_of(f[j + 3], scale) << 24;
+            for (int j = 0; j < N; j += 4) {
+                w[j / 4] = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[j / 4] |= (uint32_t)(code_of(f[j + i], scale) & 255) << (8 * i);
+            }
         }
     }
 };
+
+// Four codes of a word, or of one byte of four words, as 32-bit values times a
+// scale: code + 128 in the low bits of 2^23, less 2^23 + 128.
+__device__ __forceinline__ float2 code_pair(uint32_t lo, uint32_t hi, float scale) {
+    const float2 x = add2(make_float2(__uint_as_float(lo), __uint_as_float(hi)), make_float2(-8388736.0f, -8388736.0f));
+    return mul2(x, make_float2(scale, scale));
+}
+__device__ __forceinline__ uint32_t code_byte(uint32_t w, int i) { return __byte_perm(w, 0x4b000000u, 0x7440 | i); }   // w with its signs flipped
 
 // A launch that may start while the kernel before it on the stream ends; the
 // kernel calls chain_wait() before it reads what that one wrote.
