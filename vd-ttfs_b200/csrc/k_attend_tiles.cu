@@ -287,10 +287,14 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
                         for (int i = 0; i < kHold; ++i) r[i / 32][i % 32] = from + i < left ? r[i / 32][i % 32] : 0xff800000u;
 #pragma unroll
                     for (int i = 0; i < kHold; i += P < 32 ? P : 32) {
-                        float m = __uint_as_float(r[i / 32][i % 32]);
+                        constexpr int kRun = P < 32 ? P : 32;          // in four chains
+                        float m[4];
 #pragma unroll
-                        for (int q = 1; q < (P < 32 ? P : 32); ++q) m = fmaxf(m, __uint_as_float(r[i / 32][i % 32 + q]));
-                        top = fmaxf(top, m * c[(from + i) / P]);
+                        for (int q = 0; q < kRun; ++q) {
+                            const float x = __uint_as_float(r[i / 32][i % 32 + q]);
+                            m[q % 4] = q < 4 ? x : fmaxf(m[q % 4], x);
+                        }
+                        top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * c[(from + i) / P]);
                     }
                 }
                 const float v_most = st.v_most[slot];
@@ -330,21 +334,21 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
                         float f = st.v_log[slot][i] - v_shift;
                         f = f < -100.0f ? -100.0f : f;
                         const float d = shift + f;
-                        float l0 = 0.0f, l1 = 0.0f;
+                        const float2 by = make_float2(c[i], c[i]), add = make_float2(d, d);
+                        float2 l[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                         for (int a = i * P; a < (i + 1) * P; a += 2) {
                             const int q = a - from;
-                            float x = exp2_fast(fmaf(__uint_as_float(r[q / 32][q % 32]), c[i], d));
-                            float y = exp2_fast(fmaf(__uint_as_float(r[q / 32][q % 32 + 1]), c[i], d));
+                            float2 x = fma2(make_float2(__uint_as_float(r[q / 32][q % 32]), __uint_as_float(r[q / 32][q % 32 + 1])), by, add);
+                            x = make_float2(exp2_fast(x.x), exp2_fast(x.y));
                             if (partial) {                             // also for scales that are not numbers
-                                x = a < left ? x : 0.0f;
-                                y = a + 1 < left ? y : 0.0f;
+                                x.x = a < left ? x.x : 0.0f;
+                                x.y = a + 1 < left ? x.y : 0.0f;
                             }
-                            l0 += x;
-                            l1 += y;
-                            r[q / 64][q / 2 % 32] = pack_f16(x, y);
+                            l[a / 2 % 2] = add2(l[a / 2 % 2], x);
+                            r[q / 64][q / 2 % 32] = pack_f16(x.x, x.y);
                         }
-                        l0 += l1;
+                        const float l0 = (l[0].x + l[1].x) + (l[0].y + l[1].y);
                         sum = partial && i * P >= left ? sum : fmaf(l0, exp2_fast(-f), sum);
                     }
 #pragma unroll

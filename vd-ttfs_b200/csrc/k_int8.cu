@@ -335,25 +335,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_int8_tiles(const __grid_con
                     }
                 }
                 __syncwarp();
-                // eight lanes write a row's 128 bytes
-                const int col = col0 + b * kCols + lane % 8 * kPer;
+                const int col1 = col0 + b * kCols;
+                if (wide && col1 + kCols <= p.cols) {
+                    // eight lanes write a row's 128 bytes
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int r = k * 4 + lane / 8;
-                    const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((lane % 8 ^ (r & 7)) << 4));
-                    const long long row = row0 + r;
-                    if (row < p.rows && col < p.cols) {
-                        T* to = out + row * p.out_stride + col;
-                        if (wide && col + kPer <= p.cols) {
-                            *reinterpret_cast<uint4*>(to) = v;
-                        } else {
-                            T t[kPer];
-                            memcpy(t, &v, 16);
-#pragma unroll
-                            for (int j = 0; j < kPer; ++j)
-                                if (col + j < p.cols) to[j] = t[j];
-                        }
+                    for (int k = 0; k < 8; ++k) {
+                        const int r = k * 4 + lane / 8;
+                        const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((lane % 8 ^ (r & 7)) << 4));
+                        if (row0 + r < p.rows) *reinterpret_cast<uint4*>(out + (row0 + r) * p.out_stride + col1 + lane % 8 * kPer) = v;
                     }
+                } else {
+                    // rows that do not start on 16 bytes, or end in this block: value by value
+                    for (int r = 0; r < 32 && row0 + r < p.rows; ++r)
+#pragma unroll
+                        for (int c = lane; c < kCols; c += 32) {
+                            const int at = c * (int)sizeof(T);
+                            if (col1 + c < p.cols)
+                                out[(row0 + r) * p.out_stride + col1 + c] =
+                                    *reinterpret_cast<const T*>(stage + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15));
+                        }
                 }
                 __syncwarp();
             }
