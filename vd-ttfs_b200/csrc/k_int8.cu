@@ -37,7 +37,17 @@ __global__ void __launch_bounds__(THREADS) k_quantize_rows(const T* __restrict__
         const int at = thread + i * THREADS;
         held[i].raw = at < vecs ? *reinterpret_cast<const uint4*>(row + (long long)at * N) : make_uint4(0, 0, 0, 0);
     }
-    for (int i = vecs * N + thread; i < cols; i += THREADS) m = max_nan(fabsf(to_f32(row[i])), m);
+    // single values: what is left of the vectors, or the whole row
+    constexpr int kSingle = HELD ? 1 : 8;
+    T single[kSingle];
+#pragma unroll
+    for (int i = 0; i < kSingle; ++i) {
+        const int at = vecs * N + thread + i * THREADS;
+        single[i] = at < cols ? row[at] : from_f32<T>(0.0f);
+    }
+    for (int i = vecs * N + thread + kSingle * THREADS; i < cols; i += THREADS) m = max_nan(fabsf(to_f32(row[i])), m);
+#pragma unroll
+    for (int i = 0; i < kSingle; ++i) m = max_nan(fabsf(to_f32(single[i])), m);
     for (int i = thread + HELD * THREADS; i < vecs; i += THREADS) {
         Vec16<T> v;
         v.raw = *reinterpret_cast<const uint4*>(row + (long long)i * N);
@@ -70,7 +80,14 @@ __global__ void __launch_bounds__(THREADS) k_quantize_rows(const T* __restrict__
         v.raw = *reinterpret_cast<const uint4*>(row + (long long)i * N);
         store(v, i);
     }
-    for (int i = vecs * N + thread; i < cols; i += THREADS) out[i] = (int8_t)code_of(to_f32(row[i]), coder.scale);
+    auto put = [&](T x, int at) {
+        const float q = to_f32(x) * coder.inverse, n = rintf(q);
+        out[at] = (int8_t)(coder.exact && fabsf(q - n) <= 0.5f - 1.0f / 32768 ? (int)n : code_of(to_f32(x), coder.scale));
+    };
+#pragma unroll
+    for (int i = 0; i < kSingle; ++i)
+        if (vecs * N + thread + i * THREADS < cols) put(single[i], vecs * N + thread + i * THREADS);
+    for (int i = vecs * N + thread + kSingle * THREADS; i < cols; i += THREADS) put(row[i], i);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -346,13 +363,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_int8_tiles(const __grid_con
                     }
                 } else {
                     // rows that do not start on 16 bytes, or end in this block: value by value
-                    for (int r = 0; r < 32 && row0 + r < p.rows; ++r)
+                    T* const to = out + row0 * p.out_stride + col1;
+#pragma unroll 8
+                    for (int r = 0; r < 32; ++r)
 #pragma unroll
                         for (int c = lane; c < kCols; c += 32) {
                             const int at = c * (int)sizeof(T);
-                            if (col1 + c < p.cols)
-                                out[(row0 + r) * p.out_stride + col1 + c] =
-                                    *reinterpret_cast<const T*>(stage + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15));
+                            const T x = *reinterpret_cast<const T*>(stage + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15));
+                            if (row0 + r < p.rows && col1 + c < p.cols) to[r * p.out_stride + c] = x;
                         }
                 }
                 __syncwarp();
