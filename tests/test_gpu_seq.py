@@ -614,3 +614,52 @@ def test_the_operators_replay_in_a_graph(S):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+# --------------------------------------------------------------- refusals --
+def test_tensors_that_do_not_fit_are_refused(S):
+    """Before any launch, with ValueError (a tensor's shape, type or place) or TypeError (no tensor at all)."""
+    x = torch.zeros(4, 32, device="cuda")
+    w, ws = S.quantize_rows(torch.ones(8, 32, device="cuda"))
+    cache = make_cache(S, 4, 2, 64, 16)
+    q = torch.zeros(2, 4, 64, dtype=torch.float16, device="cuda")
+    one, starts = ints([1]), ints([0, 2])
+    table = ints([[0]])
+    rope = S.rope_table(8, 64)
+    bad = [
+        lambda: S.quantize_rows(x.cpu()), lambda: S.quantize_rows(x.int()), lambda: S.quantize_rows(x[0]), lambda: S.quantize_rows(x[:, :0]),
+        lambda: S.int8_linear(x[:, :31], w, ws), lambda: S.int8_linear(x, w.float(), ws), lambda: S.int8_linear(x, w, ws[:7]),
+        lambda: S.int8_linear(x, w, ws, ws.half()), lambda: S.int8_linear(x, w, ws, out=torch.empty(4, 7, device="cuda")),
+        lambda: S.int8_linear(x, w, ws, out_dtype=torch.int32), lambda: S.int8_linear(x, w[:, 1:], ws),
+        lambda: S.int8_linear(x[:, :20], torch.zeros(8, 20, dtype=torch.int8, device="cuda"), ws),       # rows 20 bytes apart
+        lambda: S.int8_matmul(w[:, :20].contiguous(), ws, w[:, :20], ws),
+        lambda: S.qk_norm_rope(q, q[:1], None, None, ints([0, 1]), rope), lambda: S.qk_norm_rope(q, q.float(), None, None, ints([0, 1]), rope),
+        lambda: S.qk_norm_rope(q, None, q[0, 0, :63], None, ints([0, 1]), rope), lambda: S.qk_norm_rope(q, None, None, None, ints([0]), rope),
+        lambda: S.qk_norm_rope(q, None, None, None, ints([0, 1]), rope, norm="layer"), lambda: S.qk_norm_rope(q.transpose(1, 2), None, None, None, None, None),
+        lambda: S.rope_table(8, 64, scaling="more"),
+        lambda: S.cache_append(cache, q[:, :2], q[:, :1], table, one, starts, 2), lambda: S.cache_append(cache, q, q, table, one, starts, 2),
+        lambda: S.cache_append(cache, q[:, :2], q[:, :2], table, starts, starts, 2), lambda: S.cache_append(cache, q[:, :2], q[:, :2], table.long(), one, starts, 2),
+        lambda: S.cache_load(cache, table, one, starts, -1, 1), lambda: S.cache_load(cache, table, one, starts, 2, 1, torch.int8),
+        lambda: S.cache_attention(q[..., :32], cache, table, one, starts, 2, 16), lambda: S.cache_attention(q, cache, table, one, starts[:1], 2, 16),
+        lambda: S.cache_attention(q, (cache[0], cache[0], cache[2], cache[3]), table, one, starts, 2, 16),
+        lambda: S.cache_attention(q, cache, table, one, starts, 2, 16, out=q.bfloat16()),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")
+    for call in (lambda: S.quantize_rows(3), lambda: S.cache_attention(q, cache[:3], table, one, starts, 2, 16), lambda: S.int8_linear(x, w, ws, out_dtype=3)):
+        with pytest.raises(TypeError):
+            call()
+
+
+def test_what_the_library_refuses_raises_its_error(S):
+    from vdttfs._lib import VdtError
+    cache = make_cache(S, 4, 2, 64, 16)
+    q = torch.zeros(2, 4, 64, device="cuda")
+    args = (ints([[0]]), ints([1]), ints([0, 2]), 2, 16)
+    for call, status in ((lambda: S.cache_attention(q, cache, *args), 5), (lambda: S.cache_attention(q[:, :3].half(), cache, *args), 1),
+                         (lambda: S.cache_attention(q.half(), cache, *args, scale=math.inf), 1), (lambda: S.rope_table(4, 3), 1)):
+        with pytest.raises(VdtError) as e:
+            call()
+        assert e.value.status == status

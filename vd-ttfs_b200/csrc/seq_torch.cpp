@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <initializer_list>
+#include <string>
 
 #include "vdttfs.h"
 
@@ -22,9 +23,32 @@ using at::Tensor;
 
 const Tensor kNone;
 
+// ---------------------------------------------------------------- messages --
+// Put together without streams: a message with a number in it, formatted through
+// c10::str's std::ostream, ended the process (SIGSEGV) once CUDA was initialised,
+// and not before; why is not known.
+std::string show(const char* x) { return x; }
+std::string show(int64_t x) { return std::to_string(x); }
+std::string show(int x) { return std::to_string(x); }
+std::string show(at::ScalarType x) { return c10::toString(x); }
+std::string show(at::Device x) { return x.is_cuda() ? "cuda:" + std::to_string((int)x.index()) : "another device"; }
+std::string show(at::IntArrayRef x) {
+    std::string s = "[";
+    for (size_t i = 0; i < x.size(); ++i) s += (i ? ", " : "") + std::to_string(x[i]);
+    return s + "]";
+}
+template <typename... Parts>
+std::string text(const Parts&... parts) {
+    std::string s;
+    ((s += show(parts)), ...);
+    return s;
+}
+#define CHECK_VALUE(cond, ...) TORCH_CHECK_VALUE(cond, text(__VA_ARGS__))
+#define CHECK_TYPE(cond, ...) TORCH_CHECK_TYPE(cond, text(__VA_ARGS__))
+
 // ------------------------------------------------------------- arguments --
 const Tensor& tensor(PyObject* o, const char* what) {
-    TORCH_CHECK_TYPE(THPVariable_Check(o), what, ": a tensor is wanted, got ", Py_TYPE(o)->tp_name);
+    CHECK_TYPE(THPVariable_Check(o), what, ": a tensor is wanted, got ", Py_TYPE(o)->tp_name);
     return THPVariable_Unpack(o);
 }
 const Tensor& tensor_or_none(PyObject* o, const char* what) { return o == Py_None ? kNone : tensor(o, what); }
@@ -33,20 +57,20 @@ int64_t integer(PyObject* o, const char* what) {
     const long long v = PyLong_AsLongLong(o);
     if (v == -1 && PyErr_Occurred()) {
         PyErr_Clear();
-        TORCH_CHECK_TYPE(false, what, ": a whole number is wanted");
+        CHECK_TYPE(false, what, ": a whole number is wanted");
     }
     return v;
 }
 int small_integer(PyObject* o, const char* what) {
     const int64_t v = integer(o, what);
-    TORCH_CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, what, ": out of range");
+    CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, what, ": out of range");
     return (int)v;
 }
 double number(PyObject* o, const char* what) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) {
         PyErr_Clear();
-        TORCH_CHECK_TYPE(false, what, ": a number is wanted");
+        CHECK_TYPE(false, what, ": a number is wanted");
     }
     return v;
 }
@@ -55,26 +79,26 @@ bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
 int type_of(at::ScalarType t, const char* what) {
     if (t == at::kBFloat16) return VDT_BF16;
     if (t == at::kHalf) return VDT_F16;
-    TORCH_CHECK_VALUE(t == at::kFloat, what, ": float32, float16 or bfloat16 is wanted, got ", t);
+    CHECK_VALUE(t == at::kFloat, what, ": float32, float16 or bfloat16 is wanted, got ", t);
     return VDT_F32;
 }
 at::ScalarType dtype(PyObject* o, const char* what) {
-    TORCH_CHECK_TYPE(THPDtype_Check(o), what, ": a torch dtype is wanted");
+    CHECK_TYPE(THPDtype_Check(o), what, ": a torch dtype is wanted");
     return reinterpret_cast<THPDtype*>(o)->scalar_type;
 }
 
 void on_device(const Tensor& t, const char* what, int64_t dims) {
-    TORCH_CHECK_VALUE(t.is_cuda(), what, ": a CUDA tensor is wanted");
-    TORCH_CHECK_VALUE(t.dim() == dims, what, ": ", dims, " dimensions are wanted, got ", t.sizes());
+    CHECK_VALUE(t.is_cuda(), what, ": a CUDA tensor is wanted");
+    CHECK_VALUE(t.dim() == dims, what, ": ", dims, " dimensions are wanted, got ", t.sizes());
 }
 void flat(const Tensor& t, const char* what, at::ScalarType type, int64_t n) {
-    TORCH_CHECK_VALUE(t.is_cuda() && t.scalar_type() == type && t.numel() == n && t.is_contiguous(), what, ": ", n,
+    CHECK_VALUE(t.is_cuda() && t.scalar_type() == type && t.numel() == n && t.is_contiguous(), what, ": ", n,
                       " contiguous CUDA values of ", type, " are wanted, got ", t.sizes(), " of ", t.scalar_type(), " on ", t.device());
 }
 void heads(const Tensor& t, const char* what, int64_t dim) {
     on_device(t, what, 3);
-    TORCH_CHECK_VALUE(dim < 0 || t.size(2) == dim, what, ": heads of ", dim, " are wanted, got ", t.sizes());
-    TORCH_CHECK_VALUE(t.size(2) == 1 || t.stride(2) == 1, what, ": a head's values must be consecutive");
+    CHECK_VALUE(dim < 0 || t.size(2) == dim, what, ": heads of ", dim, " are wanted, got ", t.sizes());
+    CHECK_VALUE(t.size(2) == 1 || t.stride(2) == 1, what, ": a head's values must be consecutive");
 }
 
 Tensor room(at::IntArrayRef size, at::ScalarType type, at::Device device) {
@@ -87,7 +111,7 @@ void* stream_of(PyObject* o, at::Device device, std::initializer_list<const Tens
     void* handle = PyLong_AsVoidPtr(o);
     if (!handle && PyErr_Occurred()) {
         PyErr_Clear();
-        TORCH_CHECK_TYPE(false, "stream: a raw handle is wanted");
+        CHECK_TYPE(false, "stream: a raw handle is wanted");
     }
     const auto s = handle ? c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(handle), device.index())
                           : c10::cuda::getDefaultCUDAStream(device.index());
@@ -138,13 +162,13 @@ bool arguments(Py_ssize_t n, Py_ssize_t want) {
 // --------------------------------------------------------- 8-bit product --
 void code_rows(const Tensor& t, const char* what) {
     on_device(t, what, 2);
-    TORCH_CHECK_VALUE(t.scalar_type() == at::kChar, what, ": int8 is wanted, got ", t.scalar_type());
+    CHECK_VALUE(t.scalar_type() == at::kChar, what, ": int8 is wanted, got ", t.scalar_type());
     const int64_t n = t.size(0), k = t.size(1);
-    TORCH_CHECK_VALUE(k > 0 && t.stride(1) == 1 && (n <= 1 || t.stride(0) >= k) && t.stride(0) % 16 == 0 &&
+    CHECK_VALUE(k > 0 && t.stride(1) == 1 && (n <= 1 || t.stride(0) >= k) && t.stride(0) % 16 == 0 &&
                           reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
                       what, ": rows that start on 16-byte boundaries are wanted (see quantize_rows), got ", t.sizes(), ", strides ",
                       t.strides());
-    TORCH_CHECK_VALUE(!n || t.storage_offset() + (n - 1) * t.stride(0) + (k + 15) / 16 * 16 <= (int64_t)t.storage().nbytes(), what,
+    CHECK_VALUE(!n || t.storage_offset() + (n - 1) * t.stride(0) + (k + 15) / 16 * 16 <= (int64_t)t.storage().nbytes(), what,
                       ": the last row's storage must reach to the next multiple of 16 bytes");
 }
 int64_t row_stride(const Tensor& t) { return std::max(t.stride(0), (t.size(1) + 15) / 16 * 16); }
@@ -154,12 +178,12 @@ Tensor product_out(int64_t rows, int64_t inner, const Tensor& w, const Tensor& w
                    at::ScalarType type) {
     code_rows(w, "w");
     const int64_t n = w.size(0);
-    TORCH_CHECK_VALUE(n > 0 && inner == w.size(1), "rows of ", inner, " and weights ", w.sizes(), " do not multiply");
+    CHECK_VALUE(n > 0 && inner == w.size(1), "rows of ", inner, " and weights ", w.sizes(), " do not multiply");
     flat(w_scale, "w_scale", at::kFloat, n);
     if (bias.defined()) flat(bias, "bias", at::kFloat, n);
     if (!out.defined()) return room({rows, n}, type, w.device());
     on_device(out, "out", 2);
-    TORCH_CHECK_VALUE(out.size(0) == rows && out.size(1) == n && (n == 1 || out.stride(1) == 1) && (rows <= 1 || out.stride(0) >= n),
+    CHECK_VALUE(out.size(0) == rows && out.size(1) == n && (n == 1 || out.stride(1) == 1) && (rows <= 1 || out.stride(0) >= n),
                       "out: [", rows, ", ", n, "] with consecutive columns is wanted, got ", out.sizes(), ", strides ", out.strides());
     return out;
 }
@@ -171,7 +195,7 @@ PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t count) {
     on_device(x, "x", 2);
     const int type = type_of(x.scalar_type(), "x");
     const int64_t rows = x.size(0), cols = x.size(1);
-    TORCH_CHECK_VALUE(cols > 0 && cols <= INT32_MAX, "x: no columns, or too many");
+    CHECK_VALUE(cols > 0 && cols <= INT32_MAX, "x: no columns, or too many");
     if (x.stride(1) != 1 || (rows > 1 && x.stride(0) < cols)) x = x.contiguous();
     const int64_t step = (cols + 15) / 16 * 16;
     const Tensor codes = room({rows, step}, at::kChar, x.device()), scale = room({rows}, at::kFloat, x.device());
@@ -241,7 +265,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const int type = type_of(q.scalar_type(), "q");
     if (k.defined()) {
         heads(k, "k", dim);
-        TORCH_CHECK_VALUE(k.size(0) == tokens && k.scalar_type() == q.scalar_type(), "k: ", tokens, " tokens of ", q.scalar_type(),
+        CHECK_VALUE(k.size(0) == tokens && k.scalar_type() == q.scalar_type(), "k: ", tokens, " tokens of ", q.scalar_type(),
                           " are wanted, got ", k.sizes(), " of ", k.scalar_type());
     }
     if (wq.defined()) flat(wq, "q_weight", q.scalar_type(), dim);
@@ -264,9 +288,9 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
             out[i] = room(in[i]->sizes(), q.scalar_type(), q.device());
         } else {
             out[i] = *given[i];
-            TORCH_CHECK_VALUE(out[i].defined(), "out: a pair is wanted");
+            CHECK_VALUE(out[i].defined(), "out: a pair is wanted");
             heads(out[i], "out", dim);
-            TORCH_CHECK_VALUE(out[i].sizes() == in[i]->sizes() && out[i].scalar_type() == q.scalar_type(), "out: ", in[i]->sizes(), " of ",
+            CHECK_VALUE(out[i].sizes() == in[i]->sizes() && out[i].scalar_type() == q.scalar_type(), "out: ", in[i]->sizes(), " of ",
                               q.scalar_type(), " is wanted");
         }
     }
@@ -290,7 +314,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
 
 // ------------------------------------------------------------- the cache --
 vdt_cache8 cache_of(PyObject* o) {
-    TORCH_CHECK_TYPE(PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 4, "cache: a tuple of keys, values and their scales is wanted");
+    CHECK_TYPE(PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 4, "cache: a tuple of keys, values and their scales is wanted");
     const Tensor &k = tensor(PyTuple_GET_ITEM(o, 0), "cache keys"), &v = tensor(PyTuple_GET_ITEM(o, 1), "cache values");
     const Tensor &ks = tensor(PyTuple_GET_ITEM(o, 2), "cache key scales"), &vs = tensor(PyTuple_GET_ITEM(o, 3), "cache value scales");
     on_device(k, "cache keys", 4);
@@ -298,11 +322,11 @@ vdt_cache8 cache_of(PyObject* o) {
     const int64_t pages = k.size(0), n = k.size(1), page = k.size(2), dim = k.size(3);
     flat(k, "cache keys", at::kChar, k.numel());
     flat(v, "cache values", at::kChar, k.numel());
-    TORCH_CHECK_VALUE(v.size(0) == pages && v.size(1) == n && v.size(2) == dim && v.size(3) == page, "cache values: [", pages, ", ", n, ", ", dim,
+    CHECK_VALUE(v.size(0) == pages && v.size(1) == n && v.size(2) == dim && v.size(3) == page, "cache values: [", pages, ", ", n, ", ", dim,
                       ", ", page, "] is wanted, got ", v.sizes());
     flat(ks, "cache key scales", at::kFloat, pages * n);
     flat(vs, "cache value scales", at::kFloat, pages * n);
-    TORCH_CHECK_VALUE(pages <= INT32_MAX && n <= INT32_MAX && page <= INT32_MAX && dim <= INT32_MAX, "cache: too large");
+    CHECK_VALUE(pages <= INT32_MAX && n <= INT32_MAX && page <= INT32_MAX && dim <= INT32_MAX, "cache: too large");
     return {static_cast<int8_t*>(k.data_ptr()), static_cast<int8_t*>(v.data_ptr()), static_cast<float*>(ks.data_ptr()),
             static_cast<float*>(vs.data_ptr()), (int)pages, (int)page, (int)n, (int)dim};
 }
@@ -319,7 +343,7 @@ Rows rows_of(PyObject* pages, PyObject* held, PyObject* starts) {
     const Tensor &h = tensor(held, "tokens held"), &s = tensor(starts, "starts");
     flat(h, "tokens held", at::kInt, n);
     flat(s, "starts", at::kInt, n + 1);
-    TORCH_CHECK_VALUE(n <= INT32_MAX && p.size(1) <= INT32_MAX, "pages: too large");
+    CHECK_VALUE(n <= INT32_MAX && p.size(1) <= INT32_MAX, "pages: too large");
     return {static_cast<int32_t*>(p.data_ptr()), static_cast<int32_t*>(h.data_ptr()), static_cast<int32_t*>(s.data_ptr()), (int)n, (int)p.size(1)};
 }
 
@@ -333,7 +357,7 @@ PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t count) {
     heads(v, "v", c.dim);
     const int type = type_of(k.scalar_type(), "k");
     const int64_t total = k.size(0);
-    TORCH_CHECK_VALUE(k.size(1) == c.heads && v.size(1) == c.heads && v.size(0) == total && v.scalar_type() == k.scalar_type(),
+    CHECK_VALUE(k.size(1) == c.heads && v.size(1) == c.heads && v.size(0) == total && v.scalar_type() == k.scalar_type(),
                       "k and v: [tokens, ", c.heads, ", ", c.dim, "] of one type are wanted, got ", k.sizes(), " of ", k.scalar_type(), " and ",
                       v.sizes(), " of ", v.scalar_type());
     void* s = stream_of(a[7], k.device(), {});
@@ -351,7 +375,7 @@ PyObject* cache_load(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const vdt_cache8 c = cache_of(a[0]);
     const Rows r = rows_of(a[1], a[2], a[3]);
     const int64_t total = integer(a[4], "total");
-    TORCH_CHECK_VALUE(total >= 0, "total: negative");
+    CHECK_VALUE(total >= 0, "total: negative");
     const int most = (int)std::min<int64_t>(small_integer(a[5], "most"), total);
     const at::ScalarType type = dtype(a[6], "dtype");
     const int kind = type_of(type, "dtype");
@@ -378,7 +402,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const Tensor out = given.defined() ? given : room(q.sizes(), q.scalar_type(), q.device());
     if (given.defined()) {
         heads(out, "out", c.dim);
-        TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out: ", q.sizes(), " of ", q.scalar_type(), " is wanted");
+        CHECK_VALUE(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out: ", q.sizes(), " of ", q.scalar_type(), " is wanted");
     }
     const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)c.dim) : number(a[8], "scale");
     const size_t need = vdt_cache_attention_scratch_bytes(total, (int)n, c.heads, c.dim, r.seqs, most, most_kept);
