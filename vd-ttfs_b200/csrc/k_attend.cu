@@ -474,10 +474,10 @@ __device__ __forceinline__ void add_four(float (&sum)[4], const float4& v, float
 __global__ void __launch_bounds__(128) k_attend_join_few(AttendParams p, int chunk, int count, int tile) {
     const int lane = threadIdx.x % 32, four = p.c.dim / 4;
     const long long i = (long long)blockIdx.x * 4 + threadIdx.x / 32;
-    if (i >= p.r.total * p.heads) return;
-    const JoinRow r = join_row(p, i / p.heads, (int)(i % p.heads), chunk, count, tile);
+    const bool in = i < p.r.total * p.heads;
+    const JoinRow r = in ? join_row(p, i / p.heads, (int)(i % p.heads), chunk, count, tile) : JoinRow{0, -1};
+    chain_wait();                            // before any return: what follows on the stream may count on it
     if (r.chunks == -1) return;
-    chain_wait();
     const Partial from = partial_of(p, i, count, 0);
     const float2 own = lane < r.chunks ? from.stats[lane] : make_float2(-inf_f(), 0.0f);
     float top = own.x;
@@ -521,8 +521,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(AttendParams p, in
     __shared__ float factor[kJoinChunks], part[4][256], side[2][4];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, four = p.c.dim / 4;
     const JoinRow r = join_row(p, blockIdx.x / p.heads, blockIdx.x % p.heads, chunk, count, tile);
-    if (r.chunks == -1) return;
     chain_wait();
+    if (r.chunks == -1) return;
     float top = -inf_f(), l = 0.0f, sum[2][4] = {};
     for (int first = 0; first < r.chunks; first += kJoinChunks) {
         const int here = min(r.chunks - first, kJoinChunks);

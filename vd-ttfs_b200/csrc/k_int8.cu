@@ -235,6 +235,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_int8_tiles(const __grid_con
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int steps = (p.inner + kStageBytes - 1) / kStageBytes;
     if (threadIdx.x == 0) {
+        map_ahead(&map_w);
+        map_ahead(&map_a);
         for (int i = 0; i < Shape::kStages; ++i) {
             bar_init(shared_address(&bars.full[i]), 1);
             bar_init(shared_address(&bars.empty[i]), 1);
@@ -250,6 +252,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_int8_tiles(const __grid_con
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = bars.tmem;
+    // the weights are the caller's: the first stages' need not wait for the codes
+    const int ahead = min(steps, Shape::kStages);
+    if (threadIdx.x == 0)
+        for (int s = 0; s < ahead; ++s) {
+            const uint32_t bar = shared_address(&bars.full[s]);
+            bar_expect(bar, Shape::kStage);
+            tile_load(stages + s * Shape::kStage + kTileRows * kStageBytes, &map_w, s * kStageBytes, blockIdx.x / tiles_m * BN, bar);
+        }
     chain_wait();
 
     if (warp == 0) {
@@ -260,11 +270,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_int8_tiles(const __grid_con
                 const int y = tile % tiles_m * kTileRows, c = tile / tiles_m * BN;
                 for (int s = 0; s < steps; ++s, ++n) {
                     const int slot = n % Shape::kStages;
-                    if (!(alive = bar_wait(shared_address(&bars.empty[slot]), (n / Shape::kStages & 1) ^ 1))) break;
                     const uint32_t at = stages + slot * Shape::kStage, bar = shared_address(&bars.full[slot]);
-                    bar_expect(bar, Shape::kStage);
+                    if (n >= ahead) {
+                        if (!(alive = bar_wait(shared_address(&bars.empty[slot]), (n / Shape::kStages & 1) ^ 1))) break;
+                        bar_expect(bar, Shape::kStage);
+                        tile_load(at + kTileRows * kStageBytes, &map_w, s * kStageBytes, c, bar);
+                    }
                     tile_load(at, &map_a, s * kStageBytes, y, bar);
-                    tile_load(at + kTileRows * kStageBytes, &map_w, s * kStageBytes, c, bar);
                 }
             }
             // every load has landed before the CTA ends: the last ones' stages
@@ -302,7 +314,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_int8_tiles(const __grid_con
         unsigned char* stage = smem + Shape::kStages * Shape::kStage + (warp - 2) * 4096;
         float* const scales = reinterpret_cast<float*>(smem + Shape::kStages * Shape::kStage + Shape::kOut);
         T* const out = static_cast<T*>(p.out);
-        constexpr int kCols = 128 / sizeof(T), kPer = 16 / sizeof(T);   // columns of a block; of 16 bytes
+        constexpr int kPer = 16 / sizeof(T), kCols = 8 * kPer < BN ? 8 * kPer : BN;   // columns of 16 bytes; of a block
+        constexpr int kPieces = kCols / kPer;                         // 16-byte pieces of a block's row
         const bool wide = p.out_stride * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
         bool alive = true;
         int i = 0;
@@ -348,29 +361,35 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_int8_tiles(const __grid_con
                         Vec16<T> v;
                         v.set(f);
                         const int chunk = part * (32 / kPer) + q;
-                        *reinterpret_cast<uint4*>(stage + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = v.raw;
+                        *reinterpret_cast<uint4*>(stage + lane * 128 + ((chunk ^ (lane & (kPieces - 1))) << 4)) = v.raw;
                     }
                 }
                 __syncwarp();
                 const int col1 = col0 + b * kCols;
                 if (wide && col1 + kCols <= p.cols) {
-                    // eight lanes write a row's 128 bytes
+                    // kPieces lanes write a row's bytes
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int r = k * 4 + lane / 8;
-                        const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((lane % 8 ^ (r & 7)) << 4));
-                        if (row0 + r < p.rows) *reinterpret_cast<uint4*>(out + (row0 + r) * p.out_stride + col1 + lane % 8 * kPer) = v;
+                    for (int k = 0; k < kPieces; ++k) {
+                        const int r = k * (32 / kPieces) + lane / kPieces, c = lane % kPieces;
+                        const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & (kPieces - 1))) << 4));
+                        if (row0 + r < p.rows) *reinterpret_cast<uint4*>(out + (row0 + r) * p.out_stride + col1 + c * kPer) = v;
                     }
                 } else {
-                    // rows that do not start on 16 bytes, or end in this block: value by value
-                    T* const to = out + row0 * p.out_stride + col1;
-#pragma unroll 8
-                    for (int r = 0; r < 32; ++r)
+                    // rows that do not start on 16 bytes, or end in this block:
+                    // value by value, eight rows read before they are written
+                    T* to = out + row0 * p.out_stride + col1;
+                    for (int r0 = 0; r0 < 32; r0 += 8, to += 8 * p.out_stride)
 #pragma unroll
-                        for (int c = lane; c < kCols; c += 32) {
-                            const int at = c * (int)sizeof(T);
-                            const T x = *reinterpret_cast<const T*>(stage + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15));
-                            if (row0 + r < p.rows && col1 + c < p.cols) to[r * p.out_stride + c] = x;
+                        for (int c0 = 0; c0 < kCols; c0 += 32) {
+                            const int c = c0 + lane, at = c * (int)sizeof(T);
+                            T x[8];
+#pragma unroll
+                            for (int r = 0; r < 8; ++r)
+                                x[r] = *reinterpret_cast<const T*>(stage + (r0 + r) * 128 + (((at >> 4) ^ (r & (kPieces - 1))) << 4) + (at & 15));
+                            if (col1 + c < p.cols)
+#pragma unroll
+                                for (int r = 0; r < 8; ++r)
+                                    if (row0 + r0 + r < p.rows) to[r * p.out_stride + c] = x[r];
                         }
                 }
                 __syncwarp();
@@ -436,7 +455,7 @@ cudaError_t tiles_by_width(const Int8Params& p, bool after, cudaStream_t s) {
     const long long tiles_m = (p.rows + kTileRows - 1) / kTileRows;
     int best = 0;
     long long cost = 0;
-    for (const int bn : {256, 128, 64}) {
+    for (const int bn : {256, 128, 64, 32}) {
         const long long tiles = tiles_m * ((p.cols + bn - 1) / bn), c = (tiles + kSmCount - 1) / kSmCount * (bn + 64);
         if (!best || c < cost) {
             best = bn;
@@ -445,7 +464,8 @@ cudaError_t tiles_by_width(const Int8Params& p, bool after, cudaStream_t s) {
     }
     if (best == 256) return tiles_launch<T, 256>(p, after, s);
     if (best == 128) return tiles_launch<T, 128>(p, after, s);
-    return tiles_launch<T, 64>(p, after, s);
+    if (best == 64) return tiles_launch<T, 64>(p, after, s);
+    return tiles_launch<T, 32>(p, after, s);
 }
 
 template <typename T>

@@ -262,6 +262,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  : "memory");
 }
 
+__device__ __forceinline__ void map_ahead(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 // a two-dimensional box through a tensor map; x counts values, and x times the
 // value's size is a multiple of 16 bytes
 __device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
