@@ -437,7 +437,8 @@ int vdt_int8_matmul(const int8_t* d_a, int64_t a_stride, const float* d_a_scale,
 
 /* The two together for rows x [rows, inner] of `type`: each row's codes into
    d_scratch (256-byte aligned, vdt_int8_linear_scratch_bytes; VDT_ERR_CAPACITY
-   when smaller), then the product. */
+   when smaller), then the product; a few rows are rounded by the product's
+   own kernel. */
 size_t vdt_int8_linear_scratch_bytes(int64_t rows, int inner);
 int vdt_int8_linear(const void* d_x, int type, int64_t x_stride, const int8_t* d_w, int64_t w_stride,
                     const float* d_w_scale, const float* d_bias, int64_t rows, int cols, int inner, int out_type,
@@ -479,8 +480,8 @@ int vdt_rope_table(int positions, int rot, double base, int scaling, double fact
 /* A paged cache of keys and values in 8 bits: a page holds `page` tokens (16,
    32 or 64) of one sequence; k [pages, heads, page, dim], v [pages, heads,
    dim, page] (16-byte aligned), and a scale for each page and head, k_scale
-   and v_scale [pages, heads].  dim: 32, 64, 96, 128, 192 or 256.  All memory
-   is the caller's.
+   and v_scale [pages, heads], never negative.  dim: 32, 64, 96, 128, 192 or
+   256.  All memory is the caller's.
    A sequence's pages are d_pages[seq][0 .. width), its token t in page
    t / page; packed rows of sequence s are d_starts[s] .. d_starts[s + 1] of
    `total` rows, `most` the longest such run. */
@@ -497,7 +498,9 @@ typedef struct {
    page that tokens are in already keeps its scale or, when a new token is
    larger, gets a larger one, and its old codes are rounded anew.  d_held is
    not changed.  Two sequences of one call must not append to the same page;
-   tokens for which the table has no page of the cache are dropped. */
+   tokens for which the table has no page of the cache are dropped, and so are
+   a sequence's whose rows do not fit `total` and `most`, or whose d_held is
+   negative or above 2^30. */
 int vdt_cache_append(const vdt_cache8* cache, const void* d_k, int64_t k_token, int64_t k_head, const void* d_v,
                      int64_t v_token, int64_t v_head, int type, const int32_t* d_pages, int width,
                      const int32_t* d_held, const int32_t* d_starts, int seqs, int64_t total, int most,

@@ -20,6 +20,15 @@
 // than 2^8 over what its weights are relative to (the weights are 16-bit
 // floats, which have room for that: at most 2^8 x 2^4 below), or a page's value
 // scale by more than 2^4.
+//
+// Three prompts of up to 2049 tokens behind up to 4096 cached ones, 32 heads of
+// 128 over 8: 401 us, 750 TFLOP/s (44% of the measured bf16 peak).  A step of
+// two tiles is 2,048 cycles of products and as many of exponentials (16 a
+// cycle); both tiles' softmaxes run side by side, then wait for the products,
+// since the tensor memory has no room for the next step's scores beside two
+// tiles' scores and sums.  Taking turns instead: 451 us, as one tile's softmax
+// alone does not fill the SM.  One tile a CTA reads and turns the codes twice as
+// often and is taken where there are no rows for two.
 #include "attend_internal.h"
 
 namespace vdt {

@@ -13,6 +13,8 @@ namespace vdt {
 namespace {
 
 // ------------------------------------------------------------------ quantise
+// Reads every value once, writes a byte for it: bound by memory for many rows
+// (8192 x 4096 bf16: 29 us, 3.5 TB/s; the floor is 16), by latency for few.
 // One CTA a row: the largest magnitude, then the codes.  Rows of up to HELD
 // vectors a thread are read once and stay in registers; longer ones, and rows
 // that are not on 16 bytes (HELD 0), are read twice, the second time from L1
@@ -95,7 +97,11 @@ __global__ void __launch_bounds__(THREADS) k_quantize_rows(const T* __restrict__
 // m16n8k32 with the channels as its rows and 8 tokens as its columns.  The
 // order of the inner dimension is free as long as both sides keep the same,
 // so a lane takes 16 consecutive bytes of a row (one wide load) and feeds
-// them to two products.
+// them to two products.  What bounds it is the weights' way from memory: 16
+// channels a CTA and eight warps along the inner dimension put every SM to
+// work for a few thousand channels, four steps of loads in flight a warp, the
+// first before the codes are there.  24 x 4096 x 4096: 9.3 us with the rows'
+// rounding (16.7 MB of weights, from L2 where they fit).
 constexpr int kRowsWarps = 8;
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -113,8 +119,60 @@ __device__ __forceinline__ uint32_t keep_below(uint32_t v, int word, int inner) 
 
 constexpr int kFewRows = 32;
 
-template <typename T, int NT>
+// Up to kOwnRows rows of up to kOwnValues values together are rounded by every
+// CTA for itself, into shared memory: one launch instead of two (one row of
+// 1024: 8.7 us a call with two, the host's side of a launch some 2).  The
+// values are read from L2 by all CTAs, so more of them would cost more.
+constexpr int kOwnRows = 4, kOwnValues = 16384;
+
+template <typename X>
+__device__ __forceinline__ void round_rows(const Int8Params& p, int8_t* codes, float* scale) {
+    constexpr int N = Vec16<X>::N, kThreads = kRowsWarps * 32;
+    __shared__ float part[kOwnRows][kRowsWarps];
+    const X* const x = static_cast<const X*>(p.x);
+    const int stride = (p.inner + 15) / 16 * 16, rows = (int)p.rows;
+    const bool wide = p.x_stride % N == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    const int vecs = wide ? p.inner / N : 0;
+    float m[kOwnRows] = {};
+#pragma unroll
+    for (int r = 0; r < kOwnRows; ++r) {
+        if (r >= rows) break;
+        const X* const row = x + r * p.x_stride;
+        Largest<X> most;
+        for (int i = threadIdx.x; i < vecs; i += kThreads) most.add(Vec16<X>{*reinterpret_cast<const uint4*>(row + i * N)});
+        m[r] = most.value();
+        for (int i = vecs * N + threadIdx.x; i < p.inner; i += kThreads) m[r] = max_nan(fabsf(to_f32(row[i])), m[r]);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m[r] = max_nan(__shfl_xor_sync(0xffffffffu, m[r], d), m[r]);
+        if (threadIdx.x % 32 == 0) part[r][threadIdx.x / 32] = m[r];
+    }
+    __syncthreads();
+    for (int r = 0; r < rows; ++r) {
+        const X* const row = x + r * p.x_stride;
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kRowsWarps; ++i) top = max_nan(part[r][i], top);
+        const Coder coder(top * kCodeStep);
+        if (threadIdx.x == 0) scale[r] = coder.scale;
+        for (int i = threadIdx.x; i < vecs; i += kThreads) {
+            Vec16<X> v;
+            v.raw = *reinterpret_cast<const uint4*>(row + i * N);
+            float f[N];
+            uint32_t w[N / 4];
+            v.get(f);
+            coder.words<N>(f, w);
+#pragma unroll
+            for (int j = 0; j < N / 4; ++j) reinterpret_cast<uint32_t*>(codes + r * stride)[i * (N / 4) + j] = w[j];
+        }
+        for (int i = vecs * N + threadIdx.x; i < p.inner; i += kThreads) codes[r * stride + i] = (int8_t)code_of(to_f32(row[i]), coder.scale);
+    }
+    __syncthreads();
+}
+
+// X: the type of rows that are still to be rounded; void: they are codes
+template <typename T, int NT, typename X = void>
 __global__ void __launch_bounds__(kRowsWarps * 32) k_int8_rows(Int8Params p) {
+    extern __shared__ __align__(16) int8_t own[];            // rows' codes, then their scales
     __shared__ int part[kRowsWarps][16][8 * NT + 1];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const int col0 = blockIdx.x * 16;
@@ -124,6 +182,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_int8_rows(Int8Params p) {
     const int8_t* w0 = p.w + (long long)min(col0 + g, p.cols - 1) * p.w_stride;
     const int8_t* w1 = p.w + (long long)min(col0 + g + 8, p.cols - 1) * p.w_stride;
     const int8_t* a[NT];
+    const float* a_scale = p.a_scale;
 #pragma unroll
     for (int n = 0; n < NT; ++n) a[n] = p.a + min(row0 + 8 * n + g, p.rows - 1) * p.a_stride;
     const int steps = (p.inner + 63) / 64;
@@ -145,6 +204,13 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_int8_rows(Int8Params p) {
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) weights(warp + d * kRowsWarps, u[d]);
     chain_wait();
+    if constexpr (!std::is_void_v<X>) {
+        const int stride = (p.inner + 15) / 16 * 16;
+        float* const scale = reinterpret_cast<float*>(own + p.rows * stride);
+        round_rows<X>(p, own, scale);
+        a_scale = scale;
+        a[0] = own + min(g, (int)p.rows - 1) * stride;
+    }
     for (int s0 = warp; s0 < steps; s0 += kDeep * kRowsWarps) {
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) rows(s0 + d * kRowsWarps, x[d]);
@@ -182,7 +248,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_int8_rows(Int8Params p) {
         const int col = col0 + c;
         const long long row = row0 + r;
         if (col < p.cols && row < p.rows) {
-            float y = (float)sum * p.a_scale[row] * p.w_scale[col];
+            float y = (float)sum * a_scale[row] * p.w_scale[col];
             if (p.bias) y += p.bias[col];
             static_cast<T*>(p.out)[row * p.out_stride + col] = from_f32<T>(y);
         }
@@ -199,13 +265,29 @@ cudaError_t rows_launch(const Int8Params& p, bool after, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+template <typename T, typename X>
+cudaError_t own_launch(const Int8Params& p, cudaStream_t s) {
+    const size_t bytes = (size_t)p.rows * ((p.inner + 15) / 16 * 16) + p.rows * sizeof(float);
+    k_int8_rows<T, 1, X><<<(p.cols + 15) / 16, kRowsWarps * 32, bytes, s>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t own_by_type(const Int8Params& p, int type, cudaStream_t s) {
+    if (type == VDT_F32) return own_launch<T, float>(p, s);
+    if (type == VDT_F16) return own_launch<T, __half>(p, s);
+    return own_launch<T, __nv_bfloat16>(p, s);
+}
+
 // --------------------------------------------------------------- many rows
 // Persistent CTAs over tiles of 128 rows x BN channels.  One thread keeps a
 // ring of stages (128 bytes of the inner dimension of both sides) full with
 // tile loads, one issues the products into the tensor memory, four warps turn
 // finished sums into outputs while the next tile's are made in the other half
 // of the tensor memory.  Loads past the rows, the channels and the inner size
-// give zeros.
+// give zeros.  A stage is 128 bytes because a swizzled row is; 256 channels a
+// tile halve the reads of the rows' codes against 128.  8192 x 4096 x 8192:
+// 169 us, 3.25 POP/s, bound by the tensor cores and, back to back, by power.
 constexpr int kTileRows = 128, kStageBytes = 128;    // bytes of the inner dimension a stage
 constexpr int kGemmThreads = 192;
 
@@ -499,6 +581,14 @@ cudaError_t launch_quantize_rows(const void* x, int type, long long rows, int co
     if (type == VDT_F32) return quant_launch<float>(x, rows, cols, x_stride, codes, codes_stride, scale, s);
     if (type == VDT_F16) return quant_launch<__half>(x, rows, cols, x_stride, codes, codes_stride, scale, s);
     return quant_launch<__nv_bfloat16>(x, rows, cols, x_stride, codes, codes_stride, scale, s);
+}
+
+bool int8_rounds_itself(long long rows, int inner) { return rows <= kOwnRows && rows * inner <= kOwnValues; }
+
+cudaError_t launch_int8_own(const Int8Params& p, int type, cudaStream_t s) {
+    if (p.out_type == VDT_F32) return own_by_type<float>(p, type, s);
+    if (p.out_type == VDT_F16) return own_by_type<__half>(p, type, s);
+    return own_by_type<__nv_bfloat16>(p, type, s);
 }
 
 cudaError_t launch_int8_matmul(const Int8Params& p, bool after_codes, cudaStream_t s) {

@@ -6,7 +6,9 @@
 //   (a, b) -> (a cos - b sin, b cos + a sin)  for the pairs of the first `rot` values
 //
 // VDT_ROPE_HALF pairs value i with i + rot / 2, VDT_ROPE_PAIRS 2i with 2i + 1.
-// Everything between the load and the store is 32-bit.
+// Everything between the load and the store is 32-bit.  Each value is read and
+// written once: 16381 tokens of 40 heads of 128 in bf16 take 80 us, 4.2 TB/s
+// (floor 53 us); what is left is the latency of position, angles and rows.
 #include "seq_internal.h"
 
 namespace vdt {

@@ -89,7 +89,7 @@ extern "C" int vdt_int8_matmul(const int8_t* d_a, int64_t a_stride, const float*
     SEQ_REQUIRE(d_a && d_a_scale, "NULL buffer");
     SEQ_REQUIRE(a_stride >= inner && a_stride % 16 == 0 && aligned(d_a, 16), "code rows must start on 16-byte boundaries");
     if (int s = api_check_buffers(-1, {d_a, d_a_scale, d_w, d_w_scale, d_bias, d_out})) return s;
-    Int8Params p{d_a, d_a_scale, d_w, d_w_scale, d_bias, d_out, rows, a_stride, w_stride, out_stride, cols, inner, out_type};
+    Int8Params p{d_a, d_a_scale, d_w, d_w_scale, d_bias, d_out, rows, a_stride, w_stride, out_stride, cols, inner, out_type, nullptr, 0};
     return launched(launch_int8_matmul(p, false, static_cast<cudaStream_t>(stream)), "int8_matmul");
 }
 
@@ -113,11 +113,15 @@ extern "C" int vdt_int8_linear(const void* d_x, int type, int64_t x_stride, cons
         return api_fail(VDT_ERR_CAPACITY, "scratch smaller than vdt_int8_linear_scratch_bytes");
     if (int s = api_check_buffers(-1, {d_x, d_w, d_w_scale, d_bias, d_out, d_scratch})) return s;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (int8_rounds_itself(rows, inner)) {              // a few rows: the scratch is not used
+        Int8Params p{nullptr, nullptr, d_w, d_w_scale, d_bias, d_out, rows, 0, w_stride, out_stride, cols, inner, out_type, d_x, x_stride};
+        return launched(launch_int8_own(p, type, st), "int8_linear");
+    }
     int8_t* codes = static_cast<int8_t*>(d_scratch);
     float* scale = reinterpret_cast<float*>(codes + round256((size_t)rows * (size_t)code_stride(inner)));
     cudaError_t e = launch_quantize_rows(d_x, type, rows, inner, x_stride, codes, code_stride(inner), scale, st);
     if (e != cudaSuccess) return api_cuda_fail(e, "quantize_rows");
-    Int8Params p{codes, scale, d_w, d_w_scale, d_bias, d_out, rows, code_stride(inner), w_stride, out_stride, cols, inner, out_type};
+    Int8Params p{codes, scale, d_w, d_w_scale, d_bias, d_out, rows, code_stride(inner), w_stride, out_stride, cols, inner, out_type, nullptr, 0};
     return launched(launch_int8_matmul(p, true, st), "int8_matmul");
 }
 

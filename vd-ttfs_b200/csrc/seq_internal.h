@@ -330,7 +330,12 @@ struct Int8Params {
     void* out;              // [rows, cols], rows out_stride values apart
     long long rows, a_stride, w_stride, out_stride;
     int cols, inner, out_type;
+    const void* x;          // launch_int8_own: the rows, x_stride values apart, instead of a and a_scale
+    long long x_stride;
 };
+// a few rows that the product's kernel rounds itself
+bool int8_rounds_itself(long long rows, int inner);
+cudaError_t launch_int8_own(const Int8Params& p, int type, cudaStream_t s);
 // after_codes: the kernel before it on the stream is the one that writes `a`
 cudaError_t launch_int8_matmul(const Int8Params& p, bool after_codes, cudaStream_t s);
 
