@@ -119,6 +119,18 @@ def test_linear_output_type(S, out_dtype):
         check_linear(S, rows, 96, 100, torch.float32, True, 5, out_dtype=out_dtype)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,inner", [(1, 16384), (1, 16385), (4, 4096), (4, 4097), (5, 64), (2, 37)])
+def test_linear_is_its_two_steps(S, kind, rows, inner):
+    """A few rows are rounded by the product's kernel, more by one of their own: the bits are those of the two calls."""
+    x = normal(rows, rows, inner, kind=kind).cuda()
+    w, ws = S.quantize_rows(normal(1, 33, inner).cuda())
+    b = normal(2, 33).cuda()
+    codes, scale = S.quantize_rows(x)
+    for out in KINDS:
+        assert torch.equal(S.int8_linear(x, w, ws, b, out_dtype=out), S.int8_matmul(codes, scale, w, ws, b, out_dtype=out))
+
+
 def test_linear_extremes_are_exact(S):
     """All codes at +-127, a long inner dimension: the largest sums there are."""
     for rows, inner in ((2, 131072), (140, 16384)):
