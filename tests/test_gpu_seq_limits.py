@@ -1,0 +1,114 @@
+"""The sequence operators where their bounds lie: values of very different size in one cache.
+
+Tolerances are derived as in test_gpu_seq.py; each test states what it adds.
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_seq import S, U, ints, make_cache, make_table, normal, sums  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# -------------------------------------------------------------- attention --
+def cached(cache, row, n, page):
+    """A sequence's keys, values and value scales in 64 bits: [heads, n, dim] twice, [heads, n]."""
+    at = torch.tensor(row[: -(-n // page)], device="cuda")
+    scale = [c[at].double().repeat_interleave(page, 0).T[:, :n] for c in cache[2:]]
+    k = cache[0][at].double().transpose(0, 1).flatten(1, 2)[:, :n] * scale[0][..., None]
+    v = cache[1][at].double().permute(1, 0, 3, 2).flatten(1, 2)[:, :n] * scale[1][..., None]
+    return k, v, scale[1]
+
+
+def strict(S, q, cache, table, kept, new, causal, scale, page):
+    """Attention against 64 bits.  A weight (the probability with its page's value scale) is off by 2^-11 of itself or by
+    2^-25 of the row's largest, and multiplies a code of up to 127; its exponent, of numbers up to 256, is rounded three
+    times at 2^-17: 2^-15 of the weight; the rest is the scores' error and the output's rounding."""
+    starts = sums(new)
+    heads, dim = q.shape[1:]
+    group = heads // cache[0].shape[1]
+    out = S.cache_attention(q, cache, ints(table), ints(kept), ints(starts), max(new), max(kept), causal=causal, scale=scale).double()
+    for b, n in enumerate(kept):
+        k, v, vs = (x.repeat_interleave(group, 0) for x in cached(cache, table[b], n, page))
+        x = q[starts[b]: starts[b + 1]].double().transpose(0, 1)
+        s = x @ k.transpose(1, 2) * scale
+        last = torch.arange(n - new[b] + 1, n + 1, device="cuda") if causal else torch.full((new[b],), n, device="cuda")
+        s = s.masked_fill(torch.arange(n, device="cuda")[None] >= last[:, None], -math.inf)
+        p = torch.softmax(s, -1)
+        want = p @ v
+        size = (x.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) * abs(scale)
+        d = (dim + 16) * 2.0 ** -23 * size + abs(scale) * 2.0 ** -24 * x.abs().amax(-1, keepdim=True) * k.abs().sum(2).amax(1)[:, None, None]
+        tol = U[q.dtype] * want.abs() + (2.0 ** -11 + 2.0 ** -15 + 2 * d) * (p @ v.abs()) \
+            + n * 127 * 2.0 ** -25 * (p * vs[:, None]).amax(-1, keepdim=True) + (2.0 ** -25 if q.dtype == torch.float16 else 0)
+        off = (out[starts[b]: starts[b + 1]].transpose(0, 1) - want).abs()
+        assert (off <= tol).all(), (b, float((off / tol).max()))
+
+
+@pytest.mark.parametrize("page", [16, 32])
+@pytest.mark.parametrize("power", [14, 20, 28])
+@pytest.mark.parametrize("new,dim", [(5, 64), (16, 128), (40, 64), (150, 64), (150, 128), (300, 128), (40, 256)])
+def test_attention_does_not_change_with_values_that_a_row_does_not_see(S, new, dim, power, page):
+    """The last page's values grow by 2^power: the causal rows before it give the bits they gave."""
+    kept = 256
+    table, pages = make_table([kept], page)
+    cache = make_cache(S, pages, 1, dim, page)
+    q = normal(1, new, 1, dim, kind=torch.bfloat16).cuda()
+    in_last = min(page, new // 2)                         # queries that see the last page
+    args = (ints(table), ints([kept - page + in_last]), ints([0, new]), new, kept)
+    blind = new - in_last
+    before = S.cache_attention(q, cache, *args)
+    cache.v_scale[table[0][-1]] *= 2.0 ** power
+    after = S.cache_attention(q, cache, *args)
+    assert torch.equal(after[:blind], before[:blind])
+    assert not torch.equal(after[blind:], before[blind:])
+
+
+@pytest.mark.parametrize("new", [1, 12, 40, 200])
+@pytest.mark.parametrize("power", [10, 16, 24, 30])
+def test_attention_keeps_its_bits_beside_large_values_of_no_weight(S, new, power):
+    """One page has values 2^power times the others' and keys that give it next to no probability, first or last."""
+    dim, page, kept = 64, 16, 240
+    for where in (0, 7, 14):
+        table, pages = make_table([kept], page)
+        cache = make_cache(S, pages, 1, dim, page)
+        q = normal(2, new, 2, dim).abs().add(0.5).to(torch.bfloat16).cuda()
+        at = table[0][where]
+        cache.k[at] = -100                                # against every query: scores some 40 to 120 below the others'
+        cache.k_scale[at] = 1.0 / 32
+        cache.v_scale[at] *= 2.0 ** power
+        strict(S, q, cache, table, [kept], [new], False, 0.25, page)
+
+
+@pytest.mark.parametrize("new", [1, 16, 33, 150])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 32), (256, 64)])
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
+def test_attention_value_scales_of_every_size(S, new, dim, page, kind):
+    """Value scales from 2^-20 to 2^20 (f16: of their usual size and below), in every order, pages of zeros among them."""
+    kept = [400, 333]
+    table, pages = make_table(kept, page)
+    for seed in range(3):
+        cache = make_cache(S, pages, 2, dim, page, seed)
+        g = torch.Generator().manual_seed(seed)
+        most = 0 if kind == torch.float16 else 20
+        cache.v_scale.mul_(2.0 ** (torch.rand(cache.v_scale.shape, generator=g) * (most + 20) - 20).cuda())
+        zero = torch.randint(0, pages, (2,), generator=g).cuda()
+        cache.v_scale[zero] = 0
+        q = normal(seed, 2 * new, 4, dim, kind=kind).cuda()
+        strict(S, q, cache, table, kept, [new, new], bool(seed % 2), 0.3 / math.sqrt(dim), page)
+
+
+@pytest.mark.parametrize("new", [1, 150])
+def test_attention_over_values_that_are_all_zero_then_not(S, new):
+    """Pages of zeros with the largest scores: their weights count in the sum, and the values after them are whole."""
+    dim, page, kept = 64, 16, 256
+    table, pages = make_table([kept], page)
+    cache = make_cache(S, pages, 1, dim, page)
+    for j in range(4):
+        cache.v_scale[table[0][j]] = 0
+        cache.k[table[0][j]] = 60
+    q = normal(3, new, 1, dim).abs().to(torch.float16).cuda()
+    for power in (0, -30):
+        cache.v_scale[table[0][9]] = 2.0 ** power
+        strict(S, q, cache, table, [kept], [new], False, 0.02, page)

@@ -81,9 +81,35 @@ __device__ __forceinline__ Partial partial_of(const AttendParams& p, long long r
     return {reinterpret_cast<float2*>(p.scratch) + i, p.scratch + partial_pairs(p.r.total * p.heads, count) + i * p.c.dim};
 }
 
-// By how much (powers of two) a weight may pass 1, and a page's value scale what
-// the sums are relative to, before both are taken anew
-constexpr float kSlack = 8.0f, kValueSlack = 4.0f;
+// What a row's running sums are relative to, in powers of two: 2^ref the
+// weights' sum, 2^(ref + vref) the outputs.  Both references follow what the
+// row itself sees: its largest score, and its largest score with the page's
+// value scale.  By how much one may be passed before both are taken anew:
+constexpr float kSlack = 8.0f, kSlackFactor = 256.0f;
+__device__ __forceinline__ bool passes(float x, float ref) { return x > ref + kSlack || (!(ref > -inf_f()) && x > -inf_f()); }
+
+// The references for new maxima, and the factors of the sums so far
+struct Rescale {
+    float sum, out;
+};
+__device__ __forceinline__ Rescale move_references(float top, float v_top, float& ref, float& vref) {
+    const float to = fmaxf(top, ref);
+    const float v_to = fmaxf(v_top, vref == -inf_f() ? vref : ref + vref);
+    const float v = v_to == -inf_f() ? v_to : v_to - to;
+    Rescale by;
+    by.sum = ref == -inf_f() ? 0.0f : exp2f(ref - to);
+    by.out = vref == -inf_f() ? 0.0f : exp2f((ref - to) + (vref - v));
+    ref = to;
+    vref = v;
+    return by;
+}
+// A page's value scale over that of the row's references, as the power of two
+// that its weights take with them and their sum gives back.  Not under 2^-100:
+// a page of zeros still has weights.
+__device__ __forceinline__ float page_shift(float v_log, float vref) {
+    const float d = v_log - (vref == -inf_f() ? 0.0f : vref);
+    return d < -100.0f ? -100.0f : d;
+}
 
 // many query rows: one CTA for up to 256 rows (k_attend_tiles.cu)
 Chunks plan_tiles(int dim, int heads, int kv_heads, int seqs, int most, int most_kept);

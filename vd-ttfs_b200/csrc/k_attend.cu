@@ -9,16 +9,21 @@
 //
 // The queries' rounding: q is scaled by a power of two for each row so that
 // its largest magnitude is in [1, 2); a 16-bit float then holds every bf16 or
-// f16 value whole down to 2^-14 of that (below, to 2^-24 of it).  The weights
-// exp(s - max) take their page's vs with them, relative to the largest vs so
-// far: exp2(s - m + log2(vs) - log2(vs_max)), and the sum of a page's weights
-// takes it out again.  Their rounding to 16 bits is at most 2^-11: that of an
-// f16 output, an eighth of a bf16 one's, and it averages over the tokens.
+// f16 value whole down to 2^-14 of that (below, to 2^-24 of it).
 //
-// m is not the running maximum itself: it moves only when a score passes it by
-// more than 2^8 (as a factor), and vs_max when a scale passes it by more than
-// 2^4; 16-bit floats have room for that, and the sums are rescaled a few times
-// instead of at every step.
+// A token's weight is its score's power and its page's vs together, in powers
+// of two: 2^(s + log2(vs)), and it is made relative to the largest such weight
+// that its own row sees (2^o).  A page that the row does not see, or that has
+// next to no probability, then takes no bits from the others however large its
+// values are.  The 16-bit weight is off by at most 2^-11 of itself, or, below
+// 2^-14 of the largest, by 2^-25 of that: the former is the rounding of an f16
+// output, an eighth of a bf16 one's, and it averages over the tokens.  The
+// weights' own sum is 32-bit and relative to the largest score (2^m): a page's
+// weights before the rounding, times 2^(o - m) / vs.
+//
+// m and o are not the running maxima themselves: they move only when a row
+// passes one of them by more than 2^8 (as a factor); 16-bit floats have room
+// for that, and the sums are rescaled a few times instead of at every step.
 #include "attend_internal.h"
 
 namespace vdt {
@@ -218,13 +223,15 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
     if (lane == 0)
         for (int e = 0; e < kRing; ++e) fetch(e);
 
-    float f[NR][2], ref[NR][2], sum[NR][2], vref = -inf_f();     // the lane's columns: factor, what the weights are relative to, their sum
+    // the lane's columns: factor, what their sum (2^ref) and the outputs
+    // (2^(ref + vref)) are relative to, the weights' sum
+    float f[NR][2], ref[NR][2], vref[NR][2], sum[NR][2];
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             f[n][i] = q_scale[8 * n + 2 * t + i];
-            ref[n][i] = -inf_f();
+            ref[n][i] = vref[n][i] = -inf_f();
             sum[n][i] = 0.0f;
         }
     float o[D / 16][NR][4] = {};
@@ -234,21 +241,6 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
         const bool partial = base + kUnit > least;
         const unsigned char* kt = smem + (warp * kRing + ek % kRing) * (kUnit * D);
         const unsigned char* vt = smem + (warp * kRing + ev % kRing) * (kUnit * D);
-        // pages' value scales that pass what the sums are relative to
-        float v_most = -inf_f();
-#pragma unroll
-        for (int pg = 0; pg < kPages; ++pg) v_most = fmaxf(v_most, v_log[u * kPages + pg]);
-        if (v_most > vref + kValueSlack || (vref == -inf_f() && v_most > vref)) {
-            const float by = exp2f(vref - v_most);
-#pragma unroll
-            for (int m = 0; m < D / 16; ++m)
-#pragma unroll
-                for (int n = 0; n < NR; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[m][n][e] *= by;
-            vref = v_most;
-        }
-        const float v_shift = vref == -inf_f() ? 0.0f : vref;
         alive = bar_wait_all(bars + (ek % kRing) * 8, (ek / kRing) & 1);
         if (!alive) break;
         {
@@ -292,45 +284,56 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
             if (lane == 0) fetch(ek + kRing);
             // scores, in powers of two; the lane's tokens are base + page + t' (P / 4) + ... of rows g and g + 8
             bool over = false;
-            float top[NR][2];
+            float top[NR][2], v_top[NR][2];                  // largest score; largest with its page's value scale
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) top[n][e] = -inf_f();
+                for (int e = 0; e < 2; ++e) top[n][e] = v_top[n][e] = -inf_f();
 #pragma unroll
-            for (int m = 0; m < kPart; ++m) {
-                const int pg = m / kGroups, j16 = m % kGroups;
-                const float ks = k_scale[u * kPages + pg];
-                const int token = base + pg * P + (g / 2) * (P / 4) + 4 * j16 + g % 2;
+            for (int pg = 0; pg < kPages; ++pg) {
+                const float ks = k_scale[u * kPages + pg], vl = v_log[u * kPages + pg];
 #pragma unroll
-                for (int n = 0; n < NR; ++n)
+                for (int n = 0; n < NR; ++n) {
+                    float most[2] = {-inf_f(), -inf_f()};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float v = sc[m][n][e] * (f[n][e % 2] * ks);
-                        if (partial) v = token + e / 2 * 2 < limit[n][e % 2] ? v : -inf_f();
-                        sc[m][n][e] = v;
-                        top[n][e % 2] = fmaxf(top[n][e % 2], v);
+                    for (int m = pg * kGroups; m < (pg + 1) * kGroups; ++m) {
+                        const int token = base + pg * P + (g / 2) * (P / 4) + 4 * (m % kGroups) + g % 2;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float v = sc[m][n][e] * (f[n][e % 2] * ks);
+                            if (partial) v = token + e / 2 * 2 < limit[n][e % 2] ? v : -inf_f();
+                            sc[m][n][e] = v;
+                            most[e % 2] = fmaxf(most[e % 2], v);
+                        }
                     }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        top[n][e] = fmaxf(top[n][e], most[e]);
+                        v_top[n][e] = fmaxf(v_top[n][e], most[e] + vl);
+                    }
+                }
             }
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) over = over || top[n][e] > ref[n][e] + kSlack || (ref[n][e] == -inf_f() && top[n][e] > ref[n][e]);
+                for (int e = 0; e < 2; ++e) over = over || passes(top[n][e], ref[n][e]) || passes(v_top[n][e], ref[n][e] + vref[n][e]);
             if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                 for (int n = 0; n < NR; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float x = top[n][e];
+                        float x = top[n][e], y = v_top[n][e];
 #pragma unroll
-                        for (int d = 4; d <= 16; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                        const float old = ref[n][e], to = fmaxf(x, old), by = to == -inf_f() ? 1.0f : exp2f(old - to);
-                        ref[n][e] = to;
-                        sum[n][e] *= by;
+                        for (int d = 4; d <= 16; d <<= 1) {
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
+                        }
+                        const Rescale by = move_references(x, y, ref[n][e], vref[n][e]);
+                        sum[n][e] *= by.sum;
 #pragma unroll
                         for (int m = 0; m < D / 16; ++m) {
-                            o[m][n][e] *= by;
-                            o[m][n][e + 2] *= by;
+                            o[m][n][e] *= by.out;
+                            o[m][n][e + 2] *= by.out;
                         }
                     }
             }
@@ -341,23 +344,23 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
             for (int m = 0; m < kPart; ++m) {
                 const int pg = m / kGroups, j16 = m % kGroups;
                 const int token = base + pg * P + (g / 2) * (P / 4) + 4 * j16 + g % 2;
-                // the page's scale, over what the sums are relative to; not
-                // under 2^-100: a page of zeros still has weights
-                float d = v_log[u * kPages + pg] - v_shift;
-                d = d < -100.0f ? -100.0f : d;
-                const float back = exp2_fast(-d);
+                const float vl = v_log[u * kPages + pg];
 #pragma unroll
                 for (int n = 0; n < NR; ++n) {
-                    float x[4];
+                    float x[4], d[2], r[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        d[e] = page_shift(vl, vref[n][e]);
+                        r[e] = ref[n][e] == -inf_f() ? 0.0f : ref[n][e];
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float r = ref[n][e % 2] == -inf_f() ? 0.0f : ref[n][e % 2];
-                        x[e] = exp2_fast(sc[m][n][e] - r + d);
+                        x[e] = exp2_fast(sc[m][n][e] - r[e % 2] + d[e % 2]);
                         if (partial) x[e] = token + e / 2 * 2 < limit[n][e % 2] ? x[e] : 0.0f;     // also for scales that are not numbers
                     }
                     const float a = x[0] + x[2], c = x[1] + x[3];
-                    sum[n][0] = partial && a == 0.0f ? sum[n][0] : fmaf(a, back, sum[n][0]);
-                    sum[n][1] = partial && c == 0.0f ? sum[n][1] : fmaf(c, back, sum[n][1]);
+                    sum[n][0] = partial && a == 0.0f ? sum[n][0] : fmaf(a, exp2_fast(-d[0]), sum[n][0]);
+                    sum[n][1] = partial && c == 0.0f ? sum[n][1] : fmaf(c, exp2_fast(-d[1]), sum[n][1]);
                     w[m][n][0] = transposed(pack_f16(x[0], x[1]));
                     w[m][n][1] = transposed(pack_f16(x[2], x[3]));
                 }
@@ -395,19 +398,19 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
     const bool dead = __syncthreads_or(!alive);
     float* sums = reinterpret_cast<float*>(smem);            // [warp][row][D], then [warp][row][2]
     float* tops = sums + kRowsWarps * kRows * D;
-    const float v_scale = exp2f(vref);
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+            const float v_scale = exp2f(vref[n][e] - kSlack);          // 2^vref may be too large for 32 bits where its product is not
 #pragma unroll
             for (int d = 4; d <= 16; d <<= 1) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], d);
             const int row = warp * kRows + 8 * n + 2 * t + e;
             if (!dead) {
 #pragma unroll
                 for (int m = 0; m < D / 16; ++m) {
-                    sums[row * D + m * 16 + g] = o[m][n][e] * v_scale;
-                    sums[row * D + m * 16 + g + 8] = o[m][n][e + 2] * v_scale;
+                    sums[row * D + m * 16 + g] = o[m][n][e] * v_scale * kSlackFactor;
+                    sums[row * D + m * 16 + g + 8] = o[m][n][e + 2] * v_scale * kSlackFactor;
                 }
                 if (g == 0) {
                     tops[row * 2] = ref[n][e];

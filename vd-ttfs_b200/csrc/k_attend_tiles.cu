@@ -16,10 +16,9 @@
 //     value row's tokens are so in the cache already);
 //   - one thread issues the products: with two tiles, one tile's run while the
 //     other's softmax does.
-// O is not divided or rescaled on the way unless a row's maximum grows by more
-// than 2^8 over what its weights are relative to (the weights are 16-bit
-// floats, which have room for that: at most 2^8 x 2^4 below), or a page's value
-// scale by more than 2^4.
+// O is not divided or rescaled on the way unless a row's largest score, or its
+// largest weight with the page's value scale, grows by more than 2^8 over what
+// they are relative to (the weights are 16-bit floats, which have room for that).
 //
 // Three prompts of up to 2049 tokens behind up to 4096 cached ones, 32 heads of
 // 128 over 8: 401 us, 750 TFLOP/s (44% of the measured bf16 peak).  A step of
@@ -71,7 +70,7 @@ struct State {
     uint64_t k_full[2], k_free[2], v_full[2], v_free[2], raw_full[2], raw_free[2], s_full[NT], p_full[NT], o_done[NT];
     uint64_t list_full[kAhead], list_free[kAhead];
     uint32_t tmem;
-    float k_scale[kAhead][PAGES], v_log[kAhead][PAGES], v_most[kAhead];    // of the values' scales, the logarithm
+    float k_scale[kAhead][PAGES], v_log[kAhead][PAGES];    // of the values' scales, the logarithm
 };
 
 // d (128 x N, 32-bit) (+)= a b^T for 16 columns of 16-bit floats
@@ -258,7 +257,6 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
         int my_steps = 0;
 #pragma unroll
         for (int i = 0; i < NT; ++i) my_steps = i == t ? steps[i] : my_steps;
-        // what the weights and O are relative to: 2^ref, 2^vref
         float ref = -inf_f(), vref = -inf_f(), sum = 0.0f;
         const bool busy = __any_sync(0xffffffffu, mine < rows);
         for (int j = 0; j < most; ++j) {
@@ -283,7 +281,7 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
 #pragma unroll
                     for (int i = 0; i < kHold / 32; ++i) tmem_load(at_s + from + i * 32, r[i]);
                 };
-                float c[kPages], top = -inf_f();
+                float c[kPages], top = -inf_f(), v_top = -inf_f();
 #pragma unroll
                 for (int from = kStep - kHold; from >= 0; from -= kHold) {
                     load(from);
@@ -303,15 +301,16 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
                             const float x = __uint_as_float(r[i / 32][i % 32 + q]);
                             m[q % 4] = q < 4 ? x : fmaxf(m[q % 4], x);
                         }
-                        top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * c[(from + i) / P]);
+                        const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * c[(from + i) / P];
+                        top = fmaxf(top, most);
+                        v_top = fmaxf(v_top, most + st.v_log[slot][(from + i) / P]);
                     }
                 }
-                const float v_most = st.v_most[slot];
-                const bool up = top > ref + kSlack || (ref == -inf_f() && top > ref), v_up = v_most > vref + kValueSlack || (vref == -inf_f() && v_most > vref);
-                if (v_up || __any_sync(0xffffffffu, up)) {
-                    const float to = up ? top : ref, by = ref == -inf_f() ? 0.0f : exp2_fast(ref - to);
-                    const float v_by = !v_up ? 1.0f : vref == -inf_f() ? 0.0f : exp2_fast(vref - v_most);
-                    sum *= by;
+                const bool up = passes(top, ref) || passes(v_top, ref + vref);
+                if (__any_sync(0xffffffffu, up)) {
+                    Rescale by = {1.0f, 1.0f};
+                    if (up) by = move_references(top, v_top, ref, vref);
+                    sum *= by.sum;
                     if (j > 0) {
                         alive = bar_wait_all(shared_address(&st.o_done[t]), (j - 1) & 1);
                         if (!alive) break;
@@ -321,17 +320,14 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
                             tmem_load16(at_o + i, o);
                             tmem_load_wait();
 #pragma unroll
-                            for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * (by * v_by));
+                            for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * by.out);
                             tmem_store16(at_o + i, o);
                         }
                     }
-                    ref = to;
-                    if (v_up) vref = v_most;
                 }
                 // a weight times its page's scale over 2^vref is one power of
-                // two; the sum of the weights takes the scale out again.  Not
-                // under 2^-100: a page of zeros still has weights.
-                const float shift = ref == -inf_f() ? 0.0f : -ref, v_shift = vref == -inf_f() ? 0.0f : vref;
+                // two; the sum of the weights takes the scale out again
+                const float shift = ref == -inf_f() ? 0.0f : -ref;
 #pragma unroll
                 for (int from = 0; from < kStep; from += kHold) {
                     if (from) {
@@ -340,9 +336,7 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
                     }
 #pragma unroll
                     for (int i = from / P; i < (from + kHold) / P; ++i) {
-                        float f = st.v_log[slot][i] - v_shift;
-                        f = f < -100.0f ? -100.0f : f;
-                        const float d = shift + f;
+                        const float f = page_shift(st.v_log[slot][i], vref), d = shift + f;
                         const float2 by = make_float2(c[i], c[i]), add = make_float2(d, d);
                         float2 l[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
@@ -374,7 +368,8 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
         if (alive && my_steps) alive = bar_wait_all(shared_address(&st.o_done[t]), (my_steps - 1) & 1);
         tmem_fence_after();
         const bool bad = !alive || s.kept < 0;
-        const float scale = bad ? nan_f() : count > 1 ? exp2f(vref) : sum == 0.0f ? 0.0f : exp2f(vref) / sum;
+        const float v_scale = exp2f(vref - kSlack);                     // 2^vref may be too large for 32 bits where its product is not
+        const float scale = bad ? nan_f() : count > 1 ? v_scale : sum == 0.0f ? 0.0f : v_scale / sum;
         const bool nothing = !bad && sum == 0.0f;                       // no token seen (O may not have been written)
         const long long out = token * p.out_token + (long long)head * p.out_head;
         const Partial rest = partial_of(p, token * p.heads + head, count, part);
@@ -392,7 +387,7 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
                 for (int q = 0; q < 32; q += 4) {
                     float f[4];
 #pragma unroll
-                    for (int a = 0; a < 4; ++a) f[a] = nothing ? 0.0f : __uint_as_float(r[q + a]) * scale;
+                    for (int a = 0; a < 4; ++a) f[a] = nothing ? 0.0f : __uint_as_float(r[q + a]) * scale * kSlackFactor;
                     *reinterpret_cast<float4*>(rest.sums + i + q) = make_float4(f[0], f[1], f[2], f[3]);
                 }
             } else if (wide) {
@@ -400,7 +395,7 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
                 for (int q = 0; q < 32; q += 8) {
                     float f[8];
 #pragma unroll
-                    for (int a = 0; a < 8; ++a) f[a] = nothing ? 0.0f : __uint_as_float(r[q + a]) * scale;
+                    for (int a = 0; a < 8; ++a) f[a] = nothing ? 0.0f : __uint_as_float(r[q + a]) * scale * kSlackFactor;
                     uint4* to = reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + out + i + q);
                     if (p.type == VDT_F16) {
                         Vec16<__half> v;
@@ -414,7 +409,7 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
                 }
             } else {
 #pragma unroll
-                for (int q = 0; q < 32; ++q) store_value(p.out, out + i + q, p.type, nothing ? 0.0f : __uint_as_float(r[q]) * scale);
+                for (int q = 0; q < 32; ++q) store_value(p.out, out + i + q, p.type, nothing ? 0.0f : __uint_as_float(r[q]) * scale * kSlackFactor);
             }
         }
     } else if (warp < Sh::kIssue) {
@@ -541,15 +536,11 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
             const int slot = j % kAhead;
             alive = bar_wait_all(shared_address(&st.list_free[slot]), (j / kAhead & 1) ^ 1);
             if (!alive) break;
-            float m = vs > 0.0f ? log2f(vs) : vs == 0.0f || no == -1 ? -inf_f() : nan_f();
+            const float m = vs > 0.0f ? log2f(vs) : vs == 0.0f || no == -1 ? -inf_f() : nan_f();
             if (on) {
                 st.k_scale[slot][lane] = ks;
                 st.v_log[slot][lane] = m;
             }
-            m = m == m && on ? m : -inf_f();
-#pragma unroll
-            for (int d = 1; d < kPages; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            if (lane == 0) st.v_most[slot] = m;
             __syncwarp();
             if (lane == 0) bar_arrive(shared_address(&st.list_full[slot]));
             const int now = no;
