@@ -1,4 +1,4 @@
-"""The sequence operators where their bounds lie: values of very different size in one cache.
+"""The sequence operators where their bounds lie: values of very different size in one cache, streams of the caller's own.
 
 Tolerances are derived as in test_gpu_seq.py; each test states what it adds.
 """
@@ -112,3 +112,71 @@ def test_attention_over_values_that_are_all_zero_then_not(S, new):
     for power in (0, -30):
         cache.v_scale[table[0][9]] = 2.0 ** power
         strict(S, q, cache, table, [kept], [new], False, 0.02, page)
+
+
+# ---------------------------------------------------------------- streams --
+def calls(S):
+    """Every call that copies or allocates."""
+    x = normal(1, 96, 64, kind=torch.bfloat16).cuda()
+    w, ws = S.quantize_rows(normal(2, 48, 96).cuda())
+    codes, scale = S.quantize_rows(x.T)
+    table, pages = make_table([200], 32)
+    cache = make_cache(S, pages, 2, 64, 32)
+    q = normal(3, 150, 4, 64, kind=torch.bfloat16).cuda()
+    rope, at = S.rope_table(300, 64), torch.arange(150, dtype=torch.int32, device="cuda")
+    pt, kept = ints(table), ints([200])
+    packed, new = ints([0, 200]), ints([0, 150])
+    return {
+        "quantize_rows": lambda s: S.quantize_rows(x.T, stream=s),
+        "quantize_rows of few": lambda s: S.quantize_rows(x[:, :3].T, stream=s),
+        "int8_linear": lambda s: S.int8_linear(x.T, w, ws, stream=s),
+        "int8_linear of few": lambda s: S.int8_linear(x[:, :3].T, w, ws, stream=s),
+        "int8_matmul": lambda s: S.int8_matmul(codes, scale, w, ws, stream=s),
+        "rope_table": lambda s: S.rope_table(300, 64, stream=s),
+        "qk_norm_rope": lambda s: S.qk_norm_rope(q, q[:, :2], None, None, at, rope, stream=s),
+        "cache_load": lambda s: S.cache_load(cache, pt, kept, packed, 200, 200, stream=s),
+        "cache_attention": lambda s: S.cache_attention(q, cache, pt, kept, new, 150, 200, stream=s),
+        "cache_attention of one": lambda s: S.cache_attention(q[:1], cache, pt, kept, ints([0, 1]), 1, 3000, stream=s),
+    }
+
+
+def flat(result):
+    return [t.clone() for t in (result if isinstance(result, tuple) else (result,))]
+
+
+def test_calls_on_a_stream_of_their_own_with_work_queued_on_the_current_one(S):
+    """The inputs are there; the current stream is busy for some 20 ms, and behind that writes blocks that were let go:
+    nothing of a call on another stream may wait there or lie in those blocks."""
+    side = torch.cuda.Stream()
+    for name, call in calls(S).items():
+        want = flat(call(None))
+        torch.cuda.synchronize()
+        for handle in (side.cuda_stream, 0):
+            current = torch.cuda.Stream() if handle == 0 else torch.cuda.current_stream()
+            with torch.cuda.stream(current):
+                torch.cuda._sleep(40_000_000)
+                for n in (1 << 8, 1 << 12, 1 << 14, 1 << 16, 1 << 18, 1 << 20):
+                    for _ in range(4):
+                        torch.full((n,), -7, dtype=torch.int8, device="cuda")     # blocks whose last kernel is still queued
+                got = call(handle)
+            torch.cuda.synchronize()
+            for g, t in zip(flat(got), want):
+                assert torch.equal(g, t), (name, handle)
+
+
+def test_a_result_of_another_stream_may_be_used_and_let_go_on_the_current_one(S):
+    """Its block is not given out again to that stream while the current one reads it."""
+    side = torch.cuda.Stream()
+    w, ws = S.quantize_rows(normal(2, 700, 512).cuda())
+    x = normal(1, 333, 512, kind=torch.bfloat16).cuda()
+    want = S.int8_linear(x, w, ws)
+    torch.cuda.synchronize()
+    y = S.int8_linear(x, w, ws, stream=side.cuda_stream)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda._sleep(40_000_000)
+    kept = y.clone()                                      # queued behind the sleep
+    del y
+    for _ in range(4):
+        S.int8_linear(-x, w, ws, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(kept, want)

@@ -10,9 +10,10 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
-#include <initializer_list>
+#include <optional>
 #include <string>
 
 #include "vdttfs.h"
@@ -105,20 +106,36 @@ Tensor room(at::IntArrayRef size, at::ScalarType type, at::Device device) {
     return Tensor(at::detail::empty_cuda(size, type, device, std::nullopt));
 }
 
-// The call's stream; what the call allocated is tied to one that is not torch's own
-void* stream_of(PyObject* o, at::Device device, std::initializer_list<const Tensor*> made) {
-    if (o == Py_None) return c10::cuda::getCurrentCUDAStream(device.index()).stream();
-    void* handle = PyLong_AsVoidPtr(o);
-    if (!handle && PyErr_Occurred()) {
-        PyErr_Clear();
-        CHECK_TYPE(false, "stream: a raw handle is wanted");
+// The call's stream.  One of the caller's own is torch's current one for the
+// length of the call: copies that the call makes of its inputs run on it, and
+// what the call allocates comes from that stream's memory.  A block of another
+// stream's could still be in use by what is queued there.
+class OnStream {
+public:
+    OnStream(PyObject* o, at::Device device) : before_(c10::cuda::getCurrentCUDAStream(device.index())), handle_(before_.stream()) {
+        if (o == Py_None) return;
+        handle_ = PyLong_AsVoidPtr(o);
+        if (!handle_ && PyErr_Occurred()) {
+            PyErr_Clear();
+            CHECK_TYPE(false, "stream: a raw handle is wanted");
+        }
+        if (handle_ == before_.stream()) return;
+        guard_.emplace(handle_ ? c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(handle_), device.index())
+                               : c10::cuda::getDefaultCUDAStream(device.index()));
     }
-    const auto s = handle ? c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(handle), device.index())
-                          : c10::cuda::getDefaultCUDAStream(device.index());
-    for (const Tensor* t : made)
-        if (t && t->defined() && t->numel()) t->record_stream(s.unwrap());
-    return handle;
-}
+    void* handle() const { return handle_; }
+    // A result that the call made: it may go on on the stream that was current,
+    // so its memory waits for that one, too, once it is let go
+    const Tensor& result(const Tensor& t) const {
+        if (guard_ && t.defined() && t.numel()) t.record_stream(before_.unwrap());
+        return t;
+    }
+
+private:
+    c10::cuda::CUDAStream before_;
+    void* handle_;
+    std::optional<c10::cuda::CUDAStreamGuard> guard_;
+};
 
 template <typename T = void>
 T* at_or_null(const Tensor& t) {
@@ -196,14 +213,14 @@ PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const int type = type_of(x.scalar_type(), "x");
     const int64_t rows = x.size(0), cols = x.size(1);
     CHECK_VALUE(cols > 0 && cols <= INT32_MAX, "x: no columns, or too many");
+    const OnStream on(a[1], x.device());
     if (x.stride(1) != 1 || (rows > 1 && x.stride(0) < cols)) x = x.contiguous();
     const int64_t step = (cols + 15) / 16 * 16;
     const Tensor codes = room({rows, step}, at::kChar, x.device()), scale = room({rows}, at::kFloat, x.device());
-    void* s = stream_of(a[1], x.device(), {&codes, &scale, &x});
     if (const int e = vdt_quantize_rows(x.data_ptr(), type, rows, (int)cols, x.stride(0), static_cast<int8_t*>(codes.data_ptr()), step,
-                                        static_cast<float*>(scale.data_ptr()), s))
+                                        static_cast<float*>(scale.data_ptr()), on.handle()))
         return status_error(e, "vdt_quantize_rows");
-    return pair(codes.narrow(1, 0, cols), scale);
+    return pair(on.result(codes).narrow(1, 0, cols), on.result(scale));
     END_HANDLE_TH_ERRORS
 }
 
@@ -213,17 +230,17 @@ PyObject* int8_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const Tensor &x = tensor(a[0], "a"), &xs = tensor(a[1], "a_scale"), &w = tensor(a[2], "w"), &ws = tensor(a[3], "w_scale");
     const Tensor &bias = tensor_or_none(a[4], "bias"), &given = tensor_or_none(a[6], "out");
     code_rows(x, "a");
+    const OnStream on(a[7], x.device());
     const int64_t rows = x.size(0);
     flat(xs, "a_scale", at::kFloat, rows);
     const Tensor out = product_out(rows, x.size(1), w, ws, bias, given, given.defined() ? given.scalar_type() : dtype(a[5], "out_dtype"));
     const int type = type_of(out.scalar_type(), "out");
-    void* s = stream_of(a[7], x.device(), {given.defined() ? nullptr : &out});
     const int n = (int)w.size(0);
     if (const int e = vdt_int8_matmul(static_cast<int8_t*>(x.data_ptr()), row_stride(x), at_or_null<float>(xs),
                                       static_cast<int8_t*>(w.data_ptr()), row_stride(w), at_or_null<float>(ws), at_or_null<float>(bias),
-                                      rows, n, (int)x.size(1), type, out.data_ptr(), std::max<int64_t>(out.stride(0), n), s))
+                                      rows, n, (int)x.size(1), type, out.data_ptr(), std::max<int64_t>(out.stride(0), n), on.handle()))
         return status_error(e, "vdt_int8_matmul");
-    return THPVariable_Wrap(out);
+    return THPVariable_Wrap(given.defined() ? out : on.result(out));
     END_HANDLE_TH_ERRORS
 }
 
@@ -234,6 +251,7 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const Tensor &w = tensor(a[1], "w"), &ws = tensor(a[2], "w_scale"), &bias = tensor_or_none(a[3], "bias");
     const Tensor& given = tensor_or_none(a[5], "out");
     on_device(x, "x", 2);
+    const OnStream on(a[6], x.device());
     const int type = type_of(x.scalar_type(), "x");
     const int64_t rows = x.size(0), inner = x.size(1);
     const Tensor out = product_out(rows, inner, w, ws, bias, given,
@@ -242,13 +260,12 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if ((inner > 1 && x.stride(1) != 1) || (rows > 1 && x.stride(0) < inner)) x = x.contiguous();
     const int64_t need = (int64_t)vdt_int8_linear_scratch_bytes(rows, (int)inner);
     const Tensor scratch = room({need}, at::kByte, x.device());
-    void* s = stream_of(a[6], x.device(), {&scratch, &x, given.defined() ? nullptr : &out});
     const int n = (int)w.size(0);
     if (const int e = vdt_int8_linear(x.data_ptr(), type, std::max(x.stride(0), inner), static_cast<int8_t*>(w.data_ptr()), row_stride(w),
                                       at_or_null<float>(ws), at_or_null<float>(bias), rows, n, (int)inner, out_type, out.data_ptr(),
-                                      std::max<int64_t>(out.stride(0), n), scratch.data_ptr(), (size_t)need, s))
+                                      std::max<int64_t>(out.stride(0), n), scratch.data_ptr(), (size_t)need, on.handle()))
         return status_error(e, "vdt_int8_linear");
-    return THPVariable_Wrap(out);
+    return THPVariable_Wrap(given.defined() ? out : on.result(out));
     END_HANDLE_TH_ERRORS
 }
 
@@ -278,6 +295,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
         flat(table, "table", at::kFloat, n * rot);
         flat(at, "positions", at::kInt, tokens);
     }
+    const OnStream on(a[11], q.device());
     Tensor out[2];
     const Tensor* in[2] = {&q, &k};
     const Tensor* given[2] = {&given_q, &given_k};
@@ -294,14 +312,17 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
                               q.scalar_type(), " is wanted");
         }
     }
-    void* s = stream_of(a[11], q.device(), {mine ? &out[0] : nullptr, mine ? &out[1] : nullptr});
     auto stride = [](const Tensor& t, int i) { return t.defined() ? t.stride(i) : 0; };
     if (const int e = vdt_qk_norm_rope(q.data_ptr(), q.stride(0), q.stride(1), at_or_null(k), stride(k, 0), stride(k, 1), at_or_null(wq),
                                        at_or_null(wk), rot ? at_or_null<int32_t>(at) : nullptr, rot ? at_or_null<float>(table) : nullptr, (int)n,
                                        (int)rot, layout, norm, (float)number(a[8], "eps"), tokens, (int)q.size(1), (int)kv, (int)dim, type,
                                        out[0].data_ptr(), out[0].stride(0), out[0].stride(1), at_or_null(out[1]), stride(out[1], 0),
-                                       stride(out[1], 1), s))
+                                       stride(out[1], 1), on.handle()))
         return status_error(e, "vdt_qk_norm_rope");
+    if (mine) {
+        on.result(out[0]);
+        on.result(out[1]);
+    }
     if (!out[1].defined()) {
         PyObject* x = THPVariable_Wrap(out[0]);
         PyObject* t = x ? PyTuple_Pack(2, x, Py_None) : nullptr;
@@ -360,10 +381,10 @@ PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t count) {
     CHECK_VALUE(k.size(1) == c.heads && v.size(1) == c.heads && v.size(0) == total && v.scalar_type() == k.scalar_type(),
                       "k and v: [tokens, ", c.heads, ", ", c.dim, "] of one type are wanted, got ", k.sizes(), " of ", k.scalar_type(), " and ",
                       v.sizes(), " of ", v.scalar_type());
-    void* s = stream_of(a[7], k.device(), {});
+    const OnStream on(a[7], k.device());
     const int most = (int)std::min<int64_t>(small_integer(a[6], "most"), total);
     if (const int e = vdt_cache_append(&c, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), type, r.pages,
-                                       r.width, r.held, r.starts, r.seqs, total, most, s))
+                                       r.width, r.held, r.starts, r.seqs, total, most, on.handle()))
         return status_error(e, "vdt_cache_append");
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
@@ -380,11 +401,11 @@ PyObject* cache_load(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const at::ScalarType type = dtype(a[6], "dtype");
     const int kind = type_of(type, "dtype");
     const at::Device device = tensor(PyTuple_GET_ITEM(a[0], 0), "cache keys").device();
+    const OnStream on(a[7], device);
     const Tensor k = room({total, c.heads, c.dim}, type, device), v = room({total, c.heads, c.dim}, type, device);
-    void* s = stream_of(a[7], device, {&k, &v});
-    if (const int e = vdt_cache_load(&c, r.pages, r.width, r.held, r.starts, r.seqs, total, most, kind, k.data_ptr(), v.data_ptr(), s))
+    if (const int e = vdt_cache_load(&c, r.pages, r.width, r.held, r.starts, r.seqs, total, most, kind, k.data_ptr(), v.data_ptr(), on.handle()))
         return status_error(e, "vdt_cache_load");
-    return pair(k, v);
+    return pair(on.result(k), on.result(v));
     END_HANDLE_TH_ERRORS
 }
 
@@ -399,6 +420,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const int type = type_of(q.scalar_type(), "q");
     const int most = (int)std::min<int64_t>(small_integer(a[5], "most"), total), most_kept = small_integer(a[6], "most_kept");
     const Tensor& given = tensor_or_none(a[9], "out");
+    const OnStream on(a[10], q.device());
     const Tensor out = given.defined() ? given : room(q.sizes(), q.scalar_type(), q.device());
     if (given.defined()) {
         heads(out, "out", c.dim);
@@ -407,12 +429,11 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)c.dim) : number(a[8], "scale");
     const size_t need = vdt_cache_attention_scratch_bytes(total, (int)n, c.heads, c.dim, r.seqs, most, most_kept);
     const Tensor scratch = need ? room({(int64_t)need}, at::kByte, q.device()) : Tensor();
-    void* s = stream_of(a[10], q.device(), {&scratch, given.defined() ? nullptr : &out});
     if (const int e = vdt_cache_attention(&c, q.data_ptr(), q.stride(0), q.stride(1), (int)n, type, r.pages, r.width, r.held, r.starts, r.seqs,
                                           total, most, most_kept, truth(a[7]), (float)scale, out.data_ptr(), out.stride(0), out.stride(1),
-                                          at_or_null(scratch), need, s))
+                                          at_or_null(scratch), need, on.handle()))
         return status_error(e, "vdt_cache_attention");
-    return THPVariable_Wrap(out);
+    return THPVariable_Wrap(given.defined() ? out : on.result(out));
     END_HANDLE_TH_ERRORS
 }
 

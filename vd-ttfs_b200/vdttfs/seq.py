@@ -16,9 +16,11 @@ cache_attention        attention over it, causal or not                    vdt_c
 
 Inference only, like the rest of the package.  Tensors are CUDA tensors of the
 current device; a call runs on ``stream`` (a raw handle) or torch's current
-stream.  With a ``stream`` of the caller's own, what the call allocates is
-tied to that stream; ordering the inputs is the caller's.  Tensors that do not
-fit raise ValueError, what the library refuses raises VdtError.
+stream.  A ``stream`` of the caller's own is the current one for the length of
+the call, with all that the call copies and allocates; the results' memory also
+waits for the stream that was current.  Ordering the inputs before the call, and
+keeping them until it is done, is the caller's.  Tensors that do not fit raise
+ValueError, what the library refuses raises VdtError.
 """
 from __future__ import annotations
 
@@ -65,13 +67,17 @@ def rope_table(positions, rot, base=10000.0, scaling="none", factor=1.0, trained
     that bound the ramp), for contexts ``factor`` times as long as the trained one."""
     if scaling not in SCALINGS:
         raise ValueError(f"scaling: one of {sorted(SCALINGS)}, got {scaling!r}")
-    table = torch.empty((positions, rot), dtype=torch.float32, device=device or "cuda")
-    if stream is None:
-        stream = torch.cuda.current_stream().cuda_stream
+    before = torch.cuda.current_stream()
+    if stream is None or stream == before.cuda_stream:
+        on = before
     else:
-        table.record_stream(torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream())
-    check(lib().vdt_rope_table(positions, rot, base, SCALINGS[scaling], factor, trained, fast, slow, table.data_ptr(), stream),
-          "vdt_rope_table")
+        on = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+    with torch.cuda.stream(on):
+        table = torch.empty((positions, rot), dtype=torch.float32, device=device or "cuda")
+        check(lib().vdt_rope_table(positions, rot, base, SCALINGS[scaling], factor, trained, fast, slow, table.data_ptr(), on.cuda_stream),
+              "vdt_rope_table")
+    if on is not before and table.is_cuda:
+        table.record_stream(before)
     return table
 
 
