@@ -421,7 +421,8 @@ enum { VDT_F32 = 0, VDT_F16 = 1, VDT_BF16 = 2 };
 /* Codes of rows: scale[i] = max_k |x[i][k]| * (1/127) (32-bit product),
    codes[i][k] = x / scale rounded to nearest even, in -127..127.  A row of
    zeros has scale 0 and codes 0; one with an infinity or NaN a scale that is
-   not finite (its products are NaN).  type: VDT_F32 / VDT_F16 / VDT_BF16. */
+   not finite (its products are NaN).  type: VDT_F32 / VDT_F16 / VDT_BF16.
+   d_codes must not lie over d_x. */
 int vdt_quantize_rows(const void* d_x, int type, int64_t rows, int cols, int64_t x_stride, int8_t* d_codes,
                       int64_t codes_stride, float* d_scale, vdt_stream stream);
 
@@ -430,7 +431,7 @@ int vdt_quantize_rows(const void* d_x, int type, int64_t rows, int cols, int64_t
    rows start on 16-byte boundaries (strides multiples of 16) and whose last
    row's storage reaches to the next multiple of 16 bytes; what lies between
    `inner` and there does not matter.  inner <= 131072: the sums are exact
-   32-bit integers. */
+   32-bit integers.  d_out must not lie over a or w. */
 int vdt_int8_matmul(const int8_t* d_a, int64_t a_stride, const float* d_a_scale, const int8_t* d_w,
                     int64_t w_stride, const float* d_w_scale, const float* d_bias, int64_t rows, int cols,
                     int inner, int out_type, void* d_out, int64_t out_stride, vdt_stream stream);
@@ -438,7 +439,8 @@ int vdt_int8_matmul(const int8_t* d_a, int64_t a_stride, const float* d_a_scale,
 /* The two together for rows x [rows, inner] of `type`: each row's codes into
    d_scratch (256-byte aligned, vdt_int8_linear_scratch_bytes; VDT_ERR_CAPACITY
    when smaller), then the product; a few rows are rounded by the product's
-   own kernel. */
+   own kernel, which does not use the scratch.  d_out may lie over d_x, whose
+   rows are all read before the first is written. */
 size_t vdt_int8_linear_scratch_bytes(int64_t rows, int inner);
 int vdt_int8_linear(const void* d_x, int type, int64_t x_stride, const int8_t* d_w, int64_t w_stride,
                     const float* d_w_scale, const float* d_bias, int64_t rows, int cols, int inner, int out_type,

@@ -1,4 +1,4 @@
-"""The sequence operators where their bounds lie: values of very different size in one cache, streams of the caller's own.
+"""The sequence operators where their bounds lie: values of very different size in one cache, streams of the caller's own, results in place.
 
 Tolerances are derived as in test_gpu_seq.py; each test states what it adds.
 """
@@ -180,3 +180,25 @@ def test_a_result_of_another_stream_may_be_used_and_let_go_on_the_current_one(S)
         S.int8_linear(-x, w, ws, stream=side.cuda_stream)
     torch.cuda.synchronize()
     assert torch.equal(kept, want)
+
+
+# ---------------------------------------------------------------- in place --
+@pytest.mark.parametrize("kind", list(U))
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 12, 40, 200])
+def test_linear_into_its_own_rows(S, kind, rows):
+    """A few rows are read by every CTA of the product, whose outputs must not stand there yet."""
+    for n in (64, 1024, 1000):
+        x = normal(rows, rows, n, kind=kind).cuda()
+        w, ws = S.quantize_rows(normal(1, n, n).cuda())
+        want = S.int8_linear(x, w, ws)
+        for _ in range(5):
+            y = x.clone()
+            assert S.int8_linear(y, w, ws, out=y) is not None and torch.equal(y, want)
+        # an output that begins inside the rows, of the type of twice or half the size
+        other = torch.float32 if kind != torch.float32 else torch.bfloat16
+        room = torch.zeros(rows * n * 4 + 4096, dtype=torch.uint8, device="cuda")
+        y = room[: rows * n * x.element_size()].view(kind).view(rows, n)
+        y.copy_(x)
+        out = room[2048: 2048 + rows * n * other.itemsize].view(other).view(rows, n)
+        S.int8_linear(y, w, ws, out=out)
+        assert torch.equal(out, S.int8_linear(x, w, ws, out_dtype=other))

@@ -31,6 +31,11 @@ int check_product(const int8_t* d_w, int64_t w_stride, const float* d_w_scale, i
     return VDT_OK;
 }
 
+// whether two buffers of rows share any byte
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
 int64_t code_stride(int inner) { return ((int64_t)inner + 15) / 16 * 16; }
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
@@ -113,7 +118,11 @@ extern "C" int vdt_int8_linear(const void* d_x, int type, int64_t x_stride, cons
         return api_fail(VDT_ERR_CAPACITY, "scratch smaller than vdt_int8_linear_scratch_bytes");
     if (int s = api_check_buffers(-1, {d_x, d_w, d_w_scale, d_bias, d_out, d_scratch})) return s;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (int8_rounds_itself(rows, inner)) {              // a few rows: the scratch is not used
+    // a few rows: the scratch is not used; every CTA reads all of them, so not
+    // into an output that lies over them
+    const bool over = overlap(d_x, ((rows - 1) * x_stride + inner) * type_size(type), d_out,
+                              ((rows - 1) * out_stride + cols) * type_size(out_type));
+    if (int8_rounds_itself(rows, inner) && !over) {
         Int8Params p{nullptr, nullptr, d_w, d_w_scale, d_bias, d_out, rows, 0, w_stride, out_stride, cols, inner, out_type, d_x, x_stride};
         return launched(launch_int8_own(p, type, st), "int8_linear");
     }

@@ -55,7 +55,7 @@ def int8_linear(x, w, w_scale, bias=None, out_dtype=None, out=None, stream=None)
     """x [rows, k] (float32, float16 or bfloat16), w [n, k] int8 and w_scale [n]
     from quantize_rows, bias [n] float32 or None: each row of x is rounded to 8
     bits under its own scale and multiplied.  Returns [rows, n], of x's type
-    unless out_dtype or out says otherwise."""
+    unless out_dtype or out says otherwise; out may be x, or lie over it."""
     return _seq.int8_linear(x, w, w_scale, bias, out_dtype, out, stream)
 
 
