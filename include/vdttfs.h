@@ -509,8 +509,10 @@ int vdt_cache_append(const vdt_cache8* cache, const void* d_k, int64_t k_token, 
                      vdt_stream stream);
 
 /* The sequences' d_kept[s] tokens as values of `type`, packed at d_starts[s]
-   into k, v [total, heads, dim] (contiguous, 16-byte aligned).  Tokens of pages that are not
-   in the cache become NaN. */
+   into k, v [total, heads, dim] (contiguous, 16-byte aligned).  Tokens of pages
+   that are not in the cache become NaN, and so do all rows of a sequence that
+   has more tokens than its run has rows or than `most`, or whose run does not
+   fit `total`.  Rows behind a sequence's tokens, and of no sequence, are left. */
 int vdt_cache_load(const vdt_cache8* cache, const int32_t* d_pages, int width, const int32_t* d_kept,
                    const int32_t* d_starts, int seqs, int64_t total, int most, int type, void* d_k, void* d_v,
                    vdt_stream stream);
@@ -520,8 +522,9 @@ int vdt_cache_load(const vdt_cache8* cache, const int32_t* d_pages, int width, c
    consecutive heads share one).  causal: the queries are their sequence's last
    tokens and see those up to themselves; else they see all d_kept[s] of them
    (an encoder's states).  most_kept bounds d_kept.  A query that sees no token
-   gives 0.  A sequence with more tokens than most_kept or its table hold, and
-   rows that see a page that is not in the cache, give NaN.  d_scratch:
+   gives 0.  A sequence with more tokens than most_kept or its table hold, a run
+   of queries that does not fit `most` or `total`, and rows that see a page that
+   is not in the cache give NaN.  Rows of no sequence are left.  d_scratch:
    vdt_cache_attention_scratch_bytes (may be 0), 16-byte aligned. */
 size_t vdt_cache_attention_scratch_bytes(int64_t total, int heads, int kv_heads, int dim, int seqs, int most,
                                          int most_kept);

@@ -1,4 +1,4 @@
-"""The sequence operators where their bounds lie: values of very different size in one cache, streams of the caller's own, results in place.
+"""The sequence operators where their bounds lie: values of very different size in one cache, streams of the caller's own, results in place, lengths beyond the bounds.
 
 Tolerances are derived as in test_gpu_seq.py; each test states what it adds.
 """
@@ -202,3 +202,73 @@ def test_linear_into_its_own_rows(S, kind, rows):
         out = room[2048: 2048 + rows * n * other.itemsize].view(other).view(rows, n)
         S.int8_linear(y, w, ws, out=out)
         assert torch.equal(out, S.int8_linear(x, w, ws, out_dtype=other))
+
+
+# ------------------------------------------------- lengths beyond the bounds --
+@pytest.mark.parametrize("new", [2, 40, 300])
+@pytest.mark.parametrize("kept", [100, 3000])
+def test_attention_of_runs_beyond_the_bounds_gives_nan(S, new, kept):
+    """A run of more queries than was said, or one that ends outside the rows: NaN there, the other sequences as they are."""
+    table, pages = make_table([kept] * 3, 64)
+    cache = make_cache(S, pages, 2, 64, 64)
+    q = normal(1, 3 * new, 4, 64, kind=torch.bfloat16).cuda()
+    args = (ints(table), ints([kept] * 3))
+    good = S.cache_attention(q, cache, *args, ints([0, new, 2 * new, 3 * new]), new, kept)
+    for starts, most, broken in (([0, new, 2 * new + 1, 3 * new], new, slice(new, 2 * new + 1)),
+                                 ([0, new - 1, 2 * new, 3 * new], new, slice(new - 1, 2 * new)),
+                                 ([0, new, 2 * new, 3 * new + 1], new + 1, slice(2 * new, 3 * new)),
+                                 ([-1, new, 2 * new, 3 * new], new + 1, slice(0, new))):
+        out = torch.full_like(q, 7)
+        S.cache_attention(q, cache, *args, ints(starts), most, kept, out=out)
+        assert torch.isnan(out[broken]).all()
+        whole = torch.ones(3 * new, dtype=torch.bool)
+        whole[broken] = False
+        assert torch.isfinite(out[whole.cuda()]).all()
+        for b in range(3):                                # sequences of the lengths that `good` has
+            if starts[b] == b * new and starts[b + 1] == (b + 1) * new and most == new:
+                assert torch.equal(out[starts[b]: starts[b + 1]], good[starts[b]: starts[b + 1]])
+
+
+def test_attention_leaves_rows_of_no_sequence(S):
+    for new in (3, 50):
+        table, pages = make_table([90], 16)
+        cache = make_cache(S, pages, 1, 64, 16)
+        q = normal(1, new + 4, 2, 64, kind=torch.float16).cuda()
+        out = torch.full_like(q, 7)
+        S.cache_attention(q, cache, ints(table), ints([90]), ints([1, new + 1]), new, 90, out=out)
+        assert (out[0] == 7).all() and (out[new + 1:] == 7).all() and not (out[1: new + 1] == 7).all()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("kind,code", [(torch.float32, 0), (torch.float16, 1), (torch.bfloat16, 2)])
+def test_load_of_lengths_beyond_the_bounds_gives_nan(S, kind, code, page):
+    """More tokens than the run has rows or than was said, or a run that ends outside: NaN there, other sequences whole."""
+    import ctypes as C
+    from vdttfs import _lib
+    heads, dim, n = 2, 64, 70
+    table, pages = make_table([n] * 3, page)
+    cache = make_cache(S, pages, heads, dim, page)
+    pt = ints(table)
+    desc = _lib.Cache8Desc(*(t.data_ptr() for t in cache), pages, page, heads, dim)
+    good = S.cache_load(cache, pt, ints([n] * 3), ints(sums([n] * 3)), 3 * n, n, kind)
+
+    def load(kept, starts, total, most):
+        k, v = (torch.full((total, heads, dim), 7, dtype=kind, device="cuda") for _ in range(2))
+        lengths, rows = ints(kept), ints(starts)
+        assert _lib.lib().vdt_cache_load(C.byref(desc), pt.data_ptr(), pt.shape[1], lengths.data_ptr(), rows.data_ptr(), 3, total, most, code,
+                                         k.data_ptr(), v.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        return k, v
+
+    for out, want in zip(load([n] * 3, [0, n, 2 * n, 3 * n], 3 * n, n), good):
+        assert torch.equal(out, want)
+    for kept, starts, most, broken in (([n, n, n], [0, n, 2 * n - 1, 3 * n - 1], n, (1,)), ([n, n, n], [0, n, 2 * n, 3 * n], n - 1, (0, 1, 2)),
+                                       ([5, n, 5], [0, n, 2 * n, 3 * n], 20, (1,)), ([n, n, n], [0, n, 2 * n, 3 * n + 1], n, (2,)),
+                                       ([n, n, n], [-1, n, 2 * n, 3 * n], n, (0,))):
+        for out, want in zip(load(kept, starts, 3 * n, most), good):
+            for b in range(3):
+                rows = out[max(starts[b], 0): starts[b + 1]]
+                if b in broken:
+                    assert torch.isnan(rows).all()
+                else:
+                    assert torch.equal(rows[: kept[b]], want[b * n: b * n + kept[b]]) and (rows[kept[b]:] == 7).all()

@@ -59,6 +59,24 @@ __device__ __forceinline__ void store_value(void* p, long long i, int type, floa
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
 }
 
+// A run of queries that does not fit the buffers or `most` is not computed: NaN
+// to those of its rows that there are, for the heads that share head h of the
+// cache.  All threads of one CTA.  Out of line, and given single values: a
+// reference to the kernel's parameters would put all of them on the stack (7%
+// of the kernels' time).
+static __device__ __noinline__ void spoil_rows(void* out, int type, long long token, long long head, long long first, long long end, int head0,
+                                               int group, int dim) {
+    for (long long i = threadIdx.x; i < (end - first) * group * dim; i += blockDim.x) {
+        const int at = (int)(i % (group * dim));
+        store_value(out, (first + i / (group * dim)) * token + (head0 + at / dim) * head + at % dim, type, nan_f());
+    }
+}
+__device__ __forceinline__ void spoil_run(const AttendParams& p, int b, int h) {
+    const long long first = max((long long)p.r.starts[b], 0LL), end = min((long long)p.r.starts[b + 1], p.r.total);
+    const int group = p.heads / p.c.heads;
+    spoil_rows(p.out, p.type, p.out_token, p.out_head, first, end, h * group, group, p.c.dim);
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -131,7 +131,10 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
     const int tile = blockIdx.y / p.c.heads, h = blockIdx.y % p.c.heads;
     const Queries s = queries_of(p, b);
     const int rows = s.rows * group - tile * kRows;           // rows of this tile
-    if (rows <= 0) return;
+    if (rows <= 0) {
+        if (s.rows == 0 && blockIdx.x == 0 && tile == 0) spoil_run(p, b, h);       // nothing to do for an empty run
+        return;
+    }
     const bool split = gridDim.x > 1;
     // tokens that a row sees: all, or up to its own place at the sequence's end
     auto sees = [&](int r) {

@@ -139,7 +139,10 @@ __global__ void __launch_bounds__(Shape<D, NT, P>::kThreads, Shape<D, NT, P>::kP
     const int part = blockIdx.x % count, row0 = (gridDim.x / count - 1 - blockIdx.x / count) * (NT * kTile);
     const Queries s = queries_of(p, b);
     const int rows = s.rows * group;
-    if (row0 >= rows) return;
+    if (row0 >= rows) {
+        if (rows == 0 && blockIdx.x == 0) spoil_run(p, b, h);          // nothing to do for an empty run
+        return;
+    }
     auto sees = [&](int r) {                       // tokens that row r of the sequence sees
         if (r >= rows || s.kept < 0) return 0;
         return p.causal ? max(0, s.kept - s.rows + r / group + 1) : s.kept;

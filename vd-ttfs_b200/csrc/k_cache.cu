@@ -241,8 +241,15 @@ __global__ void __launch_bounds__(kCacheThreads) k_cache_load(vdt_cache8 c, Cach
     const int b = blockIdx.z, h = blockIdx.y - (side ? c.heads : 0), j = blockIdx.x;
     const long long start = r.starts[b], rows = (long long)r.starts[b + 1] - start;
     const int kept = r.held[b];
+    if (kept > rows || kept > r.most || start < 0 || start + rows > r.total) {
+        // lengths that do not fit the buffers or `most`: NaN to those of the run's rows that there are
+        if (j == 0 && kept > 0)
+            for (long long i = max(start, 0LL) * D + threadIdx.x; i < min(start + rows, r.total) * D; i += kCacheThreads)
+                (side ? v : k)[(i / D * c.heads + h) * D + i % D] = from_f32<T>(__int_as_float(0x7fffffff));
+        return;
+    }
     const int n = min(kept - j * P, P);
-    if (n <= 0 || kept > rows || start < 0 || start + rows > r.total) return;
+    if (n <= 0) return;
     const int no = page_of(r, b, j, c.pages);
     const long long slot = (long long)max(no, 0) * c.heads + h, at = slot * (P * D);
     const float scale = no < 0 ? __int_as_float(0x7fffffff) : (side ? c.v_scale : c.k_scale)[slot];   // a page that is not in the cache: NaN

@@ -122,7 +122,8 @@ def cache_append(cache, k, v, pages, held, starts, most, stream=None):
 
 def cache_load(cache, pages, kept, starts, total, most, dtype=torch.bfloat16, stream=None):
     """The sequences' kept[s] tokens as (k, v) [total, heads, dim], sequence s at
-    rows starts[s]..starts[s + 1]; no sequence has more than ``most``."""
+    rows starts[s]..starts[s + 1]; no sequence has more than ``most``.  One that has,
+    or that does not fit its rows, gives NaN; rows of no token are not written."""
     return _seq.cache_load(cache, pages, kept, starts, total, most, dtype, stream)
 
 
@@ -131,7 +132,8 @@ def cache_attention(q, cache, pages, kept, starts, most, most_kept, causal=True,
     rows starts[s]..starts[s + 1] (at most ``most``), over its kept[s] cached
     tokens (at most ``most_kept``).  causal: the queries are the last tokens of
     their sequence, in the cache already.  scale: 1 / sqrt(dim) unless given.
-    A query that sees nothing gives zeros."""
+    A query that sees nothing gives zeros, a sequence beyond these bounds NaN; rows
+    of no sequence are not written."""
     return _seq.cache_attention(q, cache, pages, kept, starts, most, most_kept, causal, scale, out, stream)
 
 
