@@ -419,10 +419,10 @@ int vdt_measure_peaks(int device, double* fma_per_s, double* l2_read_bytes_per_s
 enum { VDT_F32 = 0, VDT_F16 = 1, VDT_BF16 = 2 };
 
 /* Codes of rows: scale[i] = max_k |x[i][k]| * (1/127) (32-bit product),
-   codes[i][k] = x / scale rounded to nearest even, in -127..127.  A row of
-   zeros has scale 0 and codes 0; one with an infinity or NaN a scale that is
-   not finite (its products are NaN).  type: VDT_F32 / VDT_F16 / VDT_BF16.
-   d_codes must not lie over d_x. */
+   codes[i][k] = x / scale rounded to nearest even, in -127..127; cols up to
+   2^30.  A row of zeros has scale 0 and codes 0; one with an infinity or NaN a
+   scale that is not finite (its products are NaN).  type: VDT_F32 / VDT_F16 /
+   VDT_BF16.  d_codes must not lie over d_x. */
 int vdt_quantize_rows(const void* d_x, int type, int64_t rows, int cols, int64_t x_stride, int8_t* d_codes,
                       int64_t codes_stride, float* d_scale, vdt_stream stream);
 
@@ -431,7 +431,7 @@ int vdt_quantize_rows(const void* d_x, int type, int64_t rows, int cols, int64_t
    rows start on 16-byte boundaries (strides multiples of 16) and whose last
    row's storage reaches to the next multiple of 16 bytes; what lies between
    `inner` and there does not matter.  inner <= 131072: the sums are exact
-   32-bit integers.  d_out must not lie over a or w. */
+   32-bit integers; cols up to 2^30.  d_out must not lie over a or w. */
 int vdt_int8_matmul(const int8_t* d_a, int64_t a_stride, const float* d_a_scale, const int8_t* d_w,
                     int64_t w_stride, const float* d_w_scale, const float* d_bias, int64_t rows, int cols,
                     int inner, int out_type, void* d_out, int64_t out_stride, vdt_stream stream);

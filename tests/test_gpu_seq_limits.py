@@ -272,3 +272,23 @@ def test_load_of_lengths_beyond_the_bounds_gives_nan(S, kind, code, page):
                     assert torch.isnan(rows).all()
                 else:
                     assert torch.equal(rows[: kept[b]], want[b * n: b * n + kept[b]]) and (rows[kept[b]:] == 7).all()
+
+
+# ------------------------------------------------------------------- sizes --
+def test_sizes_beyond_32_bits_are_refused(S):
+    """2^32 + n would otherwise be taken for n."""
+    long = (1 << 32) + 64
+    a, w = (torch.empty(1, long, dtype=torch.int8, device="cuda") for _ in range(2))
+    one = torch.ones(1, device="cuda")
+    with pytest.raises(ValueError):
+        S.int8_matmul(a, one, w, one)
+    with pytest.raises(ValueError):
+        S.int8_linear(a.view(torch.float16)[:, : long // 2].repeat(1, 2), w, one)
+    del a, w
+    x = torch.zeros(1, 1, 64, dtype=torch.float16, device="cuda")
+    many = x.expand(1, (1 << 32) + 8, 64)                 # heads that share their memory
+    with pytest.raises(ValueError):
+        S.qk_norm_rope(many, None, None, None, None, None, out=(many, None))
+    cache = make_cache(S, 2, 2, 64, 16)
+    with pytest.raises(ValueError):
+        S.cache_attention(many, cache, ints([[0]]), ints([4]), ints([0, 1]), 1, 16, out=many)

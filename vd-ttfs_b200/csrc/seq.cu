@@ -11,6 +11,7 @@ namespace {
 constexpr int kMostHeads = 1024;
 constexpr int kMostSeqs = 65535;           // grid.z
 constexpr int kMostTokens = 1 << 30;       // of one sequence
+constexpr int kMostCols = 1 << 30;         // kernels step past the last by up to a few thousand, in 32 bits
 
 #define SEQ_REQUIRE(cond, text) \
     do {                        \
@@ -22,6 +23,7 @@ int launched(cudaError_t e, const char* what) { return e == cudaSuccess ? VDT_OK
 int check_product(const int8_t* d_w, int64_t w_stride, const float* d_w_scale, int64_t rows, int cols, int inner,
                   int out_type, const void* d_out, int64_t out_stride) {
     SEQ_REQUIRE(rows >= 0 && rows < kMostTokens && cols > 0 && inner > 0, "rows, cols and inner must be positive, rows below 2^30");
+    if (cols > kMostCols) return api_fail(VDT_ERR_UNSUPPORTED, "more than 2^30 cols");
     if (inner > 131072) return api_fail(VDT_ERR_UNSUPPORTED, "inner above 131072: the sums would not fit 32-bit integers");
     SEQ_REQUIRE(type_ok(out_type), "output type");
     SEQ_REQUIRE(d_w && d_w_scale && (d_out || !rows), "NULL buffer");
@@ -76,6 +78,7 @@ extern "C" int vdt_quantize_rows(const void* d_x, int type, int64_t rows, int co
     api_clear_error();
     SEQ_REQUIRE(type_ok(type), "type");
     SEQ_REQUIRE(rows >= 0 && rows < kMostTokens && cols > 0, "rows and cols must be positive, rows below 2^30");
+    if (cols > kMostCols) return api_fail(VDT_ERR_UNSUPPORTED, "more than 2^30 cols");
     if (rows == 0) return VDT_OK;
     SEQ_REQUIRE(d_x && d_codes && d_scale, "NULL buffer");
     SEQ_REQUIRE((x_stride >= cols || rows == 1) && codes_stride >= cols, "a stride below cols");

@@ -62,11 +62,12 @@ int64_t integer(PyObject* o, const char* what) {
     }
     return v;
 }
-int small_integer(PyObject* o, const char* what) {
-    const int64_t v = integer(o, what);
+// a number or a tensor's size as the library takes it
+int size32(int64_t v, const char* what) {
     CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, what, ": out of range");
     return (int)v;
 }
+int small_integer(PyObject* o, const char* what) { return size32(integer(o, what), what); }
 double number(PyObject* o, const char* what) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) {
@@ -212,12 +213,13 @@ PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t count) {
     on_device(x, "x", 2);
     const int type = type_of(x.scalar_type(), "x");
     const int64_t rows = x.size(0), cols = x.size(1);
-    CHECK_VALUE(cols > 0 && cols <= INT32_MAX, "x: no columns, or too many");
+    CHECK_VALUE(cols > 0, "x: no columns");
+    const int n = size32(cols, "x: columns");
     const OnStream on(a[1], x.device());
     if (x.stride(1) != 1 || (rows > 1 && x.stride(0) < cols)) x = x.contiguous();
     const int64_t step = (cols + 15) / 16 * 16;
     const Tensor codes = room({rows, step}, at::kChar, x.device()), scale = room({rows}, at::kFloat, x.device());
-    if (const int e = vdt_quantize_rows(x.data_ptr(), type, rows, (int)cols, x.stride(0), static_cast<int8_t*>(codes.data_ptr()), step,
+    if (const int e = vdt_quantize_rows(x.data_ptr(), type, rows, n, x.stride(0), static_cast<int8_t*>(codes.data_ptr()), step,
                                         static_cast<float*>(scale.data_ptr()), on.handle()))
         return status_error(e, "vdt_quantize_rows");
     return pair(on.result(codes).narrow(1, 0, cols), on.result(scale));
@@ -235,10 +237,10 @@ PyObject* int8_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
     flat(xs, "a_scale", at::kFloat, rows);
     const Tensor out = product_out(rows, x.size(1), w, ws, bias, given, given.defined() ? given.scalar_type() : dtype(a[5], "out_dtype"));
     const int type = type_of(out.scalar_type(), "out");
-    const int n = (int)w.size(0);
+    const int n = size32(w.size(0), "w: rows");
     if (const int e = vdt_int8_matmul(static_cast<int8_t*>(x.data_ptr()), row_stride(x), at_or_null<float>(xs),
                                       static_cast<int8_t*>(w.data_ptr()), row_stride(w), at_or_null<float>(ws), at_or_null<float>(bias),
-                                      rows, n, (int)x.size(1), type, out.data_ptr(), std::max<int64_t>(out.stride(0), n), on.handle()))
+                                      rows, n, size32(x.size(1), "a: columns"), type, out.data_ptr(), std::max<int64_t>(out.stride(0), n), on.handle()))
         return status_error(e, "vdt_int8_matmul");
     return THPVariable_Wrap(given.defined() ? out : on.result(out));
     END_HANDLE_TH_ERRORS
@@ -258,11 +260,12 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
                                    given.defined() ? given.scalar_type() : a[4] == Py_None ? x.scalar_type() : dtype(a[4], "out_dtype"));
     const int out_type = type_of(out.scalar_type(), "out");
     if ((inner > 1 && x.stride(1) != 1) || (rows > 1 && x.stride(0) < inner)) x = x.contiguous();
-    const int64_t need = (int64_t)vdt_int8_linear_scratch_bytes(rows, (int)inner);
+    const int k = size32(inner, "x: columns");
+    const int64_t need = (int64_t)vdt_int8_linear_scratch_bytes(rows, k);
     const Tensor scratch = room({need}, at::kByte, x.device());
-    const int n = (int)w.size(0);
+    const int n = size32(w.size(0), "w: rows");
     if (const int e = vdt_int8_linear(x.data_ptr(), type, std::max(x.stride(0), inner), static_cast<int8_t*>(w.data_ptr()), row_stride(w),
-                                      at_or_null<float>(ws), at_or_null<float>(bias), rows, n, (int)inner, out_type, out.data_ptr(),
+                                      at_or_null<float>(ws), at_or_null<float>(bias), rows, n, k, out_type, out.data_ptr(),
                                       std::max<int64_t>(out.stride(0), n), scratch.data_ptr(), (size_t)need, on.handle()))
         return status_error(e, "vdt_int8_linear");
     return THPVariable_Wrap(given.defined() ? out : on.result(out));
@@ -314,8 +317,9 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
     }
     auto stride = [](const Tensor& t, int i) { return t.defined() ? t.stride(i) : 0; };
     if (const int e = vdt_qk_norm_rope(q.data_ptr(), q.stride(0), q.stride(1), at_or_null(k), stride(k, 0), stride(k, 1), at_or_null(wq),
-                                       at_or_null(wk), rot ? at_or_null<int32_t>(at) : nullptr, rot ? at_or_null<float>(table) : nullptr, (int)n,
-                                       (int)rot, layout, norm, (float)number(a[8], "eps"), tokens, (int)q.size(1), (int)kv, (int)dim, type,
+                                       at_or_null(wk), rot ? at_or_null<int32_t>(at) : nullptr, rot ? at_or_null<float>(table) : nullptr,
+                                       size32(n, "table: positions"), size32(rot, "table: columns"), layout, norm, (float)number(a[8], "eps"),
+                                       tokens, size32(q.size(1), "q: heads"), size32(kv, "k: heads"), size32(dim, "q: dimension"), type,
                                        out[0].data_ptr(), out[0].stride(0), out[0].stride(1), at_or_null(out[1]), stride(out[1], 0),
                                        stride(out[1], 1), on.handle()))
         return status_error(e, "vdt_qk_norm_rope");
@@ -416,7 +420,8 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const vdt_cache8 c = cache_of(a[1]);
     const Rows r = rows_of(a[2], a[3], a[4]);
     heads(q, "q", c.dim);
-    const int64_t total = q.size(0), n = q.size(1);
+    const int64_t total = q.size(0);
+    const int n = size32(q.size(1), "q: heads");
     const int type = type_of(q.scalar_type(), "q");
     const int most = (int)std::min<int64_t>(small_integer(a[5], "most"), total), most_kept = small_integer(a[6], "most_kept");
     const Tensor& given = tensor_or_none(a[9], "out");
@@ -427,9 +432,9 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
         CHECK_VALUE(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out: ", q.sizes(), " of ", q.scalar_type(), " is wanted");
     }
     const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)c.dim) : number(a[8], "scale");
-    const size_t need = vdt_cache_attention_scratch_bytes(total, (int)n, c.heads, c.dim, r.seqs, most, most_kept);
+    const size_t need = vdt_cache_attention_scratch_bytes(total, n, c.heads, c.dim, r.seqs, most, most_kept);
     const Tensor scratch = need ? room({(int64_t)need}, at::kByte, q.device()) : Tensor();
-    if (const int e = vdt_cache_attention(&c, q.data_ptr(), q.stride(0), q.stride(1), (int)n, type, r.pages, r.width, r.held, r.starts, r.seqs,
+    if (const int e = vdt_cache_attention(&c, q.data_ptr(), q.stride(0), q.stride(1), n, type, r.pages, r.width, r.held, r.starts, r.seqs,
                                           total, most, most_kept, truth(a[7]), (float)scale, out.data_ptr(), out.stride(0), out.stride(1),
                                           at_or_null(scratch), need, on.handle()))
         return status_error(e, "vdt_cache_attention");
