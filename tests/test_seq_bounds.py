@@ -1,7 +1,5 @@
 """CPU: sizes and pointers that the sequence operators refuse because a kernel could not take them."""
-import pytest
-
-from test_seq_checks import INVALID, P, UNSUPPORTED, call  # noqa: F401
+from test_seq_checks import INVALID, P, UNSUPPORTED, append, attend, call, desc, load
 
 
 def test_more_columns_than_the_kernels_count():
@@ -10,3 +8,23 @@ def test_more_columns_than_the_kernels_count():
         assert call("vdt_quantize_rows", P, 0, 1, cols, cols, P, cols, P, None) == UNSUPPORTED
         assert call("vdt_int8_matmul", P, 32, P, P, 32, P, None, 3, cols, 20, 2, P, cols, None) == UNSUPPORTED
         assert call("vdt_int8_linear", P, 1, 20, P, 32, P, None, 3, cols, 20, 1, P, cols, P, 1 << 20, None) == UNSUPPORTED
+
+
+def test_scales_and_lengths_off_their_alignment():
+    """A kernel's 32-bit load from such an address would fault."""
+    def matmul(a_scale=P, w_scale=P, bias=P):
+        return call("vdt_int8_matmul", P, 32, a_scale, P, 32, w_scale, bias, 3, 5, 20, 2, P, 5, None)
+
+    def linear(w_scale=P, bias=P):
+        return call("vdt_int8_linear", P, 1, 20, P, 32, w_scale, bias, 3, 5, 20, 1, P, 5, P, 1 << 20, None)
+
+    for off in (1, 2, 3):
+        for over in (dict(a_scale=P + off), dict(w_scale=P + off), dict(bias=P + off)):
+            assert matmul(**over) == INVALID, over
+            if "a_scale" not in over:
+                assert linear(**over) == INVALID, over
+        for go in (append, load, attend):
+            for over in (dict(k_scale=P + off), dict(v_scale=P + off)):
+                assert go(desc(**over)) == INVALID, over
+            for over in (dict(table=P + off), dict(held=P + off), dict(starts=P + off)):
+                assert go(desc(), **over) == INVALID, over

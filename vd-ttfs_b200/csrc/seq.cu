@@ -20,7 +20,7 @@ constexpr int kMostCols = 1 << 30;         // kernels step past the last by up t
 
 int launched(cudaError_t e, const char* what) { return e == cudaSuccess ? VDT_OK : api_cuda_fail(e, what); }
 
-int check_product(const int8_t* d_w, int64_t w_stride, const float* d_w_scale, int64_t rows, int cols, int inner,
+int check_product(const int8_t* d_w, int64_t w_stride, const float* d_w_scale, const float* d_bias, int64_t rows, int cols, int inner,
                   int out_type, const void* d_out, int64_t out_stride) {
     SEQ_REQUIRE(rows >= 0 && rows < kMostTokens && cols > 0 && inner > 0, "rows, cols and inner must be positive, rows below 2^30");
     if (cols > kMostCols) return api_fail(VDT_ERR_UNSUPPORTED, "more than 2^30 cols");
@@ -30,6 +30,7 @@ int check_product(const int8_t* d_w, int64_t w_stride, const float* d_w_scale, i
     SEQ_REQUIRE(w_stride >= inner && w_stride % 16 == 0 && aligned(d_w, 16), "weight rows must start on 16-byte boundaries");
     SEQ_REQUIRE(out_stride >= cols, "out_stride below cols");
     SEQ_REQUIRE(aligned(d_out, type_size(out_type)), "out alignment");
+    SEQ_REQUIRE(aligned(d_w_scale, 4) && aligned(d_bias, 4), "scale or bias alignment");
     return VDT_OK;
 }
 
@@ -46,6 +47,7 @@ int check_cache(const vdt_cache8* c) {
     SEQ_REQUIRE(c->k && c->v && c->k_scale && c->v_scale, "NULL cache buffer");
     SEQ_REQUIRE(c->pages > 0 && c->heads > 0 && c->heads <= kMostHeads, "cache pages or heads");
     SEQ_REQUIRE(aligned(c->k, 16) && aligned(c->v, 16), "cache codes must start on a 16-byte boundary");
+    SEQ_REQUIRE(aligned(c->k_scale, 4) && aligned(c->v_scale, 4), "cache scale alignment");
     if (c->page != 16 && c->page != 32 && c->page != 64) return api_fail(VDT_ERR_UNSUPPORTED, "pages of 16, 32 or 64 tokens");
     if (!attend_dim_ok(c->dim)) return api_fail(VDT_ERR_UNSUPPORTED, "head dimensions 32, 64, 96, 128, 192 and 256");
     return VDT_OK;
@@ -56,6 +58,7 @@ int check_rows(const int32_t* table, int width, const int32_t* held, const int32
     SEQ_REQUIRE(total < kMostTokens && most <= total, "total below 2^30, and no run longer than it");
     if (seqs > kMostSeqs) return api_fail(VDT_ERR_UNSUPPORTED, "more than 65535 sequences");
     SEQ_REQUIRE(!seqs || (held && starts && (table || !width)), "NULL buffer");
+    SEQ_REQUIRE(aligned(table, 4) && aligned(held, 4) && aligned(starts, 4), "alignment of the table or the lengths");
     return VDT_OK;
 }
 
@@ -92,9 +95,10 @@ extern "C" int vdt_int8_matmul(const int8_t* d_a, int64_t a_stride, const float*
                                int64_t w_stride, const float* d_w_scale, const float* d_bias, int64_t rows, int cols,
                                int inner, int out_type, void* d_out, int64_t out_stride, vdt_stream stream) {
     api_clear_error();
-    if (int s = check_product(d_w, w_stride, d_w_scale, rows, cols, inner, out_type, d_out, out_stride)) return s;
+    if (int s = check_product(d_w, w_stride, d_w_scale, d_bias, rows, cols, inner, out_type, d_out, out_stride)) return s;
     if (rows == 0) return VDT_OK;
     SEQ_REQUIRE(d_a && d_a_scale, "NULL buffer");
+    SEQ_REQUIRE(aligned(d_a_scale, 4), "scale alignment");
     SEQ_REQUIRE(a_stride >= inner && a_stride % 16 == 0 && aligned(d_a, 16), "code rows must start on 16-byte boundaries");
     if (int s = api_check_buffers(-1, {d_a, d_a_scale, d_w, d_w_scale, d_bias, d_out})) return s;
     Int8Params p{d_a, d_a_scale, d_w, d_w_scale, d_bias, d_out, rows, a_stride, w_stride, out_stride, cols, inner, out_type, nullptr, 0};
@@ -112,7 +116,7 @@ extern "C" int vdt_int8_linear(const void* d_x, int type, int64_t x_stride, cons
                                vdt_stream stream) {
     api_clear_error();
     SEQ_REQUIRE(type_ok(type), "type");
-    if (int s = check_product(d_w, w_stride, d_w_scale, rows, cols, inner, out_type, d_out, out_stride)) return s;
+    if (int s = check_product(d_w, w_stride, d_w_scale, d_bias, rows, cols, inner, out_type, d_out, out_stride)) return s;
     if (rows == 0) return VDT_OK;
     SEQ_REQUIRE(d_x && d_scratch, "NULL buffer");
     SEQ_REQUIRE(x_stride >= inner || rows == 1, "x_stride below inner");
