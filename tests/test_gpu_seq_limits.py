@@ -292,3 +292,10 @@ def test_sizes_beyond_32_bits_are_refused(S):
     cache = make_cache(S, 2, 2, 64, 16)
     with pytest.raises(ValueError):
         S.cache_attention(many, cache, ints([[0]]), ints([4]), ints([0, 1]), 1, 16, out=many)
+
+
+# --------------------------------------------------------------- refusals --
+def test_a_table_without_positions_is_refused(S):
+    q = torch.zeros(2, 4, 64, dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError, match="positions"):
+        S.qk_norm_rope(q, None, None, None, None, S.rope_table(8, 64))

@@ -296,6 +296,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
         n = table.size(0);
         rot = table.size(1);
         flat(table, "table", at::kFloat, n * rot);
+        CHECK_VALUE(at.defined(), "positions: wanted with a table");
         flat(at, "positions", at::kInt, tokens);
     }
     const OnStream on(a[11], q.device());
