@@ -299,3 +299,16 @@ def test_a_table_without_positions_is_refused(S):
     q = torch.zeros(2, 4, 64, dtype=torch.float16, device="cuda")
     with pytest.raises(ValueError, match="positions"):
         S.qk_norm_rope(q, None, None, None, None, S.rope_table(8, 64))
+
+
+def test_flags_that_are_neither_true_nor_false_are_refused(S):
+    class Neither:
+        def __bool__(self):
+            raise RuntimeError("neither")
+
+    cache = make_cache(S, 2, 2, 64, 16)
+    q = torch.zeros(2, 4, 64, dtype=torch.float16, device="cuda")
+    with pytest.raises(TypeError, match="interleaved"):
+        S.qk_norm_rope(q, None, None, None, None, None, interleaved=Neither())
+    with pytest.raises(TypeError, match="causal"):
+        S.cache_attention(q, cache, ints([[0]]), ints([4]), ints([0, 2]), 2, 16, causal=Neither())

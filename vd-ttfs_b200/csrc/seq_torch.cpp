@@ -76,7 +76,14 @@ double number(PyObject* o, const char* what) {
     }
     return v;
 }
-bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool truth(PyObject* o, const char* what) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) {
+        PyErr_Clear();
+        CHECK_TYPE(false, what, ": true or false is wanted");
+    }
+    return v == 1;
+}
 
 int type_of(at::ScalarType t, const char* what) {
     if (t == at::kBFloat16) return VDT_BF16;
@@ -278,7 +285,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
     WANT(12);
     const Tensor &q = tensor(a[0], "q"), &k = tensor_or_none(a[1], "k"), &wq = tensor_or_none(a[2], "q_weight");
     const Tensor &wk = tensor_or_none(a[3], "k_weight"), &at = tensor_or_none(a[4], "positions"), &table = tensor_or_none(a[5], "table");
-    const int layout = truth(a[6]) ? VDT_ROPE_PAIRS : VDT_ROPE_HALF, norm = small_integer(a[7], "norm");
+    const int layout = truth(a[6], "interleaved") ? VDT_ROPE_PAIRS : VDT_ROPE_HALF, norm = small_integer(a[7], "norm");
     const Tensor &given_q = tensor_or_none(a[9], "out (q)"), &given_k = tensor_or_none(a[10], "out (k)");
     heads(q, "q", -1);
     const int64_t tokens = q.size(0), dim = q.size(2), kv = k.defined() ? k.size(1) : 0;
@@ -436,7 +443,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const size_t need = vdt_cache_attention_scratch_bytes(total, n, c.heads, c.dim, r.seqs, most, most_kept);
     const Tensor scratch = need ? room({(int64_t)need}, at::kByte, q.device()) : Tensor();
     if (const int e = vdt_cache_attention(&c, q.data_ptr(), q.stride(0), q.stride(1), n, type, r.pages, r.width, r.held, r.starts, r.seqs,
-                                          total, most, most_kept, truth(a[7]), (float)scale, out.data_ptr(), out.stride(0), out.stride(1),
+                                          total, most, most_kept, truth(a[7], "causal"), (float)scale, out.data_ptr(), out.stride(0), out.stride(1),
                                           at_or_null(scratch), need, on.handle()))
         return status_error(e, "vdt_cache_attention");
     return THPVariable_Wrap(given.defined() ? out : on.result(out));
