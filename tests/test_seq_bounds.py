@@ -28,3 +28,12 @@ def test_scales_and_lengths_off_their_alignment():
                 assert go(desc(**over)) == INVALID, over
             for over in (dict(table=P + off), dict(held=P + off), dict(starts=P + off)):
                 assert go(desc(), **over) == INVALID, over
+
+
+def test_the_module_has_no_standard_library_of_its_own():
+    """A second libstdc++ in the process: its streams ended it when they met the first one's locales."""
+    import os
+    from conftest import ROOT
+    with open(os.path.join(ROOT, "vd-ttfs_b200", "vdttfs", "_seq.so"), "rb") as f:
+        built = f.read()
+    assert b"libstdc++.so.6\0" in built and b"_ZNSt6locale5facet" not in built

@@ -14,7 +14,6 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <optional>
-#include <string>
 
 #include "vdttfs.h"
 
@@ -24,32 +23,9 @@ using at::Tensor;
 
 const Tensor kNone;
 
-// ---------------------------------------------------------------- messages --
-// Put together without streams: a message with a number in it, formatted through
-// c10::str's std::ostream, ended the process (SIGSEGV) once CUDA was initialised,
-// and not before; why is not known.
-std::string show(const char* x) { return x; }
-std::string show(int64_t x) { return std::to_string(x); }
-std::string show(int x) { return std::to_string(x); }
-std::string show(at::ScalarType x) { return c10::toString(x); }
-std::string show(at::Device x) { return x.is_cuda() ? "cuda:" + std::to_string((int)x.index()) : "another device"; }
-std::string show(at::IntArrayRef x) {
-    std::string s = "[";
-    for (size_t i = 0; i < x.size(); ++i) s += (i ? ", " : "") + std::to_string(x[i]);
-    return s + "]";
-}
-template <typename... Parts>
-std::string text(const Parts&... parts) {
-    std::string s;
-    ((s += show(parts)), ...);
-    return s;
-}
-#define CHECK_VALUE(cond, ...) TORCH_CHECK_VALUE(cond, text(__VA_ARGS__))
-#define CHECK_TYPE(cond, ...) TORCH_CHECK_TYPE(cond, text(__VA_ARGS__))
-
 // ------------------------------------------------------------- arguments --
 const Tensor& tensor(PyObject* o, const char* what) {
-    CHECK_TYPE(THPVariable_Check(o), what, ": a tensor is wanted, got ", Py_TYPE(o)->tp_name);
+    TORCH_CHECK_TYPE(THPVariable_Check(o), what, ": a tensor is wanted, got ", Py_TYPE(o)->tp_name);
     return THPVariable_Unpack(o);
 }
 const Tensor& tensor_or_none(PyObject* o, const char* what) { return o == Py_None ? kNone : tensor(o, what); }
@@ -58,13 +34,13 @@ int64_t integer(PyObject* o, const char* what) {
     const long long v = PyLong_AsLongLong(o);
     if (v == -1 && PyErr_Occurred()) {
         PyErr_Clear();
-        CHECK_TYPE(false, what, ": a whole number is wanted");
+        TORCH_CHECK_TYPE(false, what, ": a whole number is wanted");
     }
     return v;
 }
 // a number or a tensor's size as the library takes it
 int size32(int64_t v, const char* what) {
-    CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, what, ": out of range");
+    TORCH_CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, what, ": out of range");
     return (int)v;
 }
 int small_integer(PyObject* o, const char* what) { return size32(integer(o, what), what); }
@@ -72,7 +48,7 @@ double number(PyObject* o, const char* what) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) {
         PyErr_Clear();
-        CHECK_TYPE(false, what, ": a number is wanted");
+        TORCH_CHECK_TYPE(false, what, ": a number is wanted");
     }
     return v;
 }
@@ -80,7 +56,7 @@ bool truth(PyObject* o, const char* what) {
     const int v = PyObject_IsTrue(o);
     if (v < 0) {
         PyErr_Clear();
-        CHECK_TYPE(false, what, ": true or false is wanted");
+        TORCH_CHECK_TYPE(false, what, ": true or false is wanted");
     }
     return v == 1;
 }
@@ -88,26 +64,26 @@ bool truth(PyObject* o, const char* what) {
 int type_of(at::ScalarType t, const char* what) {
     if (t == at::kBFloat16) return VDT_BF16;
     if (t == at::kHalf) return VDT_F16;
-    CHECK_VALUE(t == at::kFloat, what, ": float32, float16 or bfloat16 is wanted, got ", t);
+    TORCH_CHECK_VALUE(t == at::kFloat, what, ": float32, float16 or bfloat16 is wanted, got ", t);
     return VDT_F32;
 }
 at::ScalarType dtype(PyObject* o, const char* what) {
-    CHECK_TYPE(THPDtype_Check(o), what, ": a torch dtype is wanted");
+    TORCH_CHECK_TYPE(THPDtype_Check(o), what, ": a torch dtype is wanted");
     return reinterpret_cast<THPDtype*>(o)->scalar_type;
 }
 
 void on_device(const Tensor& t, const char* what, int64_t dims) {
-    CHECK_VALUE(t.is_cuda(), what, ": a CUDA tensor is wanted");
-    CHECK_VALUE(t.dim() == dims, what, ": ", dims, " dimensions are wanted, got ", t.sizes());
+    TORCH_CHECK_VALUE(t.is_cuda(), what, ": a CUDA tensor is wanted");
+    TORCH_CHECK_VALUE(t.dim() == dims, what, ": ", dims, " dimensions are wanted, got ", t.sizes());
 }
 void flat(const Tensor& t, const char* what, at::ScalarType type, int64_t n) {
-    CHECK_VALUE(t.is_cuda() && t.scalar_type() == type && t.numel() == n && t.is_contiguous(), what, ": ", n,
+    TORCH_CHECK_VALUE(t.is_cuda() && t.scalar_type() == type && t.numel() == n && t.is_contiguous(), what, ": ", n,
                       " contiguous CUDA values of ", type, " are wanted, got ", t.sizes(), " of ", t.scalar_type(), " on ", t.device());
 }
 void heads(const Tensor& t, const char* what, int64_t dim) {
     on_device(t, what, 3);
-    CHECK_VALUE(dim < 0 || t.size(2) == dim, what, ": heads of ", dim, " are wanted, got ", t.sizes());
-    CHECK_VALUE(t.size(2) == 1 || t.stride(2) == 1, what, ": a head's values must be consecutive");
+    TORCH_CHECK_VALUE(dim < 0 || t.size(2) == dim, what, ": heads of ", dim, " are wanted, got ", t.sizes());
+    TORCH_CHECK_VALUE(t.size(2) == 1 || t.stride(2) == 1, what, ": a head's values must be consecutive");
 }
 
 Tensor room(at::IntArrayRef size, at::ScalarType type, at::Device device) {
@@ -125,7 +101,7 @@ public:
         handle_ = PyLong_AsVoidPtr(o);
         if (!handle_ && PyErr_Occurred()) {
             PyErr_Clear();
-            CHECK_TYPE(false, "stream: a raw handle is wanted");
+            TORCH_CHECK_TYPE(false, "stream: a raw handle is wanted");
         }
         if (handle_ == before_.stream()) return;
         guard_.emplace(handle_ ? c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(handle_), device.index())
@@ -187,13 +163,13 @@ bool arguments(Py_ssize_t n, Py_ssize_t want) {
 // --------------------------------------------------------- 8-bit product --
 void code_rows(const Tensor& t, const char* what) {
     on_device(t, what, 2);
-    CHECK_VALUE(t.scalar_type() == at::kChar, what, ": int8 is wanted, got ", t.scalar_type());
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kChar, what, ": int8 is wanted, got ", t.scalar_type());
     const int64_t n = t.size(0), k = t.size(1);
-    CHECK_VALUE(k > 0 && t.stride(1) == 1 && (n <= 1 || t.stride(0) >= k) && t.stride(0) % 16 == 0 &&
+    TORCH_CHECK_VALUE(k > 0 && t.stride(1) == 1 && (n <= 1 || t.stride(0) >= k) && t.stride(0) % 16 == 0 &&
                           reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
                       what, ": rows that start on 16-byte boundaries are wanted (see quantize_rows), got ", t.sizes(), ", strides ",
                       t.strides());
-    CHECK_VALUE(!n || t.storage_offset() + (n - 1) * t.stride(0) + (k + 15) / 16 * 16 <= (int64_t)t.storage().nbytes(), what,
+    TORCH_CHECK_VALUE(!n || t.storage_offset() + (n - 1) * t.stride(0) + (k + 15) / 16 * 16 <= (int64_t)t.storage().nbytes(), what,
                       ": the last row's storage must reach to the next multiple of 16 bytes");
 }
 int64_t row_stride(const Tensor& t) { return std::max(t.stride(0), (t.size(1) + 15) / 16 * 16); }
@@ -203,12 +179,12 @@ Tensor product_out(int64_t rows, int64_t inner, const Tensor& w, const Tensor& w
                    at::ScalarType type) {
     code_rows(w, "w");
     const int64_t n = w.size(0);
-    CHECK_VALUE(n > 0 && inner == w.size(1), "rows of ", inner, " and weights ", w.sizes(), " do not multiply");
+    TORCH_CHECK_VALUE(n > 0 && inner == w.size(1), "rows of ", inner, " and weights ", w.sizes(), " do not multiply");
     flat(w_scale, "w_scale", at::kFloat, n);
     if (bias.defined()) flat(bias, "bias", at::kFloat, n);
     if (!out.defined()) return room({rows, n}, type, w.device());
     on_device(out, "out", 2);
-    CHECK_VALUE(out.size(0) == rows && out.size(1) == n && (n == 1 || out.stride(1) == 1) && (rows <= 1 || out.stride(0) >= n),
+    TORCH_CHECK_VALUE(out.size(0) == rows && out.size(1) == n && (n == 1 || out.stride(1) == 1) && (rows <= 1 || out.stride(0) >= n),
                       "out: [", rows, ", ", n, "] with consecutive columns is wanted, got ", out.sizes(), ", strides ", out.strides());
     return out;
 }
@@ -220,7 +196,7 @@ PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t count) {
     on_device(x, "x", 2);
     const int type = type_of(x.scalar_type(), "x");
     const int64_t rows = x.size(0), cols = x.size(1);
-    CHECK_VALUE(cols > 0, "x: no columns");
+    TORCH_CHECK_VALUE(cols > 0, "x: no columns");
     const int n = size32(cols, "x: columns");
     const OnStream on(a[1], x.device());
     if (x.stride(1) != 1 || (rows > 1 && x.stride(0) < cols)) x = x.contiguous();
@@ -292,7 +268,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const int type = type_of(q.scalar_type(), "q");
     if (k.defined()) {
         heads(k, "k", dim);
-        CHECK_VALUE(k.size(0) == tokens && k.scalar_type() == q.scalar_type(), "k: ", tokens, " tokens of ", q.scalar_type(),
+        TORCH_CHECK_VALUE(k.size(0) == tokens && k.scalar_type() == q.scalar_type(), "k: ", tokens, " tokens of ", q.scalar_type(),
                           " are wanted, got ", k.sizes(), " of ", k.scalar_type());
     }
     if (wq.defined()) flat(wq, "q_weight", q.scalar_type(), dim);
@@ -303,7 +279,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
         n = table.size(0);
         rot = table.size(1);
         flat(table, "table", at::kFloat, n * rot);
-        CHECK_VALUE(at.defined(), "positions: wanted with a table");
+        TORCH_CHECK_VALUE(at.defined(), "positions: wanted with a table");
         flat(at, "positions", at::kInt, tokens);
     }
     const OnStream on(a[11], q.device());
@@ -317,9 +293,9 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
             out[i] = room(in[i]->sizes(), q.scalar_type(), q.device());
         } else {
             out[i] = *given[i];
-            CHECK_VALUE(out[i].defined(), "out: a pair is wanted");
+            TORCH_CHECK_VALUE(out[i].defined(), "out: a pair is wanted");
             heads(out[i], "out", dim);
-            CHECK_VALUE(out[i].sizes() == in[i]->sizes() && out[i].scalar_type() == q.scalar_type(), "out: ", in[i]->sizes(), " of ",
+            TORCH_CHECK_VALUE(out[i].sizes() == in[i]->sizes() && out[i].scalar_type() == q.scalar_type(), "out: ", in[i]->sizes(), " of ",
                               q.scalar_type(), " is wanted");
         }
     }
@@ -347,7 +323,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t count) {
 
 // ------------------------------------------------------------- the cache --
 vdt_cache8 cache_of(PyObject* o) {
-    CHECK_TYPE(PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 4, "cache: a tuple of keys, values and their scales is wanted");
+    TORCH_CHECK_TYPE(PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 4, "cache: a tuple of keys, values and their scales is wanted");
     const Tensor &k = tensor(PyTuple_GET_ITEM(o, 0), "cache keys"), &v = tensor(PyTuple_GET_ITEM(o, 1), "cache values");
     const Tensor &ks = tensor(PyTuple_GET_ITEM(o, 2), "cache key scales"), &vs = tensor(PyTuple_GET_ITEM(o, 3), "cache value scales");
     on_device(k, "cache keys", 4);
@@ -355,11 +331,11 @@ vdt_cache8 cache_of(PyObject* o) {
     const int64_t pages = k.size(0), n = k.size(1), page = k.size(2), dim = k.size(3);
     flat(k, "cache keys", at::kChar, k.numel());
     flat(v, "cache values", at::kChar, k.numel());
-    CHECK_VALUE(v.size(0) == pages && v.size(1) == n && v.size(2) == dim && v.size(3) == page, "cache values: [", pages, ", ", n, ", ", dim,
+    TORCH_CHECK_VALUE(v.size(0) == pages && v.size(1) == n && v.size(2) == dim && v.size(3) == page, "cache values: [", pages, ", ", n, ", ", dim,
                       ", ", page, "] is wanted, got ", v.sizes());
     flat(ks, "cache key scales", at::kFloat, pages * n);
     flat(vs, "cache value scales", at::kFloat, pages * n);
-    CHECK_VALUE(pages <= INT32_MAX && n <= INT32_MAX && page <= INT32_MAX && dim <= INT32_MAX, "cache: too large");
+    TORCH_CHECK_VALUE(pages <= INT32_MAX && n <= INT32_MAX && page <= INT32_MAX && dim <= INT32_MAX, "cache: too large");
     return {static_cast<int8_t*>(k.data_ptr()), static_cast<int8_t*>(v.data_ptr()), static_cast<float*>(ks.data_ptr()),
             static_cast<float*>(vs.data_ptr()), (int)pages, (int)page, (int)n, (int)dim};
 }
@@ -376,7 +352,7 @@ Rows rows_of(PyObject* pages, PyObject* held, PyObject* starts) {
     const Tensor &h = tensor(held, "tokens held"), &s = tensor(starts, "starts");
     flat(h, "tokens held", at::kInt, n);
     flat(s, "starts", at::kInt, n + 1);
-    CHECK_VALUE(n <= INT32_MAX && p.size(1) <= INT32_MAX, "pages: too large");
+    TORCH_CHECK_VALUE(n <= INT32_MAX && p.size(1) <= INT32_MAX, "pages: too large");
     return {static_cast<int32_t*>(p.data_ptr()), static_cast<int32_t*>(h.data_ptr()), static_cast<int32_t*>(s.data_ptr()), (int)n, (int)p.size(1)};
 }
 
@@ -390,7 +366,7 @@ PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t count) {
     heads(v, "v", c.dim);
     const int type = type_of(k.scalar_type(), "k");
     const int64_t total = k.size(0);
-    CHECK_VALUE(k.size(1) == c.heads && v.size(1) == c.heads && v.size(0) == total && v.scalar_type() == k.scalar_type(),
+    TORCH_CHECK_VALUE(k.size(1) == c.heads && v.size(1) == c.heads && v.size(0) == total && v.scalar_type() == k.scalar_type(),
                       "k and v: [tokens, ", c.heads, ", ", c.dim, "] of one type are wanted, got ", k.sizes(), " of ", k.scalar_type(), " and ",
                       v.sizes(), " of ", v.scalar_type());
     const OnStream on(a[7], k.device());
@@ -408,7 +384,7 @@ PyObject* cache_load(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const vdt_cache8 c = cache_of(a[0]);
     const Rows r = rows_of(a[1], a[2], a[3]);
     const int64_t total = integer(a[4], "total");
-    CHECK_VALUE(total >= 0, "total: negative");
+    TORCH_CHECK_VALUE(total >= 0, "total: negative");
     const int most = (int)std::min<int64_t>(small_integer(a[5], "most"), total);
     const at::ScalarType type = dtype(a[6], "dtype");
     const int kind = type_of(type, "dtype");
@@ -437,7 +413,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const Tensor out = given.defined() ? given : room(q.sizes(), q.scalar_type(), q.device());
     if (given.defined()) {
         heads(out, "out", c.dim);
-        CHECK_VALUE(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out: ", q.sizes(), " of ", q.scalar_type(), " is wanted");
+        TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out: ", q.sizes(), " of ", q.scalar_type(), " is wanted");
     }
     const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)c.dim) : number(a[8], "scale");
     const size_t need = vdt_cache_attention_scratch_bytes(total, n, c.heads, c.dim, r.seqs, most, most_kept);
