@@ -37,3 +37,17 @@ def test_the_module_has_no_standard_library_of_its_own():
     with open(os.path.join(ROOT, "vd-ttfs_b200", "vdttfs", "_seq.so"), "rb") as f:
         built = f.read()
     assert b"libstdc++.so.6\0" in built and b"_ZNSt6locale5facet" not in built
+
+
+def test_the_library_is_built_without_torch():
+    """The default target is a C integrator's: nvcc alone.  The module for torch tensors has a target of its own."""
+    import os
+    import subprocess
+    from conftest import ROOT
+
+    def steps(*target):
+        return subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "vd-ttfs_b200"), "PYTHON=no-such-python", *target], check=True,
+                              capture_output=True, text=True).stdout
+
+    assert "libvdttfs.so" in steps() and "seq_torch" not in steps() and "no-such-python" not in steps()
+    assert "seq_torch" in steps("seq") and "libvdttfs.so" in steps("seq")

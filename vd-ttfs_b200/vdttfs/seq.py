@@ -30,7 +30,10 @@ import torch
 
 from ._lib import check, lib
 lib()                       # the library itself, which the module below links
-from . import _seq          # noqa: E402  (native: built with it by make -C vd-ttfs_b200)
+try:
+    from . import _seq
+except ModuleNotFoundError as e:
+    raise RuntimeError("vdttfs/_seq.so is not built (make -C vd-ttfs_b200 seq)") from e
 
 NORMS = {"none": 0, "rms": 1, "l2": 2}
 SCALINGS = {"none": 0, "linear": 1, "base": 2, "parts": 3}
