@@ -312,3 +312,62 @@ def test_flags_that_are_neither_true_nor_false_are_refused(S):
         S.qk_norm_rope(q, None, None, None, None, None, interleaved=Neither())
     with pytest.raises(TypeError, match="causal"):
         S.cache_attention(q, cache, ints([[0]]), ints([4]), ints([0, 2]), 2, 16, causal=Neither())
+
+
+SHIM = r"""
+#define _GNU_SOURCE
+#include <dlfcn.h>
+#include <string.h>
+static int fail;
+void shim_fail(int n) { fail = n; }
+static void* real(const char* name) { return dlsym(dlopen("libcudart.so.12", RTLD_LAZY | RTLD_NOLOAD), name); }
+int cudaFuncGetAttributes(void* a, const void* f) {
+    if (fail) return --fail, 999;
+    return ((int (*)(void*, const void*))real("cudaFuncGetAttributes"))(a, f);
+}
+int cudaGetDriverEntryPointByVersion(const char* name, void** f, unsigned v, unsigned long long flags, int* q) {
+    if (fail && !strcmp(name, "cuTensorMapEncodeTiled")) return --fail, 999;
+    return ((int (*)(const char*, void**, unsigned, unsigned long long, int*))real("cudaGetDriverEntryPointByVersion"))(name, f, v, flags, q);
+}
+"""
+
+FIRST_FAILS = """
+import ctypes, sys
+sys.path[:0] = [{tests!r}, {package!r}]
+import torch
+from vdttfs import seq as S, _lib
+from test_gpu_seq import ints, make_cache, make_table, normal
+shim = ctypes.CDLL({shim!r})
+x, (w, ws) = normal(1, 40, 64).cuda(), S.quantize_rows(normal(2, 48, 64).cuda())
+table, pages = make_table([300], 16)
+cache = make_cache(S, pages, 1, 64, 16)
+q = normal(3, 300, 1, 64, kind=torch.float16).cuda()
+for call in (lambda: S.int8_linear(x, w, ws), lambda: S.cache_attention(q, cache, ints(table), ints([300]), ints([0, 300]), 300, 300)):
+    shim.shim_fail(1)
+    try:
+        call()
+        sys.exit("the first call was taken")
+    except _lib.VdtError:
+        pass
+    assert torch.isfinite(call()).all()
+torch.cuda.synchronize()
+"""
+
+
+def test_a_call_that_fails_in_the_runtime_is_not_kept(dev, tmp_path):
+    """The runtime's answers that the launches go by are asked for again after a failure (made by a shim on the host)."""
+    import os
+    import shutil
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+    cc = shutil.which("cc") or shutil.which("gcc")
+    if not cc:
+        pytest.skip("no C compiler")
+    (tmp_path / "shim.c").write_text(SHIM)
+    shim = str(tmp_path / "shim.so")
+    subprocess.run([cc, "-shared", "-fPIC", "-o", shim, str(tmp_path / "shim.c"), "-ldl"], check=True)
+    code = FIRST_FAILS.format(tests=os.path.join(ROOT, "tests"), package=os.path.join(ROOT, "vd-ttfs_b200"), shim=shim)
+    done = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, LD_PRELOAD=shim), capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]

@@ -577,11 +577,14 @@ cudaError_t tiles_launch(const AttendParams& p, const Chunks& c, cudaStream_t s)
     if constexpr (NT == 2) {
         // the groups share out exactly what the block is launched with; with
         // less they would wait for ever
-        static const int regs = [] {
+        static std::atomic<int> regs{0};
+        if (!regs.load(std::memory_order_relaxed)) {
             cudaFuncAttributes a{};
-            return cudaFuncGetAttributes(&a, k_attend_tiles<D, NT, P>) == cudaSuccess ? a.numRegs : 0;
-        }();
-        if (regs < kRegs) return cudaErrorInvalidKernelImage;
+            e = cudaFuncGetAttributes(&a, k_attend_tiles<D, NT, P>);
+            if (e != cudaSuccess) return e;
+            regs.store(a.numRegs, std::memory_order_relaxed);
+        }
+        if (regs.load(std::memory_order_relaxed) < kRegs) return cudaErrorInvalidKernelImage;
     }
     const long long rows = (long long)p.r.most * (p.heads / p.c.heads), x = (rows + NT * kTile - 1) / (NT * kTile) * c.count;
     if (x > 0x7fffffff) return cudaErrorInvalidValue;

@@ -493,15 +493,18 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// cuTensorMapEncodeTiled, reached through the runtime (the library links the runtime only)
+// cuTensorMapEncodeTiled, reached through the runtime (the library links the
+// runtime only); asked for again after a call that did not get it
 EncodeTiled encode_tiled() {
-    static const EncodeTiled fn = [] {
-        void* f = nullptr;
+    static std::atomic<void*> found{nullptr};
+    void* f = found.load(std::memory_order_relaxed);
+    if (!f) {
         cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
         const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q);
-        return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeTiled>(f) : nullptr;
-    }();
-    return fn;
+        if (e != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
+        found.store(f, std::memory_order_relaxed);
+    }
+    return reinterpret_cast<EncodeTiled>(f);
 }
 
 bool byte_map(CUtensorMap* m, const int8_t* at, long long rows, int inner, long long stride, int box_rows) {
