@@ -104,7 +104,7 @@ __device__ __forceinline__ Partial partial_of(const AttendParams& p, long long r
 // row itself sees: its largest score, and its largest score with the page's
 // value scale.  By how much one may be passed before both are taken anew:
 constexpr float kSlack = 8.0f, kSlackFactor = 256.0f;
-__device__ __forceinline__ bool passes(float x, float ref) { return x > ref + kSlack || (!(ref > -inf_f()) && x > -inf_f()); }
+__device__ __forceinline__ bool passes(float x, float ref) { return x > ref + kSlack; }        // also what is above a ref of -inf
 
 // The references for new maxima, and the factors of the sums so far
 struct Rescale {

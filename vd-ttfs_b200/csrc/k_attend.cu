@@ -343,6 +343,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
             alive = bar_wait_all(bars + (ev % kRing) * 8, (ev / kRing) & 1);
             if (!alive) break;
             uint32_t w[kPart][NR][2];
+            float of_page[NR][2];                            // a page's weights, summed
 #pragma unroll
             for (int m = 0; m < kPart; ++m) {
                 const int pg = m / kGroups, j16 = m % kGroups;
@@ -362,8 +363,12 @@ __global__ void __launch_bounds__(kRowsWarps * 32) k_attend_rows(AttendParams p,
                         if (partial) x[e] = token + e / 2 * 2 < limit[n][e % 2] ? x[e] : 0.0f;     // also for scales that are not numbers
                     }
                     const float a = x[0] + x[2], c = x[1] + x[3];
-                    sum[n][0] = partial && a == 0.0f ? sum[n][0] : fmaf(a, exp2_fast(-d[0]), sum[n][0]);
-                    sum[n][1] = partial && c == 0.0f ? sum[n][1] : fmaf(c, exp2_fast(-d[1]), sum[n][1]);
+                    of_page[n][0] = j16 == 0 ? a : of_page[n][0] + a;
+                    of_page[n][1] = j16 == 0 ? c : of_page[n][1] + c;
+                    if (j16 == kGroups - 1)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            sum[n][e] = partial && of_page[n][e] == 0.0f ? sum[n][e] : fmaf(of_page[n][e], exp2_fast(-d[e]), sum[n][e]);
                     w[m][n][0] = transposed(pack_f16(x[0], x[1]));
                     w[m][n][1] = transposed(pack_f16(x[2], x[3]));
                 }
