@@ -438,8 +438,8 @@ int vdt_int8_matmul(const int8_t* d_a, int64_t a_stride, const float* d_a_scale,
 
 /* The two together for rows x [rows, inner] of `type`: each row's codes into
    d_scratch (256-byte aligned, vdt_int8_linear_scratch_bytes; VDT_ERR_CAPACITY
-   when smaller), then the product; a few rows are rounded by the product's
-   own kernel, which does not use the scratch.  d_out may lie over d_x, whose
+   when smaller), then the product; one or two rows may be rounded by the
+   product's own kernel, which does not use the scratch.  d_out may lie over d_x, whose
    rows are all read before the first is written. */
 size_t vdt_int8_linear_scratch_bytes(int64_t rows, int inner);
 int vdt_int8_linear(const void* d_x, int type, int64_t x_stride, const int8_t* d_w, int64_t w_stride,

@@ -119,11 +119,15 @@ __device__ __forceinline__ uint32_t keep_below(uint32_t v, int word, int inner) 
 
 constexpr int kFewRows = 32;
 
-// Up to kOwnRows rows of up to kOwnValues values together are rounded by every
-// CTA for itself, into shared memory: one launch instead of two (one row of
-// 1024: 8.7 us a call with two, the host's side of a launch some 2).  The
-// values are read from L2 by all CTAs, so more of them would cost more.
-constexpr int kOwnRows = 4, kOwnValues = 16384;
+// One row of up to 16384 values, or two short ones, are rounded by every CTA for
+// itself, into shared memory: one launch instead of two, 2 us of the host's.  The
+// values are read from L2 by all CTAs, which wait for their rounding, so more of
+// them cost more than the launch.  A call / on the GPU in us, so and with two
+// launches: 1 x 1024 x 1024 5.4 / 3.1 and 7.7 / 4.5, 1 x 4096 x 4096 8.2 / 8.3 and
+// 8.0 to 10.6 / 8.6, 1 x 16384 x 1024 14.4 / 15.5 and 14.8 / 19.3, 2 x 1024 x 1024
+// 6.2 / 4.5 and 8.1 / 4.5; not taken: 2 x 4096 x 4096 10.2 / 10.8 and 8.3 / 9.3,
+// 4 x 256 x 256 8.2 / 5.9 and 8.2 / 4.5, 4 x 4096 x 4096 12.9 / 13.6 and 8.3 / 9.4.
+constexpr int kOwnRows = 2, kOwnValues = 16384, kOwnShort = 1024;
 
 template <typename X>
 __device__ __forceinline__ void round_rows(const Int8Params& p, int8_t* codes, float* scale) {
@@ -586,7 +590,7 @@ cudaError_t launch_quantize_rows(const void* x, int type, long long rows, int co
     return quant_launch<__nv_bfloat16>(x, rows, cols, x_stride, codes, codes_stride, scale, s);
 }
 
-bool int8_rounds_itself(long long rows, int inner) { return rows <= kOwnRows && rows * inner <= kOwnValues; }
+bool int8_rounds_itself(long long rows, int inner) { return inner <= (rows == 1 ? kOwnValues : kOwnShort) && rows <= kOwnRows; }
 
 cudaError_t launch_int8_own(const Int8Params& p, int type, cudaStream_t s) {
     if (p.out_type == VDT_F32) return own_by_type<float>(p, type, s);

@@ -125,7 +125,7 @@ extern "C" int vdt_int8_linear(const void* d_x, int type, int64_t x_stride, cons
         return api_fail(VDT_ERR_CAPACITY, "scratch smaller than vdt_int8_linear_scratch_bytes");
     if (int s = api_check_buffers(-1, {d_x, d_w, d_w_scale, d_bias, d_out, d_scratch})) return s;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // a few rows: the scratch is not used; every CTA reads all of them, so not
+    // one or two rows: the scratch is not used; every CTA reads all of them, so not
     // into an output that lies over them
     const bool over = overlap(d_x, ((rows - 1) * x_stride + inner) * type_size(type), d_out,
                               ((rows - 1) * out_stride + cols) * type_size(out_type));

@@ -333,7 +333,7 @@ struct Int8Params {
     const void* x;          // launch_int8_own: the rows, x_stride values apart, instead of a and a_scale
     long long x_stride;
 };
-// a few rows that the product's kernel rounds itself
+// one or two rows that the product's kernel rounds itself
 bool int8_rounds_itself(long long rows, int inner);
 cudaError_t launch_int8_own(const Int8Params& p, int type, cudaStream_t s);
 // after_codes: the kernel before it on the stream is the one that writes `a`
