@@ -57,12 +57,19 @@ constexpr int kMostChunk = 4096;   // tokens of a chunk: bounds the page lists i
 // groups of eight rows of a CTA
 int row_groups(long long rows) { return rows <= 8 ? 1 : 2; }
 
-// Fewer tiles than the SMs have room for (three CTAs each): as many chunks as
-// fill it once (a second round of a few CTAs costs as much as the first: 100,000
-// tokens in 66 chunks of 8 heads took 63 us, in 49 50 us).  More tiles: chunks
-// of about 2048 tokens, which even out sequences of different lengths (64 of
-// 1,000 to 8,191 tokens: 121 us with 1536 or 2048, 127 with 2816).  None under
-// 64 tokens a warp.  With one chunk the CTAs write the output themselves.
+// Fewer tiles than the SMs have room for (three CTAs each, as heads of up to 128
+// have it): as many chunks as fill it once (a second round of a few CTAs costs as
+// much as the first: 100,000 tokens in 66 chunks of 8 heads of 128 took 63 us, in 49
+// 50 us).  More tiles: chunks of about 2048 tokens, which even out sequences of
+// different lengths (64 of 1,000 to 8,191 tokens: 121 us with 1536 or 2048, 127 with
+// 2816).  None under 64 tokens a warp.  With one chunk the CTAs write the output
+// themselves.
+//
+// Of heads of 192 two CTAs fit, of 256 one, and three are counted for them as well:
+// sequences of different lengths gain by the more chunks what a long one alone
+// loses (us, with three and with what fits: 16 of 1,400 to 8,000 tokens, 8 cached
+// heads of 192 49 and 59, of 256 70 and 77; one of 100,000, 8 of 192 75 and 60, of 256
+// 94 and 100; one of 30,000, 4 of 256 32 and 24).
 constexpr int kEvenChunk = 2048;
 
 Chunks plan_chunks(int heads, int kv_heads, int seqs, int most, int most_kept) {
