@@ -524,7 +524,8 @@ int vdt_cache_load(const vdt_cache8* cache, const int32_t* d_pages, int width, c
    (an encoder's states).  most_kept bounds d_kept.  A query that sees no token
    gives 0.  A sequence with more tokens than most_kept or its table hold, a run
    of queries that does not fit `most` or `total`, and rows that see a page that
-   is not in the cache give NaN.  Rows of no sequence are left.  d_scratch:
+   is not in the cache give NaN.  Rows of no sequence are left.  d_out may be
+   d_q with the same strides, and must not lie over it otherwise.  d_scratch:
    vdt_cache_attention_scratch_bytes (may be 0), 16-byte aligned. */
 size_t vdt_cache_attention_scratch_bytes(int64_t total, int heads, int kv_heads, int dim, int seqs, int most,
                                          int most_kept);

@@ -371,3 +371,16 @@ def test_a_call_that_fails_in_the_runtime_is_not_kept(dev, tmp_path):
     code = FIRST_FAILS.format(tests=os.path.join(ROOT, "tests"), package=os.path.join(ROOT, "vd-ttfs_b200"), shim=shim)
     done = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, LD_PRELOAD=shim), capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("new,kept", [(1, 90), (1, 9000), (12, 700), (40, 5000), (300, 900)])
+def test_attention_into_its_own_queries(S, new, kept):
+    table, pages = make_table([kept, kept], 64)
+    cache = make_cache(S, pages, 2, 64, 64)
+    q = normal(1, 2 * new, 4, 64, kind=torch.bfloat16).cuda()
+    args = (cache, ints(table), ints([kept] * 2), ints([0, new, 2 * new]), new, kept)
+    want = S.cache_attention(q, *args)
+    for _ in range(3):
+        x = q.clone()
+        S.cache_attention(x, *args, out=x)
+        assert torch.equal(x, want)
