@@ -40,7 +40,7 @@ constexpr int kUnit = 64;          // tokens that a warp takes at a time
 // k_attend_join.
 //
 // Bound by memory where the caches are long: 64 sequences of 1,023 to 8,191
-// tokens, 32 heads of 128 over 8, take 112 us, 5.4 TB/s of codes (floor 95);
+// tokens, 32 heads of 128 over 8, take 110 us, 5.6 TB/s of codes (floor 95);
 // the warps' instructions (some 1,100 for 64 tokens of 128 values, half of them
 // the codes' way to 16 bits) come close behind, and the start and end of a CTA.
 //

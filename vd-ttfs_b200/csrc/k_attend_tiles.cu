@@ -21,7 +21,7 @@
 // they are relative to (the weights are 16-bit floats, which have room for that).
 //
 // Three prompts of up to 2049 tokens behind up to 4096 cached ones, 32 heads of
-// 128 over 8: 401 us, 750 TFLOP/s (44% of the measured bf16 peak).  A step of
+// 128 over 8: 390 us, 773 TFLOP/s (46% of the measured bf16 peak).  A step of
 // two tiles is 2,048 cycles of products and as many of exponentials (16 a
 // cycle); both tiles' softmaxes run side by side, then wait for the products,
 // since the tensor memory has no room for the next step's scores beside two
