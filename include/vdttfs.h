@@ -535,6 +535,111 @@ int vdt_cache_attention(const vdt_cache8* cache, const void* d_q, int64_t q_toke
                         int64_t out_token, int64_t out_head, void* d_scratch, size_t scratch_bytes,
                         vdt_stream stream);
 
+/* Microscaled 4-bit floating point: rows in blocks of 32 values.  A block has a
+   power of two 2^e, the smallest with max |x| <= 6 * 2^e (e >= -127), held as
+   the byte e + 127, and 4-bit codes: x / 2^e rounded to the nearest of 0, 1/2, 1,
+   3/2, 2, 3, 4, 6 (codes 0 to 7) and their negatives (8 to 15), ties to the even
+   code.  A block with an infinity or NaN has the byte 255: its values, and every
+   product of its row, are NaN.  Codes lie two to a byte, the even column in the low
+   bits, in rows that start on 16-byte boundaries (strides multiples of 16) and whose
+   last row's storage reaches to the next multiple of 16 bytes.  Scales lie as the
+   tensor cores read them: tiles of 128 rows x 128 columns, 512 bytes each, row r's
+   four blocks at r % 32 * 16 + r % 128 / 32 * 4; the tiles of 128 rows one after
+   another, their number rounded up to an even one (vdt_fp4_scale_bytes; 16-byte
+   aligned).  Bytes of blocks past the columns are 0, of rows past the last anything. */
+size_t vdt_fp4_scale_bytes(int64_t rows, int cols);
+
+/* x [rows, cols] (VDT_F32 / VDT_F16 / VDT_BF16) in that form.  cols up to 2^30;
+   the last column's byte of an odd number of columns has a 0 in its high bits.
+   The outputs must not lie over d_x. */
+int vdt_quantize_fp4(const void* d_x, int type, int64_t rows, int cols, int64_t x_stride, uint8_t* d_codes,
+                     int64_t codes_stride, uint8_t* d_scale, vdt_stream stream);
+
+/* The values that they stand for, rounded to `type`. */
+int vdt_fp4_values(const uint8_t* d_codes, int64_t codes_stride, const uint8_t* d_scale, int64_t rows, int cols, int type,
+                   void* d_out, int64_t out_stride, vdt_stream stream);
+
+/* out[i][j] = sum_k a[i][k] w[j][k] + bias[j] (d_bias may be NULL), a [rows,
+   inner] and w [cols, inner] in that form, 32-bit sums; cols below 2^30.  An odd
+   `inner` wants 0 in the last byte's high bits, and scale bytes of blocks past
+   it are 0.  d_out must not lie over an input. */
+int vdt_fp4_matmul(const uint8_t* d_a, int64_t a_stride, const uint8_t* d_a_scale, const uint8_t* d_w, int64_t w_stride,
+                   const uint8_t* d_w_scale, const float* d_bias, int64_t rows, int cols, int inner, int out_type,
+                   void* d_out, int64_t out_stride, vdt_stream stream);
+
+/* The two together for rows x [rows, inner] of `type`: each row's codes and
+   scales into d_scratch (256-byte aligned, vdt_fp4_linear_scratch_bytes;
+   VDT_ERR_CAPACITY when smaller), then the product; a few rows may be rounded by
+   the product's own kernel, which does not use the scratch.  d_out may lie over
+   d_x, whose rows are all read before the first is written. */
+size_t vdt_fp4_linear_scratch_bytes(int64_t rows, int inner);
+int vdt_fp4_linear(const void* d_x, int type, int64_t x_stride, const uint8_t* d_w, int64_t w_stride,
+                   const uint8_t* d_w_scale, const float* d_bias, int64_t rows, int cols, int inner, int out_type,
+                   void* d_out, int64_t out_stride, void* d_scratch, size_t scratch_bytes, vdt_stream stream);
+
+/* t = x + residual (32-bit sum rounded to `type`; d_residual NULL: t = x, and no
+   sum is written), z_i = t_i weight_i (d_weight [cols] of `type`, NULL: 1) in 32
+   bits, r = 1 / sqrt(mean(t^2) + eps).  d_sum gets t; vdt_add_rms_norm writes
+   z r in `type`, vdt_add_rms_norm_int8 what vdt_int8_matmul takes: codes
+   round(z / u) with u = max |z| * (1/127), and the scale u r.  A row of zeros has
+   codes 0 (and NaN without eps), one with an infinity or NaN a scale that is not
+   finite.  d_sum may be d_residual or d_x, and d_out d_x or d_residual, with the
+   same strides; d_sum and d_out must not lie over each other, nor any output over an
+   input otherwise. */
+int vdt_add_rms_norm(const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride,
+                     const void* d_weight, int64_t rows, int cols, float eps, int type, void* d_sum, int64_t sum_stride,
+                     void* d_out, int64_t out_stride, vdt_stream stream);
+int vdt_add_rms_norm_int8(const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride,
+                          const void* d_weight, int64_t rows, int cols, float eps, int type, void* d_sum,
+                          int64_t sum_stride, int8_t* d_codes, int64_t codes_stride, float* d_scale, vdt_stream stream);
+
+/* A step's tokens from its sequences' lengths, for the calls on a cache whose
+   pages hold `page` tokens: kept[s] = held[s] + new[s] (negative lengths count
+   as 0), starts[0 .. seqs] the sums of the new tokens before each sequence, and
+   for row starts[s] + i of `total` packed rows positions = held[s] + i and
+   slots = page number * page + place in the page.  Pages that the sequences begin,
+   numbers ceil(held / page) .. ceil(kept / page) of each, are taken from the ring of
+   free ones, d_ring [ring] with d_span = {place of the first free one, how many}, in
+   the order of the sequences, and written into their rows of d_pages [seqs, width].
+   span_out = {the first one left, how many}; below zero: that many were lacking,
+   -1 is in the table in their place, and in the slots of their tokens.  Tokens
+   past a row's width take no page and have slot -1; rows past the last sequence's
+   have position and slot -1.  d_ring and d_new are not changed; kept may be held,
+   and span_out span, for a step in place; other buffers must not lie over each other.
+   d_scratch: vdt_plan_pages_scratch_bytes, 16-byte aligned. */
+size_t vdt_plan_pages_scratch_bytes(int seqs);
+int vdt_plan_pages(const int32_t* d_ring, int ring, const int32_t* d_span, int32_t* d_pages, int width,
+                   const int32_t* d_held, const int32_t* d_new, int seqs, int page, int64_t total, int32_t* d_kept,
+                   int32_t* d_starts, int32_t* d_positions, int64_t* d_slots, int32_t* d_span_out, void* d_scratch,
+                   size_t scratch_bytes, vdt_stream stream);
+
+/* The pages of the sequences with done[s] != 0, numbers 0 .. ceil(held[s] / page)
+   of their rows that are not negative, go behind the ring's last free one, as
+   far as it has room; held_out is 0 for these sequences and held for the others
+   (and may be held), span_out the ring's state after (and may be span). */
+int vdt_free_pages(int32_t* d_ring, int ring, const int32_t* d_span, const int32_t* d_pages, int width,
+                   const int32_t* d_held, const uint8_t* d_done, int seqs, int page, int32_t* d_held_out,
+                   int32_t* d_span_out, vdt_stream stream);
+
+/* The next token of each row of logits [rows, vocab] (VDT_F32 / VDT_F16 / VDT_BF16)
+   from its random number u in [0, 1): weights exp((x - max) / temperature), of
+   which, in the order of (value descending, index ascending), are kept the
+   first top_k (<= 0, or vocab and more: all), of these those before which less
+   than top_p of their sum lies (>= 1: all; always the first), and of these those
+   of at least min_p times the largest; the token is the first index, in the
+   vocabulary's order, at which the sum of the kept weights passes u times their
+   whole sum.  Temperature 0 takes the lowest index of the largest value.
+   d_temperature, d_top_p, d_min_p, d_top_k [rows] give each row its own, NULL takes
+   the number beside.  d_logp (may be NULL): the logarithm of the probability
+   that the token was drawn with.  Weights are whole multiples of 2^-45 (2^-62
+   times the vocabulary's size, above 2^17) and their sums exact, so calls on the
+   same inputs give the same tokens.  A row with a NaN, without a finite logit or +inf, or
+   with a parameter or u that is NaN or out of range gives token -1 and NaN.
+   vocab up to 524288. */
+int vdt_sample(const void* d_logits, int type, int64_t rows, int vocab, int64_t stride, const float* d_u,
+               const float* d_temperature, float temperature, const int32_t* d_top_k, int top_k, const float* d_top_p,
+               float top_p, const float* d_min_p, float min_p, int32_t* d_tokens, float* d_logp, vdt_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

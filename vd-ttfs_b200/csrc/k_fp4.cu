@@ -1,0 +1,453 @@
+// k_fp4.cu -- rows in microscaled 4-bit floating point, and their product.
+//
+// A block of 32 values x_k of a row has one power of two 2^e, the smallest with
+// max|x_k| <= 6 * 2^e, and codes c_k: x_k / 2^e rounded to the nearest of 0, 1/2,
+// 1, 3/2, 2, 3, 4, 6 and their negatives, ties to the even code.  (Rounding the exponent
+// down, as for a block whose largest value may be cut off at 6, would take up to
+// a quarter off the outlying values that a scale of their own is there for.)
+//
+//   y_ij = sum over blocks 2^(e_ib + e'_jb) sum_k c_ik c'_jk + bias_j
+//
+// The tensor cores multiply such operands as they are, codes from shared memory
+// and scales from tensor memory, with 32-bit sums.
+#include "step_internal.h"
+
+namespace vdt {
+namespace {
+
+// The block's scale byte, e + 127, from its largest magnitude's bits: max = m 2^k
+// <= 3/2 2^(e + 2), so e = k - 2, or k - 1 for m above 3/2.  255 where there is an
+// infinity or NaN.
+__device__ __forceinline__ uint32_t scale_byte(float most) {
+    const uint32_t b = __float_as_uint(most);
+    if (b >= 0x7f800000u) return 255;
+    const int e = (int)(b >> 23) - 2 + ((b & 0x7fffffu) > 0x400000u);
+    return (uint32_t)max(e, 0);
+}
+// 2^-e, a normal number for every byte but 255, whose codes are zeros
+__device__ __forceinline__ float inverse_of(uint32_t byte) { return byte == 255 ? 0.0f : __uint_as_float((254 - byte) << 23); }
+// byte 0 is 2^-127, below the normal numbers
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+    return byte == 255 ? __uint_as_float(0x7fffffffu) : byte ? __uint_as_float(byte << 23) : __uint_as_float(0x400000u);
+}
+
+// Eight values' codes, the first in the lowest bits
+__device__ __forceinline__ uint32_t codes_of(const float* f, float inverse) {
+    uint32_t w;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(w)
+        : "f"(f[0] * inverse), "f"(f[1] * inverse), "f"(f[2] * inverse), "f"(f[3] * inverse), "f"(f[4] * inverse), "f"(f[5] * inverse),
+          "f"(f[6] * inverse), "f"(f[7] * inverse));
+    return w;
+}
+// the largest magnitude; infinity and NaN order above the others as bits
+__device__ __forceinline__ float largest(const float* f, int n) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < n; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
+    return __uint_as_float(m);
+}
+
+// Where the scale of a row's block lies: tiles of 128 rows x 4 blocks, row r's
+// four bytes at r % 32 * 16 + r / 32 * 4, which is how the tensor memory takes
+// them (lane r % 32, column r / 32)
+__device__ __forceinline__ long long scale_at(long long row, int block, long long steps) {
+    const int r = (int)(row % kScaleRows);
+    return (row / kScaleRows * steps * 2 + block / 4) * kScaleTile + r % 32 * 16 + r / 32 * 4 + block % 4;
+}
+
+// ------------------------------------------------------------------ quantise
+// Four lanes a block, eight values each.  A warp takes 256 columns, the scales'
+// padding up to there included; what a row's last block lacks counts as zeros.
+constexpr int kPackWarps = 8;
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kPackWarps * 32) k_quantize_fp4(const T* __restrict__ x, long long rows, int cols, long long x_stride,
+                                                                  uint8_t* __restrict__ codes, long long codes_stride,
+                                                                  uint8_t* __restrict__ scale, long long steps) {
+    constexpr int N = Vec16<T>::N;
+    chain_release();
+    const int lane = threadIdx.x % 32;
+    const long long units = rows * steps;
+    for (long long u = (long long)blockIdx.x * kPackWarps + threadIdx.x / 32; u < units; u += (long long)gridDim.x * kPackWarps) {
+        const long long row = u / steps;
+        const long long col = (u - row * steps) * kFp4Step + lane * 8;
+        const T* const from = x + row * x_stride + col;
+        float f[8];
+        if (WIDE && col + 8 <= cols) {
+#pragma unroll
+            for (int j = 0; j < 8; j += N) {
+                Vec16<T> v;
+                v.raw = *reinterpret_cast<const uint4*>(from + j);
+                v.get(f + j);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = col + j < cols ? to_f32(from[j]) : 0.0f;
+        }
+        uint32_t m = __float_as_uint(largest(f, 8));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const uint32_t byte = scale_byte(__uint_as_float(m));
+        const uint32_t w = byte == 255 ? 0 : codes_of(f, inverse_of(byte));
+        if (col < cols) *reinterpret_cast<uint32_t*>(codes + row * codes_stride + col / 2) = w;
+        // four blocks' bytes from sixteen lanes
+        uint32_t four = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) four |= __shfl_sync(0xffffffffu, byte, (lane & 16) + 4 * i) << (8 * i);
+        if (lane % 16 == 0) *reinterpret_cast<uint32_t*>(scale + scale_at(row, (int)(col / kBlock), steps)) = four;
+    }
+}
+
+template <typename T>
+cudaError_t pack_launch(const void* x, long long rows, int cols, long long x_stride, uint8_t* codes, long long codes_stride, uint8_t* scale,
+                        cudaStream_t s) {
+    const bool wide = aligned(x, 16) && x_stride * (long long)sizeof(T) % 16 == 0;
+    const long long steps = fp4_steps(cols), blocks = (rows * steps + kPackWarps - 1) / kPackWarps;
+    auto kern = wide ? k_quantize_fp4<T, true> : k_quantize_fp4<T, false>;
+    kern<<<(unsigned)(blocks < 64 * kSmCount ? blocks : 64 * kSmCount), kPackWarps * 32, 0, s>>>(static_cast<const T*>(x), rows, cols, x_stride, codes,
+                                                                                               codes_stride, scale, steps);
+    return cudaGetLastError();
+}
+
+// --------------------------------------------------------------------- values
+__device__ __forceinline__ float value_of(uint32_t code, float scale) {
+    const uint32_t m = code & 7;
+    const float v = m < 2 ? 0.5f * m : m < 4 ? 0.5f * m : m < 6 ? (float)(m - 2) : 2.0f * (m - 4);
+    return (code & 8 ? -v : v) * scale;
+}
+template <typename T>
+__global__ void __launch_bounds__(256) k_fp4_values(const uint8_t* __restrict__ codes, long long codes_stride, const uint8_t* __restrict__ scale,
+                                                    long long rows, int cols, T* __restrict__ out, long long out_stride, long long steps) {
+    const int per = (cols + 7) / 8;
+    const long long units = rows * per;
+    for (long long u = (long long)blockIdx.x * 256 + threadIdx.x; u < units; u += (long long)gridDim.x * 256) {
+        const long long row = u / per;
+        const int col = (int)(u - row * per) * 8;
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + row * codes_stride + col / 2);
+        const float by = scale_of(scale[scale_at(row, col / kBlock, steps)]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (col + j < cols) out[row * out_stride + col + j] = from_f32<T>(value_of(w >> (4 * j) & 15, by));
+    }
+}
+
+// -------------------------------------------------- block-scaled matrix products
+// d += a b with scales: 128 rows of both operands' 64 consecutive 4-bit values
+__device__ __forceinline__ void mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t a_scale, uint32_t b_scale, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(shape),
+        "r"(a_scale), "r"(b_scale), "r"((uint32_t)add)
+        : "memory");
+}
+// a scale tile of 512 bytes into four columns of the tensor memory, the same for each of its four quarters
+__device__ __forceinline__ void scales_copy(uint32_t to, uint64_t tile) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(to), "l"(tile) : "memory");
+}
+// rows of 16 bytes without swizzle, eight to a group of 128 bytes
+__device__ __forceinline__ uint64_t scale_desc(uint32_t at) {
+    return (uint64_t)((at & 0x3ffff) >> 4) | 1ull << 16 | (uint64_t)(128 >> 4) << 32 | 1ull << 46;
+}
+// e2m1 operands, both with the inner dimension consecutive, scales of 8 exponent
+// bits; `pair`: which two of a scale column's four bytes
+__device__ __forceinline__ constexpr uint32_t fp4_shape(int n, int pair) {
+    return 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | 1u << 23 | (uint32_t)(128 >> 4) << 24 | (uint32_t)(2 * pair) << 29 | (uint32_t)(2 * pair) << 4;
+}
+
+constexpr int kStepBytes = kFp4Step / 2;             // 128: a swizzled row of a stage
+constexpr int kStepScales = 2 * kScaleTile;          // a stage's scales for 128 rows
+
+// ---------------------------------------------------------------- many rows
+// Persistent CTAs over tiles of 128 rows x BN channels, as for 8-bit integers:
+// one thread keeps a ring of stages (256 columns of both sides and their
+// scales) full, one copies scales and issues products, four warps turn sums
+// into outputs.  The scales of a stage have columns of the tensor memory of
+// their own, so they are written again only after the products that read them.
+// BN + the scales leave room for two tiles' sums up to 192 channels.
+constexpr int kTileRows = 128, kTileThreads = 192;
+
+template <int BN>
+struct TileShape {
+    static constexpr int kWTiles = BN <= 128 ? 1 : 2;                      // scale tiles that BN channels may touch
+    static constexpr int kCodes = (kTileRows + BN) * kStepBytes;
+    static constexpr int kStage = kCodes + (1 + kWTiles) * kStepScales;
+    static constexpr int kStages = BN >= 192 ? 4 : BN == 128 ? 5 : 6;
+    static constexpr int kSums = BN == 256 ? 1 : 2;                        // tiles whose sums fit beside the scales
+    static constexpr int kScaleCols = 8 * (1 + kWTiles);                   // of a stage
+    static constexpr int kScalesAt = kSums * BN;
+    static constexpr int kUsed = kScalesAt + kStages * kScaleCols;
+    static constexpr int kCols = kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
+    static constexpr int kOut = 4 * 4096;
+    static constexpr int kBias = 2 * BN * 4;
+    static constexpr int kBytes = 1024 + kStages * kStage + kOut + kBias;
+    static_assert(kUsed <= 512 && kBytes <= 232448 && kStage % 1024 == 0, "tile");
+};
+
+struct TileBars {
+    uint64_t full[8], empty[8], done[2], taken[2];
+    uint32_t tmem;
+};
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(kTileThreads, 1) k_fp4_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                                                               Fp4Params p, int tiles_m, int tiles) {
+    using Shape = TileShape<BN>;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ TileBars bars;
+    unsigned char* smem = smem_raw + ((1024 - (shared_address(smem_raw) & 1023)) & 1023);
+    const uint32_t stages = shared_address(smem);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int steps = (p.inner + kFp4Step - 1) / kFp4Step;
+    if (threadIdx.x == 0) {
+        map_ahead(&map_w);
+        map_ahead(&map_a);
+        for (int i = 0; i < Shape::kStages; ++i) {
+            bar_init(shared_address(&bars.full[i]), 1);
+            bar_init(shared_address(&bars.empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(shared_address(&bars.done[i]), 1);
+            bar_init(shared_address(&bars.taken[i]), 128);
+        }
+        bar_init_done();
+    }
+    if (warp == 1) tmem_alloc(shared_address(&bars.tmem), Shape::kCols);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = bars.tmem;
+    const int w_tiles = (p.cols + kScaleRows - 1) / kScaleRows;
+    // the channels' part of a stage: codes, and the scale tiles that the channels touch
+    auto load_w = [&](uint32_t at, uint32_t bar, int s, int c) {
+        tile_load(at + kTileRows * kStepBytes, &map_w, s * kStepBytes, c, bar);
+        const int t0 = c / kScaleRows;
+#pragma unroll
+        for (int i = 0; i < Shape::kWTiles; ++i)            // a tile past the last has the last one's scales; its products are not stored
+            bulk_load(at + Shape::kCodes + (1 + i) * kStepScales, p.w_scale + ((long long)min(t0 + i, w_tiles - 1) * steps + s) * kStepScales,
+                      kStepScales, bar);
+    };
+    // the weights are the caller's: the first stages' need not wait for the codes
+    const int ahead = min(steps, Shape::kStages);
+    if (threadIdx.x == 0)
+        for (int s = 0; s < ahead; ++s) {
+            const uint32_t bar = shared_address(&bars.full[s]);
+            bar_expect(bar, Shape::kStage);
+            load_w(stages + s * Shape::kStage, bar, s, blockIdx.x / tiles_m * BN);
+        }
+    chain_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int n = 0;
+            bool alive = true;
+            for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
+                const int t = tile % tiles_m, c = tile / tiles_m * BN;
+                for (int s = 0; s < steps; ++s, ++n) {
+                    const int slot = n % Shape::kStages;
+                    const uint32_t at = stages + slot * Shape::kStage, bar = shared_address(&bars.full[slot]);
+                    if (n >= ahead) {
+                        if (!(alive = bar_wait(shared_address(&bars.empty[slot]), (n / Shape::kStages & 1) ^ 1))) break;
+                        bar_expect(bar, Shape::kStage);
+                        load_w(at, bar, s, c);
+                    }
+                    tile_load(at, &map_a, s * kStepBytes, t * kTileRows, bar);
+                    bulk_load(at + Shape::kCodes, p.a_scale + ((long long)t * steps + s) * kStepScales, kStepScales, bar);
+                }
+            }
+            // every load has landed before the CTA ends: the last ones' stages
+            for (int i = max(0, n - Shape::kStages); i < n; ++i)
+                bar_wait(shared_address(&bars.full[i % Shape::kStages]), i / Shape::kStages & 1);
+        }
+    } else if (warp == 1) {
+        const uint32_t sums = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t a = tile_desc(stages), w = tile_desc(stages + kTileRows * kStepBytes), f = scale_desc(stages + Shape::kCodes);
+        const bool one = elected();
+        int n = 0, i = 0;
+        bool alive = true;
+        for (int tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x, ++i) {
+            const int half = i % Shape::kSums;
+            // the first channel's place in its scale tile, a column for 32
+            const uint32_t shift = tile / tiles_m * BN % kScaleRows / 32;
+            if (!(alive = bar_wait_all(shared_address(&bars.taken[half]), (i / Shape::kSums & 1) ^ 1))) break;
+            tmem_fence_after();
+            for (int s = 0; s < steps; ++s, ++n) {
+                const int slot = n % Shape::kStages;
+                if (!(alive = bar_wait_all(shared_address(&bars.full[slot]), n / Shape::kStages & 1))) break;
+                tmem_fence_after();
+                if (one) {
+                    const uint32_t sc = sums + Shape::kScalesAt + slot * Shape::kScaleCols;
+                    // columns: 128 columns of the inner dimension after another, in each the rows' tile, then the channels' tiles
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < 1 + Shape::kWTiles; ++j)
+                            scales_copy(sc + h * (Shape::kScaleCols / 2) + j * 4, f + (slot * Shape::kStage + j * kStepScales + h * kScaleTile) / 16);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t at = sc + k / 2 * (Shape::kScaleCols / 2);
+                        mma_fp4(sums + half * BN, a + (slot * Shape::kStage + k * 32) / 16, w + (slot * Shape::kStage + k * 32) / 16, fp4_shape(BN, k % 2),
+                                at, at + 4 + shift, s > 0 || k > 0);
+                    }
+                    mma_commit(shared_address(&bars.empty[slot]));
+                }
+            }
+            if (alive && one) mma_commit(shared_address(&bars.done[half]));
+        }
+    } else {
+        const int quarter = warp % 4, thread = threadIdx.x - 64;     // a warp reads the rows of its quarter
+        unsigned char* stage = smem + Shape::kStages * Shape::kStage + (warp - 2) * 4096;
+        float* const bias = reinterpret_cast<float*>(smem + Shape::kStages * Shape::kStage + Shape::kOut);
+        T* const out = static_cast<T*>(p.out);
+        constexpr int kPer = 16 / sizeof(T), kCols = 8 * kPer < BN ? 8 * kPer : BN;   // columns of 16 bytes; of a block
+        constexpr int kPieces = kCols / kPer;                         // 16-byte pieces of a block's row
+        const bool wide = p.out_stride * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+        bool alive = true;
+        int i = 0;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++i) {
+            const int half = i % Shape::kSums;
+            const long long row0 = (long long)(tile % tiles_m) * kTileRows + quarter * 32;
+            const int col0 = tile / tiles_m * BN;
+            // the tile before last's are not in use any more: every warp has been past this barrier for the one between
+            float* const bs = bias + (i & 1) * BN;
+            if (p.bias)
+                for (int c = thread; c < BN; c += 128) bs[c] = p.bias[min(col0 + c, p.cols - 1)];
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            alive = alive && bar_wait_all(shared_address(&bars.done[half]), i / Shape::kSums & 1);
+            tmem_fence_after();
+#pragma unroll 1
+            for (int b = 0; b < BN / kCols; ++b) {
+#pragma unroll
+                for (int part = 0; part < kCols / 32; ++part) {
+                    uint32_t r[32];
+                    tmem_load(tmem + half * BN + (quarter * 32 << 16) + b * kCols + part * 32, r);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int q = 0; q < 32 / kPer; ++q) {
+                        float f[kPer];
+                        const int c = b * kCols + part * 32 + q * kPer;
+#pragma unroll
+                        for (int j = 0; j < kPer; ++j) f[j] = __uint_as_float(r[q * kPer + j]);
+                        if (p.bias)
+#pragma unroll
+                            for (int j = 0; j < kPer; ++j) f[j] += bs[c + j];
+                        if (!alive)
+#pragma unroll
+                            for (int j = 0; j < kPer; ++j) f[j] = __int_as_float(0x7fffffff);
+                        Vec16<T> v;
+                        v.set(f);
+                        const int chunk = part * (32 / kPer) + q;
+                        *reinterpret_cast<uint4*>(stage + lane * 128 + ((chunk ^ (lane & (kPieces - 1))) << 4)) = v.raw;
+                    }
+                }
+                __syncwarp();
+                const int col1 = col0 + b * kCols;
+                if (wide && col1 + kCols <= p.cols) {
+                    // kPieces lanes write a row's bytes
+#pragma unroll
+                    for (int k = 0; k < kPieces; ++k) {
+                        const int r = k * (32 / kPieces) + lane / kPieces, c = lane % kPieces;
+                        const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & (kPieces - 1))) << 4));
+                        if (row0 + r < p.rows) *reinterpret_cast<uint4*>(out + (row0 + r) * p.out_stride + col1 + c * kPer) = v;
+                    }
+                } else {
+                    // rows that do not start on 16 bytes, or end in this block: value by value, eight rows read before they are written
+                    T* to = out + row0 * p.out_stride + col1;
+                    for (int r0 = 0; r0 < 32; r0 += 8, to += 8 * p.out_stride)
+#pragma unroll
+                        for (int c0 = 0; c0 < kCols; c0 += 32) {
+                            const int c = c0 + lane, at = c * (int)sizeof(T);
+                            T x[8];
+#pragma unroll
+                            for (int r = 0; r < 8; ++r)
+                                x[r] = *reinterpret_cast<const T*>(stage + (r0 + r) * 128 + (((at >> 4) ^ (r & (kPieces - 1))) << 4) + (at & 15));
+                            if (col1 + c < p.cols)
+#pragma unroll
+                                for (int r = 0; r < 8; ++r)
+                                    if (row0 + r0 + r < p.rows) to[r * p.out_stride + c] = x[r];
+                        }
+                }
+                __syncwarp();
+            }
+            tmem_fence_before();
+            bar_arrive(shared_address(&bars.taken[half]));
+        }
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tmem_fence_after();
+        tmem_free(tmem, Shape::kCols);
+    }
+}
+
+template <typename T, int BN>
+cudaError_t tiles_launch(const Fp4Params& p, bool after, cudaStream_t s) {
+    using Shape = TileShape<BN>;
+    CUtensorMap a, w;
+    const int bytes = (p.inner + 1) / 2;
+    if (!byte_rows_map(&a, p.a, p.rows, bytes, p.a_stride, kStepBytes, kTileRows) ||
+        !byte_rows_map(&w, p.w, p.cols, bytes, p.w_stride, kStepBytes, BN))
+        return cudaErrorInvalidValue;
+    const cudaError_t e = allow_shared<k_fp4_tiles<T, BN>>(Shape::kBytes);
+    if (e != cudaSuccess) return e;
+    const long long tiles_m = (p.rows + kTileRows - 1) / kTileRows, tiles = tiles_m * ((p.cols + BN - 1) / BN);
+    if (tiles > 0x7fffffff - 1024) return cudaErrorInvalidValue;
+    const dim3 grid((unsigned)(tiles < kSmCount ? tiles : kSmCount));
+    if (after) return launch_after(k_fp4_tiles<T, BN>, grid, dim3(kTileThreads), Shape::kBytes, s, a, w, p, (int)tiles_m, (int)tiles);
+    k_fp4_tiles<T, BN><<<grid, kTileThreads, Shape::kBytes, s>>>(a, w, p, (int)tiles_m, (int)tiles);
+    return cudaGetLastError();
+}
+
+// The widest tile whose last round of CTAs is not much emptier than a narrower one's
+template <typename T>
+cudaError_t tiles_by_width(const Fp4Params& p, bool after, cudaStream_t s) {
+    const long long tiles_m = (p.rows + kTileRows - 1) / kTileRows;
+    int best = 0;
+    long long cost = 0;
+    for (const int bn : {256, 192, 128, 64}) {
+        const long long tiles = tiles_m * ((p.cols + bn - 1) / bn), c = (tiles + kSmCount - 1) / kSmCount * (bn + 64);
+        if (!best || c < cost) {
+            best = bn;
+            cost = c;
+        }
+    }
+    if (best == 256) return tiles_launch<T, 256>(p, after, s);
+    if (best == 192) return tiles_launch<T, 192>(p, after, s);
+    if (best == 128) return tiles_launch<T, 128>(p, after, s);
+    return tiles_launch<T, 64>(p, after, s);
+}
+
+}  // namespace
+
+cudaError_t launch_quantize_fp4(const void* x, int type, long long rows, int cols, long long x_stride, uint8_t* codes, long long codes_stride,
+                                uint8_t* scale, cudaStream_t s) {
+    if (type == VDT_F32) return pack_launch<float>(x, rows, cols, x_stride, codes, codes_stride, scale, s);
+    if (type == VDT_F16) return pack_launch<__half>(x, rows, cols, x_stride, codes, codes_stride, scale, s);
+    return pack_launch<__nv_bfloat16>(x, rows, cols, x_stride, codes, codes_stride, scale, s);
+}
+
+cudaError_t launch_fp4_values(const uint8_t* codes, long long codes_stride, const uint8_t* scale, long long rows, int cols, int type, void* out,
+                              long long out_stride, cudaStream_t s) {
+    const long long blocks = (rows * ((cols + 7) / 8) + 255) / 256;
+    const unsigned grid = (unsigned)(blocks < 32 * kSmCount ? blocks : 32 * kSmCount);
+    auto go = [&](auto* to) { k_fp4_values<<<grid, 256, 0, s>>>(codes, codes_stride, scale, rows, cols, to, out_stride, fp4_steps(cols)); };
+    if (type == VDT_F32) go(static_cast<float*>(out));
+    else if (type == VDT_F16) go(static_cast<__half*>(out));
+    else go(static_cast<__nv_bfloat16*>(out));
+    return cudaGetLastError();
+}
+
+bool fp4_rounds_itself(long long) { return false; }
+cudaError_t launch_fp4_own(const Fp4Params&, int, cudaStream_t) { return cudaErrorInvalidValue; }
+
+cudaError_t launch_fp4_matmul(const Fp4Params& p, bool after_codes, cudaStream_t s) {
+    if (p.out_type == VDT_F32) return tiles_by_width<float>(p, after_codes, s);
+    if (p.out_type == VDT_F16) return tiles_by_width<__half>(p, after_codes, s);
+    return tiles_by_width<__nv_bfloat16>(p, after_codes, s);
+}
+
+}  // namespace vdt

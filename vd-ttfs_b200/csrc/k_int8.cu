@@ -516,20 +516,24 @@ EncodeTiled encode_tiled() {
     return reinterpret_cast<EncodeTiled>(f);
 }
 
-bool byte_map(CUtensorMap* m, const int8_t* at, long long rows, int inner, long long stride, int box_rows) {
+}  // namespace
+
+bool byte_rows_map(CUtensorMap* m, const void* at, long long rows, int bytes, long long stride, int box_bytes, int box_rows) {
     const EncodeTiled fn = encode_tiled();
     if (!fn) return false;
-    const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
-    const cuuint32_t box[2] = {kStageBytes, (cuuint32_t)box_rows}, ones[2] = {1, 1};
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(at), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const cuuint64_t dims[2] = {(cuuint64_t)bytes, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {(cuuint32_t)box_bytes, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(at), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+
+namespace {
 
 template <typename T, int BN>
 cudaError_t tiles_launch(const Int8Params& p, bool after, cudaStream_t s) {
     using Shape = GemmShape<BN>;
     CUtensorMap a, w;
-    if (!byte_map(&a, p.a, p.rows, p.inner, p.a_stride, kTileRows) || !byte_map(&w, p.w, p.cols, p.inner, p.w_stride, BN))
+    if (!byte_rows_map(&a, p.a, p.rows, p.inner, p.a_stride, kStageBytes, kTileRows) || !byte_rows_map(&w, p.w, p.cols, p.inner, p.w_stride, kStageBytes, BN))
         return cudaErrorInvalidValue;
     const cudaError_t e = allow_shared<k_int8_tiles<T, BN>>(Shape::kBytes);
     if (e != cudaSuccess) return e;

@@ -272,6 +272,10 @@ __device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap* map, 
         : "memory");
 }
 
+// The map of rows of bytes, `stride` apart, by boxes of box_bytes x box_rows,
+// swizzled over 128 bytes; false where the driver does not make it
+bool byte_rows_map(CUtensorMap* m, const void* at, long long rows, int bytes, long long stride, int box_bytes, int box_rows);
+
 // ---------------------------------------------------- fifth-generation tensor cores
 // A tile in shared memory, rows of 128 bytes swizzled over 1024 (eight rows)
 __device__ __forceinline__ uint64_t tile_desc(uint32_t at) {

@@ -426,9 +426,343 @@ PyObject* cache_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------- microscaled 4-bit floating point
+// codes of rows, two to a byte; their columns, as far as the bytes go
+int64_t fp4_rows(const Tensor& t, const Tensor& scale, const char* what) {
+    on_device(t, what, 2);
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kByte, what, ": uint8 is wanted, got ", t.scalar_type());
+    const int64_t n = t.size(0), k = t.size(1);
+    TORCH_CHECK_VALUE(k > 0 && (k == 1 || t.stride(1) == 1) && (n <= 1 || t.stride(0) >= k) && t.stride(0) % 16 == 0 &&
+                          reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+                      what, ": rows that start on 16-byte boundaries are wanted (see quantize_fp4), got ", t.sizes(), ", strides ", t.strides());
+    TORCH_CHECK_VALUE(!n || t.storage_offset() + (n - 1) * t.stride(0) + (k + 15) / 16 * 16 <= (int64_t)t.storage().nbytes(), what,
+                      ": the last row's storage must reach to the next multiple of 16 bytes");
+    size32(2 * k, what);
+    const int64_t need = (int64_t)vdt_fp4_scale_bytes(n, (int)(2 * k));
+    TORCH_CHECK_VALUE(scale.is_cuda() && scale.scalar_type() == at::kByte && scale.is_contiguous() && scale.numel() == need, what, "'s scales: ", need,
+                      " contiguous CUDA bytes are wanted (see quantize_fp4), got ", scale.sizes(), " of ", scale.scalar_type());
+    return 2 * k;
+}
+
+PyObject* quantize_fp4(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    WANT(2);
+    Tensor x = tensor(a[0], "x");
+    on_device(x, "x", 2);
+    const int type = type_of(x.scalar_type(), "x");
+    const int64_t rows = x.size(0), cols = x.size(1);
+    TORCH_CHECK_VALUE(cols > 0, "x: no columns");
+    const int n = size32(cols, "x: columns");
+    const OnStream on(a[1], x.device());
+    if ((cols > 1 && x.stride(1) != 1) || (rows > 1 && x.stride(0) < cols)) x = x.contiguous();
+    const int64_t bytes = (cols + 1) / 2, step = (bytes + 15) / 16 * 16;
+    const Tensor codes = room({rows, step}, at::kByte, x.device());
+    const Tensor scale = room({(rows + 127) / 128, (cols + 255) / 256 * 2, 32, 16}, at::kByte, x.device());
+    if (const int e = vdt_quantize_fp4(x.data_ptr(), type, rows, n, x.stride(0), static_cast<uint8_t*>(codes.data_ptr()), step,
+                                       static_cast<uint8_t*>(scale.data_ptr()), on.handle()))
+        return status_error(e, "vdt_quantize_fp4");
+    return pair(on.result(codes).narrow(1, 0, bytes), on.result(scale));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* fp4_values(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    WANT(5);
+    const Tensor &codes = tensor(a[0], "codes"), &scale = tensor(a[1], "scale");
+    const int64_t most = fp4_rows(codes, scale, "codes"), cols = a[2] == Py_None ? most : integer(a[2], "cols");
+    TORCH_CHECK_VALUE(cols == most || cols == most - 1, "cols: ", most, " or ", most - 1, " is wanted");
+    const at::ScalarType type = dtype(a[3], "dtype");
+    const int kind = type_of(type, "dtype");
+    const OnStream on(a[4], codes.device());
+    const Tensor out = room({codes.size(0), cols}, type, codes.device());
+    if (cols)
+        if (const int e = vdt_fp4_values(static_cast<uint8_t*>(codes.data_ptr()), row_stride(codes), static_cast<uint8_t*>(scale.data_ptr()),
+                                         codes.size(0), (int)cols, kind, out.data_ptr(), cols, on.handle()))
+            return status_error(e, "vdt_fp4_values");
+    return THPVariable_Wrap(on.result(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// checks of what both products take; the output, new or the caller's
+Tensor fp4_out(int64_t rows, int64_t inner, const Tensor& w, const Tensor& w_scale, const Tensor& bias, const Tensor& out, at::ScalarType type) {
+    const int64_t have = fp4_rows(w, w_scale, "w"), n = w.size(0);
+    TORCH_CHECK_VALUE(n > 0 && (inner + 1) / 2 * 2 == have, "rows of ", inner, " and weights of ", have, " do not multiply");
+    if (bias.defined()) flat(bias, "bias", at::kFloat, n);
+    if (!out.defined()) return room({rows, n}, type, w.device());
+    on_device(out, "out", 2);
+    TORCH_CHECK_VALUE(out.size(0) == rows && out.size(1) == n && (n == 1 || out.stride(1) == 1) && (rows <= 1 || out.stride(0) >= n),
+                      "out: [", rows, ", ", n, "] with consecutive columns is wanted, got ", out.sizes(), ", strides ", out.strides());
+    return out;
+}
+
+PyObject* fp4_matmul(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    WANT(8);
+    const Tensor &x = tensor(a[0], "a"), &xs = tensor(a[1], "a_scale"), &w = tensor(a[2], "w"), &ws = tensor(a[3], "w_scale");
+    const Tensor &bias = tensor_or_none(a[4], "bias"), &given = tensor_or_none(a[6], "out");
+    const int64_t inner = fp4_rows(x, xs, "a"), rows = x.size(0);
+    const OnStream on(a[7], x.device());
+    const Tensor out = fp4_out(rows, inner, w, ws, bias, given, given.defined() ? given.scalar_type() : dtype(a[5], "out_dtype"));
+    const int type = type_of(out.scalar_type(), "out"), n = size32(w.size(0), "w: rows");
+    if (const int e = vdt_fp4_matmul(at_or_null<uint8_t>(x), row_stride(x), at_or_null<uint8_t>(xs), at_or_null<uint8_t>(w), row_stride(w),
+                                     at_or_null<uint8_t>(ws), at_or_null<float>(bias), rows, n, (int)inner, type, out.data_ptr(),
+                                     std::max<int64_t>(out.stride(0), n), on.handle()))
+        return status_error(e, "vdt_fp4_matmul");
+    return THPVariable_Wrap(given.defined() ? out : on.result(out));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* fp4_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    WANT(7);
+    Tensor x = tensor(a[0], "x");
+    const Tensor &w = tensor(a[1], "w"), &ws = tensor(a[2], "w_scale"), &bias = tensor_or_none(a[3], "bias");
+    const Tensor& given = tensor_or_none(a[5], "out");
+    on_device(x, "x", 2);
+    const OnStream on(a[6], x.device());
+    const int type = type_of(x.scalar_type(), "x");
+    const int64_t rows = x.size(0), inner = x.size(1);
+    const Tensor out = fp4_out(rows, inner, w, ws, bias, given,
+                               given.defined() ? given.scalar_type() : a[4] == Py_None ? x.scalar_type() : dtype(a[4], "out_dtype"));
+    const int out_type = type_of(out.scalar_type(), "out");
+    if ((inner > 1 && x.stride(1) != 1) || (rows > 1 && x.stride(0) < inner)) x = x.contiguous();
+    const int k = size32(inner, "x: columns"), n = size32(w.size(0), "w: rows");
+    const int64_t need = (int64_t)vdt_fp4_linear_scratch_bytes(rows, k);
+    const Tensor scratch = room({need}, at::kByte, x.device());
+    if (const int e = vdt_fp4_linear(x.data_ptr(), type, std::max(x.stride(0), inner), at_or_null<uint8_t>(w), row_stride(w), at_or_null<uint8_t>(ws),
+                                     at_or_null<float>(bias), rows, n, k, out_type, out.data_ptr(), std::max<int64_t>(out.stride(0), n),
+                                     scratch.data_ptr(), (size_t)need, on.handle()))
+        return status_error(e, "vdt_fp4_linear");
+    return THPVariable_Wrap(given.defined() ? out : on.result(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// -------------------------------------------- residual's addition and norm
+// What both forms take: x and the residual with consecutive columns, and the sum
+struct NormArgs {
+    Tensor x, residual, weight, sum;
+    int type, cols;
+    int64_t rows;
+};
+bool even_rows(const Tensor& t) { return (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)); }
+// rows of one type and size that the call writes to
+const Tensor& rows_like(const Tensor& t, const Tensor& x, const char* what) {
+    on_device(t, what, 2);
+    TORCH_CHECK_VALUE(t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && even_rows(t), what, ": ", x.sizes(), " of ", x.scalar_type(),
+                      " with consecutive columns is wanted, got ", t.sizes(), " of ", t.scalar_type(), ", strides ", t.strides());
+    return t;
+}
+NormArgs norm_args(PyObject* x, PyObject* residual, PyObject* weight, PyObject* sum) {
+    NormArgs n{tensor(x, "x"), tensor_or_none(residual, "residual"), tensor_or_none(weight, "weight"), tensor_or_none(sum, "sum"), 0, 0, 0};
+    on_device(n.x, "x", 2);
+    n.type = type_of(n.x.scalar_type(), "x");
+    n.rows = n.x.size(0);
+    TORCH_CHECK_VALUE(n.x.size(1) > 0, "x: no columns");
+    n.cols = size32(n.x.size(1), "x: columns");
+    if (n.weight.defined()) flat(n.weight, "weight", n.x.scalar_type(), n.cols);
+    if (n.residual.defined()) {
+        on_device(n.residual, "residual", 2);
+        TORCH_CHECK_VALUE(n.residual.sizes() == n.x.sizes() && n.residual.scalar_type() == n.x.scalar_type(), "residual: ", n.x.sizes(), " of ",
+                          n.x.scalar_type(), " is wanted, got ", n.residual.sizes(), " of ", n.residual.scalar_type());
+        if (n.sum.defined()) rows_like(n.sum, n.x, "sum_out");
+    }
+    TORCH_CHECK_VALUE(n.residual.defined() || !n.sum.defined(), "sum_out: wanted with a residual alone");
+    return n;
+}
+
+PyObject* add_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    WANT(7);
+    NormArgs n = norm_args(a[0], a[1], a[2], a[5]);
+    const float eps = (float)number(a[3], "eps");
+    const Tensor& given = tensor_or_none(a[4], "out");
+    const OnStream on(a[6], n.x.device());
+    const Tensor x = n.x;
+    if (!even_rows(n.x)) n.x = n.x.contiguous();
+    if (n.residual.defined() && !even_rows(n.residual)) n.residual = n.residual.contiguous();
+    const Tensor out = given.defined() ? rows_like(given, x, "out") : room(x.sizes(), x.scalar_type(), x.device());
+    const Tensor sum = !n.residual.defined() ? x : n.sum.defined() ? n.sum : room(x.sizes(), x.scalar_type(), x.device());
+    if (const int e = vdt_add_rms_norm(n.x.data_ptr(), n.x.stride(0), at_or_null(n.residual), n.residual.defined() ? n.residual.stride(0) : 0,
+                                       at_or_null(n.weight), n.rows, n.cols, eps, n.type, n.residual.defined() ? sum.data_ptr() : nullptr,
+                                       sum.stride(0), out.data_ptr(), out.stride(0), on.handle()))
+        return status_error(e, "vdt_add_rms_norm");
+    if (!given.defined()) on.result(out);
+    if (n.residual.defined() && !n.sum.defined()) on.result(sum);
+    return pair(out, sum);
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* triple(const Tensor& a, const Tensor& b, const Tensor& c) {
+    PyObject* t = PyTuple_New(3);
+    if (!t) return nullptr;
+    const Tensor* each[3] = {&a, &b, &c};
+    for (int i = 0; i < 3; ++i) {
+        PyObject* o = THPVariable_Wrap(*each[i]);
+        if (!o) {
+            Py_DECREF(t);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(t, i, o);
+    }
+    return t;
+}
+
+PyObject* add_rms_norm_int8(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    WANT(6);
+    NormArgs n = norm_args(a[0], a[1], a[2], a[4]);
+    const float eps = (float)number(a[3], "eps");
+    const OnStream on(a[5], n.x.device());
+    const Tensor x = n.x;
+    if (!even_rows(n.x)) n.x = n.x.contiguous();
+    if (n.residual.defined() && !even_rows(n.residual)) n.residual = n.residual.contiguous();
+    const Tensor sum = !n.residual.defined() ? x : n.sum.defined() ? n.sum : room(x.sizes(), x.scalar_type(), x.device());
+    const int64_t step = ((int64_t)n.cols + 15) / 16 * 16;
+    const Tensor codes = room({n.rows, step}, at::kChar, x.device()), scale = room({n.rows}, at::kFloat, x.device());
+    if (const int e = vdt_add_rms_norm_int8(n.x.data_ptr(), n.x.stride(0), at_or_null(n.residual), n.residual.defined() ? n.residual.stride(0) : 0,
+                                            at_or_null(n.weight), n.rows, n.cols, eps, n.type, n.residual.defined() ? sum.data_ptr() : nullptr,
+                                            sum.stride(0), static_cast<int8_t*>(codes.data_ptr()), step, static_cast<float*>(scale.data_ptr()),
+                                            on.handle()))
+        return status_error(e, "vdt_add_rms_norm_int8");
+    if (n.residual.defined() && !n.sum.defined()) on.result(sum);
+    return triple(on.result(codes).narrow(1, 0, n.cols), on.result(scale), sum);
+    END_HANDLE_TH_ERRORS
+}
+
+// ------------------------------------------------------------- page tables
+// (ring, span) of a pool of pages
+struct Pool {
+    Tensor ring, span;
+};
+Pool pool_of(PyObject* o) {
+    TORCH_CHECK_TYPE(PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 2, "pool: a tuple of the ring and its span is wanted");
+    Pool p{tensor(PyTuple_GET_ITEM(o, 0), "pool ring"), tensor(PyTuple_GET_ITEM(o, 1), "pool span")};
+    on_device(p.ring, "pool ring", 1);
+    flat(p.ring, "pool ring", at::kInt, p.ring.numel());
+    flat(p.span, "pool span", at::kInt, 2);
+    return p;
+}
+// the caller's tensor, or a new one
+Tensor ints_out(PyObject* given, const char* what, at::ScalarType type, int64_t n, const OnStream& on, at::Device device) {
+    const Tensor& t = tensor_or_none(given, what);
+    if (t.defined()) {
+        flat(t, what, type, n);
+        return t;
+    }
+    return on.result(room({n}, type, device));
+}
+
+PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    WANT(12);
+    const Pool pool = pool_of(a[0]);
+    const Tensor& pages = tensor(a[1], "pages");
+    on_device(pages, "pages", 2);
+    flat(pages, "pages", at::kInt, pages.numel());
+    const int seqs = size32(pages.size(0), "pages: rows"), width = size32(pages.size(1), "pages: columns");
+    const Tensor &held = tensor(a[2], "held"), &fresh = tensor(a[3], "new");
+    flat(held, "held", at::kInt, seqs);
+    flat(fresh, "new", at::kInt, seqs);
+    const int page = small_integer(a[4], "page");
+    const int64_t total = integer(a[5], "total");
+    TORCH_CHECK_VALUE(total >= 0 && page > 0, "page must be positive, total not negative");
+    const at::Device device = pages.device();
+    const OnStream on(a[6], device);
+    const Tensor out[5] = {ints_out(a[7], "out kept", at::kInt, seqs, on, device), ints_out(a[8], "out starts", at::kInt, (int64_t)seqs + 1, on, device),
+                           ints_out(a[9], "out positions", at::kInt, total, on, device), ints_out(a[10], "out slots", at::kLong, total, on, device),
+                           ints_out(a[11], "out span", at::kInt, 2, on, device)};
+    const size_t need = vdt_plan_pages_scratch_bytes(seqs);
+    const Tensor scratch = room({(int64_t)need}, at::kByte, device);
+    if (const int e = vdt_plan_pages(at_or_null<int32_t>(pool.ring), size32(pool.ring.numel(), "pool ring"), at_or_null<int32_t>(pool.span),
+                                     at_or_null<int32_t>(pages), width, at_or_null<int32_t>(held), at_or_null<int32_t>(fresh), seqs, page, total,
+                                     at_or_null<int32_t>(out[0]), at_or_null<int32_t>(out[1]), at_or_null<int32_t>(out[2]), at_or_null<int64_t>(out[3]),
+                                     at_or_null<int32_t>(out[4]), scratch.data_ptr(), need, on.handle()))
+        return status_error(e, "vdt_plan_pages");
+    PyObject* t = PyTuple_New(5);
+    for (int i = 0; t && i < 5; ++i) {
+        PyObject* o = THPVariable_Wrap(out[i]);
+        if (!o) Py_CLEAR(t);
+        else PyTuple_SET_ITEM(t, i, o);
+    }
+    return t;
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* free_pages(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    WANT(8);
+    const Pool pool = pool_of(a[0]);
+    const Tensor& pages = tensor(a[1], "pages");
+    on_device(pages, "pages", 2);
+    flat(pages, "pages", at::kInt, pages.numel());
+    const int seqs = size32(pages.size(0), "pages: rows"), width = size32(pages.size(1), "pages: columns");
+    const Tensor &held = tensor(a[2], "held"), &done = tensor(a[3], "done");
+    flat(held, "held", at::kInt, seqs);
+    TORCH_CHECK_VALUE(done.scalar_type() == at::kBool || done.scalar_type() == at::kByte, "done: bool or uint8 is wanted, got ", done.scalar_type());
+    flat(done, "done", done.scalar_type(), seqs);
+    const int page = small_integer(a[4], "page");
+    TORCH_CHECK_VALUE(page > 0, "page must be positive");
+    const at::Device device = pages.device();
+    const OnStream on(a[5], device);
+    const Tensor out = ints_out(a[6], "out held", at::kInt, seqs, on, device), span = ints_out(a[7], "out span", at::kInt, 2, on, device);
+    if (const int e = vdt_free_pages(at_or_null<int32_t>(pool.ring), size32(pool.ring.numel(), "pool ring"), at_or_null<int32_t>(pool.span),
+                                     at_or_null<int32_t>(pages), width, at_or_null<int32_t>(held), at_or_null<uint8_t>(done), seqs, page,
+                                     at_or_null<int32_t>(out), at_or_null<int32_t>(span), on.handle()))
+        return status_error(e, "vdt_free_pages");
+    return pair(out, span);
+    END_HANDLE_TH_ERRORS
+}
+
+// ---------------------------------------------------------------- sampling
+// a number for all rows, or a tensor with one for each
+const float* floats_or_number(PyObject* o, const char* what, int64_t rows, float* all) {
+    if (!THPVariable_Check(o)) {
+        *all = (float)number(o, what);
+        return nullptr;
+    }
+    const Tensor& t = THPVariable_Unpack(o);
+    flat(t, what, at::kFloat, rows);
+    return static_cast<const float*>(t.data_ptr());
+}
+
+PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    WANT(7);
+    Tensor x = tensor(a[0], "logits");
+    on_device(x, "logits", 2);
+    const int type = type_of(x.scalar_type(), "logits");
+    const int64_t rows = x.size(0);
+    TORCH_CHECK_VALUE(x.size(1) > 0, "logits: no columns");
+    const int vocab = size32(x.size(1), "logits: columns");
+    const Tensor& u = tensor(a[1], "u");
+    flat(u, "u", at::kFloat, rows);
+    float temperature = 0, top_p = 0, min_p = 0;
+    const float *temperatures = floats_or_number(a[2], "temperature", rows, &temperature), *top_ps = floats_or_number(a[4], "top_p", rows, &top_p);
+    const float* min_ps = floats_or_number(a[5], "min_p", rows, &min_p);
+    const int32_t* top_ks = nullptr;
+    int top_k = 0;
+    if (THPVariable_Check(a[3])) {
+        const Tensor& k = THPVariable_Unpack(a[3]);
+        flat(k, "top_k", at::kInt, rows);
+        top_ks = static_cast<const int32_t*>(k.data_ptr());
+    } else {
+        top_k = small_integer(a[3], "top_k");
+    }
+    const OnStream on(a[6], x.device());
+    if (!even_rows(x)) x = x.contiguous();
+    const Tensor tokens = room({rows}, at::kInt, x.device()), logp = room({rows}, at::kFloat, x.device());
+    if (const int e = vdt_sample(x.data_ptr(), type, rows, vocab, x.stride(0), at_or_null<float>(u), temperatures, temperature, top_ks, top_k, top_ps,
+                                 top_p, min_ps, min_p, at_or_null<int32_t>(tokens), at_or_null<float>(logp), on.handle()))
+        return status_error(e, "vdt_sample");
+    return pair(on.result(tokens), on.result(logp));
+    END_HANDLE_TH_ERRORS
+}
+
 #define METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {METHOD(quantize_rows), METHOD(int8_matmul), METHOD(int8_linear), METHOD(qk_norm_rope),
-                          METHOD(cache_append), METHOD(cache_load), METHOD(cache_attention), {nullptr, nullptr, 0, nullptr}};
+                          METHOD(cache_append), METHOD(cache_load), METHOD(cache_attention), METHOD(quantize_fp4), METHOD(fp4_values),
+                          METHOD(fp4_matmul), METHOD(fp4_linear), METHOD(add_rms_norm), METHOD(add_rms_norm_int8), METHOD(plan_pages),
+                          METHOD(free_pages), METHOD(sample), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_seq", "The sequence operators for torch tensors (see vdttfs.seq).", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};
 

@@ -123,6 +123,19 @@ SIGNATURES = {
     "vdt_cache_attention_scratch_bytes": (C.c_size_t, [_l, _i, _i, _i, _i, _i, _i]),
     "vdt_cache_attention": (_i, [_cp, _vp, _l, _l, _i, _i, _vp, _i, _vp, _vp, _i, _l, _i, _i, _i, C.c_float, _vp, _l, _l,
                                  _vp, C.c_size_t, _vp]),
+    # what runs around them in a step
+    "vdt_fp4_scale_bytes": (C.c_size_t, [_l, _i]),
+    "vdt_quantize_fp4": (_i, [_vp, _i, _l, _i, _l, _vp, _l, _vp, _vp]),
+    "vdt_fp4_values": (_i, [_vp, _l, _vp, _l, _i, _i, _vp, _l, _vp]),
+    "vdt_fp4_matmul": (_i, [_vp, _l, _vp, _vp, _l, _vp, _vp, _l, _i, _i, _i, _vp, _l, _vp]),
+    "vdt_fp4_linear_scratch_bytes": (C.c_size_t, [_l, _i]),
+    "vdt_fp4_linear": (_i, [_vp, _i, _l, _vp, _l, _vp, _vp, _l, _i, _i, _i, _vp, _l, _vp, C.c_size_t, _vp]),
+    "vdt_add_rms_norm": (_i, [_vp, _l, _vp, _l, _vp, _l, _i, C.c_float, _i, _vp, _l, _vp, _l, _vp]),
+    "vdt_add_rms_norm_int8": (_i, [_vp, _l, _vp, _l, _vp, _l, _i, C.c_float, _i, _vp, _l, _vp, _l, _vp, _vp]),
+    "vdt_plan_pages_scratch_bytes": (C.c_size_t, [_i]),
+    "vdt_plan_pages": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _l, _vp, _vp, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
+    "vdt_free_pages": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp]),
+    "vdt_sample": (_i, [_vp, _i, _l, _i, _l, _vp, _vp, C.c_float, _vp, _i, _vp, C.c_float, _vp, C.c_float, _vp, _vp, _vp]),
 }
 
 _lib = None

@@ -12,6 +12,16 @@ Cache8                 a paged cache of keys and values in 8 bits          vdt_c
 cache_append           new keys and values into it                         vdt_cache_append
 cache_load             sequences out of it, as values                      vdt_cache_load
 cache_attention        attention over it, causal or not                    vdt_cache_attention
+quantize_fp4           rows in 4-bit floating point, scales for blocks     vdt_quantize_fp4
+fp4_values             the values that they stand for                      vdt_fp4_values
+fp4_matmul             product of such rows and weights                    vdt_fp4_matmul
+fp4_linear             the two together, for 16- or 32-bit rows            vdt_fp4_linear
+add_rms_norm           the residual's addition and the norm of the sum     vdt_add_rms_norm
+add_rms_norm_int8      the same in 8 bits, for int8_matmul                 vdt_add_rms_norm_int8
+PagePool               the free pages of a cache                           (two buffers)
+plan_pages             page tables, positions, slots from lengths          vdt_plan_pages
+free_pages             finished sequences' pages back to the pool          vdt_free_pages
+sample                 the next tokens from logits and random numbers      vdt_sample
 =====================  ==================================================  =========================
 
 Inference only, like the rest of the package.  Tensors are CUDA tensors of the
@@ -140,5 +150,114 @@ def cache_attention(q, cache, pages, kept, starts, most, most_kept, causal=True,
     return _seq.cache_attention(q, cache, pages, kept, starts, most, most_kept, causal, scale, out, stream)
 
 
+# ------------------------------------- microscaled 4-bit floating point --
+def quantize_fp4(x, stream=None):
+    """x [rows, cols] -> (codes uint8 [rows, ceil(cols / 2)], scale uint8): every 32
+    values of a row are rounded to 0, 1/2, 1, 3/2, 2, 3, 4, 6 or their negatives,
+    ties to the even code, times the smallest power of two that no value passes
+    6 of.  Two codes a byte, the even column in the low bits; the scales' bytes (the
+    exponent + 127; 255: a block with an infinity or NaN) lie as the tensor cores
+    read them, [rows / 128, cols / 128, 32, 16], columns in steps of 256, row r's four
+    blocks at [r % 32, r % 128 // 32 * 4:].  Weights [out, in] are quantised
+    with this once, too."""
+    return _seq.quantize_fp4(x, stream)
+
+
+def fp4_values(codes, scale, cols=None, dtype=torch.float32, stream=None):
+    """The values [rows, cols] that quantize_fp4's results stand for (cols: two for
+    each byte, or one less)."""
+    return _seq.fp4_values(codes, scale, cols, dtype, stream)
+
+
+def fp4_matmul(a, a_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16, out=None, stream=None):
+    """a [rows, k] and w [n, k], codes and scales from quantize_fp4, bias [n] float32
+    or None -> a w^T + bias [rows, n], summed in 32 bits."""
+    return _seq.fp4_matmul(a, a_scale, w, w_scale, bias, out_dtype, out, stream)
+
+
+def fp4_linear(x, w, w_scale, bias=None, out_dtype=None, out=None, stream=None):
+    """x [rows, k] (float32, float16 or bfloat16), w and w_scale from quantize_fp4,
+    bias [n] float32 or None: x is rounded in blocks of 32 and multiplied.  Returns
+    [rows, n], of x's type unless out_dtype or out says otherwise; out may be x,
+    or lie over it."""
+    return _seq.fp4_linear(x, w, w_scale, bias, out_dtype, out, stream)
+
+
+# ------------------------------------------ residual's addition and norm --
+def add_rms_norm(x, residual=None, weight=None, eps=1e-6, out=None, sum_out=None, stream=None):
+    """x, residual [rows, cols] of one type (residual may be None) -> (y, t): t = x +
+    residual, y = t / sqrt(mean(t^2) + eps) * weight (of the same type, or None).
+    Without a residual t is x itself.  sum_out may be the residual or x, out x or the
+    residual; they may not lie over each other."""
+    return _seq.add_rms_norm(x, residual, weight, eps, out, sum_out, stream)
+
+
+def add_rms_norm_int8(x, residual=None, weight=None, eps=1e-6, sum_out=None, stream=None):
+    """The same with y in 8 bits, as int8_matmul takes it: (codes, scale, t).  The
+    codes are those of t * weight, the norm is in the scale."""
+    return _seq.add_rms_norm_int8(x, residual, weight, eps, sum_out, stream)
+
+
+# ----------------------------------------------------------- page tables --
+class PagePool(NamedTuple):
+    """The free pages of a cache: ``ring`` int32 [pages] and ``span`` int32 [2], the
+    first free one's place in it and their number; they go on round its end.  Any
+    two such tensors in a tuple serve."""
+    ring: torch.Tensor
+    span: torch.Tensor
+
+    @classmethod
+    def full(cls, pages, device="cuda"):
+        """All of ``pages`` pages free."""
+        return cls(torch.arange(pages, dtype=torch.int32, device=device), torch.tensor([0, pages], dtype=torch.int32, device=device))
+
+
+class PagePlan(NamedTuple):
+    """What plan_pages gives: tokens in the cache after the step and first packed
+    row of each sequence, position and slot of each row, the pool's span after."""
+    kept: torch.Tensor
+    starts: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    span: torch.Tensor
+
+
+def plan_pages(pool, pages, held, new, page, total, out=None, stream=None):
+    """A step's tokens, from the tokens held [seqs] and new [seqs] (int32): pages that
+    the sequences begin are taken from the pool, sequence after sequence, and
+    written into ``pages`` [seqs, width]; returns a PagePlan for ``total`` packed
+    rows.  kept, starts and pages are what cache_append (with held) and cache_attention
+    take, positions what qk_norm_rope takes; slots are page number * page + place.
+    Rows past the last sequence's get -1, and so do slots of tokens without a page:
+    those past the table's width, and those for which the pool has none (then
+    span[1] is below zero, by as many pages).  ``out``: a PagePlan to write
+    to, any of it None; its kept may be held, its span the pool's.  Nothing is
+    copied to the host."""
+    return PagePlan(*_seq.plan_pages(tuple(pool), pages, held, new, page, total, stream, *(out or (None,) * 5)))
+
+
+def free_pages(pool, pages, held, done, page, out=None, stream=None):
+    """The pages of the sequences with done [seqs] (bool) go behind the pool's last:
+    returns (held, span), 0 tokens held for these.  ``out``: the two to write
+    to, which may be held and the pool's span."""
+    return _seq.free_pages(tuple(pool), pages, held, done, page, stream, *(out or (None, None)))
+
+
+# -------------------------------------------------------------- sampling --
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, stream=None):
+    """logits [rows, vocab] (float32, float16 or bfloat16) and a random number
+    u [rows] (float32, in [0, 1)) for each row -> (tokens int32 [rows], logp float32
+    [rows]).  Weights exp((x - max) / temperature); of the tokens by (value descending,
+    index ascending) the first top_k are kept (<= 0: all), of these those before which
+    less than top_p of their sum lies, of these those of at least min_p times the
+    largest; the token is the first index at which the kept weights' sum passes
+    u times the whole.  temperature 0: the lowest index of the largest.  Each parameter a
+    number, or a tensor [rows] (float32; top_k int32).  logp: the logarithm of the
+    probability that the token was drawn with.  A row that gives no token (a NaN in
+    it, -inf alone, a parameter or u out of range) has -1 and NaN."""
+    return _seq.sample(logits, u, temperature, top_k, top_p, min_p, stream)
+
+
 __all__ = ["quantize_rows", "int8_matmul", "int8_linear", "rope_table", "qk_norm_rope", "Cache8", "cache_append",
-           "cache_load", "cache_attention", "NORMS", "SCALINGS"]
+           "cache_load", "cache_attention", "quantize_fp4", "fp4_values", "fp4_matmul", "fp4_linear", "add_rms_norm",
+           "add_rms_norm_int8", "PagePool", "PagePlan", "plan_pages", "free_pages", "sample", "NORMS", "SCALINGS"]
