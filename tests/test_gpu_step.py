@@ -495,6 +495,23 @@ def test_sample_ties(S):
                 check_sample(S, y, u, *args)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_sample_of_masked_rows(S, kind):
+    """Masks of the type's lowest value, of -inf and of both; rows in which they leave one token, or none but masked ones."""
+    low = torch.finfo(kind).min
+    x = (normal(9, 6, 5000) * 2).to(kind)
+    x[0, 10:] = low
+    x[1, 10:], x[1, :5] = -INF, low
+    x[2], x[2, 1::2] = low, -INF
+    x[3], x[3, 77] = low, 0.5
+    x[4] = low
+    x[5], x[5, 4000] = -INF, low
+    u = uniform(4, 6)
+    for t in (0.0, 1e-3, 1.0, 1e35):
+        for k, p, least in ((0, 1.0, 0.0), (7, 1.0, 0.0), (0, 0.9, 0.0), (3000, 0.5, 0.1)):
+            check_sample(S, x, u, t, k, p, least)
+
+
 def test_sample_parameters_of_each_row(S):
     g = torch.Generator().manual_seed(3)
     rows, vocab = 60, 9000

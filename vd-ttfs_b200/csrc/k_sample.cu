@@ -12,16 +12,17 @@
 // in 64 bits: sums are exact, the same in any order, and an answer differs from
 // the real numbers' one where u comes within some 2^-34 of a border.
 //
-// One CTA takes a row, or a cluster of them where rows are few; what does not fit
-// beside the histograms in shared memory is read again from L2.  A histogram of
-// the tokens over 2048 steps of log2(w), 44 an octave, gives the step of the
-// token number k, and, since a step's weights are within a 44th of an octave of
-// each other, bounds of the few steps in which the last token for p lies.  One pass
-// then sums all weights and those before these steps, and lists the steps'
-// tokens; they are told apart by finer histograms while there are many of them, and
-// sorted in the end.  Where no more than kList tokens come up to there, one CTA
-// sorts them all and finishes; else all CTAs sum what is kept, and the part of the
-// warp in which the sum passes the target is gone through again.
+// One CTA takes a row, or a cluster of them where rows are few, and reads it
+// from L2 for each pass.  A histogram of the tokens over 2048 steps of log2(w), 44 an
+// octave, gives the step of the token number k, and an estimate of the few steps
+// in which the last token for p lies: a step's weights are within a 44th of an
+// octave of its middle.  One pass then sums all weights and those before these
+// steps, and lists the steps' tokens.  The sums say whether the estimate holds; where
+// it does not, the same again with the bounds of the steps' weights, which do.  The
+// listed tokens are told apart by finer histograms while there are many of them,
+// and sorted in the end.  Where no more than kList tokens come up to there, one CTA sorts
+// them all and finishes; else all CTAs sum what is kept, and the part of the warp in
+// which the sum passes the target is gone through again.
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -34,7 +35,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = 2048, kRoom = kBins + 4, kList = 1024, kChosen = 8192;
+constexpr int kBins = 2048, kRoom = kBins + 4, kList = 1024, kChosen = 512;
 constexpr float kSteps = 44.0f;              // of an octave; kBins of them are 46.5 octaves, below which weights round to 0
 constexpr int kMostBits = 44, kBoundBits = 40;
 
@@ -95,36 +96,46 @@ struct Top<float> {
 };
 
 struct Weigher {
-    float top, bottom;      // the row's largest value; one whose weight is 0
+    // The row's largest value; a power of two that logits and temperature are taken
+    // times, 1 but for the smallest and largest of them; the largest so, and a value without weight
+    float largest, factor, top, bottom;
     float part, part_top, steps;
     double octaves;         // log2(e) / T
     int bits;
-    __device__ __forceinline__ void set(float largest, float temperature, int vocab) {
-        top = largest;
-        octaves = 1.4426950408889634 / (double)temperature;
+    __device__ __forceinline__ void set(float row_top, float temperature, int vocab) {
+        // The smallest temperatures (below large values nothing has any weight then) and the
+        // largest leave no room for what is computed from them; nor do rows of the type's
+        // lowest value, which -inf is to be below
+        largest = row_top;
+        factor = temperature < 1e-30f && fabsf(largest) < 1e9f ? 0x1p90f : temperature > 1e30f || largest < -1e30f ? 0x1p-20f : 1.0f;
+        top = largest * factor;
+        octaves = 1.4426950408889634 / (double)fmaxf(temperature * factor, 1e-30f);
         float below = value_of(key_of(top) - 1);             // the next value below (0's is not -0)
         if (below == top) below = value_of(key_of(top) - 2);
         bottom = fmaxf(fminf(__double2float_rd((double)top - 80.0 / octaves), below), -FLT_MAX);
         // of large logits halves, whose difference is always a number
-        part = fabsf(top) > 1e30f ? 0.5f : 1.0f;
-        part_top = part * top;
-        steps = (float)(octaves / (double)part * (double)kSteps);
+        const float half = fabsf(top) > 1e30f ? 0.5f : 1.0f;
+        part = half * factor;
+        part_top = part * largest;
+        steps = (float)(octaves / (double)half * (double)kSteps);
         bits = min(kMostBits, 62 - (32 - __clz(vocab - 1)));
         // the next value below the largest has no weight by far: no exponent below a double's
         const double span = (double)top - (double)bottom;
         if (span * octaves > 900.0) octaves = 80.0 / span;
     }
-    // steps below the largest; kBins for all without weight
-    __device__ __forceinline__ float depth(float x) const { return fminf(fmaf(-part, x, part_top) * steps, (float)kBins); }
-    // the step itself: floor in the low bits of 2^23 + depth
-    static __device__ __forceinline__ int step(float depth) { return __float_as_int(__fadd_rd(depth, 8388608.0f)) & (2 * kBins - 1); }
+    // steps below the largest
+    __device__ __forceinline__ float depth(float x) const { return fmaf(-part, x, part_top) * steps; }
+    // the step itself, kBins for all without weight: floor in the low bits of 2^23 + depth
+    static __device__ __forceinline__ int step(float depth) {
+        return __float_as_int(__fadd_rd(fminf(depth, (float)kBins), 8388608.0f)) & (2 * kBins - 1);
+    }
     // 2^bits exp((x - top) / T) to the nearest whole number.  2^f on [-1/2, 1/2] by the
     // interpolating polynomial of degree 8 at Chebyshev's points, off by at most 2^-39.7.
     // 3/2 2^52 added leaves the nearest whole number in the low bits; no branches, so that
     // the chains of several tokens run side by side.
     __device__ __forceinline__ u64 weight(float x) const {
         constexpr double kRound = 6755399441055744.0;
-        const double d = (double)fmaxf(x, bottom) - (double)top;
+        const double d = (double)fmaxf(x * factor, bottom) - (double)top;
         const double z = fma(d, octaves, kRound), f = fma(d, octaves, kRound - z);
         double y = 0x1.63d0e49869220p-20;
         y = fma(y, f, 0x1.00dc4b54b68d6p-16);
@@ -146,7 +157,7 @@ struct Weigher {
 // same one wait for each other), and the tokens of the steps that are looked into
 struct Work {
     uint32_t count[4][kRoom];                // (kBins: tokens without weight; later counts, and the weights' parts)
-    int chosen[kChosen];
+    u64 chosen[kWarps][kChosen];             // each warp its own
 };
 struct Shared {
     u64 list[kList];
@@ -155,7 +166,7 @@ struct Shared {
     u64 found[4];
     u64 kept[kWarps];                        // weight of what each warp's part keeps
     u64 last;
-    unsigned listed, chosen;
+    unsigned listed, chosen[kWarps];
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -190,6 +201,45 @@ __device__ __forceinline__ void block_scan(Shared& sh, u64 (&v)[K], u64 (&all)[K
         all[k] = __shfl_sync(0xffffffffu, upto, 31);
         v[k] += __shfl_sync(0xffffffffu, upto - w, warp) - own[k];
     }
+}
+__device__ __forceinline__ float warp_scan(float v) {
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const float o = __shfl_up_sync(0xffffffffu, v, d);
+        if ((int)(threadIdx.x % 32) >= d) v += o;
+    }
+    return v;
+}
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v) {
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const uint32_t o = __shfl_up_sync(0xffffffffu, v, d);
+        if ((int)(threadIdx.x % 32) >= d) v += o;
+    }
+    return v;
+}
+// the same for a count and a weight, and the sum of a third (its bits in `all`)
+__device__ __forceinline__ void block_scan(Shared& sh, uint32_t& count, u64& weight, float square, u64 (&all)[3]) {
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t own = count, c = warp_scan(count);
+    const u64 mine = weight, w = warp_scan(weight);
+    const float q = warp_scan(square);
+    __syncthreads();
+    if (lane == 31) {
+        sh.warps[0][warp] = c;
+        sh.warps[1][warp] = w;
+        sh.warps[2][warp] = __float_as_uint(q);
+    }
+    __syncthreads();
+    const bool in = lane < kWarps;
+    const uint32_t n = in ? (uint32_t)sh.warps[0][lane] : 0, n_upto = warp_scan(n);
+    const u64 o = in ? sh.warps[1][lane] : 0, o_upto = warp_scan(o);
+    const float q_upto = warp_scan(in ? __uint_as_float((uint32_t)sh.warps[2][lane]) : 0.0f);
+    all[0] = __shfl_sync(0xffffffffu, n_upto, 31);
+    all[1] = __shfl_sync(0xffffffffu, o_upto, 31);
+    all[2] = __float_as_uint(__shfl_sync(0xffffffffu, q_upto, 31));
+    count = c - own + __shfl_sync(0xffffffffu, n_upto - n, warp);
+    weight = w - mine + __shfl_sync(0xffffffffu, o_upto - o, warp);
 }
 template <int K>
 __device__ __forceinline__ void block_sum(Shared& sh, u64 (&v)[K]) {
@@ -226,9 +276,10 @@ struct Row {
     const T* slice;          // this CTA's part
     int first, n, seg;       // its first index, its length, and what a warp takes of it
     bool wide, endless;      // endless: the largest value is +inf, which counts as 0 then, and all others as -inf
-    bool tiny;               // logits and temperature count 2^90 times, for the smallest of them
     int rank, ranks, turn;
     u64 end;                 // the last token's place that counts, as far as it is known
+    float end_value;
+    int end_index;
     Weigher w;
 
     __device__ __forceinline__ void together() const {
@@ -294,10 +345,10 @@ struct Row {
         }
         return v;
     }
-    __device__ __forceinline__ float value(float x) const { return endless ? (x == INFINITY ? 0.0f : -INFINITY) : tiny ? x * 0x1p90f : x; }
+    __device__ __forceinline__ float value(float x) const { return endless ? (x == INFINITY ? 0.0f : -INFINITY) : x; }
     __device__ __forceinline__ void values(const Vec16<T>& v, float* x) const {
         v.get(x);
-        if (endless || tiny)
+        if (endless)
 #pragma unroll
             for (int j = 0; j < N; ++j) x[j] = value(x[j]);
     }
@@ -345,7 +396,12 @@ struct Row {
             atomicAdd(&wk.count[3][bin], (uint32_t)(v >> 30));
         }
     }
-    __device__ __forceinline__ bool before_end(float x, int i) const { return place_of(x, first + i) <= end; }
+    __device__ __forceinline__ void end_at(u64 place) {
+        end = place;
+        end_value = value_at(place);
+        end_index = (int)((uint32_t)place - (uint32_t)first);
+    }
+    __device__ __forceinline__ bool before_end(float x, int i) const { return x > end_value || (x == end_value && i <= end_index); }
     // The row's histogram, of the tokens up to the place `end` (PART), or of all
     template <bool PART>
     __device__ __forceinline__ void histogram() {
@@ -357,76 +413,112 @@ struct Row {
         });
     }
 
-    // The steps of the row's histogram in which the last kept token may lie, for the
-    // count k (k >= 0), or else for the share top_p of the weight: by a step's bounds
-    // of its tokens' weights, in multiples of 2^-40, of the sums and of the whole.
+    // The steps of the row's histogram in which the last kept token lies, for the count
+    // k (k >= 0), or else for the share top_p of the weight.  A step's weight is its
+    // tokens' number times that of its middle, which each of them is off by at most a
+    // factor h = 2^(1/88).  `sure`: steps that the bounds allow; else by the errors' size,
+    // 0.46% (the spread over a step) of each step's weight, four times the root of the
+    // sum of their squares.
     struct Steps {
         int from, to;               // from == kBins: there is no such token
         u64 before, upto;           // tokens before `from`, and up to `to`
     };
-    __device__ __forceinline__ Steps steps_for(int k, float top_p) {
+    __device__ __forceinline__ void gather_counts() {
         constexpr int kPer = kBins / kThreads;
         static_assert(kPer == 4, "four steps a thread");
-        const int mine = kPer * threadIdx.x;
         __syncthreads();
-        auto add = [](uint4 a, uint4 b) { return make_uint4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); };
-        uint4 sum = *reinterpret_cast<const uint4*>(&wk.count[0][mine]);
+        uint4 sum = reinterpret_cast<const uint4*>(&wk.count[0][0])[threadIdx.x];
 #pragma unroll
-        for (int k = 1; k < 4; ++k) sum = add(sum, *reinterpret_cast<const uint4*>(&wk.count[k][mine]));
-        if (ranks > 1) {
-            *reinterpret_cast<uint4*>(&wk.count[0][mine]) = sum;
-            cluster.sync();                                   // all histograms are there
-            uint4 o[8];
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-                o[r] = r < ranks ? *reinterpret_cast<const uint4*>(&cluster.map_shared_rank(&wk, r)->count[0][mine]) : make_uint4(0, 0, 0, 0);
-            sum = o[0];
-#pragma unroll
-            for (int r = 1; r < 8; ++r) sum = add(sum, o[r]);
+        for (int k = 1; k < 4; ++k) {
+            const uint4 o = reinterpret_cast<const uint4*>(&wk.count[k][0])[threadIdx.x];
+            sum = make_uint4(sum.x + o.x, sum.y + o.y, sum.z + o.z, sum.w + o.w);
         }
-        const uint32_t c[kPer] = {sum.x, sum.y, sum.z, sum.w};
-        // bounds of a step's weight; it counts as wider than it is by 2^-16, for the 32-bit depths and exponentials
-        auto under = [](int b) { return (u64)(exp2f((float)kBoundBits - (b + 1.0f) / kSteps) * (1.0f - 0x1p-16f)); };
-        auto over = [](int b) { return (u64)(exp2f((float)kBoundBits - b / kSteps) * (1.0f + 0x1p-16f)) + 1; };
-        u64 v[3] = {}, all[3];
+        reinterpret_cast<uint4*>(&wk.count[0][0])[threadIdx.x] = sum;
+        together();                                           // all histograms are there
+    }
+    __device__ __forceinline__ Steps steps_for(int k, float top_p, bool sure) {
+        constexpr int kPer = kBins / kThreads;
+        const int mine = kBins / ranks, per = (mine + kThreads - 1) / kThreads;      // this CTA's steps; a thread's, consecutive
+        const int from = rank * mine + threadIdx.x * per;
+        uint32_t c[kPer] = {}, count = 0;
+        u64 w[kPer] = {}, weight = 0;
+        float square = 0.0f;
+        if (ranks == 1) {
+            const uint4 o = reinterpret_cast<const uint4*>(&wk.count[0][0])[threadIdx.x];
+            c[0] = o.x;
+            c[1] = o.y;
+            c[2] = o.z;
+            c[3] = o.w;
+        } else if ((int)threadIdx.x * per < mine) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                if (r >= ranks) continue;
+                const uint32_t* const o = &cluster.map_shared_rank(&wk, r)->count[0][from];
+                c[0] += o[0];
+                if (per == 2) c[1] += o[1];
+            }
+        }
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            v[0] += c[i];
-            v[1] += c[i] * under(mine + i);
-            v[2] += c[i] * over(mine + i);
+            const float each = exp2f((float)kBoundBits - (from + i + 0.5f) / kSteps);
+            w[i] = c[i] * (u64)each;
+            count += c[i];
+            weight += w[i];
+            square += (float)w[i] * (float)w[i];
         }
+        u64 all[3];
+        block_scan(sh, count, weight, square, all);
         if (threadIdx.x == 0) {
-            sh.found[0] = sh.found[1] = kBins;
-            sh.found[3] = 0;
+            sh.found[0] = kBins;
+            sh.found[1] = kBins - 1;
         }
-        block_scan(sh, v, all);
+        const auto& slots = say(all);
+        float squares = 0.0f;
+        u64 tokens = 0, total = 0;
+        for (int r = 0; r < ranks; ++r) {
+            if (r < rank) {
+                count += (uint32_t)slots[r][0];
+                weight += slots[r][1];
+            }
+            tokens += slots[r][0];
+            total += slots[r][1];
+            squares += __uint_as_float((uint32_t)slots[r][2]);
+        }
+        if (threadIdx.x == 0) sh.found[3] = tokens;
+        __syncthreads();
         // the first step up to which there may be enough, and the first up to which there is
-        bool whole;
-        u64 least, most;
-        if (k >= 0) {
-            least = most = (u64)k;
-        } else {
-            least = max(share_of(fmaxf(top_p, 0.0f), all[1], &whole), 1ull);
-            most = min(share_of(fmaxf(top_p, 0.0f), all[2], &whole) + 2, all[1]);
+        // (the last, where that is nearly all); 2^(1/44), and room for the 32-bit depths and sums
+        const float whole = (float)total, share = fmaxf(top_p, 0.0f) * whole, wide = 1.0159f * 1.0002f;
+        float lower = share / wide, upper = share * wide;
+        if (!sure) {
+            const float off = 4.0f * 0.0046f * sqrtf(squares) + 1e-5f * whole;
+            lower = fmaxf(lower, share - off);
+            upper = fminf(upper, share + off);
         }
+        const u64 least = max((u64)fmaxf(lower, 0.0f), 1ull), most = upper > whole * 0.9999f ? ~0ull : max((u64)upper, 1ull);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const u64 lo = c[i] * under(mine + i), hi = c[i] * over(mine + i);
-            const u64 a = k >= 0 ? v[0] : v[2], b = k >= 0 ? v[0] : v[1];
-            if (a < least && least <= a + (k >= 0 ? c[i] : hi)) {
-                sh.found[0] = mine + i;
-                sh.found[2] = v[0];
-            }
-            if (b < most && most <= b + (k >= 0 ? c[i] : lo)) {
-                sh.found[1] = mine + i;
-                sh.found[3] = v[0] + c[i];
-            }
-            v[0] += c[i];
-            v[1] += lo;
-            v[2] += hi;
+            const bool here = k >= 0 ? count < (uint32_t)k && (uint32_t)k <= count + c[i] : weight < least && least <= weight + w[i];
+            const bool there = k >= 0 ? here : weight < most && most <= weight + w[i];
+            if (here || there)
+                for (int r = 0; r < ranks; ++r) {
+                    u64* const f = cluster.map_shared_rank(sh.found, r);
+                    if (here) {
+                        f[0] = from + i;
+                        f[2] = count;
+                    }
+                    if (there) {
+                        f[1] = from + i;
+                        f[3] = count + c[i];
+                    }
+                }
+            count += c[i];
+            weight += w[i];
         }
+        together();
+        const Steps found{(int)sh.found[0], (int)sh.found[1], sh.found[2], sh.found[3]};
         __syncthreads();
-        return {(int)sh.found[0], (int)sh.found[1], sh.found[2], sh.found[3]};
+        return found;
     }
 
     // The part of a histogram of counts and weights in which the token number `want`,
@@ -480,78 +572,87 @@ struct Row {
         return r;
     }
 
-    // into the first CTA's list
-    __device__ __forceinline__ void put(u64 place) {
+    // into the first CTA's list, from the lanes that have one; the whole warp
+    __device__ __forceinline__ void put(bool have, u64 place) {
+        const unsigned who = __ballot_sync(0xffffffffu, have);
+        if (!who) return;
+        const int lane = threadIdx.x % 32;
+        unsigned at = 0;
+        if (lane == 0) at = atomicAdd(cluster.map_shared_rank(&sh.listed, 0), (unsigned)__popc(who));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
+        if (have && at < kList) cluster.map_shared_rank(sh.list, 0)[at] = place;
+    }
+    // the same from a lane by itself
+    __device__ __forceinline__ void put_one(u64 place) {
         const unsigned at = atomicAdd(cluster.map_shared_rank(&sh.listed, 0), 1u);
         if (at < kList) cluster.map_shared_rank(sh.list, 0)[at] = place;
     }
     // its length, for the first CTA alone: the others may go on after that one has ended
     __device__ __forceinline__ unsigned in_list() const { return rank == 0 ? min(sh.listed, (unsigned)kList) : 0; }
 
-    // One pass over the row's tokens (PART: up to the place `end`): with WEIGHTS their
-    // weights' sum, and the sum of those in steps before `from`, each warp's into `kept`;
-    // and the tokens of the steps from..to into `chosen`, or of all steps up to `to`
-    // into the first CTA's list.
+    // One pass over the row's tokens (PART: up to the place `end`): with WEIGHTS the
+    // sums of their weights, of those in steps before `from`, each warp's into `kept`, and of those
+    // in steps up to `to`; and the tokens of the steps from..to into `chosen`, or of all
+    // steps up to `to` into the first CTA's list.
     template <bool PART, bool WEIGHTS>
-    __device__ __forceinline__ void look(int from, int to, bool list, u64 (&sums)[2], bool* fits) {
-        if (threadIdx.x == 0) sh.listed = sh.chosen = 0;
+    __device__ __forceinline__ void look(int from, int to, bool list, u64 (&sums)[3], bool* fits) {
+        if (threadIdx.x == 0) sh.listed = 0;
         together();
-        sums[0] = sums[1] = 0;
-        const float upto = (float)(to + 1), since = (float)from, first_step = list ? 0.0f : since;
+        unsigned have = 0;
+        sums[0] = sums[1] = sums[2] = 0;
+        const float since = (float)from, upto = (float)(to + 1), first_step = list ? 0.0f : since;
+        const int lane = threadIdx.x % 32;
         each_vector([&](const float* x, int i) {
             unsigned mine = 0, in = 0;
-            float d[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                d[j] = w.depth(x[j]);
-                if (PART && before_end(x[j], i + j)) in |= 1u << j;
-                if (d[j] < upto && d[j] >= first_step) mine |= 1u << j;
-            }
-            if constexpr (PART) mine &= in;
-            if (WEIGHTS && (!PART || __any_sync(0xffffffffu, in))) {
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const u64 o = w.weight(x[j]), v = d[j] < (float)kBins && (!PART || (in >> j & 1)) ? o : 0;      // (-inf has no weight)
-                    sums[0] += v;
-                    sums[1] += d[j] < since ? v : 0;
-                }
-            }
-            if (!__any_sync(0xffffffffu, mine)) return;
-            if (list) {
+            if constexpr (PART) {
 #pragma unroll
                 for (int j = 0; j < N; ++j)
-                    if (mine >> j & 1) put(place_of(x[j], first + i + j));
-                return;
+                    if (before_end(x[j], i + j)) in |= 1u << j;
+                if (!__any_sync(0xffffffffu, in)) return;
             }
-            const int many = __popc(mine), lane = threadIdx.x % 32;
-            int before = many;
 #pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const int o = __shfl_up_sync(0xffffffffu, before, d);
-                if (lane >= d) before += o;
-            }
-            unsigned at = 0;
-            if (lane == 31) at = atomicAdd(&sh.chosen, (unsigned)before);
-            at = __shfl_sync(0xffffffffu, at, 31) + before - many;
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (mine >> j & 1) {
-                    if (at < kChosen) wk.chosen[at] = i + j;
-                    ++at;
+            for (int j = 0; j < N; ++j) {
+                const float d = w.depth(x[j]);
+                const bool here = !PART || (in >> j & 1);
+                if (WEIGHTS) {
+                    u64 v = w.weight(x[j]);
+                    if (!here) v = 0;
+                    sums[0] += v;
+                    if (d < since) sums[1] += v;
+                    if (d < upto) sums[2] += v;
                 }
+                mine |= (unsigned)(here && d < upto && d >= first_step) << j;
+            }
+            // one of each lane's at a time, hardly ever more than two
+            for (unsigned who; (who = __ballot_sync(0xffffffffu, mine != 0)) != 0; mine &= mine - 1) {
+                const int j = __ffs(mine) - 1;
+                float y = x[0];
+#pragma unroll
+                for (int k = 1; k < N; ++k) y = j == k ? x[k] : y;
+                const u64 place = place_of(y, first + i + j);
+                if (list) {
+                    put(mine != 0, place);
+                } else {
+                    const unsigned at = have + __popc(who & ((1u << lane) - 1));
+                    if (mine && at < kChosen) wk.chosen[threadIdx.x / 32][at] = place;
+                    have += __popc(who);
+                }
+            }
         });
+        if (lane == 0) sh.chosen[threadIdx.x / 32] = have;
         if constexpr (WEIGHTS) {
             const u64 kept = warp_sum(sums[1]);
-            if (threadIdx.x % 32 == 0) sh.kept[threadIdx.x / 32] = kept;
+            if (lane == 0) sh.kept[threadIdx.x / 32] = kept;
             block_sum(sh, sums);
+            const auto& slots = say(sums);
+            sums[0] = sums[1] = sums[2] = 0;
+            for (int r = 0; r < ranks; ++r)
+#pragma unroll
+                for (int k = 0; k < 3; ++k) sums[k] += slots[r][k];
         } else {
             __syncthreads();
         }
-        u64 said[3] = {sums[0], sums[1], sh.chosen > kChosen};
-        say_sum(said);
-        sums[0] = said[0];
-        sums[1] = said[1];
-        *fits = said[2] == 0;
+        *fits = say_max(block_max(have)) <= kChosen;
     }
     // The sorted list's weights (or ones) of this thread's two places, the sum before them,
     // and the whole; those past the first `most` count nothing
@@ -571,16 +672,16 @@ struct Row {
     template <typename F>
     __device__ __forceinline__ void each_chosen(bool listed, int from, int to, F f) const {
         if (listed) {
-            const int many = (int)sh.chosen;
-            for (int k = threadIdx.x; k < many; k += kThreads) {
-                const int i = wk.chosen[k];
-                f(value(to_f32(slice[i])), i);
+            const int warp = threadIdx.x / 32, many = (int)sh.chosen[warp];
+            for (int k = threadIdx.x % 32; k < many; k += 32) {
+                const u64 place = wk.chosen[warp][k];
+                f(value_at(place), place);
             }
         } else {
             const float upto = (float)(to + 1), since = (float)from;
             each([&](float x, int i) {
                 const float d = w.depth(x);
-                if (d >= since && d < upto && before_end(x, i)) f(x, i);
+                if (d >= since && d < upto && (end == ~0ull || before_end(x, i))) f(x, place_of(x, first + i));
             });
         }
     }
@@ -609,7 +710,7 @@ __device__ __forceinline__ void sort_list(u64* a, unsigned n) {
     for (unsigned run = 2; run <= size; run *= 2)
         for (unsigned gap = run / 2; gap; gap /= 2) {
             for (unsigned i = threadIdx.x; i < size / 2; i += kThreads) {
-                const unsigned lo = i / gap * gap * 2 + i % gap, hi = lo + gap;
+                const unsigned lo = 2 * i - (i & (gap - 1)), hi = lo + gap;
                 const bool up = (lo & run) == 0;
                 const u64 x = a[lo], y = a[hi];
                 if ((x > y) == up) {
@@ -633,7 +734,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
     const int first = rank * part, n = max(0, min(p.vocab - first, part));
     const T* const row = static_cast<const T*>(p.logits) + r * p.stride + first;
     const int seg = ((part + kWarps - 1) / kWarps + 32 * N - 1) / (32 * N) * (32 * N);
-    Row<T> s{cluster, sh, wk, row, first, n, seg, reinterpret_cast<uintptr_t>(row) % 16 == 0, false, false, rank, ranks, 0, ~0ull, {}};
+    Row<T> s{cluster, sh, wk, row, first, n, seg, reinterpret_cast<uintptr_t>(row) % 16 == 0, false, rank, ranks, 0, ~0ull, -INFINITY, INT_MIN, {}};
     const float temperature = p.temperatures ? p.temperatures[r] : p.temperature, top_p = p.top_ps ? p.top_ps[r] : p.top_p;
     const float min_p = p.min_ps ? p.min_ps[r] : p.min_p, u = p.u[r];
     const int top_k = p.top_ks ? p.top_ks[r] : p.top_k;
@@ -665,9 +766,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
     }
     Weigher& w = s.w;
     s.endless = top == INFINITY;
-    s.tiny = !s.endless && temperature < 1e-30f && fabsf(top) < 1e9f;
-    // (at that temperature, below larger values nothing has any weight)
-    w.set(s.value(top), s.tiny ? temperature * 0x1p90f : fmaxf(temperature, 1e-30f), p.vocab);
+    w.set(s.value(top), temperature, p.vocab);
     const u64 least = __double2ull_ru((double)fminf(fmaxf(min_p, 0.0f), 1.0f) * (double)(1ull << w.bits));
 
     const bool by_count = top_k > 0 && top_k < p.vocab, by_weight = top_p < 1.0f;
@@ -680,15 +779,22 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         if (partly) s.template histogram<true>();
         else if (!counted) s.template histogram<false>();
         counted = true;
-        const auto at = s.steps_for(weights ? -1 : top_k, top_p);
-        if (at.from == kBins) continue;                   // fewer tokens than k have any weight
-        listed = at.upto <= kList;
-        u64 sums[2];
+        s.gather_counts();
+        typename Row<T>::Steps at;
+        u64 sums[3], want = (u64)top_k;
         bool fits;
-        if (!weights) s.template look<false, false>(at.from, at.to, listed, sums, &fits);
-        else if (partly) s.template look<true, true>(at.from, at.to, listed, sums, &fits);
-        else s.template look<false, true>(at.from, at.to, listed, sums, &fits);
-        u64 want = weights ? want_of(top_p, sums[0]) : (u64)top_k;
+        for (int sure = 0; sure < 2; ++sure) {
+            at = s.steps_for(weights ? -1 : top_k, top_p, sure != 0);
+            if (at.from == kBins) break;
+            listed = at.upto <= kList;
+            if (!weights) s.template look<false, false>(at.from, at.to, listed, sums, &fits);
+            else if (partly) s.template look<true, true>(at.from, at.to, listed, sums, &fits);
+            else s.template look<false, true>(at.from, at.to, listed, sums, &fits);
+            if (!weights) break;
+            want = want_of(top_p, sums[0]);
+            if (sums[1] < want && want <= sums[2]) break;
+        }
+        if (at.from == kBins) continue;                   // fewer tokens than k have any weight
         if (listed) {
             // few tokens up to the last step: the first CTA has them all
             (weights ? limit_w : limit_k) = want;
@@ -701,9 +807,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         const float since = (float)at.from, parts = (float)kBins / (float)(at.to + 1 - at.from);
         float low_part = 0.0f, high_part = INFINITY;
         auto part_of = [&](auto f) {
-            s.each_chosen(fits, at.from, at.to, [&](float x, int i) {
+            s.each_chosen(fits, at.from, at.to, [&](float x, u64 place) {
                 const float q = (w.depth(x) - since) * parts;
-                const u64 place = place_of(x, first + i);
                 if (q >= low_part && q < high_part && place >= lo && place <= hi) f(x, q, place);
             });
         };
@@ -734,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         }
         if (threadIdx.x == 0) sh.listed = 0;
         s.together();
-        part_of([&](float, float, u64 place) { s.put(place); });
+        part_of([&](float, float, u64 place) { s.put_one(place); });
         s.together();
         if (rank == 0) {
             const unsigned few = s.in_list();
@@ -750,12 +855,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
             }
         }
         s.together();
-        s.end = *cluster.map_shared_rank(&sh.last, 0);
+        s.end_at(*cluster.map_shared_rank(&sh.last, 0));
         s.together();
         if (weights && !least) {
             // what the steps' tokens add to each warp's part
-            s.each_chosen(fits, at.from, at.to, [&](float x, int i) {
-                if (s.before_end(x, i)) atomicAdd(&sh.kept[i / seg], w.weight(x));
+            s.each_chosen(fits, at.from, at.to, [&](float x, u64 place) {
+                if (place <= s.end) atomicAdd(&sh.kept[((int)(uint32_t)place - first) / seg], w.weight(x));
             });
             __syncthreads();
             summed = true;
@@ -809,12 +914,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
 
     // everything up to the last: each warp's sum, each CTA's, the whole; then the part of the
     // warp in which the sum passes the target once more
-    const float last_value = s.end == ~0ull ? -INFINITY : value_at(s.end);
-    const int last_index = s.end == ~0ull ? INT_MIN : (int)((uint32_t)s.end - (uint32_t)first);
-    auto weigh = [&](const float* x, int i, u64* v) {
+    const bool all_kept = s.end == ~0ull;
+    auto weigh = [&](const float* x, int i, bool in, u64* v) {
         unsigned kept = 0;
 #pragma unroll
-        for (int j = 0; j < N; ++j) kept |= (x[j] > last_value || (x[j] == last_value && i + j <= last_index)) ? 1u << j : 0u;
+        for (int j = 0; j < N; ++j) kept |= in && (all_kept || s.before_end(x[j], i + j)) ? 1u << j : 0u;
         u64 sum = 0;
 #pragma unroll
         for (int j = 0; j < N; ++j) v[j] = 0;
@@ -833,7 +937,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         u64 mine = 0;
         s.each_vector([&](const float* x, int i) {
             u64 v[N];
-            mine += weigh(x, i, v);
+            mine += weigh(x, i, true, v);
         });
         mine = warp_sum(mine);
         __syncthreads();
@@ -844,29 +948,36 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
     u64 sum[1] = {__shfl_sync(0xffffffffu, upto, 31)};
     const u64 here = sum[0], below = s.say_sum(sum), target = share_of(share, sum[0], &whole);
     if (target < below || target >= below + here) return;
-    // the part in which the target lies, by all warps
+    // the part in which the target lies, by all warps, some consecutive vectors a thread;
+    // then the thread in whose vectors it lies
     const int of = __popc(__ballot_sync(0xffffffffu, below + upto <= target));
-    u64 before = below + __shfl_sync(0xffffffffu, upto - own, of);
-    const int from = of * seg, to = min(n, from + seg);
-    for (int i0 = from; i0 < to; i0 += kThreads * N) {
-        const int i = i0 + (int)threadIdx.x * N;
-        u64 v[N] = {}, part_sum[1] = {0}, all[1];
-        if (i0 + warp * 32 * N < to) {                    // whole warps
-            float x[N];
-            s.values(s.load(i), x);
-            part_sum[0] = weigh(x, i, v);
-        }
-        block_scan(sh, part_sum, all);
-        u64 place = before + part_sum[0];
+    const u64 before = below + __shfl_sync(0xffffffffu, upto - own, of);
+    const int from = of * seg, to = min(n, from + seg), many = ((to - from + N - 1) / N + kThreads - 1) / kThreads;
+    u64 place[1] = {0}, all[1], v[N];
+    for (int k = 0; k < many; ++k) {
+        const int i = from + ((int)threadIdx.x * many + k) * N;
+        float x[N];
+        s.values(s.load(i), x);
+        place[0] += weigh(x, i, i < to, v);
+    }
+    u64 mine = place[0];
+    block_scan(sh, place, all);
+    u64 at = before + place[0];
+    const bool last = at <= target && target < at + mine;
+    if (!__any_sync(0xffffffffu, last)) return;
+    for (int k = 0; k < many; ++k) {
+        const int i = from + ((int)threadIdx.x * many + k) * N;
+        float x[N];
+        s.values(s.load(i), x);
+        weigh(x, i, i < to, v);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            if (place <= target && target < place + v[j]) {
+            if (last && at <= target && target < at + v[j]) {
                 p.tokens[r] = first + i + j;
                 if (p.logp) p.logp[r] = (float)log((double)v[j] / (double)sum[0]);
             }
-            place += v[j];
+            at += v[j];
         }
-        before += all[0];
     }
 }
 
