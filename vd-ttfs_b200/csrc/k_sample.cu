@@ -687,39 +687,62 @@ struct Row {
     }
 };
 
-// Ascending, in place; every thread of the CTA.  A few by counting the smaller ones
-// of each (equal ones, which are all of the largest number there is, keep their order).
-constexpr unsigned kCounted = 192;
+// Ascending, in place; every thread of the CTA.  A few by counting the smaller ones of
+// each (equal ones, which are all of the largest number there is, keep their order); more
+// in a bitonic network, two neighbours a thread.  Partners up
+// to 63 places apart are in the same warp and meet in registers, the others in shared
+// memory (all steps there took four times as long).
+constexpr unsigned kCounted = 128;
 __device__ __forceinline__ void sort_list(u64* a, unsigned n) {
+    static_assert(kList == 2 * kThreads, "two a thread");
+    const unsigned t = threadIdx.x;
     if (n <= kCounted) {
         u64 mine = 0;
         unsigned at = 0;
-        if (threadIdx.x < n) {
-            mine = a[threadIdx.x];
-            for (unsigned i = 0; i < n; ++i) at += a[i] < mine || (a[i] == mine && i < threadIdx.x);
+        if (t < n) {
+            mine = a[t];
+            for (unsigned i = 0; i < n; ++i) at += a[i] < mine || (a[i] == mine && i < t);
         }
         __syncthreads();
-        if (threadIdx.x < n) a[at] = mine;
+        if (t < n) a[at] = mine;
         __syncthreads();
         return;
     }
-    unsigned size = 2;
+    u64 x = 2 * t < n ? a[2 * t] : ~0ull, y = 2 * t + 1 < n ? a[2 * t + 1] : ~0ull;
+    unsigned size = 64;
     while (size < n) size *= 2;
-    for (unsigned i = n + threadIdx.x; i < size; i += kThreads) a[i] = ~0ull;
-    __syncthreads();
-    for (unsigned run = 2; run <= size; run *= 2)
-        for (unsigned gap = run / 2; gap; gap /= 2) {
-            for (unsigned i = threadIdx.x; i < size / 2; i += kThreads) {
-                const unsigned lo = 2 * i - (i & (gap - 1)), hi = lo + gap;
-                const bool up = (lo & run) == 0;
-                const u64 x = a[lo], y = a[hi];
-                if ((x > y) == up) {
-                    a[lo] = y;
-                    a[hi] = x;
-                }
+    for (unsigned run = 2; run <= size; run *= 2) {
+        const bool up = (2 * t & run) == 0;
+        for (unsigned gap = run / 2; gap >= 2; gap /= 2) {
+            u64 ox, oy;
+            if (gap < 64) {
+                if (2 * t >= size) break;                     // whole warps
+                ox = __shfl_xor_sync(0xffffffffu, x, gap / 2);
+                oy = __shfl_xor_sync(0xffffffffu, y, gap / 2);
+            } else {
+                __syncthreads();
+                a[2 * t] = x;
+                a[2 * t + 1] = y;
+                __syncthreads();
+                ox = a[2 * t ^ gap];
+                oy = a[(2 * t ^ gap) + 1];
             }
-            __syncthreads();
+            const bool smaller = ((2 * t & gap) == 0) == up;
+            x = (x < ox) == smaller ? x : ox;
+            y = (y < oy) == smaller ? y : oy;
         }
+        if ((x > y) == up) {
+            const u64 o = x;
+            x = y;
+            y = o;
+        }
+    }
+    __syncthreads();
+    if (2 * t < size) {
+        a[2 * t] = x;
+        a[2 * t + 1] = y;
+    }
+    __syncthreads();
 }
 
 template <typename T>
@@ -857,6 +880,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         s.together();
         s.end_at(*cluster.map_shared_rank(&sh.last, 0));
         s.together();
+        if (!weights && top_k <= kList) {
+            s.template look<true, false>(0, kBins - 1, true, sums, &fits);
+            limit_k = (u64)top_k;
+            in_list = s.in_list();
+            listed = true;
+        }
         if (weights && !least) {
             // what the steps' tokens add to each warp's part
             s.each_chosen(fits, at.from, at.to, [&](float x, u64 place) {
