@@ -10,10 +10,14 @@
 //
 // The tensor cores multiply such operands as they are, codes from shared memory
 // and scales from tensor memory, with 32-bit sums.
+#include <cooperative_groups.h>
+
 #include "step_internal.h"
 
 namespace vdt {
 namespace {
+
+namespace cg = cooperative_groups;
 
 // The block's scale byte, e + 127, from its largest magnitude's bits: max = m 2^k
 // <= 3/2 2^(e + 2), so e = k - 2, or k - 1 for m above 3/2.  255 where there is an
@@ -159,6 +163,252 @@ __device__ __forceinline__ constexpr uint32_t fp4_shape(int n, int pair) {
 
 constexpr int kStepBytes = kFp4Step / 2;             // 128: a swizzled row of a stage
 constexpr int kStepScales = 2 * kScaleTile;          // a stage's scales for 128 rows
+
+// ----------------------------------------------------------------- few rows
+// The channels are the products' 128 rows and the tokens their columns, so a
+// tile holds 128 channels whatever the number of tokens, and what bounds it is the
+// weights' way from memory.  A cluster of CTAs shares a tile's inner dimension, so
+// that all SMs load at once and every CTA's stages are on their way from the
+// start; the sums meet in shared memory.  X: the type of rows that are still to be
+// rounded, which eight warps do for their CTA's part of the inner dimension while
+// the weights come; void: they are codes.  24 x 4096 x 8192 f16: SEE us.
+constexpr int kFewStages = 4, kRoundWarps = 8;
+constexpr int kFewRows = 64, kOwnRows = 64;
+
+template <int NT>
+struct FewShape {
+    static constexpr int kCodes = (128 + NT) * kStepBytes;
+    static constexpr int kStage = kCodes + 2 * kStepScales;
+    static constexpr int kBytes = 1024 + kFewStages * kStage;
+    static constexpr int kScalesAt = 64, kScaleCols = 16, kCols = 128;     // tensor memory: sums, then 16 columns of scales a stage
+    static_assert(NT <= kScalesAt && kScalesAt + kFewStages * kScaleCols <= kCols && NT * 512 <= kFewStages * kStage, "tile");
+};
+struct FewBars {
+    uint64_t full[kFewStages], empty[kFewStages], done;
+    uint32_t tmem;
+};
+
+template <typename X, int NT>
+__global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarps) k_fp4_few(const __grid_constant__ CUtensorMap map_w,
+                                                                                            const __grid_constant__ CUtensorMap map_a, Fp4Params p) {
+    using Shape = FewShape<NT>;
+    constexpr bool kOwn = !std::is_void_v<X>;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ FewBars bars;
+    unsigned char* const smem = smem_raw + ((1024 - (shared_address(smem_raw) & 1023)) & 1023);
+    const uint32_t stages = shared_address(smem);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int split = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int tile = blockIdx.x / split, row0 = blockIdx.y * NT, rows = (int)min((long long)NT, p.rows - row0);
+    const int steps = (p.inner + kFp4Step - 1) / kFp4Step;
+    const int first = (int)((long long)steps * rank / split), last = (int)((long long)steps * (rank + 1) / split);
+    if (threadIdx.x == 0) {
+        map_ahead(&map_w);
+        for (int i = 0; i < kFewStages; ++i) {
+            bar_init(shared_address(&bars.full[i]), kOwn ? 1 + kRoundWarps : 1);
+            bar_init(shared_address(&bars.empty[i]), 1);
+        }
+        bar_init(shared_address(&bars.done), 1);
+        bar_init_done();
+    }
+    if (warp == 1) tmem_alloc(shared_address(&bars.tmem), Shape::kCols);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = bars.tmem;
+    bool alive = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            auto load_w = [&](int s) {
+                const int slot = (s - first) % kFewStages;
+                const uint32_t at = stages + slot * Shape::kStage, bar = shared_address(&bars.full[slot]);
+                bar_expect(bar, kOwn ? 128 * kStepBytes + kStepScales : Shape::kStage);
+                tile_load(at, &map_w, s * kStepBytes, tile * 128, bar);
+                bulk_load(at + Shape::kCodes, p.w_scale + ((long long)tile * steps + s) * kStepScales, kStepScales, bar);
+            };
+            // the weights are the caller's: the first stages' need not wait for the codes
+            const int ahead = min(last, first + kFewStages);
+            for (int s = first; s < ahead; ++s) load_w(s);
+            if constexpr (!kOwn) chain_wait();
+            for (int s = first; s < last && alive; ++s) {
+                const int slot = (s - first) % kFewStages;
+                const uint32_t at = stages + slot * Shape::kStage, bar = shared_address(&bars.full[slot]);
+                if (s >= ahead) {
+                    if (!(alive = bar_wait(shared_address(&bars.empty[slot]), ((s - first) / kFewStages & 1) ^ 1))) break;
+                    load_w(s);
+                }
+                if constexpr (!kOwn) {
+                    tile_load(at + 128 * kStepBytes, &map_a, s * kStepBytes, row0, bar);
+                    bulk_load(at + Shape::kCodes + kStepScales, p.a_scale + ((long long)(row0 / kScaleRows) * steps + s) * kStepScales, kStepScales, bar);
+                }
+            }
+            // every load has landed before the CTA ends: the last ones' stages
+            for (int s = max(first, last - kFewStages); s < last; ++s)
+                bar_wait(shared_address(&bars.full[(s - first) % kFewStages]), (s - first) / kFewStages & 1);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const uint32_t sums = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t w = tile_desc(stages), a = tile_desc(stages + 128 * kStepBytes), f = scale_desc(stages + Shape::kCodes);
+        // codes that are loaded lie in their scale tile where their rows do, a column for 32
+        const uint32_t shift = kOwn ? 0 : row0 % kScaleRows / 32;
+        const bool one = elected();
+        for (int s = first; s < last; ++s) {
+            const int slot = (s - first) % kFewStages;
+            if (!(alive = bar_wait_all(shared_address(&bars.full[slot]), (s - first) / kFewStages & 1))) break;
+            tmem_fence_after();
+            if (one) {
+                const uint32_t sc = sums + Shape::kScalesAt + slot * Shape::kScaleCols;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        scales_copy(sc + h * 8 + j * 4, f + (slot * Shape::kStage + j * kStepScales + h * kScaleTile) / 16);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    mma_fp4(sums, w + (slot * Shape::kStage + k * 32) / 16, a + (slot * Shape::kStage + k * 32) / 16, fp4_shape(NT, k % 2), sc + k / 2 * 8,
+                            sc + k / 2 * 8 + 4 + shift, s > first || k > 0);
+                mma_commit(shared_address(&bars.empty[slot]));
+            }
+        }
+        if (alive && one) mma_commit(shared_address(&bars.done));
+    } else if constexpr (kOwn) {
+        // four lanes a block, eight values each; a step's rows after another
+        constexpr int N = Vec16<X>::N, kThreads = 32 * kRoundWarps, kMost = NT * 32 / kThreads;
+        const int t = threadIdx.x - 64;
+        const X* const x = static_cast<const X*>(p.x) + (long long)row0 * p.x_stride;
+        const bool wide = p.x_stride * (long long)sizeof(X) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+        for (int s = first; s < last; ++s) {
+            const int slot = (s - first) % kFewStages;
+            unsigned char* const at = smem + slot * Shape::kStage;
+            float f[kMost][8];
+#pragma unroll
+            for (int k = 0; k < kMost; ++k) {
+                const int row = (t + k * kThreads) / 32, col = s * kFp4Step + t % 32 * 8;
+                const X* const from = x + (long long)row * p.x_stride + col;
+                if (row < rows && wide && col + 8 <= p.inner) {
+#pragma unroll
+                    for (int j = 0; j < 8; j += N) {
+                        Vec16<X> v;
+                        v.raw = *reinterpret_cast<const uint4*>(from + j);
+                        v.get(f[k] + j);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) f[k][j] = row < rows && col + j < p.inner ? to_f32(from[j]) : 0.0f;
+                }
+            }
+            if (s - first >= kFewStages) {
+                if (!bar_wait_all(shared_address(&bars.empty[slot]), ((s - first) / kFewStages & 1) ^ 1)) break;
+            }
+#pragma unroll
+            for (int k = 0; k < kMost; ++k) {
+                const int row = (t + k * kThreads) / 32;             // a warp's lanes have one row
+                if (row >= rows) break;
+                uint32_t m = __float_as_uint(largest(f[k], 8));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const uint32_t byte = scale_byte(__uint_as_float(m)), w = byte == 255 ? 0 : codes_of(f[k], inverse_of(byte));
+                const int chunk = lane / 4;                          // of 16 bytes, swizzled by the row
+                *reinterpret_cast<uint32_t*>(at + (128 + row) * kStepBytes + ((chunk ^ (row & 7)) << 4) + lane % 4 * 4) = w;
+                if (lane % 4 == 0) at[Shape::kCodes + kStepScales + chunk / 4 * kScaleTile + row % 32 * 16 + row / 32 * 4 + chunk % 4] = (unsigned char)byte;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tensor cores read what these lanes wrote
+            __syncwarp();
+            if (lane == 0) bar_arrive(shared_address(&bars.full[slot]));
+        }
+    }
+
+    // the sums: channel 32 (warp % 4) + lane, tokens side by side
+    const int quarter = warp % 4;
+    float* const part = reinterpret_cast<float*>(smem);              // [NT][128], over stages that are through
+    const bool reads = warp >= 2 && warp < 6;
+    if (reads) {
+        alive = bar_wait_all(shared_address(&bars.done), 0);
+        tmem_fence_after();
+#pragma unroll
+        for (int b = 0; b < (NT + 31) / 32; ++b) {
+            uint32_t r[32];
+            tmem_load(tmem + (quarter * 32 << 16) + b * 32, r);
+            tmem_load_wait();
+#pragma unroll
+            for (int c = 0; c < (NT < 32 ? NT : 32); ++c)
+                part[(b * 32 + c) * 128 + quarter * 32 + lane] = alive ? __uint_as_float(r[c]) : __int_as_float(0x7fffffff);
+        }
+    }
+    tmem_fence_before();
+    __syncwarp();
+    if (split > 1) cluster.sync();
+    else __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tmem_fence_after();
+        tmem_free(tmem, Shape::kCols);
+    }
+    // each CTA adds up its share of the tokens
+    const int from = rows * rank / split, to = rows * (rank + 1) / split;
+    for (int i = threadIdx.x; i < (to - from) * 128; i += blockDim.x) {
+        const int row = from + i / 128, col = tile * 128 + i % 128;
+        float y = 0.0f;
+        if (split == 1) {
+            y = part[row * 128 + i % 128];
+        } else {
+            float o[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) o[r] = r < split ? cluster.map_shared_rank(part, r)[row * 128 + i % 128] : 0.0f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) y += o[r];
+        }
+        if (col >= p.cols) continue;
+        if (p.bias) y += p.bias[col];
+        const long long at = (long long)(row0 + row) * p.out_stride + col;
+        if (p.out_type == VDT_F32) static_cast<float*>(p.out)[at] = y;
+        else if (p.out_type == VDT_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(y);
+        else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+    }
+    if (split > 1) cluster.sync();                                   // until the others have read this CTA's part
+}
+
+template <typename X, int NT>
+cudaError_t few_launch(const Fp4Params& p, bool after, cudaStream_t s) {
+    using Shape = FewShape<NT>;
+    CUtensorMap w, a;
+    const int bytes = (p.inner + 1) / 2;
+    if (!byte_rows_map(&w, p.w, p.cols, bytes, p.w_stride, kStepBytes, 128)) return cudaErrorInvalidValue;
+    if (std::is_void_v<X>) {
+        if (!byte_rows_map(&a, p.a, p.rows, bytes, p.a_stride, kStepBytes, NT)) return cudaErrorInvalidValue;
+    } else {
+        a = w;
+    }
+    const cudaError_t e = allow_shared<k_fp4_few<X, NT>>(Shape::kBytes);
+    if (e != cudaSuccess) return e;
+    // as many CTAs a tile as put two on every SM, each with a step at least
+    const long long tiles = (long long)((p.cols + 127) / 128) * ((p.rows + NT - 1) / NT), steps = fp4_steps(p.inner);
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= 2 * kSmCount && steps >= split * 2) split *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((p.cols + 127) / 128 * split), (unsigned)((p.rows + NT - 1) / NT));
+    cfg.blockDim = dim3(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarps);
+    cfg.dynamicSmemBytes = Shape::kBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = after ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, k_fp4_few<X, NT>, w, a, p);
+}
+template <typename X>
+cudaError_t few_by_rows(const Fp4Params& p, bool after, cudaStream_t s) {
+    if (p.rows <= 16) return few_launch<X, 16>(p, after, s);
+    if (p.rows <= 32) return few_launch<X, 32>(p, after, s);
+    return few_launch<X, 64>(p, after, s);
+}
 
 // ---------------------------------------------------------------- many rows
 // Persistent CTAs over tiles of 128 rows x BN channels, as for 8-bit integers:
@@ -441,10 +691,16 @@ cudaError_t launch_fp4_values(const uint8_t* codes, long long codes_stride, cons
     return cudaGetLastError();
 }
 
-bool fp4_rounds_itself(long long) { return false; }
-cudaError_t launch_fp4_own(const Fp4Params&, int, cudaStream_t) { return cudaErrorInvalidValue; }
+bool fp4_rounds_itself(long long rows) { return rows <= kOwnRows; }
+
+cudaError_t launch_fp4_own(const Fp4Params& p, int type, cudaStream_t s) {
+    if (type == VDT_F32) return few_by_rows<float>(p, false, s);
+    if (type == VDT_F16) return few_by_rows<__half>(p, false, s);
+    return few_by_rows<__nv_bfloat16>(p, false, s);
+}
 
 cudaError_t launch_fp4_matmul(const Fp4Params& p, bool after_codes, cudaStream_t s) {
+    if (p.rows <= kFewRows) return few_by_rows<void>(p, after_codes, s);
     if (p.out_type == VDT_F32) return tiles_by_width<float>(p, after_codes, s);
     if (p.out_type == VDT_F16) return tiles_by_width<__half>(p, after_codes, s);
     return tiles_by_width<__nv_bfloat16>(p, after_codes, s);
