@@ -198,7 +198,7 @@ extern "C" int vdt_plan_pages(const int32_t* d_ring, int ring, const int32_t* d_
         return api_fail(VDT_ERR_CAPACITY, "scratch smaller than vdt_plan_pages_scratch_bytes");
     if (int s = api_check_buffers(-1, {d_ring, d_span, d_pages, d_held, d_new, d_kept, d_starts, d_positions, d_slots, d_span_out, d_scratch})) return s;
     PlanParams p{d_ring, d_span, d_pages, d_held, d_new, d_kept, d_starts, d_positions, d_span_out, d_slots, static_cast<int32_t*>(d_scratch),
-                 total, ring, width, seqs, page};
+                 total, ring, width, seqs, page, 0, false};
     return launched(launch_plan_pages(p, static_cast<cudaStream_t>(stream)), "plan_pages");
 }
 
@@ -209,7 +209,7 @@ extern "C" int vdt_free_pages(int32_t* d_ring, int ring, const int32_t* d_span, 
     STEP_REQUIRE(d_span_out && (!seqs || (d_done && d_held_out)), "NULL buffer");
     STEP_REQUIRE(aligned(d_held_out, 4) && aligned(d_span_out, 4), "alignment");
     if (int s = api_check_buffers(-1, {d_ring, d_span, d_pages, d_held, d_done, d_held_out, d_span_out})) return s;
-    FreeParams p{d_ring, d_span, d_pages, d_held, d_done, d_held_out, d_span_out, ring, width, seqs, page};
+    FreeParams p{d_ring, d_span, d_pages, d_held, d_done, d_held_out, d_span_out, ring, width, seqs, page, 0};
     return launched(launch_free_pages(p, static_cast<cudaStream_t>(stream)), "free_pages");
 }
 

@@ -59,7 +59,8 @@ struct PlanParams {
     int64_t* slots;
     int32_t* scratch;
     long long total;
-    int size, width, seqs, page;
+    int size, width, seqs, page, shift;     // shift: set by the launch, log2(page) or -1
+    bool wide;                              // so is this: positions and slots on 16 bytes
 };
 size_t plan_scratch_bytes(int seqs);
 cudaError_t launch_plan_pages(const PlanParams& p, cudaStream_t s);
@@ -69,7 +70,7 @@ struct FreeParams {
     const int32_t *span, *pages, *held;
     const uint8_t* done;
     int32_t *held_out, *span_out;
-    int size, width, seqs, page;
+    int size, width, seqs, page, shift;
 };
 cudaError_t launch_free_pages(const FreeParams& p, cudaStream_t s);
 

@@ -233,14 +233,14 @@ def plan_pages(pool, pages, held, new, page, total, out=None, stream=None):
     span[1] is below zero, by as many pages).  ``out``: a PagePlan to write
     to, any of it None; its kept may be held, its span the pool's.  Nothing is
     copied to the host."""
-    return PagePlan(*_seq.plan_pages(tuple(pool), pages, held, new, page, total, stream, *(out or (None,) * 5)))
+    return PagePlan._make(_seq.plan_pages(pool, pages, held, new, page, total, stream, *(out or (None,) * 5)))
 
 
 def free_pages(pool, pages, held, done, page, out=None, stream=None):
     """The pages of the sequences with done [seqs] (bool) go behind the pool's last:
     returns (held, span), 0 tokens held for these.  ``out``: the two to write
     to, which may be held and the pool's span."""
-    return _seq.free_pages(tuple(pool), pages, held, done, page, stream, *(out or (None, None)))
+    return _seq.free_pages(pool, pages, held, done, page, stream, *(out or (None, None)))
 
 
 # -------------------------------------------------------------- sampling --
