@@ -64,23 +64,26 @@ __device__ __forceinline__ long long scale_at(long long row, int block, long lon
 }
 
 // ------------------------------------------------------------------ quantise
-// Four lanes a block, eight values each.  A warp takes 256 columns, the scales'
-// padding up to there included; what a row's last block lacks counts as zeros.
+// Four lanes a block, eight values each.  A warp takes 256 columns of a row, the
+// scales' padding up to there included; what a row's last block lacks counts as
+// zeros.  Rows of few columns share a CTA, 2^across warps each.  Bound by memory:
+// 8192 x 4096 bf16 SEE us.
 constexpr int kPackWarps = 8;
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kPackWarps * 32) k_quantize_fp4(const T* __restrict__ x, long long rows, int cols, long long x_stride,
                                                                   uint8_t* __restrict__ codes, long long codes_stride,
-                                                                  uint8_t* __restrict__ scale, long long steps) {
+                                                                  uint8_t* __restrict__ scale, int steps, int across) {
     constexpr int N = Vec16<T>::N;
     chain_release();
-    const int lane = threadIdx.x % 32;
-    const long long units = rows * steps;
-    for (long long u = (long long)blockIdx.x * kPackWarps + threadIdx.x / 32; u < units; u += (long long)gridDim.x * kPackWarps) {
-        const long long row = u / steps;
-        const long long col = (u - row * steps) * kFp4Step + lane * 8;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int step = (blockIdx.x << across) + (warp & ((1 << across) - 1)), per = kPackWarps >> across;
+    if (step >= steps) return;
+    const int col = step * kFp4Step + lane * 8;
+    const bool whole = WIDE && col + 8 <= cols;
+    for (long long row = (long long)blockIdx.y * per + (warp >> across); row < rows; row += (long long)gridDim.y * per) {
         const T* const from = x + row * x_stride + col;
         float f[8];
-        if (WIDE && col + 8 <= cols) {
+        if (whole) {
 #pragma unroll
             for (int j = 0; j < 8; j += N) {
                 Vec16<T> v;
@@ -94,25 +97,27 @@ __global__ void __launch_bounds__(kPackWarps * 32) k_quantize_fp4(const T* __res
         uint32_t m = __float_as_uint(largest(f, 8));
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const uint32_t byte = scale_byte(__uint_as_float(m));
+        uint32_t byte = scale_byte(__uint_as_float(m));
         const uint32_t w = byte == 255 ? 0 : codes_of(f, inverse_of(byte));
         if (col < cols) *reinterpret_cast<uint32_t*>(codes + row * codes_stride + col / 2) = w;
         // four blocks' bytes from sixteen lanes
-        uint32_t four = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) four |= __shfl_sync(0xffffffffu, byte, (lane & 16) + 4 * i) << (8 * i);
-        if (lane % 16 == 0) *reinterpret_cast<uint32_t*>(scale + scale_at(row, (int)(col / kBlock), steps)) = four;
+        byte |= __shfl_down_sync(0xffffffffu, byte, 4) << 8;
+        byte |= __shfl_down_sync(0xffffffffu, byte, 8) << 16;
+        if (lane % 16 == 0) *reinterpret_cast<uint32_t*>(scale + scale_at(row, col / kBlock, steps)) = byte;
     }
 }
 
 template <typename T>
 cudaError_t pack_launch(const void* x, long long rows, int cols, long long x_stride, uint8_t* codes, long long codes_stride, uint8_t* scale,
                         cudaStream_t s) {
-    const bool wide = aligned(x, 16) && x_stride * (long long)sizeof(T) % 16 == 0;
-    const long long steps = fp4_steps(cols), blocks = (rows * steps + kPackWarps - 1) / kPackWarps;
+    const bool wide = aligned(x, 16) && (rows == 1 || x_stride * (long long)sizeof(T) % 16 == 0);
+    const int steps = (int)fp4_steps(cols);
+    int across = 0;
+    while (across < 3 && (1 << across) < steps) ++across;
+    const long long per = kPackWarps >> across, down = (rows + per - 1) / per;
+    const dim3 grid((unsigned)((steps + (1 << across) - 1) >> across), (unsigned)(down < 65535 ? down : 65535));
     auto kern = wide ? k_quantize_fp4<T, true> : k_quantize_fp4<T, false>;
-    kern<<<(unsigned)(blocks < 64 * kSmCount ? blocks : 64 * kSmCount), kPackWarps * 32, 0, s>>>(static_cast<const T*>(x), rows, cols, x_stride, codes,
-                                                                                               codes_stride, scale, steps);
+    kern<<<grid, kPackWarps * 32, 0, s>>>(static_cast<const T*>(x), rows, cols, x_stride, codes, codes_stride, scale, steps, across);
     return cudaGetLastError();
 }
 
@@ -413,11 +418,15 @@ cudaError_t few_by_rows(const Fp4Params& p, bool after, cudaStream_t s) {
 // ---------------------------------------------------------------- many rows
 // Persistent CTAs over tiles of 128 rows x BN channels, as for 8-bit integers:
 // one thread keeps a ring of stages (256 columns of both sides and their
-// scales) full, one copies scales and issues products, four warps turn sums
+// scales) full, one copies scales and issues products, eight warps turn sums
 // into outputs.  The scales of a stage have columns of the tensor memory of
 // their own, so they are written again only after the products that read them.
-// BN + the scales leave room for two tiles' sums up to 192 channels.
-constexpr int kTileRows = 128, kTileThreads = 192;
+// Beside them there is no room for two tiles' sums of 256 channels, so the eight
+// warps take all of a tile's sums into registers at once (128 a thread) and the
+// next tile's products start before the first output is written.  What bounds it
+// is the way of the stages from L2, some 19 TB/s; tiles of 192 channels, whose sums fit
+// twice, read a sixth more of them.  8192 x 4096 x 8192: SEE us.
+constexpr int kTileRows = 128, kOutWarps = 8, kTileThreads = 64 + 32 * kOutWarps;
 
 template <int BN>
 struct TileShape {
@@ -430,7 +439,7 @@ struct TileShape {
     static constexpr int kScalesAt = kSums * BN;
     static constexpr int kUsed = kScalesAt + kStages * kScaleCols;
     static constexpr int kCols = kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
-    static constexpr int kOut = 4 * 4096;
+    static constexpr int kOut = kOutWarps * 2048;                          // 32 rows of 64 bytes for each warp, where outputs are not on 32 bytes
     static constexpr int kBias = 2 * BN * 4;
     static constexpr int kBytes = 1024 + kStages * kStage + kOut + kBias;
     static_assert(kUsed <= 512 && kBytes <= 232448 && kStage % 1024 == 0, "tile");
@@ -460,7 +469,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_fp4_tiles(const __grid_cons
         }
         for (int i = 0; i < 2; ++i) {
             bar_init(shared_address(&bars.done[i]), 1);
-            bar_init(shared_address(&bars.taken[i]), 128);
+            bar_init(shared_address(&bars.taken[i]), 32 * kOutWarps);
         }
         bar_init_done();
     }
@@ -547,82 +556,97 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_fp4_tiles(const __grid_cons
             if (alive && one) mma_commit(shared_address(&bars.done[half]));
         }
     } else {
-        const int quarter = warp % 4, thread = threadIdx.x - 64;     // a warp reads the rows of its quarter
-        unsigned char* stage = smem + Shape::kStages * Shape::kStage + (warp - 2) * 4096;
+        // a warp reads the rows of its quarter, half of the channels
+        constexpr int kCols = BN / 2, kWords = kCols * (int)sizeof(T) / 4;
+        const int quarter = warp % 4, thread = threadIdx.x - 64, half_col = (warp - 2) / 4 * kCols;
+        unsigned char* stage = smem + Shape::kStages * Shape::kStage + (warp - 2) * 2048;
         float* const bias = reinterpret_cast<float*>(smem + Shape::kStages * Shape::kStage + Shape::kOut);
         T* const out = static_cast<T*>(p.out);
-        constexpr int kPer = 16 / sizeof(T), kCols = 8 * kPer < BN ? 8 * kPer : BN;   // columns of 16 bytes; of a block
-        constexpr int kPieces = kCols / kPer;                         // 16-byte pieces of a block's row
-        const bool wide = p.out_stride * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+        const bool wide = p.out_stride * sizeof(T) % 32 == 0 && reinterpret_cast<uintptr_t>(out) % 32 == 0;
         bool alive = true;
         int i = 0;
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++i) {
             const int half = i % Shape::kSums;
             const long long row0 = (long long)(tile % tiles_m) * kTileRows + quarter * 32;
-            const int col0 = tile / tiles_m * BN;
+            const int col0 = tile / tiles_m * BN + half_col;
             // the tile before last's are not in use any more: every warp has been past this barrier for the one between
             float* const bs = bias + (i & 1) * BN;
             if (p.bias)
-                for (int c = thread; c < BN; c += 128) bs[c] = p.bias[min(col0 + c, p.cols - 1)];
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+                for (int c = thread; c < BN; c += 32 * kOutWarps) bs[c] = p.bias[min(tile / tiles_m * BN + c, p.cols - 1)];
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kOutWarps) : "memory");
             alive = alive && bar_wait_all(shared_address(&bars.done[half]), i / Shape::kSums & 1);
             tmem_fence_after();
-#pragma unroll 1
-            for (int b = 0; b < BN / kCols; ++b) {
+            uint32_t words[kWords];                       // the row's outputs, two to a word for 16 bits
+            {
+                uint32_t r[kCols / 32][32];
 #pragma unroll
-                for (int part = 0; part < kCols / 32; ++part) {
-                    uint32_t r[32];
-                    tmem_load(tmem + half * BN + (quarter * 32 << 16) + b * kCols + part * 32, r);
-                    tmem_load_wait();
+                for (int b = 0; b < kCols / 32; ++b) tmem_load(tmem + half * BN + (quarter * 32 << 16) + half_col + b * 32, r[b]);
+                tmem_load_wait();
+                tmem_fence_before();
+                bar_arrive(shared_address(&bars.taken[half]));
 #pragma unroll
-                    for (int q = 0; q < 32 / kPer; ++q) {
-                        float f[kPer];
-                        const int c = b * kCols + part * 32 + q * kPer;
+                for (int b = 0; b < kCols; b += 4) {
+                    float f[4];
 #pragma unroll
-                        for (int j = 0; j < kPer; ++j) f[j] = __uint_as_float(r[q * kPer + j]);
-                        if (p.bias)
+                    for (int j = 0; j < 4; ++j) f[j] = alive ? __uint_as_float(r[b / 32][b % 32 + j]) : __int_as_float(0x7fffffff);
+                    if (p.bias) {
+                        const float4 d = *reinterpret_cast<const float4*>(bs + half_col + b);
+                        f[0] += d.x;
+                        f[1] += d.y;
+                        f[2] += d.z;
+                        f[3] += d.w;
+                    }
+                    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                            for (int j = 0; j < kPer; ++j) f[j] += bs[c + j];
-                        if (!alive)
-#pragma unroll
-                            for (int j = 0; j < kPer; ++j) f[j] = __int_as_float(0x7fffffff);
-                        Vec16<T> v;
-                        v.set(f);
-                        const int chunk = part * (32 / kPer) + q;
-                        *reinterpret_cast<uint4*>(stage + lane * 128 + ((chunk ^ (lane & (kPieces - 1))) << 4)) = v.raw;
+                        for (int j = 0; j < 4; ++j) words[b + j] = __float_as_uint(f[j]);
+                    } else {
+                        words[b / 2] = pack2<T>(f[0], f[1]);
+                        words[b / 2 + 1] = pack2<T>(f[2], f[3]);
                     }
                 }
-                __syncwarp();
-                const int col1 = col0 + b * kCols;
-                if (wide && col1 + kCols <= p.cols) {
-                    // kPieces lanes write a row's bytes
-#pragma unroll
-                    for (int k = 0; k < kPieces; ++k) {
-                        const int r = k * (32 / kPieces) + lane / kPieces, c = lane % kPieces;
-                        const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & (kPieces - 1))) << 4));
-                        if (row0 + r < p.rows) *reinterpret_cast<uint4*>(out + (row0 + r) * p.out_stride + col1 + c * kPer) = v;
-                    }
-                } else {
-                    // rows that do not start on 16 bytes, or end in this block: value by value, eight rows read before they are written
-                    T* to = out + row0 * p.out_stride + col1;
-                    for (int r0 = 0; r0 < 32; r0 += 8, to += 8 * p.out_stride)
-#pragma unroll
-                        for (int c0 = 0; c0 < kCols; c0 += 32) {
-                            const int c = c0 + lane, at = c * (int)sizeof(T);
-                            T x[8];
-#pragma unroll
-                            for (int r = 0; r < 8; ++r)
-                                x[r] = *reinterpret_cast<const T*>(stage + (r0 + r) * 128 + (((at >> 4) ^ (r & (kPieces - 1))) << 4) + (at & 15));
-                            if (col1 + c < p.cols)
-#pragma unroll
-                                for (int r = 0; r < 8; ++r)
-                                    if (row0 + r0 + r < p.rows) to[r * p.out_stride + c] = x[r];
-                        }
-                }
-                __syncwarp();
             }
-            tmem_fence_before();
-            bar_arrive(shared_address(&bars.taken[half]));
+            if (wide && col0 + kCols <= p.cols) {
+                // each lane its own row, whole sectors
+                if (row0 + lane < p.rows) {
+                    T* const to = out + (row0 + lane) * p.out_stride + col0;
+#pragma unroll
+                    for (int c = 0; c < kWords; c += 8)
+                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + c * 4 / (int)sizeof(T)), "r"(words[c]),
+                                     "r"(words[c + 1]), "r"(words[c + 2]), "r"(words[c + 3]), "r"(words[c + 4]), "r"(words[c + 5]), "r"(words[c + 6]),
+                                     "r"(words[c + 7])
+                                     : "memory");
+                }
+            } else {
+                // rows that do not start on 32 bytes, or end in this block: 64 bytes of them at a
+                // time, value by value, a row's side by side, eight rows read before they are written
+                constexpr int kSide = 64 / (int)sizeof(T);
+#pragma unroll
+                for (int c0 = 0; c0 < kCols; c0 += kSide) {
+                    __syncwarp();
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int w = c0 * (int)sizeof(T) / 4 + 4 * q;
+                        *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ (lane / 2 & 3)) << 4)) = make_uint4(words[w], words[w + 1], words[w + 2], words[w + 3]);
+                    }
+                    __syncwarp();
+                    const int c = lane % kSide, at = c * (int)sizeof(T), col = col0 + c0 + c;
+#pragma unroll
+                    for (int r0 = 0; r0 < kSide; r0 += 8) {
+                        T x[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const int row = (r0 + k) * (32 / kSide) + lane / kSide;
+                            x[k] = *reinterpret_cast<const T*>(stage + row * 64 + (((at >> 4) ^ (row / 2 & 3)) << 4) + (at & 15));
+                        }
+                        if (col < p.cols)
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                const long long row = row0 + (r0 + k) * (32 / kSide) + lane / kSide;
+                                if (row < p.rows) out[row * p.out_stride + col] = x[k];
+                            }
+                    }
+                }
+            }
         }
     }
     tmem_fence_before();
