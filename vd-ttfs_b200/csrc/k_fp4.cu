@@ -12,6 +12,8 @@
 // and scales from tensor memory, with 32-bit sums.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
 #include "step_internal.h"
 
 namespace vdt {
@@ -36,23 +38,120 @@ __device__ __forceinline__ float scale_of(uint32_t byte) {
 }
 
 // Eight values' codes, the first in the lowest bits
-__device__ __forceinline__ uint32_t codes_of(const float* f, float inverse) {
+__device__ __forceinline__ uint32_t codes_of(const float* f) {
     uint32_t w;
     asm("{\n\t.reg .b8 a, b, c, d;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
         "mov.b32 %0, {a, b, c, d};\n\t}"
         : "=r"(w)
-        : "f"(f[0] * inverse), "f"(f[1] * inverse), "f"(f[2] * inverse), "f"(f[3] * inverse), "f"(f[4] * inverse), "f"(f[5] * inverse),
-          "f"(f[6] * inverse), "f"(f[7] * inverse));
+        : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
     return w;
 }
-// the largest magnitude; infinity and NaN order above the others as bits
-__device__ __forceinline__ float largest(const float* f, int n) {
-    uint32_t m = 0;
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
+// A block of 32 values as they lie in memory -> its 16 bytes of codes; returns the
+// scale's byte.  One thread a block: no exchange, and the scale is made once.
+// bf16 values are scaled as they are (a power of two changes no bit but the
+// exponent's, and what falls below the smallest number has code 0 anyway).
+template <typename T>
+__device__ __forceinline__ uint32_t round_block(const uint32_t (&raw)[8 * sizeof(T)], uint4& codes) {
+    float most;
+    uint32_t w[4];
+    if constexpr (sizeof(T) == 4) {
+        most = fabsf(__uint_as_float(raw[0]));
 #pragma unroll
-    for (int j = 0; j < n; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
-    return __uint_as_float(m);
+        for (int i = 1; i < 32; ++i) most = max_or_nan(most, fabsf(__uint_as_float(raw[i])));
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        __nv_bfloat162 m, o;
+        memcpy(&m, &raw[0], 4);
+        m = __habs2(m);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) {
+            memcpy(&o, &raw[i], 4);
+            m = __hmax2_nan(m, __habs2(o));
+        }
+        most = max_or_nan(__low2float(m), __high2float(m));
+    } else {
+        __half2 m, o;
+        memcpy(&m, &raw[0], 4);
+        m = __habs2(m);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) {
+            memcpy(&o, &raw[i], 4);
+            m = __hmax2_nan(m, __habs2(o));
+        }
+        most = max_or_nan(__low2float(m), __high2float(m));
+    }
+    const uint32_t byte = scale_byte(fabsf(most));
+    const float inverse = inverse_of(byte);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float f[8];
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(raw[8 * q + j]) * inverse;
+        } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            const __nv_bfloat162 by = __float2bfloat162_rn(inverse);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                __nv_bfloat162 o;
+                memcpy(&o, &raw[4 * q + j], 4);
+                o = __hmul2(o, by);
+                uint32_t u;
+                memcpy(&u, &o, 4);
+                unpack2<T>(u, f[2 * j], f[2 * j + 1]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                unpack2<T>(raw[4 * q + j], f[2 * j], f[2 * j + 1]);
+                f[2 * j] *= inverse;
+                f[2 * j + 1] *= inverse;
+            }
+        }
+        w[q] = codes_of(f);
+    }
+    codes = byte == 255 ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]);
+    return byte;
+}
+// The block's values, those at or past `left` as zeros.  ALIGN: the bytes that it starts on a multiple of.
+template <typename T, int ALIGN>
+__device__ __forceinline__ void load_block(const T* from, int left, uint32_t (&raw)[8 * sizeof(T)]) {
+    constexpr int kWords = 8 * sizeof(T);
+    if (ALIGN == 32 && left >= 32) {
+#pragma unroll
+        for (int i = 0; i < kWords; i += 8)
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(raw[i]), "=r"(raw[i + 1]), "=r"(raw[i + 2]), "=r"(raw[i + 3]), "=r"(raw[i + 4]), "=r"(raw[i + 5]), "=r"(raw[i + 6]),
+                           "=r"(raw[i + 7])
+                         : "l"(reinterpret_cast<const uint32_t*>(from) + i));
+    } else if (ALIGN >= 16 && left >= 32) {
+#pragma unroll
+        for (int i = 0; i < kWords; i += 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(from) + i);
+            raw[i] = v.x;
+            raw[i + 1] = v.y;
+            raw[i + 2] = v.z;
+            raw[i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                raw[i] = i < left ? __float_as_uint(from[i]) : 0u;
+            } else {
+                uint16_t lo = 0, hi = 0;
+                if (2 * i < left) memcpy(&lo, from + 2 * i, 2);
+                if (2 * i + 1 < left) memcpy(&hi, from + 2 * i + 1, 2);
+                raw[i] = lo | (uint32_t)hi << 16;
+            }
+        }
+    }
 }
 
 // Where the scale of a row's block lies: tiles of 128 rows x 4 blocks, row r's
@@ -64,60 +163,41 @@ __device__ __forceinline__ long long scale_at(long long row, int block, long lon
 }
 
 // ------------------------------------------------------------------ quantise
-// Four lanes a block, eight values each.  A warp takes 256 columns of a row, the
-// scales' padding up to there included; what a row's last block lacks counts as
-// zeros.  Rows of few columns share a CTA, 2^across warps each.  Bound by memory:
-// 8192 x 4096 bf16 SEE us.
-constexpr int kPackWarps = 8;
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kPackWarps * 32) k_quantize_fp4(const T* __restrict__ x, long long rows, int cols, long long x_stride,
-                                                                  uint8_t* __restrict__ codes, long long codes_stride,
-                                                                  uint8_t* __restrict__ scale, int steps, int across) {
-    constexpr int N = Vec16<T>::N;
+// A thread a block.  2^across threads (8, 16 or 32) side by side take a row's
+// blocks, the scales' padding included, so rows of few columns share a warp.  Bound
+// by memory: 8192 x 4096 bf16 SEE us.
+constexpr int kPackThreads = 128;
+template <typename T, int ALIGN>
+__global__ void __launch_bounds__(kPackThreads) k_quantize_fp4(const T* __restrict__ x, long long rows, int cols, long long x_stride,
+                                                               uint8_t* __restrict__ codes, long long codes_stride, uint8_t* __restrict__ scale,
+                                                               int steps, int across) {
     chain_release();
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int step = (blockIdx.x << across) + (warp & ((1 << across) - 1)), per = kPackWarps >> across;
-    if (step >= steps) return;
-    const int col = step * kFp4Step + lane * 8;
-    const bool whole = WIDE && col + 8 <= cols;
-    for (long long row = (long long)blockIdx.y * per + (warp >> across); row < rows; row += (long long)gridDim.y * per) {
-        const T* const from = x + row * x_stride + col;
-        float f[8];
-        if (whole) {
-#pragma unroll
-            for (int j = 0; j < 8; j += N) {
-                Vec16<T> v;
-                v.raw = *reinterpret_cast<const uint4*>(from + j);
-                v.get(f + j);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = col + j < cols ? to_f32(from[j]) : 0.0f;
-        }
-        uint32_t m = __float_as_uint(largest(f, 8));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        uint32_t byte = scale_byte(__uint_as_float(m));
-        const uint32_t w = byte == 255 ? 0 : codes_of(f, inverse_of(byte));
-        if (col < cols) *reinterpret_cast<uint32_t*>(codes + row * codes_stride + col / 2) = w;
-        // four blocks' bytes from sixteen lanes
-        byte |= __shfl_down_sync(0xffffffffu, byte, 4) << 8;
-        byte |= __shfl_down_sync(0xffffffffu, byte, 8) << 16;
-        if (lane % 16 == 0) *reinterpret_cast<uint32_t*>(scale + scale_at(row, col / kBlock, steps)) = byte;
+    const int block = (blockIdx.x << across) + (threadIdx.x & ((1 << across) - 1)), per = kPackThreads >> across;
+    const int col = block * kBlock;
+    for (long long row = (long long)blockIdx.y * per + (threadIdx.x >> across); row - (threadIdx.x >> across) < rows; row += (long long)gridDim.y * per) {
+        const bool in = row < rows && block < steps * (kFp4Step / kBlock);
+        uint32_t raw[8 * sizeof(T)];
+        load_block<T, ALIGN>(x + row * x_stride + col, in ? cols - col : 0, raw);
+        uint4 w;
+        uint32_t byte = round_block<T>(raw, w);
+        // (the last row's storage reaches to the next 16 bytes)
+        if (in && col < cols) *reinterpret_cast<uint4*>(codes + row * codes_stride + col / 2) = w;
+        // four blocks' bytes together
+        byte |= __shfl_down_sync(0xffffffffu, byte, 1) << 8;
+        byte |= __shfl_down_sync(0xffffffffu, byte, 2) << 16;
+        if (in && block % 4 == 0) *reinterpret_cast<uint32_t*>(scale + scale_at(row, block, steps)) = byte;
     }
 }
 
 template <typename T>
 cudaError_t pack_launch(const void* x, long long rows, int cols, long long x_stride, uint8_t* codes, long long codes_stride, uint8_t* scale,
                         cudaStream_t s) {
-    const bool wide = aligned(x, 16) && (rows == 1 || x_stride * (long long)sizeof(T) % 16 == 0);
-    const int steps = (int)fp4_steps(cols);
-    int across = 0;
-    while (across < 3 && (1 << across) < steps) ++across;
-    const long long per = kPackWarps >> across, down = (rows + per - 1) / per;
-    const dim3 grid((unsigned)((steps + (1 << across) - 1) >> across), (unsigned)(down < 65535 ? down : 65535));
-    auto kern = wide ? k_quantize_fp4<T, true> : k_quantize_fp4<T, false>;
-    kern<<<grid, kPackWarps * 32, 0, s>>>(static_cast<const T*>(x), rows, cols, x_stride, codes, codes_stride, scale, steps, across);
+    auto on = [&](int bytes) { return aligned(x, bytes) && (rows == 1 || x_stride * (long long)sizeof(T) % bytes == 0); };
+    const int steps = (int)fp4_steps(cols), blocks = steps * (kFp4Step / kBlock), across = steps == 1 ? 3 : steps == 2 ? 4 : 5;
+    const long long per = kPackThreads >> across, down = (rows + per - 1) / per;
+    const dim3 grid((unsigned)((blocks + (1 << across) - 1) >> across), (unsigned)std::min(down, 65535LL));
+    auto kern = on(32) ? k_quantize_fp4<T, 32> : on(16) ? k_quantize_fp4<T, 16> : k_quantize_fp4<T, 1>;
+    kern<<<grid, kPackThreads, 0, s>>>(static_cast<const T*>(x), rows, cols, x_stride, codes, codes_stride, scale, steps, across);
     return cudaGetLastError();
 }
 
@@ -280,46 +360,38 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarp
         }
         if (alive && one) mma_commit(shared_address(&bars.done));
     } else if constexpr (kOwn) {
-        // four lanes a block, eight values each; a step's rows after another
-        constexpr int N = Vec16<X>::N, kThreads = 32 * kRoundWarps, kMost = NT * 32 / kThreads;
-        const int t = threadIdx.x - 64;
+        // a thread a block of a step, eight of them a row; the next step's values on their way meanwhile
+        constexpr int kThreads = 32 * kRoundWarps, kMost = (NT * 8 + kThreads - 1) / kThreads, kWords = 8 * sizeof(X);
+        const int t = threadIdx.x - 64, block = t % 8;
         const X* const x = static_cast<const X*>(p.x) + (long long)row0 * p.x_stride;
-        const bool wide = p.x_stride * (long long)sizeof(X) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+        const bool wide = p.x_stride * (long long)sizeof(X) % 32 == 0 && reinterpret_cast<uintptr_t>(x) % 32 == 0;
+        uint32_t raw[kMost][kWords];
+        auto load = [&](int s) {
+            const int col = s * kFp4Step + block * kBlock;
+#pragma unroll
+            for (int k = 0; k < kMost; ++k) {
+                const int row = (t + k * kThreads) / 8, left = row < rows ? p.inner - col : 0;
+                if (wide) load_block<X, 32>(x + (long long)row * p.x_stride + col, left, raw[k]);
+                else load_block<X, 1>(x + (long long)row * p.x_stride + col, left, raw[k]);
+            }
+        };
+        load(first);
         for (int s = first; s < last; ++s) {
             const int slot = (s - first) % kFewStages;
             unsigned char* const at = smem + slot * Shape::kStage;
-            float f[kMost][8];
-#pragma unroll
-            for (int k = 0; k < kMost; ++k) {
-                const int row = (t + k * kThreads) / 32, col = s * kFp4Step + t % 32 * 8;
-                const X* const from = x + (long long)row * p.x_stride + col;
-                if (row < rows && wide && col + 8 <= p.inner) {
-#pragma unroll
-                    for (int j = 0; j < 8; j += N) {
-                        Vec16<X> v;
-                        v.raw = *reinterpret_cast<const uint4*>(from + j);
-                        v.get(f[k] + j);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) f[k][j] = row < rows && col + j < p.inner ? to_f32(from[j]) : 0.0f;
-                }
-            }
             if (s - first >= kFewStages) {
                 if (!bar_wait_all(shared_address(&bars.empty[slot]), ((s - first) / kFewStages & 1) ^ 1)) break;
             }
 #pragma unroll
             for (int k = 0; k < kMost; ++k) {
-                const int row = (t + k * kThreads) / 32;             // a warp's lanes have one row
+                const int row = (t + k * kThreads) / 8;
                 if (row >= rows) break;
-                uint32_t m = __float_as_uint(largest(f[k], 8));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                const uint32_t byte = scale_byte(__uint_as_float(m)), w = byte == 255 ? 0 : codes_of(f[k], inverse_of(byte));
-                const int chunk = lane / 4;                          // of 16 bytes, swizzled by the row
-                *reinterpret_cast<uint32_t*>(at + (128 + row) * kStepBytes + ((chunk ^ (row & 7)) << 4) + lane % 4 * 4) = w;
-                if (lane % 4 == 0) at[Shape::kCodes + kStepScales + chunk / 4 * kScaleTile + row % 32 * 16 + row / 32 * 4 + chunk % 4] = (unsigned char)byte;
+                uint4 w;
+                const uint32_t byte = round_block<X>(raw[k], w);
+                *reinterpret_cast<uint4*>(at + (128 + row) * kStepBytes + ((block ^ (row & 7)) << 4)) = w;      // swizzled by the row
+                at[Shape::kCodes + kStepScales + block / 4 * kScaleTile + row % 32 * 16 + row / 32 * 4 + block % 4] = (unsigned char)byte;
             }
+            if (s + 1 < last) load(s + 1);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tensor cores read what these lanes wrote
             __syncwarp();
             if (lane == 0) bar_arrive(shared_address(&bars.full[slot]));
