@@ -165,7 +165,8 @@ __device__ __forceinline__ long long scale_at(long long row, int block, long lon
 // ------------------------------------------------------------------ quantise
 // A thread a block.  2^across threads (8, 16 or 32) side by side take a row's
 // blocks, the scales' padding included, so rows of few columns share a warp.  Bound
-// by memory: 8192 x 4096 bf16 SEE us.
+// by memory: 8192 x 4096 bf16 14.7 us, 5.8 TB/s (four lanes a block, which exchange
+// their maxima, took 26 us and four times the instructions).
 constexpr int kPackThreads = 128;
 template <typename T, int ALIGN>
 __global__ void __launch_bounds__(kPackThreads) k_quantize_fp4(const T* __restrict__ x, long long rows, int cols, long long x_stride,
@@ -177,7 +178,26 @@ __global__ void __launch_bounds__(kPackThreads) k_quantize_fp4(const T* __restri
     for (long long row = (long long)blockIdx.y * per + (threadIdx.x >> across); row - (threadIdx.x >> across) < rows; row += (long long)gridDim.y * per) {
         const bool in = row < rows && block < steps * (kFp4Step / kBlock);
         uint32_t raw[8 * sizeof(T)];
-        load_block<T, ALIGN>(x + row * x_stride + col, in ? cols - col : 0, raw);
+        if constexpr (ALIGN >= 16) {
+            load_block<T, ALIGN>(x + row * x_stride + col, in ? cols - col : 0, raw);
+        } else {
+            // a block's 32 values by the warp's lanes, then each lane its block; rows of 33 words (f32) or 17
+            constexpr int kPitch = sizeof(T) == 4 ? 33 : 34;
+            __shared__ T side[kPackThreads / 32][32 * kPitch];
+            T* const mine = side[threadIdx.x / 32];
+            const int lane = threadIdx.x % 32, mask = (1 << across) - 1;
+            __syncwarp();
+#pragma unroll 8
+            for (int i = 0; i < 32; ++i) {
+                const int from = (threadIdx.x & ~31) + i;             // the thread whose block it is
+                const long long r = row + (from >> across) - (threadIdx.x >> across);
+                const int c = ((blockIdx.x << across) + (from & mask)) * kBlock + lane;
+                mine[i * kPitch + lane] = r < rows && c < cols ? x[r * x_stride + c] : from_f32<T>(0.0f);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < (int)(8 * sizeof(T)); ++i) memcpy(&raw[i], mine + lane * kPitch + i * (4 / (int)sizeof(T)), 4);
+        }
         uint4 w;
         uint32_t byte = round_block<T>(raw, w);
         // (the last row's storage reaches to the next 16 bytes)
@@ -256,17 +276,27 @@ constexpr int kStepScales = 2 * kScaleTile;          // a stage's scales for 128
 // that all SMs load at once and every CTA's stages are on their way from the
 // start; the sums meet in shared memory.  X: the type of rows that are still to be
 // rounded, which eight warps do for their CTA's part of the inner dimension while
-// the weights come; void: they are codes.  24 x 4096 x 8192 f16: SEE us.
+// the weights come; void: they are codes.  24 x 4096 x 8192 f16:
+// 9.2 us (17.8 MB of weights, from L2 where they fit; without the rounding 6.7).
 constexpr int kFewStages = 4, kRoundWarps = 8;
-constexpr int kFewRows = 64, kOwnRows = 64;
+
+// Up to kOwnRows the kernel rounds the rows itself.  A call / on the GPU in us, so and
+// with two launches, f16: 1 x 4096 x 8192 9.6 / 7.5 and 12.5 / 8.0, 16 x 1024 x 1024
+// 7.0 / 4.6 and 9.8 / 6.2, 32 x 4096 x 8192 11.3 / 9.2 and 14.1 / 8.7, 32 x 8192 x 1024
+// 8.8 / 6.7 and 12.0 / 7.5; not taken: 64 x 4096 x 8192 15.6 / 13.5 and 14.3 / 11.8.
+// Up to kFewRows the tokens may be the columns; above kOwnRows where sharing the
+// inner dimension takes more than kFewSteps steps off each CTA (us, so and with the
+// tiles below): 64 x 4096 x 4096 6.7 and 8.0, 64 x 8192 x 1024 6.3 and 12.4, 64 x
+// 4096 x 8192 8.2 and 7.9, not taken: 64 x 1024 x 1024 5.3 and 4.5.
+constexpr int kFewRows = 64, kOwnRows = 32, kFewSteps = 6;
 
 template <int NT>
 struct FewShape {
     static constexpr int kCodes = (128 + NT) * kStepBytes;
     static constexpr int kStage = kCodes + 2 * kStepScales;
-    static constexpr int kBytes = 1024 + kFewStages * kStage;
+    static constexpr int kBytes = 1024 + kFewStages * kStage + NT * 512;
     static constexpr int kScalesAt = 64, kScaleCols = 16, kCols = 128;     // tensor memory: sums, then 16 columns of scales a stage
-    static_assert(NT <= kScalesAt && kScalesAt + kFewStages * kScaleCols <= kCols && NT * 512 <= kFewStages * kStage, "tile");
+    static_assert(NT <= kScalesAt && kScalesAt + kFewStages * kScaleCols <= kCols, "tile");
 };
 struct FewBars {
     uint64_t full[kFewStages], empty[kFewStages], done;
@@ -291,7 +321,7 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarp
     if (threadIdx.x == 0) {
         map_ahead(&map_w);
         for (int i = 0; i < kFewStages; ++i) {
-            bar_init(shared_address(&bars.full[i]), kOwn ? 1 + kRoundWarps : 1);
+            bar_init(shared_address(&bars.full[i]), kOwn ? 1 + NT / 4 : 1);
             bar_init(shared_address(&bars.empty[i]), 1);
         }
         bar_init(shared_address(&bars.done), 1);
@@ -360,38 +390,35 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarp
         }
         if (alive && one) mma_commit(shared_address(&bars.done));
     } else if constexpr (kOwn) {
-        // a thread a block of a step, eight of them a row; the next step's values on their way meanwhile
-        constexpr int kThreads = 32 * kRoundWarps, kMost = (NT * 8 + kThreads - 1) / kThreads, kWords = 8 * sizeof(X);
-        const int t = threadIdx.x - 64, block = t % 8;
-        const X* const x = static_cast<const X*>(p.x) + (long long)row0 * p.x_stride;
-        const bool wide = p.x_stride * (long long)sizeof(X) % 32 == 0 && reinterpret_cast<uintptr_t>(x) % 32 == 0;
-        uint32_t raw[kMost][kWords];
+        // A thread a block of a step, eight of them a row; the next step's values on their
+        // way meanwhile.  What a step leaves over of the threads takes the next one, so that
+        // the steps' loads do not wait for each other.
+        constexpr int kGroup = NT * 8, kGroups = 32 * kRoundWarps / kGroup;
+        static_assert(kGroups >= 1, "a thread a block");
+        const int t = (threadIdx.x - 64) % kGroup, block = t % 8, row = t / 8;
+        const X* const x = static_cast<const X*>(p.x) + (long long)(row0 + row) * p.x_stride + block * kBlock;
+        const bool wide = p.x_stride * (long long)sizeof(X) % 32 == 0 && reinterpret_cast<uintptr_t>(p.x) % 32 == 0;
+        uint32_t raw[8 * sizeof(X)];
         auto load = [&](int s) {
-            const int col = s * kFp4Step + block * kBlock;
-#pragma unroll
-            for (int k = 0; k < kMost; ++k) {
-                const int row = (t + k * kThreads) / 8, left = row < rows ? p.inner - col : 0;
-                if (wide) load_block<X, 32>(x + (long long)row * p.x_stride + col, left, raw[k]);
-                else load_block<X, 1>(x + (long long)row * p.x_stride + col, left, raw[k]);
-            }
+            const int col = s * kFp4Step, left = row < rows && s < last ? p.inner - col - block * kBlock : 0;
+            if (wide) load_block<X, 32>(x + col, left, raw);
+            else load_block<X, 1>(x + col, left, raw);
         };
-        load(first);
-        for (int s = first; s < last; ++s) {
+        int s = first + (threadIdx.x - 64) / kGroup;
+        load(s);
+        for (; s < last; s += kGroups) {
             const int slot = (s - first) % kFewStages;
             unsigned char* const at = smem + slot * Shape::kStage;
+            uint4 w;
+            const uint32_t byte = round_block<X>(raw, w);
+            load(s + kGroups);
             if (s - first >= kFewStages) {
                 if (!bar_wait_all(shared_address(&bars.empty[slot]), ((s - first) / kFewStages & 1) ^ 1)) break;
             }
-#pragma unroll
-            for (int k = 0; k < kMost; ++k) {
-                const int row = (t + k * kThreads) / 8;
-                if (row >= rows) break;
-                uint4 w;
-                const uint32_t byte = round_block<X>(raw[k], w);
+            if (row < rows) {
                 *reinterpret_cast<uint4*>(at + (128 + row) * kStepBytes + ((block ^ (row & 7)) << 4)) = w;      // swizzled by the row
                 at[Shape::kCodes + kStepScales + block / 4 * kScaleTile + row % 32 * 16 + row / 32 * 4 + block % 4] = (unsigned char)byte;
             }
-            if (s + 1 < last) load(s + 1);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tensor cores read what these lanes wrote
             __syncwarp();
             if (lane == 0) bar_arrive(shared_address(&bars.full[slot]));
@@ -400,9 +427,8 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarp
 
     // the sums: channel 32 (warp % 4) + lane, tokens side by side
     const int quarter = warp % 4;
-    float* const part = reinterpret_cast<float*>(smem);              // [NT][128], over stages that are through
-    const bool reads = warp >= 2 && warp < 6;
-    if (reads) {
+    float* const part = reinterpret_cast<float*>(smem + kFewStages * Shape::kStage);      // [NT][128]
+    if (warp >= 2 && warp < 6) {
         alive = bar_wait_all(shared_address(&bars.done), 0);
         tmem_fence_after();
 #pragma unroll
@@ -424,30 +450,54 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarp
         tmem_fence_after();
         tmem_free(tmem, Shape::kCols);
     }
-    // each CTA adds up its share of the tokens
+    // each CTA adds up its share of the tokens, four channels a thread
     const int from = rows * rank / split, to = rows * (rank + 1) / split;
-    for (int i = threadIdx.x; i < (to - from) * 128; i += blockDim.x) {
-        const int row = from + i / 128, col = tile * 128 + i % 128;
-        float y = 0.0f;
-        if (split == 1) {
-            y = part[row * 128 + i % 128];
-        } else {
-            float o[8];
+    const bool wide = p.out_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+    for (int i = threadIdx.x; i < (to - from) * 32; i += blockDim.x) {
+        const int row = from + i / 32, c = i % 32 * 4, col = tile * 128 + c;
+        float4 o[8];
 #pragma unroll
-            for (int r = 0; r < 8; ++r) o[r] = r < split ? cluster.map_shared_rank(part, r)[row * 128 + i % 128] : 0.0f;
+        for (int r = 0; r < 8; ++r)
+            if (r < split) o[r] = *reinterpret_cast<const float4*>((split > 1 ? cluster.map_shared_rank(part, r) : part) + row * 128 + c);
+        float y[4] = {o[0].x, o[0].y, o[0].z, o[0].w};
 #pragma unroll
-            for (int r = 0; r < 8; ++r) y += o[r];
-        }
-        if (col >= p.cols) continue;
-        if (p.bias) y += p.bias[col];
+        for (int r = 1; r < 8; ++r)
+            if (r < split) {
+                y[0] += o[r].x;
+                y[1] += o[r].y;
+                y[2] += o[r].z;
+                y[3] += o[r].w;
+            }
+        if (p.bias)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < p.cols) y[j] += p.bias[col + j];
         const long long at = (long long)(row0 + row) * p.out_stride + col;
-        if (p.out_type == VDT_F32) static_cast<float*>(p.out)[at] = y;
-        else if (p.out_type == VDT_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(y);
-        else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+        auto put = [&](auto* out) {
+            using T = std::remove_pointer_t<decltype(out)>;
+            if (wide && col + 4 <= p.cols) {
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out + at) = make_float4(y[0], y[1], y[2], y[3]);
+                else *reinterpret_cast<uint2*>(out + at) = make_uint2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (col + j < p.cols) out[at + j] = from_f32<T>(y[j]);
+            }
+        };
+        if (p.out_type == VDT_F32) put(static_cast<float*>(p.out));
+        else if (p.out_type == VDT_F16) put(static_cast<__half*>(p.out));
+        else put(static_cast<__nv_bfloat16*>(p.out));
     }
     if (split > 1) cluster.sync();                                   // until the others have read this CTA's part
 }
 
+// CTAs a tile: as many as the SMs hold at a time (two each, or one with 64 tokens), each with a step at least
+int few_split(int cols, int inner, int tokens) {
+    const long long tiles = (cols + 127) / 128, steps = fp4_steps(inner);
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= (tokens == 64 ? 1 : 2) * kSmCount && steps >= split * 2) split *= 2;
+    return split;
+}
 template <typename X, int NT>
 cudaError_t few_launch(const Fp4Params& p, bool after, cudaStream_t s) {
     using Shape = FewShape<NT>;
@@ -461,10 +511,7 @@ cudaError_t few_launch(const Fp4Params& p, bool after, cudaStream_t s) {
     }
     const cudaError_t e = allow_shared<k_fp4_few<X, NT>>(Shape::kBytes);
     if (e != cudaSuccess) return e;
-    // as many CTAs a tile as put two on every SM, each with a step at least
-    const long long tiles = (long long)((p.cols + 127) / 128) * ((p.rows + NT - 1) / NT), steps = fp4_steps(p.inner);
-    int split = 1;
-    while (split < 8 && tiles * split * 2 <= 2 * kSmCount && steps >= split * 2) split *= 2;
+    const int split = few_split(p.cols, p.inner, NT);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((p.cols + 127) / 128 * split), (unsigned)((p.rows + NT - 1) / NT));
     cfg.blockDim = dim3(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarps);
@@ -483,8 +530,10 @@ cudaError_t few_launch(const Fp4Params& p, bool after, cudaStream_t s) {
 template <typename X>
 cudaError_t few_by_rows(const Fp4Params& p, bool after, cudaStream_t s) {
     if (p.rows <= 16) return few_launch<X, 16>(p, after, s);
-    if (p.rows <= 32) return few_launch<X, 32>(p, after, s);
-    return few_launch<X, 64>(p, after, s);
+    if constexpr (std::is_void_v<X>) {
+        if (p.rows > 32) return few_launch<X, 64>(p, after, s);
+    }
+    return few_launch<X, 32>(p, after, s);
 }
 
 // ---------------------------------------------------------------- many rows
@@ -497,7 +546,9 @@ cudaError_t few_by_rows(const Fp4Params& p, bool after, cudaStream_t s) {
 // warps take all of a tile's sums into registers at once (128 a thread) and the
 // next tile's products start before the first output is written.  What bounds it
 // is the way of the stages from L2, some 19 TB/s; tiles of 192 channels, whose sums fit
-// twice, read a sixth more of them.  8192 x 4096 x 8192: SEE us.
+// twice, read a sixth more of them.  8192 x 4096 x 8192:
+// 103 us, 5.3 PFLOP/s (113 with 192 channels; 79 without the weights' loads, 88 without
+// the outputs' stores).
 constexpr int kTileRows = 128, kOutWarps = 8, kTileThreads = 64 + 32 * kOutWarps;
 
 template <int BN>
@@ -796,7 +847,8 @@ cudaError_t launch_fp4_own(const Fp4Params& p, int type, cudaStream_t s) {
 }
 
 cudaError_t launch_fp4_matmul(const Fp4Params& p, bool after_codes, cudaStream_t s) {
-    if (p.rows <= kFewRows) return few_by_rows<void>(p, after_codes, s);
+    const long long steps = fp4_steps(p.inner), split = few_split(p.cols, p.inner, 64);
+    if (p.rows <= kOwnRows || (p.rows <= kFewRows && steps - steps / split > kFewSteps)) return few_by_rows<void>(p, after_codes, s);
     if (p.out_type == VDT_F32) return tiles_by_width<float>(p, after_codes, s);
     if (p.out_type == VDT_F16) return tiles_by_width<__half>(p, after_codes, s);
     return tiles_by_width<__nv_bfloat16>(p, after_codes, s);
