@@ -551,6 +551,20 @@ def test_sample_rows_that_give_no_token(S):
     check_sample(S, x, u, 1.0, 0, 0.9, p)
 
 
+def test_sample_of_several_ctas_a_row_again_and_again(S):
+    """Rows that clusters of CTAs share, with parameters that send them different ways: the same tokens every time."""
+    g = torch.Generator().manual_seed(8)
+    rows, vocab = 64, 40000
+    pick = lambda *v: torch.tensor(v)[torch.randint(0, len(v), (rows,), generator=g)].cuda()  # noqa: E731
+    x = (torch.randn(rows, vocab, generator=g) * 3).to(torch.bfloat16).cuda()
+    args = (uniform(3, rows).cuda(), pick(0.0, 0.6, 1.0, 1.3), pick(0, 20, 1000, 3000).int(), pick(0.8, 0.95, 1.0), pick(0.0, 0.02))
+    first = S.sample(x, *args)
+    check_sample(S, x, *args)
+    for _ in range(200):
+        tokens, logp = S.sample(x, *args)
+        assert torch.equal(tokens, first[0]) and torch.equal(logp, first[1])
+
+
 def test_sample_of_strided_rows(S):
     x = normal(6, 20, 4111, kind=torch.bfloat16).cuda()
     u = uniform(6, 20)

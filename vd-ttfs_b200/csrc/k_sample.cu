@@ -469,8 +469,7 @@ struct Row {
         u64 all[3];
         block_scan(sh, count, weight, square, all);
         if (threadIdx.x == 0) {
-            sh.found[0] = kBins;
-            sh.found[1] = kBins - 1;
+            sh.found[0] = sh.found[1] = kBins;
         }
         const auto& slots = say(all);
         float squares = 0.0f;
@@ -484,8 +483,7 @@ struct Row {
             total += slots[r][1];
             squares += __uint_as_float((uint32_t)slots[r][2]);
         }
-        if (threadIdx.x == 0) sh.found[3] = tokens;
-        __syncthreads();
+        // (from here on the other CTAs may write to `found`)
         // the first step up to which there may be enough, and the first up to which there is
         // (the last, where that is nearly all); 2^(1/44), and room for the 32-bit depths and sums
         const float whole = (float)total, share = fmaxf(top_p, 0.0f) * whole, wide = 1.0159f * 1.0002f;
@@ -516,7 +514,8 @@ struct Row {
             weight += w[i];
         }
         together();
-        const Steps found{(int)sh.found[0], (int)sh.found[1], sh.found[2], sh.found[3]};
+        const bool open = sh.found[1] == kBins;               // no step reaches so far: all of them
+        const Steps found{(int)sh.found[0], open ? kBins - 1 : (int)sh.found[1], sh.found[2], open ? tokens : sh.found[3]};
         __syncthreads();
         return found;
     }
