@@ -631,8 +631,8 @@ int vdt_free_pages(int32_t* d_ring, int ring, const int32_t* d_span, const int32
    whole sum.  Temperature 0 takes the lowest index of the largest value.
    d_temperature, d_top_p, d_min_p, d_top_k [rows] give each row its own, NULL takes
    the number beside.  d_logp (may be NULL): the logarithm of the probability
-   that the token was drawn with.  Weights are whole multiples of 2^-45 (2^-62
-   times the vocabulary's size, above 2^17) and their sums exact, so calls on the
+   that the token was drawn with.  Weights are whole multiples of 2^-44 of the
+   largest (2^-43 for vocabularies above 2^18) and their sums exact, so calls on the
    same inputs give the same tokens.  A row with a NaN, without a finite logit or +inf, or
    with a parameter or u that is NaN or out of range gives token -1 and NaN.
    vocab up to 524288. */

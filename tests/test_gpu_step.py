@@ -580,3 +580,153 @@ def test_sample_frequencies(S):
     tokens, _ = S.sample(x, ((torch.arange(n) + 0.5) / n).cuda(), top_k=4)
     p = torch.softmax(torch.tensor([1.0, -INF, 2.0, -INF, 0.5, 3.0]).double(), 0)
     assert ((torch.bincount(tokens.long(), minlength=6).cpu() - p * n).abs() <= 1.0).all()
+
+
+# --------------------------------------------------- streams, graphs, places --
+def step_calls(S):
+    """One call of each operator, on inputs of its own: name -> (call(stream), results)."""
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(40, 300, generator=g).to(torch.bfloat16).cuda()
+    w, ws = S.quantize_fp4(torch.randn(200, 300, generator=g).cuda())
+    c, cs = S.quantize_fp4(x)
+    few, weight = x[:3].clone(), torch.ones(300, dtype=torch.bfloat16, device="cuda")
+    logits, u = (torch.randn(9, 30000, generator=g) * 3).cuda(), torch.rand(9, generator=g).cuda()
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    pool, pages, held, new = S.PagePool.full(50), torch.full((3, 9), -1, dtype=torch.int32, device="cuda"), ints(0, 0, 0), ints(5, 100, 33)
+    done = torch.tensor([True, False, True]).cuda()
+    S.plan_pages(pool, pages, held, new, 16, 140)
+    return {
+        "quantize_fp4": lambda st: S.quantize_fp4(x, stream=st), "fp4_values": lambda st: (S.fp4_values(c, cs, stream=st),),
+        "fp4_matmul": lambda st: (S.fp4_matmul(c, cs, w, ws, stream=st),), "fp4_linear": lambda st: (S.fp4_linear(x, w, ws, stream=st),),
+        "fp4_linear few": lambda st: (S.fp4_linear(few, w, ws, stream=st),), "add_rms_norm": lambda st: S.add_rms_norm(x, x, weight, stream=st),
+        "add_rms_norm_int8": lambda st: S.add_rms_norm_int8(x, x, weight, stream=st),
+        "plan_pages": lambda st: tuple(S.plan_pages(pool, pages, held, new, 16, 140, stream=st)),
+        "free_pages": lambda st: S.free_pages((pool.ring.clone(), pool.span), pages, new, done, 16, stream=st),
+        "sample": lambda st: S.sample(logits, u, 0.8, 0, 0.9, stream=st), "sample k": lambda st: S.sample(logits, u, 0.8, 2000, 0.9, stream=st),
+    }
+
+
+# rows past the packed codes of quantised rows, and the padding rows of scale tiles, hold anything
+def same(name, a, b):
+    if name == "quantize_fp4":
+        return all(torch.equal(p[:, :9] if i else p, q[:, :9] if i else q) for i, (p, q) in enumerate(zip(unpacked(*a, 300), unpacked(*b, 300))))
+    return all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_calls_on_a_stream_of_the_callers_own(S):
+    side = torch.cuda.Stream()
+    for name, call in step_calls(S).items():
+        want = call(None)
+        torch.cuda.synchronize()
+        got = call(side.cuda_stream)
+        side.synchronize()
+        assert same(name, got, want), name
+        assert torch.cuda.current_stream() == torch.cuda.default_stream()
+
+
+def test_two_calls_at_once(S):
+    """The same calls on two streams, many times over: nothing is shared between calls."""
+    calls = step_calls(S)
+    want = {name: call(None) for name, call in calls.items()}
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    for name, call in calls.items():
+        if name == "plan_pages":
+            continue                                         # its table is one
+        got = []
+        for _ in range(20):
+            for s in sides:
+                with torch.cuda.stream(s):
+                    got.append(call(None))
+        torch.cuda.synchronize()
+        assert all(same(name, g, want[name]) for g in got), name
+
+
+def test_calls_in_a_graph(S):
+    calls = step_calls(S)
+    want = {name: call(None) for name, call in calls.items()}
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = {name: call(None) for name, call in calls.items()}
+        graphs.append((g, got))
+    for _ in range(3):
+        for g, _ in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for _, got in graphs:
+        for name in calls:
+            assert same(name, got[name], want[name]), name
+
+
+def test_a_step_in_place_in_a_graph(S):
+    """Lengths and the pool's state advance with every replay."""
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    pool, pages, held, new = S.PagePool.full(40), torch.full((3, 9), -1, dtype=torch.int32, device="cuda"), ints(3, 15, 16), ints(1, 1, 1)
+    S.plan_pages(pool, pages, ints(0, 0, 0), held, 16, 34, S.PagePlan(None, None, None, None, pool.span))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        plan = S.plan_pages(pool, pages, held, new, 16, 3, S.PagePlan(held, None, None, None, pool.span))
+    state = (pool.ring.tolist(), tuple(pool.span.tolist()), pages.tolist(), held.tolist())
+    for _ in range(40):
+        g.replay()
+        want = plan_definition(*state[:2], state[2], state[3], [1, 1, 1], 16, 3)
+        assert [t.tolist() for t in plan] == list(want[:5]) and pages.tolist() == want[5] and held.tolist() == want[0]
+        state = (pool.ring.tolist(), tuple(pool.span.tolist()), pages.tolist(), held.tolist())
+
+
+def test_results_of_a_stream_go_on_on_the_current_one(S):
+    """A result that is dropped while the current stream still reads it is not given out again before that is done."""
+    side = torch.cuda.Stream()
+    x = normal(1, 512, 2048, kind=torch.bfloat16).cuda()
+    want, _ = S.add_rms_norm(x)
+    for _ in range(20):
+        y, _ = S.add_rms_norm(x, stream=side.cuda_stream)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda._sleep(200000)
+        z = y.clone()
+        del y
+        S.add_rms_norm(-x, stream=side.cuda_stream)
+        assert torch.equal(z, want)
+
+
+def test_tensors_that_do_not_fit_are_refused(S):
+    x = normal(1, 4, 64, kind=torch.bfloat16).cuda()
+    w, ws = S.quantize_fp4(normal(2, 10, 64).cuda())
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    pool, pages, u = S.PagePool.full(4), torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.rand(4, device="cuda")
+    held = ints(1, 2)
+    for bad in (lambda: S.quantize_fp4(x.cpu()), lambda: S.quantize_fp4(x[0]), lambda: S.quantize_fp4(x.long()), lambda: S.fp4_linear(x[:, :60], w, ws),
+                lambda: S.fp4_linear(x, w[:5], ws[:, :1]), lambda: S.fp4_linear(x, w, ws.flatten()[:512]), lambda: S.fp4_linear(x, w.view(torch.int8), ws),
+                lambda: S.fp4_linear(x, w, ws, x[0]), lambda: S.fp4_linear(x, w, ws, out=x), lambda: S.fp4_matmul(x, ws, w, ws),
+                lambda: S.fp4_linear(x, w[:, 1:], ws), lambda: S.fp4_values(w, ws, 40), lambda: S.add_rms_norm(x, x[:3]), lambda: S.add_rms_norm(x, x.float()),
+                lambda: S.add_rms_norm(x, None, x[0].float()), lambda: S.add_rms_norm(x, sum_out=x), lambda: S.add_rms_norm(x, x, out=x[:, ::2]),
+                lambda: S.add_rms_norm_int8(x, None, x[0, :5]), lambda: S.plan_pages(pool, pages.long(), held, held, 16, 2),
+                lambda: S.plan_pages(pool, pages, held[:1], held, 16, 2), lambda: S.plan_pages(pool, pages, held, held, 0, 2),
+                lambda: S.plan_pages(pool, pages, held, held, 16, -1), lambda: S.plan_pages(pool, pages, held, held, 16, 2, S.PagePlan(held[:1], *[None] * 4)),
+                lambda: S.free_pages(pool, pages, held, held, 16), lambda: S.free_pages((pool.ring.view(2, 2), pool.span), pages, held, held.bool(), 16),
+                lambda: S.sample(x, u[:3]), lambda: S.sample(x, u.double()), lambda: S.sample(x, u, u[:2]), lambda: S.sample(x, u, 1.0, u),
+                lambda: S.sample(x.int(), u), lambda: S.sample(x[:, :0], u)):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: S.quantize_fp4(3), lambda: S.plan_pages(pool.ring, pages, held, held, 16, 2), lambda: S.sample(x, u, "a"), lambda: S.sample(x, u, 1.0, 0.5),
+                lambda: S.add_rms_norm(x, eps="b")):
+        with pytest.raises(TypeError):
+            bad()
+    from vdttfs._lib import VdtError
+    for bad in (lambda: S.sample(x, u, -1.0), lambda: S.sample(x, u, math.nan), lambda: S.add_rms_norm(x, eps=-1.0),
+                lambda: S.sample(torch.zeros(1, 524289, device="cuda"), u[:1])):
+        with pytest.raises(VdtError):
+            bad()
+
+
+def test_calls_of_nothing(S):
+    x = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")
+    w, ws = S.quantize_fp4(normal(2, 10, 64).cuda())
+    codes, scale = S.quantize_fp4(x)
+    assert codes.shape == (0, 32) and S.fp4_values(codes, scale).shape == (0, 64) and S.fp4_linear(x, w, ws).shape == (0, 10)
+    assert S.fp4_matmul(codes, scale, w, ws).shape == (0, 10)
+    assert [t.shape[0] for t in S.add_rms_norm(x, x)] == [0, 0] and [t.shape[0] for t in S.add_rms_norm_int8(x, x)] == [0, 0, 0]
+    assert [t.shape[0] for t in S.sample(x, torch.empty(0, device="cuda"))] == [0, 0]

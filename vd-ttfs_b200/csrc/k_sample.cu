@@ -123,6 +123,11 @@ struct Weigher {
         const double span = (double)top - (double)bottom;
         if (span * octaves > 900.0) octaves = 80.0 / span;
     }
+    // the logarithm of a token's probability, from the kept weights' sum (1 for the largest)
+    __device__ __forceinline__ double log_sum(u64 sum) const { return log((double)sum * __hiloint2double((1023 - bits) << 20, 0)); }
+    __device__ __forceinline__ float log_share(float x, double log_sum) const {
+        return (float)(((double)fmaxf(x * factor, bottom) - (double)top) * octaves * 0.6931471805599453 - log_sum);
+    }
     // steps below the largest
     __device__ __forceinline__ float depth(float x) const { return fmaf(-part, x, part_top) * steps; }
     // the step itself, kBins for all without weight: floor in the low bits of 2^23 + depth
@@ -166,6 +171,7 @@ struct Shared {
     u64 found[4];
     u64 kept[kWarps];                        // weight of what each warp's part keeps
     u64 last;
+    double log_sum;
     unsigned listed, chosen[kWarps];
 };
 
@@ -459,15 +465,26 @@ struct Row {
             }
         }
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const float each = exp2f((float)kBoundBits - (from + i + 0.5f) / kSteps);
-            w[i] = c[i] * (u64)each;
-            count += c[i];
-            weight += w[i];
-            square += (float)w[i] * (float)w[i];
+        for (int i = 0; i < kPer; ++i) count += c[i];
+        if (k < 0) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const float each = exp2f((float)kBoundBits - (from + i + 0.5f) / kSteps);
+                w[i] = c[i] * (u64)each;
+                weight += w[i];
+                square += (float)w[i] * (float)w[i];
+            }
         }
         u64 all[3];
-        block_scan(sh, count, weight, square, all);
+        if (k < 0) {
+            block_scan(sh, count, weight, square, all);
+        } else {
+            u64 v[1] = {count}, sum[1];
+            block_scan(sh, v, sum);
+            count = (uint32_t)v[0];
+            all[0] = sum[0];
+            all[1] = all[2] = 0;
+        }
         if (threadIdx.x == 0) {
             sh.found[0] = sh.found[1] = kBins;
         }
@@ -486,14 +503,18 @@ struct Row {
         // (from here on the other CTAs may write to `found`)
         // the first step up to which there may be enough, and the first up to which there is
         // (the last, where that is nearly all); 2^(1/44), and room for the 32-bit depths and sums
-        const float whole = (float)total, share = fmaxf(top_p, 0.0f) * whole, wide = 1.0159f * 1.0002f;
-        float lower = share / wide, upper = share * wide;
-        if (!sure) {
-            const float off = 4.0f * 0.0046f * sqrtf(squares) + 1e-5f * whole;
-            lower = fmaxf(lower, share - off);
-            upper = fminf(upper, share + off);
+        u64 least = 0, most = 0;
+        if (k < 0) {
+            const float whole = (float)total, share = fmaxf(top_p, 0.0f) * whole, wide = 1.0159f * 1.0002f;
+            float lower = share / wide, upper = share * wide;
+            if (!sure) {
+                const float off = 4.0f * 0.0046f * sqrtf(squares) + 1e-5f * whole;
+                lower = fmaxf(lower, share - off);
+                upper = fminf(upper, share + off);
+            }
+            least = max((u64)fmaxf(lower, 0.0f), 1ull);
+            most = upper > whole * 0.9999f ? ~0ull : max((u64)upper, 1ull);
         }
-        const u64 least = max((u64)fmaxf(lower, 0.0f), 1ull), most = upper > whole * 0.9999f ? ~0ull : max((u64)upper, 1ull);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const bool here = k >= 0 ? count < (uint32_t)k && (uint32_t)k <= count + c[i] : weight < least && least <= weight + w[i];
@@ -700,7 +721,11 @@ __device__ __forceinline__ void sort_list(u64* a, unsigned n) {
         unsigned at = 0;
         if (t < n) {
             mine = a[t];
-            for (unsigned i = 0; i < n; ++i) at += a[i] < mine || (a[i] == mine && i < t);
+#pragma unroll 8
+            for (unsigned i = 0; i < n; ++i) {
+                const u64 o = a[i];
+                at += o < mine || (o == mine && i < t);
+            }
         }
         __syncthreads();
         if (t < n) a[at] = mine;
@@ -914,6 +939,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
             all[0] = kept[0] + kept[1];
             block_sum(sh, all);
             const u64 target = share_of(share, all[0], &whole);
+            if (threadIdx.x == kThreads - 1) sh.log_sum = p.logp ? w.log_sum(all[0]) : 0.0;      // while the others sort
             // the kept ones again, in the vocabulary's order
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -932,7 +958,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
             for (int i = 0; i < 2; ++i) {
                 if (v[0] <= target && target < v[0] + own[i]) {
                     p.tokens[r] = (int)(turned[i] >> 32);
-                    if (p.logp) p.logp[r] = (float)log((double)own[i] / (double)all[0]);
+                    if (p.logp) p.logp[r] = w.log_share(value_of(~(uint32_t)turned[i]), sh.log_sum);
                 }
                 v[0] += own[i];
             }
@@ -1002,15 +1028,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         for (int j = 0; j < N; ++j) {
             if (last && at <= target && target < at + v[j]) {
                 p.tokens[r] = first + i + j;
-                if (p.logp) p.logp[r] = (float)log((double)v[j] / (double)sum[0]);
+                if (p.logp) p.logp[r] = w.log_share(x[j], w.log_sum(sum[0]));
             }
             at += v[j];
         }
     }
 }
 
-// CTAs a row: one, as long as the rows alone put two on every SM or the parts get
-// small, and as many as keep a part's tokens within what the histograms count.
+// CTAs a row: as many as put two on every SM, with parts of kLeastPart tokens at
+// least, and as keep a part's tokens within what the histograms count.  us with
+// parts of 4096 and 32768 at least: 1 x 32768 bf16 top-k 15.9 and 17.8, 1 x 131072 bf16
+// top-p 41 and 47, 8 x 50001 f32 top-p 34 and 59; 16 x 131072 bf16 top-k 23.7 and 21.4.
 template <typename T>
 cudaError_t sample_launch(const SampleParams& p, cudaStream_t s) {
     constexpr int N = Vec16<T>::N, kMostPart = 1 << 17, kLeastPart = 4096;
