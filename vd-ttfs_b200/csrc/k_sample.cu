@@ -166,7 +166,7 @@ struct Work {
 };
 struct Shared {
     u64 list[kList];
-    u64 said[2][8][3];                       // what the CTAs tell each other, two exchanges in turn
+    u64 said[2][8][4];                       // what the CTAs tell each other, two exchanges in turn
     u64 warps[3][kWarps];
     u64 found[4];
     u64 kept[kWarps];                        // weight of what each warp's part keeps
@@ -294,8 +294,8 @@ struct Row {
     }
     // What each CTA has to say, to all of them
     template <int K>
-    __device__ __forceinline__ u64 (&say(const u64 (&mine)[K]))[8][3] {
-        u64 (&slots)[8][3] = sh.said[turn];
+    __device__ __forceinline__ u64 (&say(const u64 (&mine)[K]))[8][4] {
+        u64 (&slots)[8][4] = sh.said[turn];
         turn ^= 1;
         if ((int)threadIdx.x < ranks) {
             u64* const to = cluster.map_shared_rank(&slots[rank][0], threadIdx.x);
@@ -592,18 +592,8 @@ struct Row {
         return r;
     }
 
-    // into the first CTA's list, from the lanes that have one; the whole warp
-    __device__ __forceinline__ void put(bool have, u64 place) {
-        const unsigned who = __ballot_sync(0xffffffffu, have);
-        if (!who) return;
-        const int lane = threadIdx.x % 32;
-        unsigned at = 0;
-        if (lane == 0) at = atomicAdd(cluster.map_shared_rank(&sh.listed, 0), (unsigned)__popc(who));
-        at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
-        if (have && at < kList) cluster.map_shared_rank(sh.list, 0)[at] = place;
-    }
-    // the same from a lane by itself
-    __device__ __forceinline__ void put_one(u64 place) {
+    // a token into the first CTA's list, from a lane by itself
+    __device__ __forceinline__ void put(u64 place) {
         const unsigned at = atomicAdd(cluster.map_shared_rank(&sh.listed, 0), 1u);
         if (at < kList) cluster.map_shared_rank(sh.list, 0)[at] = place;
     }
@@ -612,15 +602,13 @@ struct Row {
 
     // One pass over the row's tokens (PART: up to the place `end`): with WEIGHTS the
     // sums of their weights, of those in steps before `from`, each warp's into `kept`, and of those
-    // in steps up to `to`; and the tokens of the steps from..to into `chosen`, or of all
-    // steps up to `to` into the first CTA's list.
+    // in steps up to `to`; and the tokens of the steps first..to into `chosen`, as far as each warp
+    // has room for its own (`fits`: all have), `before`: how many the CTAs of lower rank have.
     template <bool PART, bool WEIGHTS>
-    __device__ __forceinline__ void look(int from, int to, bool list, u64 (&sums)[3], bool* fits) {
-        if (threadIdx.x == 0) sh.listed = 0;
-        together();
+    __device__ __forceinline__ void look(int from, int to, int first_of, u64 (&sums)[3], bool* fits, unsigned* before) {
         unsigned have = 0;
         sums[0] = sums[1] = sums[2] = 0;
-        const float since = (float)from, upto = (float)(to + 1), first_step = list ? 0.0f : since;
+        const float since = (float)from, upto = (float)(to + 1), first_step = (float)first_of;
         const int lane = threadIdx.x % 32;
         each_vector([&](const float* x, int i) {
             unsigned mine = 0, in = 0;
@@ -649,31 +637,50 @@ struct Row {
                 float y = x[0];
 #pragma unroll
                 for (int k = 1; k < N; ++k) y = j == k ? x[k] : y;
-                const u64 place = place_of(y, first + i + j);
-                if (list) {
-                    put(mine != 0, place);
-                } else {
-                    const unsigned at = have + __popc(who & ((1u << lane) - 1));
-                    if (mine && at < kChosen) wk.chosen[threadIdx.x / 32][at] = place;
-                    have += __popc(who);
-                }
+                const unsigned at = have + __popc(who & ((1u << lane) - 1));
+                if (mine && at < kChosen) wk.chosen[threadIdx.x / 32][at] = place_of(y, first + i + j);
+                have += __popc(who);
             }
         });
         if (lane == 0) sh.chosen[threadIdx.x / 32] = have;
+        u64 said[4] = {0, 0, 0, 0}, many[1] = {lane == 0 ? have + (have > kChosen ? 1ull << 40 : 0) : 0};
         if constexpr (WEIGHTS) {
             const u64 kept = warp_sum(sums[1]);
             if (lane == 0) sh.kept[threadIdx.x / 32] = kept;
             block_sum(sh, sums);
-            const auto& slots = say(sums);
-            sums[0] = sums[1] = sums[2] = 0;
-            for (int r = 0; r < ranks; ++r)
-#pragma unroll
-                for (int k = 0; k < 3; ++k) sums[k] += slots[r][k];
-        } else {
-            __syncthreads();
+            said[0] = sums[0];
+            said[1] = sums[1];
+            said[2] = sums[2];
         }
-        *fits = say_max(block_max(have)) <= kChosen;
+        block_sum(sh, many);
+        said[3] = many[0];
+        const auto& slots = say(said);
+        sums[0] = sums[1] = sums[2] = 0;
+        u64 all = 0;
+        for (int r = 0; r < ranks; ++r) {
+            if (r == rank) *before = (unsigned)all;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) sums[k] += slots[r][k];
+            all += slots[r][3];
+        }
+        *fits = all >> 40 == 0;
     }
+    // What `look` listed, at most kList tokens, into the first CTA's list
+    __device__ __forceinline__ void send(bool fits, int from, int to, unsigned before) {
+        if (fits) {
+            const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, many = (int)sh.chosen[warp];
+            for (int i = 0; i < warp; ++i) before += sh.chosen[i];
+            u64* const list = cluster.map_shared_rank(sh.list, 0);
+            for (int k = lane; k < many; k += 32)
+                if (before + k < kList) list[before + k] = wk.chosen[warp][k];
+        } else {
+            if (threadIdx.x == 0) sh.listed = 0;
+            together();
+            each_chosen(false, from, to, [&](float, u64 place) { put(place); });
+        }
+        together();
+    }
+
     // The sorted list's weights (or ones) of this thread's two places, the sum before them,
     // and the whole; those past the first `most` count nothing
     __device__ __forceinline__ u64 before_each(unsigned many, bool weights, u64 (&own)[2], u64* before, u64 most = ~0ull) {
@@ -830,13 +837,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         typename Row<T>::Steps at;
         u64 sums[3], want = (u64)top_k;
         bool fits;
+        unsigned before = 0;
         for (int sure = 0; sure < 2; ++sure) {
             at = s.steps_for(weights ? -1 : top_k, top_p, sure != 0);
             if (at.from == kBins) break;
             listed = at.upto <= kList;
-            if (!weights) s.template look<false, false>(at.from, at.to, listed, sums, &fits);
-            else if (partly) s.template look<true, true>(at.from, at.to, listed, sums, &fits);
-            else s.template look<false, true>(at.from, at.to, listed, sums, &fits);
+            const int first_of = listed ? 0 : at.from;
+            if (!weights) s.template look<false, false>(at.from, at.to, first_of, sums, &fits, &before);
+            else if (partly) s.template look<true, true>(at.from, at.to, first_of, sums, &fits, &before);
+            else s.template look<false, true>(at.from, at.to, first_of, sums, &fits, &before);
             if (!weights) break;
             want = want_of(top_p, sums[0]);
             if (sums[1] < want && want <= sums[2]) break;
@@ -844,8 +853,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         if (at.from == kBins) continue;                   // fewer tokens than k have any weight
         if (listed) {
             // few tokens up to the last step: the first CTA has them all
+            s.send(fits, 0, at.to, before);
             (weights ? limit_w : limit_k) = want;
-            in_list = s.in_list();
+            in_list = (unsigned)at.upto;
             break;
         }
         want -= weights ? sums[1] : at.before;
@@ -886,7 +896,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         }
         if (threadIdx.x == 0) sh.listed = 0;
         s.together();
-        part_of([&](float, float, u64 place) { s.put_one(place); });
+        part_of([&](float, float, u64 place) { s.put(place); });
         s.together();
         if (rank == 0) {
             const unsigned few = s.in_list();
@@ -905,9 +915,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         s.end_at(*cluster.map_shared_rank(&sh.last, 0));
         s.together();
         if (!weights && top_k <= kList) {
-            s.template look<true, false>(0, kBins - 1, true, sums, &fits);
+            s.template look<true, false>(0, kBins - 1, 0, sums, &fits, &before);
+            s.send(fits, 0, kBins - 1, before);
             limit_k = (u64)top_k;
-            in_list = s.in_list();
+            in_list = (unsigned)top_k;
             listed = true;
         }
         if (weights && !least) {
