@@ -397,11 +397,12 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarp
         static_assert(kGroups >= 1, "a thread a block");
         const int t = (threadIdx.x - 64) % kGroup, block = t % 8, row = t / 8;
         const X* const x = static_cast<const X*>(p.x) + (long long)(row0 + row) * p.x_stride + block * kBlock;
-        const bool wide = p.x_stride * (long long)sizeof(X) % 32 == 0 && reinterpret_cast<uintptr_t>(p.x) % 32 == 0;
+        const uintptr_t off = reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(rows > 1 ? p.x_stride * (long long)sizeof(X) : 0);
         uint32_t raw[8 * sizeof(X)];
         auto load = [&](int s) {
             const int col = s * kFp4Step, left = row < rows && s < last ? p.inner - col - block * kBlock : 0;
-            if (wide) load_block<X, 32>(x + col, left, raw);
+            if (off % 32 == 0) load_block<X, 32>(x + col, left, raw);
+            else if (off % 16 == 0) load_block<X, 16>(x + col, left, raw);
             else load_block<X, 1>(x + col, left, raw);
         };
         int s = first + (threadIdx.x - 64) / kGroup;
