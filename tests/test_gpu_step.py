@@ -730,3 +730,38 @@ def test_calls_of_nothing(S):
     assert S.fp4_matmul(codes, scale, w, ws).shape == (0, 10)
     assert [t.shape[0] for t in S.add_rms_norm(x, x)] == [0, 0] and [t.shape[0] for t in S.add_rms_norm_int8(x, x)] == [0, 0, 0]
     assert [t.shape[0] for t in S.sample(x, torch.empty(0, device="cuda"))] == [0, 0]
+
+
+def test_rows_further_apart_than_32_bits_count(S):
+    far = 2 ** 31 + 64
+    store = torch.zeros(far + 4096, dtype=torch.bfloat16, device="cuda")
+    near = normal(5, 2, 1000, kind=torch.bfloat16).cuda()
+
+    def view(t=None):
+        v = store.as_strided((2, 1000), (far, 1))
+        if t is not None:
+            v.copy_(t)
+        return v
+
+    w, ws = S.quantize_fp4(normal(6, 1000, 1000).cuda())
+    u = torch.tensor([0.3, 0.9], device="cuda")
+    x = view(near)
+    assert torch.equal(S.fp4_values(*S.quantize_fp4(x)), S.fp4_values(*S.quantize_fp4(near)))
+    for a, b in zip(S.add_rms_norm(x, near) + S.add_rms_norm_int8(x, near) + S.sample(x, u, 1.0, 0, 0.9), S.add_rms_norm(near, near) + S.add_rms_norm_int8(near, near)
+                    + S.sample(near, u, 1.0, 0, 0.9)):
+        assert torch.equal(a, b)
+    want = S.fp4_linear(near, w, ws)
+    assert torch.equal(S.fp4_linear(x, w, ws), want)
+    S.fp4_linear(near, w, ws, out=view())
+    assert torch.equal(view(), want)
+    codes, scale = S.quantize_fp4(near)
+    S.fp4_matmul(codes, scale, w, ws, out=view(near))
+    assert torch.equal(view(), want)
+    S.add_rms_norm(near, near, out=view(), sum_out=near.clone())
+    assert torch.equal(view(), S.add_rms_norm(near, near)[0])
+    # many rows, the tiles' way
+    wide = torch.zeros(200 * 2 ** 24, dtype=torch.bfloat16, device="cuda").as_strided((200, 256), (2 ** 24 + 32, 1))
+    m, ms = S.quantize_fp4(normal(7, 256, 96).cuda())
+    y = normal(8, 200, 96, kind=torch.bfloat16).cuda()
+    S.fp4_linear(y, m, ms, out=wide)
+    assert torch.equal(wide, S.fp4_linear(y, m, ms))
