@@ -95,12 +95,24 @@ struct Top<float> {
     __device__ __forceinline__ float value() const { return a; }
 };
 
+// 2^(i / 32)
+__device__ const double kRoots[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+
 struct Weigher {
     // The row's largest value; a power of two that logits and temperature are taken
     // times, 1 but for the smallest and largest of them; the largest so, and a value without weight
     float largest, factor, top, bottom;
     float part, part_top, steps;
-    double octaves;         // log2(e) / T
+    double octaves, parts;  // log2(e) / T, and 32 times that
+    const double* roots;    // kRoots in shared memory
     int bits;
     __device__ __forceinline__ void set(float row_top, float temperature, int vocab) {
         // The smallest temperatures (below large values nothing has any weight then) and the
@@ -122,6 +134,7 @@ struct Weigher {
         // the next value below the largest has no weight by far: no exponent below a double's
         const double span = (double)top - (double)bottom;
         if (span * octaves > 900.0) octaves = 80.0 / span;
+        parts = 32.0 * octaves;
     }
     // the logarithm of a token's probability, from the kept weights' sum (1 for the largest)
     __device__ __forceinline__ double log_sum(u64 sum) const { return log((double)sum * __hiloint2double((1023 - bits) << 20, 0)); }
@@ -134,24 +147,24 @@ struct Weigher {
     static __device__ __forceinline__ int step(float depth) {
         return __float_as_int(__fadd_rd(fminf(depth, (float)kBins), 8388608.0f)) & (2 * kBins - 1);
     }
-    // 2^bits exp((x - top) / T) to the nearest whole number.  2^f on [-1/2, 1/2] by the
-    // interpolating polynomial of degree 8 at Chebyshev's points, off by at most 2^-39.7.
-    // 3/2 2^52 added leaves the nearest whole number in the low bits; no branches, so that
-    // the chains of several tokens run side by side.
+    // 2^bits exp((x - top) / T) to the nearest whole number: the next 32nd of an octave from
+    // a table, its exponent moved by the whole octaves, and the rest, at most a 64th, by the
+    // interpolating polynomial of degree 4 at Chebyshev's points, off by at most 2^-43.  (Without
+    // the table degree 8 is wanted: 14 operations in 64 bits a token, of which the SM does
+    // 1.6 a cycle for a warp, and not 9.)  3/2 2^52 added leaves the nearest whole number in the
+    // low bits; no branches, so that the chains of several tokens run side by side.
     __device__ __forceinline__ u64 weight(float x) const {
         constexpr double kRound = 6755399441055744.0;
         const double d = (double)fmaxf(x * factor, bottom) - (double)top;
-        const double z = fma(d, octaves, kRound), f = fma(d, octaves, kRound - z);
-        double y = 0x1.63d0e49869220p-20;
-        y = fma(y, f, 0x1.00dc4b54b68d6p-16);
-        y = fma(y, f, 0x1.4308acd88a0d7p-13);
-        y = fma(y, f, 0x1.5d8745a58ae45p-10);
-        y = fma(y, f, 0x1.3b2ab717e98f6p-7);
-        y = fma(y, f, 0x1.c6b08dd6fe736p-5);
-        y = fma(y, f, 0x1.ebfbdff823ef1p-3);
-        y = fma(y, f, 0x1.62e42fef84ceep-1);
+        const double z = fma(d, parts, kRound), f = fma(d, parts, kRound - z);
+        const int whole = __double2loint(z);
+        const double root = roots[whole & 31];
+        double y = 0x1.3b2b18fa66654p-27;
+        y = fma(y, f, 0x1.c6b167e61eadap-20);
+        y = fma(y, f, 0x1.ebfbdff817570p-13);
+        y = fma(y, f, 0x1.62e42fef6d03fp-6);
         y = fma(y, f, 1.0);
-        y = fma(y, __hiloint2double((1023 + bits + __double2loint(z)) << 20, 0), 4503599627370496.0);
+        y = fma(y, __hiloint2double(__double2hiint(root) + ((bits + (whole >> 5)) << 20), __double2loint(root)), 4503599627370496.0);
         return (u64)__double_as_longlong(y) & 0xfffffffffffffull;
     }
 };
@@ -171,7 +184,7 @@ struct Shared {
     u64 found[4];
     u64 kept[kWarps];                        // weight of what each warp's part keeps
     u64 last;
-    double log_sum;
+    double roots[32], log_sum;
     unsigned listed, chosen[kWarps];
 };
 
@@ -720,7 +733,7 @@ struct Row {
 // to 63 places apart are in the same warp and meet in registers, the others in shared
 // memory (all steps there took four times as long).
 constexpr unsigned kCounted = 128;
-__device__ __forceinline__ void sort_list(u64* a, unsigned n) {
+__device__ __noinline__ void sort_list(u64* a, unsigned n) {
     static_assert(kList == 2 * kThreads, "two a thread");
     const unsigned t = threadIdx.x;
     if (n <= kCounted) {
@@ -795,6 +808,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
     const bool greedy = temperature == 0.0f;
     if (ranks > 1) cluster.barrier_arrive();
 
+    if (threadIdx.x < 32) sh.roots[threadIdx.x] = kRoots[threadIdx.x];
     // the largest value; NaN orders above the others
     Top<T> most;
     s.each_load([&](const Vec16<T>& v) { most.add(v); });
@@ -821,6 +835,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
     Weigher& w = s.w;
     s.endless = top == INFINITY;
     w.set(s.value(top), temperature, p.vocab);
+    w.roots = sh.roots;
     const u64 least = __double2ull_ru((double)fminf(fmaxf(min_p, 0.0f), 1.0f) * (double)(1ull << w.bits));
 
     const bool by_count = top_k > 0 && top_k < p.vocab, by_weight = top_p < 1.0f;
