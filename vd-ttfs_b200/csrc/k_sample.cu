@@ -25,6 +25,7 @@
 // which the sum passes the target is gone through again.
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <cfloat>
 
 #include "step_internal.h"
@@ -292,9 +293,9 @@ struct Row {
     cg::cluster_group cluster;
     Shared& sh;
     Work& wk;
-    const T* slice;          // this CTA's part
-    int first, n, seg;       // its first index, its length, and what a warp takes of it
-    bool wide, endless;      // endless: the largest value is +inf, which counts as 0 then, and all others as -inf
+    const T* slice;          // this CTA's part, on 16 bytes: the row's may begin up to N - 1 values before it does
+    int first, n, seg;       // its first index (below 0 then), its length, and what a warp takes of it
+    bool endless;            // endless: the largest value is +inf, which counts as 0 then, and all others as -inf
     int rank, ranks, turn;
     u64 end;                 // the last token's place that counts, as far as it is known
     float end_value;
@@ -351,19 +352,21 @@ struct Row {
         return v;
     }
 
-    // N values; past the end of the part there is -inf
-    __device__ __forceinline__ Vec16<T> load(int i) const {
+    // N values; what is not the part's counts as -inf
+    __device__ __forceinline__ Vec16<T> load(int i, bool edge) const {
         Vec16<T> v;
-        if (wide && i + N <= n) {
-            v.raw = *reinterpret_cast<const uint4*>(slice + i);
+        if (!edge) {
+            v.raw = __ldg(reinterpret_cast<const uint4*>(slice + i));
         } else {
             float x[N];
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = i + j < n ? to_f32(slice[i + j]) : -INFINITY;
+            for (int j = 0; j < N; ++j) x[j] = i + j < n && first + i + j >= 0 ? to_f32(slice[i + j]) : -INFINITY;
             v.set(x);
         }
         return v;
     }
+    // whether some of a warp's vectors from i0 on are not the part's
+    __device__ __forceinline__ bool edge_at(int i0) const { return i0 + 32 * N > n || (first < 0 && i0 == 0); }
     __device__ __forceinline__ float value(float x) const { return endless ? (x == INFINITY ? 0.0f : -INFINITY) : x; }
     __device__ __forceinline__ void values(const Vec16<T>& v, float* x) const {
         v.get(x);
@@ -378,10 +381,10 @@ struct Row {
         const int from = threadIdx.x / 32 * seg, to = min(n, from + seg), step = 32 * N;
         if (from >= to) return;
         int i = from + (int)(threadIdx.x % 32) * N;
-        Vec16<T> next = load(i);
+        Vec16<T> next = load(i, edge_at(from));
         for (int i0 = from; i0 < to; i0 += step, i += step) {
             const Vec16<T> v = next;
-            if (i0 + step < to) next = load(i + step);
+            if (i0 + step < to) next = load(i + step, edge_at(i0 + step));
             float x[N];
             values(v, x);
             f(x, i);
@@ -392,7 +395,7 @@ struct Row {
     __device__ __forceinline__ void each_load(F f) const {
         const int from = threadIdx.x / 32 * seg, to = min(n, from + seg);
 #pragma unroll 4
-        for (int i0 = from; i0 < to; i0 += 32 * N) f(load(i0 + (int)(threadIdx.x % 32) * N));
+        for (int i0 = from; i0 < to; i0 += 32 * N) f(load(i0 + (int)(threadIdx.x % 32) * N, edge_at(i0)));
     }
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
@@ -798,10 +801,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
     const cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const long long r = blockIdx.x / ranks;
-    const int first = rank * part, n = max(0, min(p.vocab - first, part));
-    const T* const row = static_cast<const T*>(p.logits) + r * p.stride + first;
+    const T* const row = static_cast<const T*>(p.logits) + r * p.stride;
+    const int first = rank * part - (int)(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T)), n = max(0, min(p.vocab - first, part));
     const int seg = ((part + kWarps - 1) / kWarps + 32 * N - 1) / (32 * N) * (32 * N);
-    Row<T> s{cluster, sh, wk, row, first, n, seg, reinterpret_cast<uintptr_t>(row) % 16 == 0, false, rank, ranks, 0, ~0ull, -INFINITY, INT_MIN, {}};
+    Row<T> s{cluster, sh, wk, row + first, first, n, seg, false, rank, ranks, 0, ~0ull, -INFINITY, INT_MIN, {}};
     const float temperature = p.temperatures ? p.temperatures[r] : p.temperature, top_p = p.top_ps ? p.top_ps[r] : p.top_p;
     const float min_p = p.min_ps ? p.min_ps[r] : p.min_p, u = p.u[r];
     const int top_k = p.top_ks ? p.top_ks[r] : p.top_k;
@@ -847,8 +850,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         if (weights ? !by_weight : !by_count) continue;
         if (partly) s.template histogram<true>();
         else if (!counted) s.template histogram<false>();
+        if (partly || !counted) s.gather_counts();
         counted = true;
-        s.gather_counts();
         typename Row<T>::Steps at;
         u64 sums[3], want = (u64)top_k;
         bool fits;
@@ -1037,7 +1040,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
     for (int k = 0; k < many; ++k) {
         const int i = from + ((int)threadIdx.x * many + k) * N;
         float x[N];
-        s.values(s.load(i), x);
+        s.values(s.load(i, i + N > n || first + i < 0), x);
         place[0] += weigh(x, i, i < to, v);
     }
     u64 mine = place[0];
@@ -1048,7 +1051,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
     for (int k = 0; k < many; ++k) {
         const int i = from + ((int)threadIdx.x * many + k) * N;
         float x[N];
-        s.values(s.load(i), x);
+        s.values(s.load(i, i + N > n || first + i < 0), x);
         weigh(x, i, i < to, v);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
@@ -1068,9 +1071,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
 template <typename T>
 cudaError_t sample_launch(const SampleParams& p, cudaStream_t s) {
     constexpr int N = Vec16<T>::N, kMostPart = 1 << 17, kLeastPart = 4096;
-    auto part_of = [&](int ranks) { return ((p.vocab + ranks - 1) / ranks + N - 1) / N * N; };
+    // rows that are not on 16 bytes begin up to N - 1 values into their first ones
+    const bool on16 = aligned(p.logits, 16) && (p.rows == 1 || p.stride * (long long)sizeof(T) % 16 == 0);
+    const int places = p.vocab + (on16 ? 0 : N - 1);
+    auto part_of = [&](int ranks) { return ((places + ranks - 1) / ranks + N - 1) / N * N; };
     int ranks = 1;
-    while (part_of(ranks) > kMostPart || (ranks < 8 && p.rows * ranks * 2 <= 2 * kSmCount && part_of(ranks * 2) >= kLeastPart)) ranks *= 2;
+    while (std::min(part_of(ranks), p.vocab) > kMostPart || (ranks < 8 && p.rows * ranks * 2 <= 2 * kSmCount && part_of(ranks * 2) >= kLeastPart)) ranks *= 2;
     const cudaError_t e = allow_shared<k_sample<T>>((int)sizeof(Work));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
