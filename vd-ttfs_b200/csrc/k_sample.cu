@@ -57,43 +57,65 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
     return m;
 }
+// Eight values side by side, on a multiple of their size
+template <typename T>
+struct Eight {
+    static constexpr int kWords = 2 * sizeof(T);
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const T* from) {
+        if constexpr (sizeof(T) == 4) {
+            asm("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                : "l"(from));
+        } else {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(from));
+            w[0] = v.x;
+            w[1] = v.y;
+            w[2] = v.z;
+            w[3] = v.w;
+        }
+    }
+    __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) f[i] = __uint_as_float(w[i]);
+            else unpack2<T>(w[i], f[2 * i], f[2 * i + 1]);
+        }
+    }
+    __device__ __forceinline__ void set(const float* f) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+            else w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+        }
+    }
+};
 // the largest of many values; NaN where one is
 template <typename T>
 struct Top {
-    __nv_bfloat162 a = {__ushort_as_bfloat16(0xff80), __ushort_as_bfloat16(0xff80)};
-    __device__ __forceinline__ void add(const Vec16<T>& v) {
-        const uint32_t w[4] = {v.raw.x, v.raw.y, v.raw.z, v.raw.w};
+    using Pair = std::conditional_t<sizeof(T) == 4, float, std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>>;
+    Pair a;
+    __device__ __forceinline__ Top() {
+        const uint32_t lowest = sizeof(T) == 4 || std::is_same_v<T, __nv_bfloat16> ? 0xff80ff80u : 0xfc00fc00u;
+        if constexpr (sizeof(T) == 4) a = -INFINITY;
+        else memcpy(&a, &lowest, 4);
+    }
+    __device__ __forceinline__ void add(const Eight<T>& v) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            __nv_bfloat162 b;
-            memcpy(&b, &w[i], 4);
-            a = __hmax2_nan(a, b);
+        for (int i = 0; i < Eight<T>::kWords; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                a = max_or_nan(a, __uint_as_float(v.w[i]));
+            } else {
+                Pair b;
+                memcpy(&b, &v.w[i], 4);
+                a = __hmax2_nan(a, b);
+            }
         }
     }
-    __device__ __forceinline__ float value() const { return max_or_nan(__low2float(a), __high2float(a)); }
-};
-template <>
-struct Top<__half> {
-    __half2 a = {__ushort_as_half(0xfc00), __ushort_as_half(0xfc00)};
-    __device__ __forceinline__ void add(const Vec16<__half>& v) {
-        const uint32_t w[4] = {v.raw.x, v.raw.y, v.raw.z, v.raw.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            __half2 b;
-            memcpy(&b, &w[i], 4);
-            a = __hmax2_nan(a, b);
-        }
+    __device__ __forceinline__ float value() const {
+        if constexpr (sizeof(T) == 4) return a;
+        else return max_or_nan(__low2float(a), __high2float(a));
     }
-    __device__ __forceinline__ float value() const { return max_or_nan(__low2float(a), __high2float(a)); }
-};
-template <>
-struct Top<float> {
-    float a = -INFINITY;
-    __device__ __forceinline__ void add(const Vec16<float>& v) {
-        a = max_or_nan(a, max_or_nan(max_or_nan(__uint_as_float(v.raw.x), __uint_as_float(v.raw.y)),
-                                     max_or_nan(__uint_as_float(v.raw.z), __uint_as_float(v.raw.w))));
-    }
-    __device__ __forceinline__ float value() const { return a; }
 };
 
 // 2^(i / 32)
@@ -108,42 +130,45 @@ __device__ const double kRoots[32] = {
     0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
 
 struct Weigher {
-    // The row's largest value; a power of two that logits and temperature are taken
-    // times, 1 but for the smallest and largest of them; the largest so, and a value without weight
-    float largest, factor, top, bottom;
-    float part, part_top, steps;
-    double octaves, parts;  // log2(e) / T, and 32 times that
+    // How a row's values are taken.  As they are, mostly; `alone`: the largest as 0, all
+    // others as -inf, where it is +inf or the next value below it has no weight; `shift`: less
+    // the largest, where that is many temperatures (what has any weight is near to
+    // it then, and the difference exact); times `factor`, a power of two, for the smallest temperatures
+    bool odd, alone, shift;
+    float largest, factor;
+    float top, bottom;      // the largest then, and a value without weight (-inf is not weighed)
+    float slope, start;     // steps of the histogram below the largest: start + slope x
+    double parts;           // 32 log2(e) / T
     const double* roots;    // kRoots in shared memory
     int bits;
+    __device__ __forceinline__ float value(float x) const {
+        return alone ? (x == largest ? 0.0f : -INFINITY) : (shift ? x - largest : x) * factor;
+    }
     __device__ __forceinline__ void set(float row_top, float temperature, int vocab) {
-        // The smallest temperatures (below large values nothing has any weight then) and the
-        // largest leave no room for what is computed from them; nor do rows of the type's
-        // lowest value, which -inf is to be below
+        constexpr double kLog2e = 1.4426950408889634;
         largest = row_top;
-        factor = temperature < 1e-30f && fabsf(largest) < 1e9f ? 0x1p90f : temperature > 1e30f || largest < -1e30f ? 0x1p-20f : 1.0f;
-        top = largest * factor;
-        octaves = 1.4426950408889634 / (double)fmaxf(temperature * factor, 1e-30f);
-        float below = value_of(key_of(top) - 1);             // the next value below (0's is not -0)
-        if (below == top) below = value_of(key_of(top) - 2);
-        bottom = fmaxf(fminf(__double2float_rd((double)top - 80.0 / octaves), below), -FLT_MAX);
-        // of large logits halves, whose difference is always a number
-        const float half = fabsf(top) > 1e30f ? 0.5f : 1.0f;
-        part = half * factor;
-        part_top = part * largest;
-        steps = (float)(octaves / (double)half * (double)kSteps);
+        float below = value_of(key_of(largest) - 1);             // the next value below (0's is not -0)
+        if (below == largest) below = value_of(key_of(largest) - 2);
+        const double octaves = kLog2e / (double)temperature, far = fabs((double)largest) * octaves * (double)kSteps;
+        alone = largest == INFINITY || ((double)largest - (double)below) * octaves > 60.0;
+        shift = !alone && far > 1e4;
+        factor = !alone && temperature < 1e-30f ? 0x1p90f : 1.0f;
+        odd = alone || shift || factor != 1.0f;
+        top = value(largest);
+        const double each = alone ? 1.0 : octaves / (double)factor;
+        parts = 32.0 * each;
+        bottom = fmaxf(__double2float_rd((double)top - 80.0 / each), -FLT_MAX);
+        slope = (float)(-(double)kSteps * each);
+        // a little above, so that the largest is not below 0
+        start = (float)((double)kSteps * each * (double)top) + (float)(shift || alone ? 0.0 : far) * 0x1p-22f;
         bits = min(kMostBits, 62 - (32 - __clz(vocab - 1)));
-        // the next value below the largest has no weight by far: no exponent below a double's
-        const double span = (double)top - (double)bottom;
-        if (span * octaves > 900.0) octaves = 80.0 / span;
-        parts = 32.0 * octaves;
     }
     // the logarithm of a token's probability, from the kept weights' sum (1 for the largest)
     __device__ __forceinline__ double log_sum(u64 sum) const { return log((double)sum * __hiloint2double((1023 - bits) << 20, 0)); }
     __device__ __forceinline__ float log_share(float x, double log_sum) const {
-        return (float)(((double)fmaxf(x * factor, bottom) - (double)top) * octaves * 0.6931471805599453 - log_sum);
+        return (float)(((double)x - (double)top) * parts * (0.6931471805599453 / 32.0) - log_sum);
     }
-    // steps below the largest
-    __device__ __forceinline__ float depth(float x) const { return fmaf(-part, x, part_top) * steps; }
+    __device__ __forceinline__ float depth(float x) const { return fmaf(slope, x, start); }
     // the step itself, kBins for all without weight: floor in the low bits of 2^23 + depth
     static __device__ __forceinline__ int step(float depth) {
         return __float_as_int(__fadd_rd(fminf(depth, (float)kBins), 8388608.0f)) & (2 * kBins - 1);
@@ -156,7 +181,7 @@ struct Weigher {
     // low bits; no branches, so that the chains of several tokens run side by side.
     __device__ __forceinline__ u64 weight(float x) const {
         constexpr double kRound = 6755399441055744.0;
-        const double d = (double)fmaxf(x * factor, bottom) - (double)top;
+        const double d = (double)fmaxf(x, bottom) - (double)top;
         const double z = fma(d, parts, kRound), f = fma(d, parts, kRound - z);
         const int whole = __double2loint(z);
         const double root = roots[whole & 31];
@@ -289,13 +314,12 @@ __device__ __forceinline__ u64 want_of(float top_p, u64 sum) {
 
 template <typename T>
 struct Row {
-    static constexpr int N = Vec16<T>::N;
+    static constexpr int N = 8;
     cg::cluster_group cluster;
     Shared& sh;
     Work& wk;
-    const T* slice;          // this CTA's part, on 16 bytes: the row's may begin up to N - 1 values before it does
+    const T* slice;          // this CTA's part, on whole vectors: the row's may begin up to N - 1 values before it does
     int first, n, seg;       // its first index (below 0 then), its length, and what a warp takes of it
-    bool endless;            // endless: the largest value is +inf, which counts as 0 then, and all others as -inf
     int rank, ranks, turn;
     u64 end;                 // the last token's place that counts, as far as it is known
     float end_value;
@@ -353,10 +377,10 @@ struct Row {
     }
 
     // N values; what is not the part's counts as -inf
-    __device__ __forceinline__ Vec16<T> load(int i, bool edge) const {
-        Vec16<T> v;
+    __device__ __forceinline__ Eight<T> load(int i, bool edge) const {
+        Eight<T> v;
         if (!edge) {
-            v.raw = __ldg(reinterpret_cast<const uint4*>(slice + i));
+            v.load(slice + i);
         } else {
             float x[N];
 #pragma unroll
@@ -367,12 +391,11 @@ struct Row {
     }
     // whether some of a warp's vectors from i0 on are not the part's
     __device__ __forceinline__ bool edge_at(int i0) const { return i0 + 32 * N > n || (first < 0 && i0 == 0); }
-    __device__ __forceinline__ float value(float x) const { return endless ? (x == INFINITY ? 0.0f : -INFINITY) : x; }
-    __device__ __forceinline__ void values(const Vec16<T>& v, float* x) const {
+    __device__ __forceinline__ void values(const Eight<T>& v, float* x) const {
         v.get(x);
-        if (endless)
+        if (w.odd)
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = value(x[j]);
+            for (int j = 0; j < N; ++j) x[j] = w.value(x[j]);
     }
     // Every N tokens of this thread: a warp's are consecutive, a lane's N of them too;
     // the next are on their way meanwhile
@@ -381,9 +404,9 @@ struct Row {
         const int from = threadIdx.x / 32 * seg, to = min(n, from + seg), step = 32 * N;
         if (from >= to) return;
         int i = from + (int)(threadIdx.x % 32) * N;
-        Vec16<T> next = load(i, edge_at(from));
+        Eight<T> next = load(i, edge_at(from));
         for (int i0 = from; i0 < to; i0 += step, i += step) {
-            const Vec16<T> v = next;
+            const Eight<T> v = next;
             if (i0 + step < to) next = load(i + step, edge_at(i0 + step));
             float x[N];
             values(v, x);
@@ -641,7 +664,7 @@ struct Row {
                 if (WEIGHTS) {
                     u64 v = w.weight(x[j]);
                     if (!here) v = 0;
-                    sums[0] += v;
+                    if (d < (float)kBins) sums[0] += v;              // (not -inf)
                     if (d < since) sums[1] += v;
                     if (d < upto) sums[2] += v;
                 }
@@ -724,7 +747,7 @@ struct Row {
             const float upto = (float)(to + 1), since = (float)from;
             each([&](float x, int i) {
                 const float d = w.depth(x);
-                if (d >= since && d < upto && (end == ~0ull || before_end(x, i))) f(x, place_of(x, first + i));
+                if (d >= since && d < upto && before_end(x, i)) f(x, place_of(x, first + i));
             });
         }
     }
@@ -797,14 +820,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
     extern __shared__ __align__(16) unsigned char memory[];
     __shared__ Shared sh;
     Work& wk = *reinterpret_cast<Work*>(memory);
-    constexpr int N = Vec16<T>::N;
+    constexpr int N = Row<T>::N;
     const cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const long long r = blockIdx.x / ranks;
     const T* const row = static_cast<const T*>(p.logits) + r * p.stride;
-    const int first = rank * part - (int)(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T)), n = max(0, min(p.vocab - first, part));
+    const int first = rank * part - (int)(reinterpret_cast<uintptr_t>(row) % (N * sizeof(T)) / sizeof(T)), n = max(0, min(p.vocab - first, part));
     const int seg = ((part + kWarps - 1) / kWarps + 32 * N - 1) / (32 * N) * (32 * N);
-    Row<T> s{cluster, sh, wk, row + first, first, n, seg, false, rank, ranks, 0, ~0ull, -INFINITY, INT_MIN, {}};
+    Row<T> s{cluster, sh, wk, row + first, first, n, seg, rank, ranks, 0, ~0ull, -INFINITY, INT_MIN, {}};
     const float temperature = p.temperatures ? p.temperatures[r] : p.temperature, top_p = p.top_ps ? p.top_ps[r] : p.top_p;
     const float min_p = p.min_ps ? p.min_ps[r] : p.min_p, u = p.u[r];
     const int top_k = p.top_ks ? p.top_ks[r] : p.top_k;
@@ -814,7 +837,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
     if (threadIdx.x < 32) sh.roots[threadIdx.x] = kRoots[threadIdx.x];
     // the largest value; NaN orders above the others
     Top<T> most;
-    s.each_load([&](const Vec16<T>& v) { most.add(v); });
+    s.each_load([&](const Eight<T>& v) { most.add(v); });
     if (ranks > 1) cluster.barrier_wait();                // all CTAs are there to be told
     const float mine_top = most.value();
     const u64 top_key = s.say_max(s.block_max(mine_top != mine_top ? ~0ull : (u64)key_of(mine_top)));
@@ -836,8 +859,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         return;
     }
     Weigher& w = s.w;
-    s.endless = top == INFINITY;
-    w.set(s.value(top), temperature, p.vocab);
+    w.set(top, temperature, p.vocab);
     w.roots = sh.roots;
     const u64 least = __double2ull_ru((double)fminf(fmaxf(min_p, 0.0f), 1.0f) * (double)(1ull << w.bits));
 
@@ -997,11 +1019,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
 
     // everything up to the last: each warp's sum, each CTA's, the whole; then the part of the
     // warp in which the sum passes the target once more
-    const bool all_kept = s.end == ~0ull;
     auto weigh = [&](const float* x, int i, bool in, u64* v) {
         unsigned kept = 0;
 #pragma unroll
-        for (int j = 0; j < N; ++j) kept |= in && (all_kept || s.before_end(x[j], i + j)) ? 1u << j : 0u;
+        for (int j = 0; j < N; ++j) kept |= in && s.before_end(x[j], i + j) ? 1u << j : 0u;
         u64 sum = 0;
 #pragma unroll
         for (int j = 0; j < N; ++j) v[j] = 0;
@@ -1070,10 +1091,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
 // top-p 41 and 47, 8 x 50001 f32 top-p 34 and 59; 16 x 131072 bf16 top-k 23.7 and 21.4.
 template <typename T>
 cudaError_t sample_launch(const SampleParams& p, cudaStream_t s) {
-    constexpr int N = Vec16<T>::N, kMostPart = 1 << 17, kLeastPart = 4096;
-    // rows that are not on 16 bytes begin up to N - 1 values into their first ones
-    const bool on16 = aligned(p.logits, 16) && (p.rows == 1 || p.stride * (long long)sizeof(T) % 16 == 0);
-    const int places = p.vocab + (on16 ? 0 : N - 1);
+    constexpr int N = Row<T>::N, kMostPart = 1 << 17, kLeastPart = 4096;
+    // rows that are not on whole vectors begin up to N - 1 values into their first ones
+    const bool whole = aligned(p.logits, N * sizeof(T)) && (p.rows == 1 || p.stride % N == 0);
+    const int places = p.vocab + (whole ? 0 : N - 1);
     auto part_of = [&](int ranks) { return ((places + ranks - 1) / ranks + N - 1) / N * N; };
     int ranks = 1;
     while (std::min(part_of(ranks), p.vocab) > kMostPart || (ranks < 8 && p.rows * ranks * 2 <= 2 * kSmCount && part_of(ranks * 2) >= kLeastPart)) ranks *= 2;
