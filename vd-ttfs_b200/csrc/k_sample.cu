@@ -720,6 +720,21 @@ struct Row {
         together();
     }
 
+    // Each warp's sum of the weights up to `end` of at least `least`, into `kept`
+    __device__ __forceinline__ void sum_kept(u64 least) {
+        u64 mine = 0;
+        each_vector([&](const float* x, int i) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const u64 o = w.weight(x[j]);
+                if (before_end(x[j], i + j) && o >= least) mine += o;
+            }
+        });
+        mine = warp_sum(mine);
+        __syncthreads();
+        if (threadIdx.x % 32 == 0) sh.kept[threadIdx.x / 32] = mine;
+        __syncthreads();
+    }
     // The sorted list's weights (or ones) of this thread's two places, the sum before them,
     // and the whole; those past the first `most` count nothing
     __device__ __forceinline__ u64 before_each(unsigned many, bool weights, u64 (&own)[2], u64* before, u64 most = ~0ull) {
@@ -1036,18 +1051,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
         }
         return sum;
     };
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (!summed) {
-        u64 mine = 0;
-        s.each_vector([&](const float* x, int i) {
-            u64 v[N];
-            mine += weigh(x, i, true, v);
-        });
-        mine = warp_sum(mine);
-        __syncthreads();
-        if (lane == 0) sh.kept[warp] = mine;
-        __syncthreads();
-    }
+    const int lane = threadIdx.x % 32;
+    if (!summed) s.sum_kept(least);
     const u64 own = lane < kWarps ? sh.kept[lane] : 0, upto = warp_scan(own);   // each warp has them all
     u64 sum[1] = {__shfl_sync(0xffffffffu, upto, 31)};
     const u64 here = sum[0], below = s.say_sum(sum), target = share_of(share, sum[0], &whole);
