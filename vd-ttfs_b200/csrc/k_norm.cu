@@ -7,6 +7,10 @@
 // The norm is one factor for the whole row, so it goes into the scale alone: a
 // code does not depend on how r is rounded, and both reductions, of t^2 and of
 // |z|, run over the row at once.
+//
+// Bound by memory: 16381 x 4096 bf16 with a residual, the sum and codes written,
+// 470 MB in 75.7 us, 6.2 TB/s of the 6.5 that a plain copy reaches.  One row of
+// 1024, and 777 x 1001 f32, 4 us: a launch, the row's latency and one barrier.
 #include "step_internal.h"
 
 namespace vdt {
