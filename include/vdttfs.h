@@ -583,9 +583,9 @@ int vdt_fp4_linear(const void* d_x, int type, int64_t x_stride, const uint8_t* d
    z r in `type`, vdt_add_rms_norm_int8 what vdt_int8_matmul takes: codes
    round(z / u) with u = max |z| * (1/127), and the scale u r.  A row of zeros has
    codes 0 (and NaN without eps), one with an infinity or NaN a scale that is not
-   finite.  d_sum may be d_residual or d_x, and d_out d_x or d_residual, with the
-   same strides; d_sum and d_out must not lie over each other, nor any output over an
-   input otherwise. */
+   finite; t^2 is summed in 32 bits, so r is 0 where the sum passes 3.4e38.  d_sum may
+   be d_residual or d_x, and d_out d_x or d_residual, with the same strides; d_sum and
+   d_out must not lie over each other, nor any output over an input otherwise. */
 int vdt_add_rms_norm(const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride,
                      const void* d_weight, int64_t rows, int cols, float eps, int type, void* d_sum, int64_t sum_stride,
                      void* d_out, int64_t out_stride, vdt_stream stream);
@@ -606,6 +606,7 @@ int vdt_add_rms_norm_int8(const void* d_x, int64_t x_stride, const void* d_resid
    past a row's width take no page and have slot -1; rows past the last sequence's
    have position and slot -1.  d_ring and d_new are not changed; kept may be held,
    and span_out span, for a step in place; other buffers must not lie over each other.
+   Up to 65535 sequences, and 2^30 pages in the ring and in a row of the table.
    d_scratch: vdt_plan_pages_scratch_bytes, 16-byte aligned. */
 size_t vdt_plan_pages_scratch_bytes(int seqs);
 int vdt_plan_pages(const int32_t* d_ring, int ring, const int32_t* d_span, int32_t* d_pages, int width,

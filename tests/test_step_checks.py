@@ -85,6 +85,18 @@ def test_norm_refusals():
     refusals(codes, (dict(scale=None), dict(scale=P + 2)))
 
 
+def test_norm_outputs_over_each_other_are_refused():
+    def values(x=P, xs=20, r=2 * P, rs=20, rows=3, total=3 * P, ss=20, out=4 * P, stride=20):
+        return call("vdt_add_rms_norm", x, xs, r, rs, None, rows, 20, 1e-6, 2, total, ss, out, stride, None)
+
+    def codes(x=P, xs=20, r=2 * P, rs=20, rows=3, total=3 * P, ss=20):
+        return call("vdt_add_rms_norm_int8", x, xs, r, rs, None, rows, 20, 1e-6, 2, total, ss, 4 * P, 20, 5 * P, None)
+
+    for go in (values, codes):
+        refusals(go, (dict(total=P, ss=24), dict(total=2 * P, rs=24), dict(x=2 * P, total=2 * P, xs=24)))
+    refusals(values, (dict(out=3 * P), dict(out=3 * P, rows=1), dict(out=P, stride=24), dict(out=2 * P, stride=24), dict(r=None, out=P, stride=24)))
+
+
 def plan(**over):
     a = dict(ring=P, n=8, span=P, pages=P, width=3, held=P, new=P, seqs=2, page=16, total=5, kept=P, starts=P, positions=P, slots=P, out=P, scratch=P,
              size=1 << 20)
@@ -110,6 +122,12 @@ def test_page_table_refusals():
     refusals(free, (dict(done=None),))
     need = call("vdt_plan_pages_scratch_bytes", 2)
     assert need > 0 and plan(size=need - 1) == CAPACITY and call("vdt_plan_pages_scratch_bytes", -1) == 0
+
+
+def test_page_tables_past_32_bits_count_are_refused():
+    for go in (plan, free):
+        for over in (dict(width=(1 << 30) + 1), dict(n=(1 << 30) + 1), dict(width=(1 << 31) - 1), dict(n=(1 << 31) - 1)):
+            assert go(**over) == UNSUPPORTED, over
 
 
 def test_sample_refusals():

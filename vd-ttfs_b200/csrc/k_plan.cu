@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(THREADS) k_free(FreeParams p) {
         __syncthreads();
         at = (int)threadIdx.x < many ? counts[threadIdx.x] : 0;
         scan2<THREADS>(at, none, all);
-        if ((int)threadIdx.x < many) counts[threadIdx.x] = clamp32(before + at);
+        if ((int)threadIdx.x < many) counts[threadIdx.x] = (int)min(before + at, (long long)p.size);
         __syncthreads();
         for (int i = warp; i < many; i += kWarps) {
             int to = counts[i];

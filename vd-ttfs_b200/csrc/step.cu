@@ -12,6 +12,7 @@ namespace {
 constexpr int kMostSeqs = 65535;
 constexpr long long kMostRows = 1 << 30;
 constexpr int kMostCols = 1 << 30;         // kernels step past the last by up to a few thousand, in 32 bits
+constexpr int kMostPages = 1 << 30;        // likewise, by a warp's
 
 #define STEP_REQUIRE(cond, text) \
     do {                         \
@@ -49,6 +50,10 @@ int check_product(const uint8_t* d_w, int64_t w_stride, const uint8_t* d_w_scale
     return VDT_OK;
 }
 
+// in place: the same rows, not others that begin there
+bool same_rows(const void* a, int64_t a_stride, const void* b, int64_t b_stride, int64_t rows) {
+    return a != b || !a || rows <= 1 || a_stride == b_stride;
+}
 int check_norm(const void* d_x, int64_t x_stride, const void* d_residual, int64_t residual_stride, const void* d_weight, int64_t rows, int cols,
                float eps, int type, const void* d_sum, int64_t sum_stride) {
     STEP_REQUIRE(type_ok(type), "type");
@@ -58,6 +63,8 @@ int check_norm(const void* d_x, int64_t x_stride, const void* d_residual, int64_
     if (!rows) return VDT_OK;
     STEP_REQUIRE(d_x && (!d_residual || d_sum), "NULL buffer");
     STEP_REQUIRE(rows == 1 || (x_stride >= cols && (!d_residual || (residual_stride >= cols && sum_stride >= cols))), "a stride below cols");
+    STEP_REQUIRE(!d_residual || (same_rows(d_sum, sum_stride, d_x, x_stride, rows) && same_rows(d_sum, sum_stride, d_residual, residual_stride, rows)),
+                 "a sum in place has the strides of what it replaces");
     const int e = type_size(type);
     STEP_REQUIRE(aligned(d_x, e) && aligned(d_residual, e) && aligned(d_weight, e) && aligned(d_sum, e), "alignment");
     return VDT_OK;
@@ -76,6 +83,7 @@ NormParams norm_params(const void* d_x, int64_t x_stride, const void* d_residual
 int check_tables(const void* d_ring, int ring, const void* d_span, const void* d_pages, int width, const void* d_held, int seqs, int page) {
     STEP_REQUIRE(seqs >= 0 && width >= 0 && ring >= 0 && page > 0, "negative size");
     if (seqs > kMostSeqs) return api_fail(VDT_ERR_UNSUPPORTED, "more than 65535 sequences");
+    if (width > kMostPages || ring > kMostPages) return api_fail(VDT_ERR_UNSUPPORTED, "more than 2^30 pages in the ring or a table's row");
     STEP_REQUIRE(d_span && (d_ring || !ring) && (!seqs || (d_held && (d_pages || !width))), "NULL buffer");
     STEP_REQUIRE(aligned(d_ring, 4) && aligned(d_span, 4) && aligned(d_pages, 4) && aligned(d_held, 4), "alignment");
     return VDT_OK;
@@ -163,6 +171,9 @@ extern "C" int vdt_add_rms_norm(const void* d_x, int64_t x_stride, const void* d
     if (int s = check_norm(d_x, x_stride, d_residual, residual_stride, d_weight, rows, cols, eps, type, d_sum, sum_stride)) return s;
     if (!rows) return VDT_OK;
     STEP_REQUIRE(d_out && (out_stride >= cols || rows == 1) && aligned(d_out, type_size(type)), "output");
+    STEP_REQUIRE(!d_residual || d_out != d_sum, "the output over the sum");
+    STEP_REQUIRE(same_rows(d_out, out_stride, d_x, x_stride, rows) && same_rows(d_out, out_stride, d_residual, residual_stride, rows),
+                 "an output in place has the strides of what it replaces");
     if (int s = api_check_buffers(-1, {d_x, d_residual, d_weight, d_sum, d_out})) return s;
     NormParams p = norm_params(d_x, x_stride, d_residual, residual_stride, d_weight, rows, cols, eps, type, d_sum, sum_stride, out_stride);
     p.out = d_out;
