@@ -673,7 +673,6 @@ struct Row {
                     if (!here) v = 0;
                     if (d < (float)kBins) sums[0] += v;              // (not -inf)
                     if (d < since) sums[1] += v;
-                    if (d < upto) sums[2] += v;
                 }
                 mine |= (unsigned)(here && d < upto && d >= first_step) << j;
             }
@@ -688,6 +687,19 @@ struct Row {
                 have += __popc(who);
             }
         });
+        if constexpr (WEIGHTS) {
+            // up to `to`: the ones before `from` and the chosen, where these do not begin at the largest
+            if (first_of) sums[2] = sums[1];
+            __syncwarp();
+            if (have <= kChosen) {
+                for (unsigned k = lane; k < have; k += 32) sums[2] += w.weight(value_at(wk.chosen[threadIdx.x / 32][k]));
+            } else {
+                each([&](float x, int i) {
+                    const float d = w.depth(x);
+                    if (d < upto && d >= first_step && (!PART || before_end(x, i))) sums[2] += w.weight(x);
+                });
+            }
+        }
         if (lane == 0) sh.chosen[threadIdx.x / 32] = have;
         u64 said[4] = {0, 0, 0, 0}, many[1] = {lane == 0 ? have + (have > kChosen ? 1ull << 40 : 0) : 0};
         if constexpr (WEIGHTS) {
