@@ -46,6 +46,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048, kRoom = kBins + 4, kList = 1024, kChosen = 512;
 constexpr float kSteps = 44.0f;              // of an octave; kBins of them are 46.5 octaves, below which weights round to 0
 constexpr int kMostBits = 44, kBoundBits = 40;
+constexpr int kMostPart = 1 << 17;           // tokens of a CTA
 
 using u64 = unsigned long long;
 
@@ -146,8 +147,9 @@ struct Weigher {
     float top, bottom;      // the largest then, and a value without weight (-inf is not weighed)
     float slope, start;     // steps of the histogram below the largest: start + slope x
     double parts;           // 32 log2(e) / T
-    const double* roots;    // kRoots in shared memory
+    const double* roots;    // kRoots times 2^bits, in shared memory
     int bits;
+    static __device__ __forceinline__ int bits_of(int vocab) { return min(kMostBits, 62 - (32 - __clz(vocab - 1))); }
     __device__ __forceinline__ float value(float x) const {
         return alone ? (x == largest ? 0.0f : -INFINITY) : (shift ? x - largest : x) * factor;
     }
@@ -168,7 +170,7 @@ struct Weigher {
         slope = (float)(-(double)kSteps * each);
         // a little above, so that the largest is not below 0
         start = (float)((double)kSteps * each * (double)top) + (float)(shift || alone ? 0.0 : far) * 0x1p-22f;
-        bits = min(kMostBits, 62 - (32 - __clz(vocab - 1)));
+        bits = bits_of(vocab);
     }
     // the logarithm of a token's probability, from the kept weights' sum (1 for the largest)
     __device__ __forceinline__ double log_sum(u64 sum) const { return log((double)sum * __hiloint2double((1023 - bits) << 20, 0)); }
@@ -180,26 +182,28 @@ struct Weigher {
     static __device__ __forceinline__ int step(float depth) {
         return __float_as_int(__fadd_rd(fminf(depth, (float)kBins), 8388608.0f)) & (2 * kBins - 1);
     }
-    // 2^bits exp((x - top) / T) to the nearest whole number: the next 32nd of an octave from
-    // a table, its exponent moved by the whole octaves, and the rest, at most a 64th, by the
-    // interpolating polynomial of degree 4 at Chebyshev's points, off by at most 2^-43.  (Without
-    // the table degree 8 is wanted: 14 operations in 64 bits a token, of which the SM does
-    // 1.6 a cycle for a warp, and not 9.)  3/2 2^52 added leaves the nearest whole number in the
-    // low bits; no branches, so that the chains of several tokens run side by side.
-    __device__ __forceinline__ u64 weight(float x) const {
+    // 2^bits exp((x - top) / T) to the nearest whole number, and 2^52: the next 32nd of an
+    // octave from a table, its exponent moved by the whole octaves, and the rest, at most a
+    // 64th, by the interpolating polynomial of degree 4 at Chebyshev's points, off by at most
+    // 2^-43.  (Without the table degree 8 is wanted: 14 operations in 64 bits a token, of
+    // which the SM does 1.6 a cycle for a warp, and not 9.)  3/2 2^52 added leaves the nearest
+    // whole number in the low bits; no branches, so that the chains of several tokens run side by side.
+    __device__ __forceinline__ double raised(float x) const {
         constexpr double kRound = 6755399441055744.0;
         const double d = (double)fmaxf(x, bottom) - (double)top;
         const double z = fma(d, parts, kRound), f = fma(d, parts, kRound - z);
-        const int whole = __double2loint(z);
+        const unsigned whole = (unsigned)__double2loint(z);
         const double root = roots[whole & 31];
         double y = 0x1.3b2b18fa66654p-27;
         y = fma(y, f, 0x1.c6b167e61eadap-20);
         y = fma(y, f, 0x1.ebfbdff817570p-13);
         y = fma(y, f, 0x1.62e42fef6d03fp-6);
         y = fma(y, f, 1.0);
-        y = fma(y, __hiloint2double(__double2hiint(root) + ((bits + (whole >> 5)) << 20), __double2loint(root)), 4503599627370496.0);
-        return (u64)__double_as_longlong(y) & 0xfffffffffffffull;
+        return fma(y, __hiloint2double((int)((unsigned)__double2hiint(root) + ((whole & ~31u) << 15)), __double2loint(root)), 4503599627370496.0);
     }
+    // as 64-bit floating point, sums of which are exact up to 2^53: 2^9 of the largest
+    __device__ __forceinline__ double weight_f(float x) const { return raised(x) - 4503599627370496.0; }
+    __device__ __forceinline__ u64 weight(float x) const { return (u64)__double_as_longlong(raised(x)) & 0xfffffffffffffull; }
 };
 
 // A histogram, weights in three parts of 15 bits (a CTA's sums of each stay below
@@ -603,6 +607,7 @@ struct Row {
         for (int i = 0; i < kPer; ++i) {
             const int b = threadIdx.x * per + i;
             if (i >= per || b >= mine) continue;
+#pragma unroll 4
             for (int r = 0; r < ranks; ++r) {
                 const Work* const o = cluster.map_shared_rank(&wk, r);
                 c[i] += o->count[0][from + b];
@@ -638,9 +643,12 @@ struct Row {
         return r;
     }
 
-    // a token into the first CTA's list, from a lane by itself
+    // a token into the first CTA's list, from some of a warp's lanes: one of them counts for all
     __device__ __forceinline__ void put(u64 place) {
-        const unsigned at = atomicAdd(cluster.map_shared_rank(&sh.listed, 0), 1u);
+        const unsigned who = __activemask(), below = __popc(who & ((1u << threadIdx.x % 32) - 1));
+        unsigned at = 0;
+        if (!below) at = atomicAdd(cluster.map_shared_rank(&sh.listed, 0), (unsigned)__popc(who));
+        at = __shfl_sync(who, at, __ffs(who) - 1) + below;
         if (at < kList) cluster.map_shared_rank(sh.list, 0)[at] = place;
     }
     // its length, for the first CTA alone: the others may go on after that one has ended
@@ -653,7 +661,8 @@ struct Row {
     template <bool PART, bool WEIGHTS>
     __device__ __forceinline__ void look(int from, int to, int first_of, u64 (&sums)[3], bool* fits, unsigned* before) {
         unsigned have = 0;
-        sums[0] = sums[1] = sums[2] = 0;
+        static_assert(kMostPart / kThreads + N <= 1 << (53 - kMostBits), "a thread's sums are exact in 64-bit floating point");
+        double all = 0.0, head = 0.0;
         const float since = (float)from, upto = (float)(to + 1), first_step = (float)first_of;
         const int lane = threadIdx.x % 32;
         each_vector([&](const float* x, int i) {
@@ -669,10 +678,9 @@ struct Row {
                 const float d = w.depth(x[j]);
                 const bool here = !PART || (in >> j & 1);
                 if (WEIGHTS) {
-                    u64 v = w.weight(x[j]);
-                    if (!here) v = 0;
-                    if (d < (float)kBins) sums[0] += v;              // (not -inf)
-                    if (d < since) sums[1] += v;
+                    const double v = w.weight_f(x[j]);
+                    if (here && d < (float)kBins) all += v;          // (not -inf)
+                    if (here && d < since) head += v;
                 }
                 mine |= (unsigned)(here && d < upto && d >= first_step) << j;
             }
@@ -687,6 +695,9 @@ struct Row {
                 have += __popc(who);
             }
         });
+        sums[0] = (u64)all;
+        sums[1] = (u64)head;
+        sums[2] = 0;
         if constexpr (WEIGHTS) {
             // up to `to`: the ones before `from` and the chosen, where these do not begin at the largest
             if (first_of) sums[2] = sums[1];
@@ -714,14 +725,14 @@ struct Row {
         said[3] = many[0];
         const auto& slots = say(said);
         sums[0] = sums[1] = sums[2] = 0;
-        u64 all = 0;
+        u64 listed = 0;
         for (int r = 0; r < ranks; ++r) {
-            if (r == rank) *before = (unsigned)all;
+            if (r == rank) *before = (unsigned)listed;
 #pragma unroll
             for (int k = 0; k < 3; ++k) sums[k] += slots[r][k];
-            all += slots[r][3];
+            listed += slots[r][3];
         }
-        *fits = all >> 40 == 0;
+        *fits = listed >> 40 == 0;
     }
     // What `look` listed, at most kList tokens, into the first CTA's list
     __device__ __forceinline__ void send(bool fits, int from, int to, unsigned before) {
@@ -741,15 +752,16 @@ struct Row {
 
     // Each warp's sum of the weights up to `end` of at least `least`, into `kept`
     __device__ __forceinline__ void sum_kept(u64 least) {
-        u64 mine = 0;
+        const double least_f = (double)least;
+        double sum = 0.0;
         each_vector([&](const float* x, int i) {
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const u64 o = w.weight(x[j]);
-                if (before_end(x[j], i + j) && o >= least) mine += o;
+                const double o = w.weight_f(x[j]);
+                if (before_end(x[j], i + j) && o >= least_f) sum += o;
             }
         });
-        mine = warp_sum(mine);
+        const u64 mine = warp_sum((u64)sum);
         __syncthreads();
         if (threadIdx.x % 32 == 0) sh.kept[threadIdx.x / 32] = mine;
         __syncthreads();
@@ -868,7 +880,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
     const bool greedy = temperature == 0.0f;
     if (ranks > 1) cluster.barrier_arrive();
 
-    if (threadIdx.x < 32) sh.roots[threadIdx.x] = kRoots[threadIdx.x];
+    if (threadIdx.x < 32) sh.roots[threadIdx.x] = kRoots[threadIdx.x] * (double)(1ull << Weigher::bits_of(p.vocab));
     // the largest value; NaN orders above the others
     Top<T> most;
     s.each_load([&](const Eight<T>& v) { most.add(v); });
@@ -996,10 +1008,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
             listed = true;
         }
         if (weights && !least) {
-            // what the steps' tokens add to each warp's part
+            // what the steps' tokens add to each warp's part, which are its own
+            u64 mine = 0;
             s.each_chosen(fits, at.from, at.to, [&](float x, u64 place) {
-                if (place <= s.end) atomicAdd(&sh.kept[((int)(uint32_t)place - first) / seg], w.weight(x));
+                if (place <= s.end) mine += w.weight(x);
             });
+            mine = warp_sum(mine);
+            if (threadIdx.x % 32 == 0) sh.kept[threadIdx.x / 32] += mine;
             __syncthreads();
             summed = true;
         }
@@ -1115,7 +1130,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(SampleParams p, int part
 // top-p 41 and 47, 8 x 50001 f32 top-p 34 and 59; 16 x 131072 bf16 top-k 23.7 and 21.4.
 template <typename T>
 cudaError_t sample_launch(const SampleParams& p, cudaStream_t s) {
-    constexpr int N = Row<T>::N, kMostPart = 1 << 17, kLeastPart = 4096;
+    constexpr int N = Row<T>::N, kLeastPart = 4096;
     // rows that are not on whole vectors begin up to N - 1 values into their first ones
     const bool whole = aligned(p.logits, N * sizeof(T)) && (p.rows == 1 || p.stride % N == 0);
     const int places = p.vocab + (whole ? 0 : N - 1);
