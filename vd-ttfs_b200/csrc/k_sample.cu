@@ -27,8 +27,8 @@
 // Bound by instructions, some 100 a token with top_p in three passes, and by 64
 // registers a thread, with which two CTAs share an SM so that one computes while
 // the other waits for a barrier (one CTA with 128: each row is faster, all of them
-// slower).  us, replayed: 250 x 100003 f32, top_p, 155, against 15 for reading the
-// logits once; 64 x 131072 bf16, mixed parameters, 66; one row of 32768 17.4, which
+// slower).  us, replayed: 250 x 100003 f32, top_p, 137, against 15 for reading the
+// logits once; 64 x 131072 bf16, mixed parameters, 62; one row of 32768 16.5, which
 // are some ten exchanges in the cluster and code that runs once.
 #include <cooperative_groups.h>
 
