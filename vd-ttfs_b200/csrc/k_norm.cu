@@ -16,6 +16,8 @@
 namespace vdt {
 namespace {
 
+constexpr int kMostHeld = 2048;              // vectors of a row that its threads hold at most
+
 // THREADS a row, by its length alone, so that a row's bits do not hang on the
 // rows beside it; nor on where it lies: rows that are not on 16 bytes (WIDE
 // false) are read value by value, by the same threads in the same order.  A row
@@ -23,6 +25,7 @@ namespace {
 // ones the sum is read (or made) a second time.
 template <typename T, int HELD, int THREADS, bool CODES, bool WIDE>
 __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) k_add_rms_norm(NormParams p) {
+    constexpr bool kLong = HELD * THREADS == kMostHeld;      // the others' rows are all held
     constexpr int N = Vec16<T>::N, kWarps = THREADS / 32, kRows = THREADS < 128 ? 128 / THREADS : 1;
     __shared__ float squares[kWarps], largest[kWarps];
     const long long r = (long long)blockIdx.x * kRows + threadIdx.x / THREADS;
@@ -64,8 +67,8 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) k_add_rms_norm(
 #pragma unroll
         for (int j = 0; j < N; ++j) f[j] *= g[j];
     };
-    // the sum's values, as it holds them; stored on the way, which may be over x or the residual
-    auto take = [&](int at, Vec16<T> v, const Vec16<T>& o) {
+    // the sum's values, as it holds them, their squares added to `into`; stored on the way, which may be over x or the residual
+    auto take = [&](int at, Vec16<T> v, const Vec16<T>& o, float& into) {
         float f[N];
         v.get(f);
         if (residual) {
@@ -78,7 +81,7 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) k_add_rms_norm(
             put(sum, at, v);
         }
 #pragma unroll
-        for (int j = 0; j < N; ++j) square = fmaf(f[j], f[j], square);
+        for (int j = 0; j < N; ++j) into = fmaf(f[j], f[j], into);
         if constexpr (CODES) {
             times(at, f);
 #pragma unroll
@@ -96,10 +99,20 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) k_add_rms_norm(
     }
 #pragma unroll
     for (int i = 0; i < HELD; ++i)
-        if (thread + i * THREADS < vecs) held[i] = take(thread + i * THREADS, held[i], other[i]);
-    for (int at = thread + HELD * THREADS; at < vecs; at += THREADS) {
-        const Vec16<T> v = get(x, at);
-        take(at, v, residual ? get(residual, at) : v);
+        if (thread + i * THREADS < vecs) held[i] = take(thread + i * THREADS, held[i], other[i], square);
+    // Of the rest a vector at a time, what an addition rounds off brought into the next one: a sum is off
+    // by two roundings however long the row (added one by one, a row of 2^24 equal values was off by
+    // 10^4 of them).  An infinite sum stays so.
+    if constexpr (kLong) {
+        float excess = 0.0f;
+        for (int at = thread + HELD * THREADS; at < vecs; at += THREADS) {
+            const Vec16<T> v = get(x, at);
+            float part = 0.0f;
+            take(at, v, residual ? get(residual, at) : v, part);
+            const float add = part - excess, to = square + add;
+            excess = to == INFINITY ? 0.0f : (to - square) - add;
+            square = to;
+        }
     }
     // values behind the last whole vector, one for each of the first threads
     const int rest = vecs * N + thread;
@@ -157,7 +170,8 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) k_add_rms_norm(
 #pragma unroll
         for (int i = 0; i < HELD; ++i)
             if (thread + i * THREADS < vecs) store(held[i], thread + i * THREADS);
-        for (int at = thread + HELD * THREADS; at < vecs; at += THREADS) store(get(again, at), at);
+        if constexpr (kLong)
+            for (int at = thread + HELD * THREADS; at < vecs; at += THREADS) store(get(again, at), at);
         if (rest < cols) out[rest] = (int8_t)code_of(tail, coder.scale);
     } else {
         T* const out = static_cast<T*>(p.out) + r * p.out_stride;
@@ -173,7 +187,8 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) k_add_rms_norm(
 #pragma unroll
         for (int i = 0; i < HELD; ++i)
             if (thread + i * THREADS < vecs) store(held[i], thread + i * THREADS);
-        for (int at = thread + HELD * THREADS; at < vecs; at += THREADS) store(get(again, at), at);
+        if constexpr (kLong)
+            for (int at = thread + HELD * THREADS; at < vecs; at += THREADS) store(get(again, at), at);
         if (rest < cols) out[rest] = from_f32<T>(tail * norm);
     }
 }
