@@ -92,3 +92,55 @@ def test_norm_in_place_at_every_length(S, kind, cols):
     assert torch.equal(S.add_rms_norm(a, None, w, out=a)[0], alone)
     a = x.clone()
     assert torch.equal(S.add_rms_norm(a, a, w, sum_out=a)[0], S.add_rms_norm(x, x, w)[0])
+
+
+# ----------------------------------------- every way through the 4-bit product --
+def check_product(S, rows, inner, outer, kind, bias=True):
+    """Against the 64-bit product of the values that codes and scales stand for; sums as in test_gpu_step.py: inner / 64 + 2
+    steps of 2^-23 of the terms' magnitudes, and the output's rounding."""
+    g = torch.Generator(device="cuda").manual_seed(rows + inner + outer)
+    x = torch.randn(rows, inner, generator=g, device="cuda").to(kind)
+    x *= (1 + torch.arange(rows, device="cuda") % 5).to(kind)[:, None]      # rows' and channels' scales differ, so that a wrong one shows
+    m = torch.randn(outer, inner, generator=g, device="cuda") * 2.0 ** (torch.arange(outer, device="cuda") % 7)[:, None]
+    b = torch.randn(outer, generator=g, device="cuda") if bias else None
+    w, ws = S.quantize_fp4(m)
+    codes, scale = S.quantize_fp4(x)
+    a, v = S.fp4_values(codes, scale, inner).double(), S.fp4_values(w, ws, inner).double()
+    want, size = a @ v.T, a.abs() @ v.abs().T
+    if bias:
+        want, size = want + b.double(), size + b.double().abs()
+    room = (inner / 64 + 2) * 2.0 ** -23 * size + 1e-37
+    # 16-bit floating point ends at 65504, and rounds what is 65520 and more, half a step of 32 past it, to infinity: the
+    # sums of 4100 terms deviate by up to 5 x 64 x 4100^1/2 = 20490, and some of 33000 of them pass that
+    past = 65520.0 if kind == torch.float16 else INF
+    for y in (S.fp4_linear(x, w, ws, b), S.fp4_matmul(codes, scale, w, ws, b, out_dtype=kind)):
+        assert y.dtype == kind
+        over = torch.isinf(y)
+        assert (want.abs() + room)[over].ge(past).all() and torch.equal(y[over].sign().double(), want[over].sign())
+        assert (want.abs() - room)[~over].lt(past).all()
+        off = torch.where(over, 0.0, (y.double() - want).abs()) - U[kind] * want.abs() - room
+        assert (off <= 0).all(), (off.amax(1).argmax().item(), off.amax(0).argmax().item())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,inner,outer", [
+    # tiles of 192 channels, which begin in the middle of a tile of scales and span two: one a CTA, two, three; 3, 6 and 2 steps
+    (200, 700, 9601), (1000, 1300, 7001), (1000, 300, 10501),
+    # of 128: one, two and three a CTA, the last past the ring's five stages
+    (777, 1001, 1531), (1000, 1300, 4701), (51100, 300, 127),
+    # of 64: three
+    (51100, 300, 50),
+    # of 256, whose sums fit once: two and three, six steps in four stages
+    (1000, 1300, 9301), (1000, 1300, 13901)])
+def test_fp4_tiles_of_every_width(S, kind, rows, inner, outer):
+    check_product(S, rows, inner, outer, kind)
+    if kind is torch.bfloat16:
+        check_product(S, rows, inner, outer, kind, bias=False)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [33, 47, 63, 64])
+def test_fp4_tokens_as_columns(S, kind, rows):
+    """33 to 64 tokens as the products' columns: a long inner dimension, shared by a cluster."""
+    check_product(S, rows, 2049, 50, kind)
+    check_product(S, rows, 4100, 1001, kind, bias=False)
