@@ -224,7 +224,7 @@ cudaError_t pack_launch(const void* x, long long rows, int cols, long long x_str
 // --------------------------------------------------------------------- values
 __device__ __forceinline__ float value_of(uint32_t code, float scale) {
     const uint32_t m = code & 7;
-    const float v = m < 2 ? 0.5f * m : m < 4 ? 0.5f * m : m < 6 ? (float)(m - 2) : 2.0f * (m - 4);
+    const float v = m < 4 ? 0.5f * m : m < 6 ? (float)(m - 2) : 2.0f * (m - 4);
     return (code & 8 ? -v : v) * scale;
 }
 template <typename T>
@@ -270,7 +270,7 @@ constexpr int kStepBytes = kFp4Step / 2;             // 128: a swizzled row of a
 constexpr int kStepScales = 2 * kScaleTile;          // a stage's scales for 128 rows
 
 // ----------------------------------------------------------------- few rows
-// The channels are the products' 128 rows and the tokens their columns, so a
+// The channels are the products' 128 rows and the tokens, at most NT, their columns, so a
 // tile holds 128 channels whatever the number of tokens, and what bounds it is the
 // weights' way from memory.  A cluster of CTAs shares a tile's inner dimension, so
 // that all SMs load at once and every CTA's stages are on their way from the
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarp
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const cg::cluster_group cluster = cg::this_cluster();
     const int split = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int tile = blockIdx.x / split, row0 = blockIdx.y * NT, rows = (int)min((long long)NT, p.rows - row0);
+    const int tile = blockIdx.x / split, rows = (int)p.rows;
     const int steps = (p.inner + kFp4Step - 1) / kFp4Step;
     const int first = (int)((long long)steps * rank / split), last = (int)((long long)steps * (rank + 1) / split);
     if (threadIdx.x == 0) {
@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarp
                     load_w(s);
                 }
                 if constexpr (!kOwn) {
-                    tile_load(at + 128 * kStepBytes, &map_a, s * kStepBytes, row0, bar);
-                    bulk_load(at + Shape::kCodes + kStepScales, p.a_scale + ((long long)(row0 / kScaleRows) * steps + s) * kStepScales, kStepScales, bar);
+                    tile_load(at + 128 * kStepBytes, &map_a, s * kStepBytes, 0, bar);
+                    bulk_load(at + Shape::kCodes + kStepScales, p.a_scale + (long long)s * kStepScales, kStepScales, bar);
                 }
             }
             // every load has landed before the CTA ends: the last ones' stages
@@ -367,8 +367,6 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarp
     } else if (warp == 1) {
         const uint32_t sums = __shfl_sync(0xffffffffu, tmem, 0);
         const uint64_t w = tile_desc(stages), a = tile_desc(stages + 128 * kStepBytes), f = scale_desc(stages + Shape::kCodes);
-        // codes that are loaded lie in their scale tile where their rows do, a column for 32
-        const uint32_t shift = kOwn ? 0 : row0 % kScaleRows / 32;
         const bool one = elected();
         for (int s = first; s < last; ++s) {
             const int slot = (s - first) % kFewStages;
@@ -384,7 +382,7 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarp
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     mma_fp4(sums, w + (slot * Shape::kStage + k * 32) / 16, a + (slot * Shape::kStage + k * 32) / 16, fp4_shape(NT, k % 2), sc + k / 2 * 8,
-                            sc + k / 2 * 8 + 4 + shift, s > first || k > 0);
+                            sc + k / 2 * 8 + 4, s > first || k > 0);
                 mma_commit(shared_address(&bars.empty[slot]));
             }
         }
@@ -396,7 +394,7 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarp
         constexpr int kGroup = NT * 8, kGroups = 32 * kRoundWarps / kGroup;
         static_assert(kGroups >= 1, "a thread a block");
         const int t = (threadIdx.x - 64) % kGroup, block = t % 8, row = t / 8;
-        const X* const x = static_cast<const X*>(p.x) + (long long)(row0 + row) * p.x_stride + block * kBlock;
+        const X* const x = static_cast<const X*>(p.x) + row * p.x_stride + block * kBlock;
         const uintptr_t off = reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(rows > 1 ? p.x_stride * (long long)sizeof(X) : 0);
         uint32_t raw[8 * sizeof(X)];
         auto load = [&](int s) {
@@ -473,7 +471,7 @@ __global__ void __launch_bounds__(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarp
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (col + j < p.cols) y[j] += p.bias[col + j];
-        const long long at = (long long)(row0 + row) * p.out_stride + col;
+        const long long at = row * p.out_stride + col;
         auto put = [&](auto* out) {
             using T = std::remove_pointer_t<decltype(out)>;
             if (wide && col + 4 <= p.cols) {
@@ -504,6 +502,7 @@ cudaError_t few_launch(const Fp4Params& p, bool after, cudaStream_t s) {
     using Shape = FewShape<NT>;
     CUtensorMap w, a;
     const int bytes = (p.inner + 1) / 2;
+    if (p.rows > NT) return cudaErrorInvalidValue;
     if (!byte_rows_map(&w, p.w, p.cols, bytes, p.w_stride, kStepBytes, 128)) return cudaErrorInvalidValue;
     if (std::is_void_v<X>) {
         if (!byte_rows_map(&a, p.a, p.rows, bytes, p.a_stride, kStepBytes, NT)) return cudaErrorInvalidValue;
@@ -514,7 +513,7 @@ cudaError_t few_launch(const Fp4Params& p, bool after, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const int split = few_split(p.cols, p.inner, NT);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((p.cols + 127) / 128 * split), (unsigned)((p.rows + NT - 1) / NT));
+    cfg.gridDim = dim3((unsigned)((p.cols + 127) / 128 * split));
     cfg.blockDim = dim3(std::is_void_v<X> ? 192 : 64 + 32 * kRoundWarps);
     cfg.dynamicSmemBytes = Shape::kBytes;
     cfg.stream = s;
