@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_step import INF, KINDS, U, normal
+from test_gpu_step import INF, KINDS, U, check_sample, normal, sample_definition, uniform
 
 pytestmark = pytest.mark.gpu
 
@@ -144,3 +144,52 @@ def test_fp4_tokens_as_columns(S, kind, rows):
     """33 to 64 tokens as the products' columns: a long inner dimension, shared by a cluster."""
     check_product(S, rows, 2049, 50, kind)
     check_product(S, rows, 4100, 1001, kind, bias=False)
+
+
+# ----------------------------------------------------- vocabularies of every size --
+def equal_rows(x):
+    """Rows in which one step of a histogram has every token, and one of two values."""
+    x[0] = 0.25
+    x[1] = -7.0
+    x[1, ::2] = -7.5
+    return x
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,vocab", [(2, 262144), (2, 262145), (3, 524287), (3, 524288)])
+def test_sample_of_the_widest_vocabularies(S, kind, rows, vocab):
+    """Up to 2^18 tokens weights have 44 bits, above it 43."""
+    x = equal_rows((normal(vocab, rows + 2, vocab) * 3).to(kind))
+    for t, k, p, least in ((1.0, 0, 1.0, 0.0), (0.7, 40, 0.9, 0.0), (1.1, 0, 0.95, 0.0), (0.9, 5000, 0.9, 0.0), (1.0, vocab - 1, 0.5, 0.01), (0.0, 0, 1.0, 0.0)):
+        check_sample(S, x, uniform(vocab, rows + 2), t, k, p, least)
+
+
+def test_sample_of_a_full_part_a_cta(S):
+    """So many rows that each has one CTA, and as many tokens as it counts: 2^17, from rows on 32 bytes and off them; one
+    more, and two CTAs share a row."""
+    rows = 150
+    for vocab, off in ((1 << 17, 0), (1 << 17, 3), ((1 << 17) + 1, 0), ((1 << 17) + 1, 5)):
+        store = (normal(vocab + off, rows, vocab + 8) * 2).cuda()
+        x = store.flatten()[off: off + rows * vocab].view(rows, vocab)
+        equal_rows(x)
+        u = uniform(off, rows)
+        some = [0, 1, *range(2, rows, 7)]
+        host = x[some].cpu().double().numpy()
+        for args in ((1.0, 0, 0.9, 0.0), (1.0, 2000, 0.8, 0.0), (1.0, 0, 1.0, 0.0)):
+            tokens, logp = S.sample(x, u.cuda(), *args)
+            for i, r in enumerate(some):
+                token, log = sample_definition(host[i], float(u[r]), args[0], args[1], float(np.float32(args[2])), args[3])
+                assert int(tokens[r]) == token and abs(float(logp[r]) - log) <= 2.0 ** -24 * abs(log) + 2.0 ** -34, (r, args)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,vocab", [(2, 40000), (2, 1200), (160, 3000)])
+def test_sample_of_fewer_weights_than_top_k(S, kind, rows, vocab):
+    """No token is the k-th with any weight: the histogram that was made for top_k serves for top_p, counted once."""
+    x = torch.full((rows, vocab), -INF)
+    x[:, 5::7] = -torch.arange(len(range(5, vocab, 7))) % 61 * 0.1
+    x[:, 1::7] = -3000.0
+    x = x.to(kind)
+    for k in (1100, vocab // 2, vocab - 1):
+        for p in (0.3, 0.9, 0.999):
+            check_sample(S, x, uniform(k, rows), 1.0, k, p, 0.0)
