@@ -634,7 +634,8 @@ int vdt_free_pages(int32_t* d_ring, int ring, const int32_t* d_span, const int32
    the number beside.  d_logp (may be NULL): the logarithm of the probability
    that the token was drawn with.  Weights are whole multiples of 2^-44 of the
    largest (2^-43 for vocabularies above 2^18) and their sums exact, so calls on the
-   same inputs give the same tokens.  A row with a NaN, without a finite logit or +inf, or
+   same inputs give the same tokens; rounding moves a border by up to as many such
+   steps as there are kept tokens.  A row with a NaN, without a finite logit or +inf, or
    with a parameter or u that is NaN or out of range gives token -1 and NaN.
    vocab up to 524288. */
 int vdt_sample(const void* d_logits, int type, int64_t rows, int vocab, int64_t stride, const float* d_u,

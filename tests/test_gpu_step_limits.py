@@ -193,3 +193,17 @@ def test_sample_of_fewer_weights_than_top_k(S, kind, rows, vocab):
     for k in (1100, vocab // 2, vocab - 1):
         for p in (0.3, 0.9, 0.999):
             check_sample(S, x, uniform(k, rows), 1.0, k, p, 0.0)
+
+
+def test_sample_tails_below_a_step(S):
+    """Weights are rounded to multiples of 2^-44 of the largest (2^-43 above 2^18 tokens), so n of them are off by up to n
+    halves of that; the polynomial by 2^-43 of each.  Here all but one token have 0.44 of such a step, and count
+    nothing: the largest error there is but for the last bits."""
+    for vocab, bits in ((1 << 17, 44), (1 << 18, 44), (1 << 19, 43)):
+        x = torch.full((1, vocab), float(np.float32(-(bits + 1.2) * math.log(2))))
+        x[0, 9] = 0
+        for rows in (1, 160):
+            tokens, logp = S.sample(x.cuda().repeat(rows, 1), torch.full((rows,), 0.5).cuda())
+            _, want = sample_definition(x[0].double().numpy(), 0.5, 1.0, 0, 1.0, 0.0)
+            assert (tokens == 9).all() and ((logp.cpu().double() - want).abs() <= vocab * 2.0 ** -(bits + 1) + 2.0 ** -42).all()
+            assert abs(want) > 0.8 * vocab * 2.0 ** -(bits + 1)

@@ -9,8 +9,11 @@
 // kept is everything up to one last token: it is found by its place, without
 // sorting the row.  A token hangs on comparisons of sums, so the weights are
 // whole numbers, w * 2^44 (2^43 for vocabularies above 2^18), from a table of roots
-// and a polynomial in 64 bits: sums are exact, the same in any order, and an answer differs from
-// the real numbers' one where u comes within some 2^-34 of a border.
+// and a polynomial in 64 bits: sums are exact, the same in any order.  A weight is rounded
+// by up to half a step, the sum of n of them by up to n / 2, and a share of it by as much, so
+// an answer can differ from the real numbers' one where u or top_p come within n steps of a
+// border: 2^-27 of the sum for 2^17 tokens, 2^-24 for 2^19.  It takes a tail whose weights all
+// round the same way (45.2 octaves down they count nothing); of others root n steps remain, 2^-35.
 //
 // One CTA takes a row, or a cluster of them where rows are few, and reads it
 // from L2 for each pass.  A histogram of the tokens over 2048 steps of log2(w), 44 an
