@@ -207,3 +207,57 @@ def test_sample_tails_below_a_step(S):
             _, want = sample_definition(x[0].double().numpy(), 0.5, 1.0, 0, 1.0, 0.0)
             assert (tokens == 9).all() and ((logp.cpu().double() - want).abs() <= vocab * 2.0 ** -(bits + 1) + 2.0 ** -42).all()
             assert abs(want) > 0.8 * vocab * 2.0 ** -(bits + 1)
+
+
+# --------------------------------------------------------------- the C ABI, step by step --
+def test_steps_of_the_c_abi(S):
+    """Lengths and pages advance from step to step as a C caller has them: held into a plan, kept out of it, the next held
+    from free_pages; no page is in two places, none is lost."""
+    from vdttfs._lib import check, lib
+    rng = np.random.default_rng(3)
+    seqs, width, page, count = 9, 5, 16, 30
+    ints = lambda v, n=torch.int32: torch.tensor(np.asarray(v), dtype=n, device="cuda")  # noqa: E731
+    ring, span, pages = ints(np.arange(count)), ints([0, count]), torch.full((seqs, width), -1, dtype=torch.int32, device="cuda")
+    held, kept, starts = ints([0] * seqs), ints([0] * seqs), ints([0] * (seqs + 1))
+    need = lib().vdt_plan_pages_scratch_bytes(seqs)
+    scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    p = lambda t: t.data_ptr()  # noqa: E731
+    lengths = [0] * seqs
+    for _ in range(60):
+        new = [min(int(rng.integers(0, 25)) if n == 0 else 1, width * page - n) for n in lengths]
+        total = sum(new)
+        fresh, positions, slots = ints(new), ints([0] * (total + 1)), ints([0] * (total + 1), torch.int64)
+        check(lib().vdt_plan_pages(p(ring), count, p(span), p(pages), width, p(held), p(fresh), seqs, page, total, p(kept), p(starts), p(positions), p(slots),
+                                   p(span), p(scratch), need, stream), "vdt_plan_pages")
+        lengths = [a + b for a, b in zip(lengths, new)]
+        assert held.tolist() == [a - b for a, b in zip(lengths, new)] and kept.tolist() == lengths
+        first, left = span.tolist()
+        if left < 0:
+            break
+        table, order = pages.tolist(), ring.tolist()
+        used = [n for row, many in zip(table, lengths) for n in row[: -(-many // page)]]
+        assert sorted(used + [order[(first + i) % count] for i in range(left)]) == list(range(count))
+        assert positions.tolist()[:total] == [a - b + i for a, b in zip(lengths, new) for i in range(b)]
+        done = rng.random(seqs) < (0.6 if left < 12 else 0.1)
+        done_t = ints(done, torch.uint8)
+        check(lib().vdt_free_pages(p(ring), count, p(span), p(pages), width, p(kept), p(done_t), seqs, page, p(held), p(span), stream), "vdt_free_pages")
+        lengths = [0 if d else n for d, n in zip(done, lengths)]
+        assert held.tolist() == lengths
+    else:
+        return
+    raise AssertionError("the pool ran out")
+
+
+@pytest.mark.parametrize("k", [1, 31, 32, 33, 63, 65])
+def test_code_rows_of_the_c_abi(S, k):
+    """Rows of ceil(k / 2) bytes, as far apart as the next multiple of 16; nearer ones are refused."""
+    from vdttfs._lib import lib
+    n, x = 7, normal(k, 7, k).cuda()
+    stride, stream = ((k + 1) // 2 + 15) // 16 * 16, torch.cuda.current_stream().cuda_stream
+    codes = torch.full((n, stride), 0xab, dtype=torch.uint8, device="cuda")
+    scale = torch.empty(lib().vdt_fp4_scale_bytes(n, k), dtype=torch.uint8, device="cuda")
+    go = lambda s: lib().vdt_quantize_fp4(x.data_ptr(), 0, n, k, k, codes.data_ptr(), s, scale.data_ptr(), stream)  # noqa: E731
+    assert go(stride) == 0 and (stride == 16 or go(stride - 16) == 1)
+    want, _ = S.quantize_fp4(x)
+    assert torch.equal(codes[:, : want.shape[1]], want)
