@@ -261,3 +261,35 @@ def test_code_rows_of_the_c_abi(S, k):
     assert go(stride) == 0 and (stride == 16 or go(stride - 16) == 1)
     want, _ = S.quantize_fp4(x)
     assert torch.equal(codes[:, : want.shape[1]], want)
+
+
+# ------------------------------------------------------------ results of one call --
+def results(S):
+    x = normal(1, 40, 300, kind=torch.bfloat16).cuda()
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    pool, pages, held, new = S.PagePool.full(50), torch.full((3, 9), -1, dtype=torch.int32, device="cuda"), ints(0, 0, 0), ints(5, 100, 33)
+    plan = S.plan_pages(pool, pages, held, new, 16, 140)
+    none = S.plan_pages(pool, torch.full((3, 9), -1, dtype=torch.int32, device="cuda"), held, ints(0, 0, 0), 16, 0)
+    return {"quantize_fp4": S.quantize_fp4(x), "add_rms_norm": S.add_rms_norm(x, x), "add_rms_norm_int8": S.add_rms_norm_int8(x, x), "plan_pages": plan,
+            "plan_pages of nothing": none, "free_pages": S.free_pages(pool, pages, new, torch.tensor([True, False, True]).cuda(), 16),
+            "sample": S.sample(normal(2, 7, 900).cuda(), uniform(1, 7).cuda())}
+
+
+def test_results_have_storage_of_their_own(S):
+    """A result that is kept holds no other one in memory, and one that is used again at another size writes over none."""
+    for name, out in results(S).items():
+        places = [t.untyped_storage().data_ptr() for t in out if t.numel()]
+        assert len(set(places)) == len(places), name
+        for i, t in enumerate(out):
+            others = [o.clone() for o in out]
+            t.resize_(0).resize_(4 * others[i].numel() + 500).fill_(77)
+            for j, o in enumerate(out):
+                assert i == j or torch.equal(o, others[j]), (name, i, j)
+            t.resize_(others[i].shape).copy_(others[i])
+
+
+def test_a_kept_result_holds_its_own_bytes(S):
+    plan = S.plan_pages(S.PagePool.full(4000), torch.full((3, 900), -1, dtype=torch.int32, device="cuda"), *(torch.zeros(3, dtype=torch.int32, device="cuda"),) * 2, 16, 50000)
+    for t, most in ((plan.kept, 12), (plan.starts, 16), (plan.span, 8), (plan.positions, 200000)):
+        assert t.untyped_storage().nbytes() == most
+    assert plan.slots.untyped_storage().nbytes() <= 400000 + 4096

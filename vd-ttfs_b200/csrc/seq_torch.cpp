@@ -90,31 +90,6 @@ Tensor room(at::IntArrayRef size, at::ScalarType type, at::Device device) {
     return Tensor(at::detail::empty_cuda(size, type, device, std::nullopt));
 }
 
-// Results that belong together share a block of memory: an allocation and a
-// view by way of torch's operators take some 0.8 and 0.5 us of host time each.
-class Block {
-public:
-    // room for n values of `type`, from the next 256 bytes on; its first byte
-    int64_t add(int64_t n, at::ScalarType type) {
-        const int64_t at = bytes_;
-        bytes_ = at + (n * (int64_t)c10::elementSize(type) + 255) / 256 * 256;
-        return at;
-    }
-    void make(at::Device device) { all_ = room({bytes_}, at::kByte, device); }
-    const Tensor& all() const { return all_; }
-    Tensor part(int64_t at, at::IntArrayRef size, at::IntArrayRef stride, at::ScalarType type) const {
-        Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all_.storage()), all_.key_set(), c10::scalarTypeToTypeMeta(type));
-        t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
-        t.unsafeGetTensorImpl()->set_sizes_and_strides(size, stride);
-        return t;
-    }
-    void* at(int64_t byte) const { return bytes_ ? static_cast<char*>(all_.data_ptr()) + byte : nullptr; }
-
-private:
-    int64_t bytes_ = 0;
-    Tensor all_;
-};
-
 // The call's stream.  One of the caller's own is torch's current one for the
 // length of the call: copies that the call makes of its inputs run on it, and
 // what the call allocates comes from that stream's memory.  A block of another
@@ -482,15 +457,13 @@ PyObject* quantize_fp4(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if ((cols > 1 && x.stride(1) != 1) || (rows > 1 && x.stride(0) < cols)) x = x.contiguous();
     const int64_t bytes = (cols + 1) / 2, step = (bytes + 15) / 16 * 16;
     const int64_t tiles = (rows + 127) / 128, steps = (cols + 255) / 256 * 2;
-    Block block;
-    const int64_t at_codes = block.add(rows * step, at::kByte), at_scale = block.add(tiles * steps * 512, at::kByte);
-    block.make(x.device());
-    if (const int e = vdt_quantize_fp4(x.data_ptr(), type, rows, n, x.stride(0), static_cast<uint8_t*>(block.at(at_codes)), step,
-                                       static_cast<uint8_t*>(block.at(at_scale)), on.handle()))
+    const Tensor codes = room({rows, step}, at::kByte, x.device()), scale = room({tiles, steps, 32, 16}, at::kByte, x.device());
+    if (const int e = vdt_quantize_fp4(x.data_ptr(), type, rows, n, x.stride(0), at_or_null<uint8_t>(codes), step, at_or_null<uint8_t>(scale), on.handle()))
         return status_error(e, "vdt_quantize_fp4");
-    on.result(block.all());
-    return pair(block.part(at_codes, {rows, bytes}, {step, 1}, at::kByte),
-                block.part(at_scale, {tiles, steps, 32, 16}, {steps * 512, 512, 16, 1}, at::kByte));
+    on.result(codes);
+    on.result(scale);
+    codes.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef({rows, bytes}), at::IntArrayRef({step, 1}));
+    return pair(codes, scale);
     END_HANDLE_TH_ERRORS
 }
 
@@ -647,17 +620,16 @@ PyObject* add_rms_norm_int8(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (n.residual.defined() && !even_rows(n.residual)) n.residual = n.residual.contiguous();
     const Tensor sum = !n.residual.defined() ? x : n.sum.defined() ? n.sum : room(x.sizes(), x.scalar_type(), x.device());
     const int64_t step = ((int64_t)n.cols + 15) / 16 * 16;
-    Block block;
-    const int64_t at_codes = block.add(n.rows * step, at::kChar), at_scale = block.add(n.rows, at::kFloat);
-    block.make(x.device());
+    const Tensor codes = room({n.rows, step}, at::kChar, x.device()), scale = room({n.rows}, at::kFloat, x.device());
     if (const int e = vdt_add_rms_norm_int8(n.x.data_ptr(), n.x.stride(0), at_or_null(n.residual), n.residual.defined() ? n.residual.stride(0) : 0,
                                             at_or_null(n.weight), n.rows, n.cols, eps, n.type, n.residual.defined() ? sum.data_ptr() : nullptr,
-                                            sum.stride(0), static_cast<int8_t*>(block.at(at_codes)), step, static_cast<float*>(block.at(at_scale)),
-                                            on.handle()))
+                                            sum.stride(0), at_or_null<int8_t>(codes), step, at_or_null<float>(scale), on.handle()))
         return status_error(e, "vdt_add_rms_norm_int8");
     if (n.residual.defined() && !n.sum.defined()) on.result(sum);
-    on.result(block.all());
-    return triple(block.part(at_codes, {n.rows, n.cols}, {step, 1}, at::kChar), block.part(at_scale, {n.rows}, {1}, at::kFloat), sum);
+    on.result(codes);
+    on.result(scale);
+    codes.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef({n.rows, (int64_t)n.cols}), at::IntArrayRef({step, 1}));
+    return triple(codes, scale, sum);
     END_HANDLE_TH_ERRORS
 }
 
@@ -674,20 +646,18 @@ Pool pool_of(PyObject* o) {
     flat(p.span, "pool span", at::kInt, 2);
     return p;
 }
-// Whole numbers that a call writes: the caller's tensor, or a part of a new block
+// Whole numbers that a call writes: the caller's tensor, or a new one (with storage for `more` of them)
 struct Ints {
-    Tensor given;
-    int64_t n, at = 0;
-    at::ScalarType type;
-    Ints(PyObject* o, const char* what, at::ScalarType t, int64_t many, Block& block) : given(tensor_or_none(o, what)), n(many), type(t) {
-        if (given.defined()) flat(given, what, t, many);
-        else at = block.add(many, t);
+    Tensor t;
+    Ints(PyObject* o, const char* what, at::ScalarType type, int64_t n, at::Device device, const OnStream& on, int64_t more = 0)
+        : t(tensor_or_none(o, what)) {
+        if (t.defined()) {
+            flat(t, what, type, n);
+            return;
+        }
+        on.result(t = room({std::max(n, more)}, type, device));
+        if (more > n) t.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef({n}), at::IntArrayRef({(int64_t)1}));
     }
-    template <typename T>
-    T* data(const Block& block) const {
-        return static_cast<T*>(given.defined() ? given.data_ptr() : n ? block.at(at) : nullptr);
-    }
-    PyObject* wrap(const Block& block) const { return THPVariable_Wrap(given.defined() ? given : block.part(at, {n}, {1}, type)); }
 };
 
 PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t count) {
@@ -706,22 +676,22 @@ PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t count) {
     TORCH_CHECK_VALUE(total >= 0 && total <= INT32_MAX && page > 0, "page must be positive, total not negative");
     const at::Device device = pages.device();
     const OnStream on(a[6], device);
-    Block block;
     const size_t need = vdt_plan_pages_scratch_bytes(seqs);
-    const int64_t scratch = block.add((int64_t)need, at::kByte);
-    const Ints out[5] = {{a[7], "out kept", at::kInt, seqs, block}, {a[8], "out starts", at::kInt, (int64_t)seqs + 1, block},
-                         {a[9], "out positions", at::kInt, total, block}, {a[10], "out slots", at::kLong, total, block},
-                         {a[11], "out span", at::kInt, 2, block}};
-    block.make(device);
+    // the scratch lies behind new slots: an allocation less, and nothing that is kept lies behind it
+    const int64_t behind = (8 * total + 15) / 16 * 16;
+    const Ints out[5] = {{a[7], "out kept", at::kInt, seqs, device, on}, {a[8], "out starts", at::kInt, (int64_t)seqs + 1, device, on},
+                         {a[9], "out positions", at::kInt, total, device, on}, {a[10], "out slots", at::kLong, total, device, on, behind / 8 + (int64_t)need / 8},
+                         {a[11], "out span", at::kInt, 2, device, on}};
+    const Tensor own = a[10] == Py_None ? Tensor() : room({(int64_t)need}, at::kByte, device);
+    void* const scratch = own.defined() ? own.data_ptr() : static_cast<char*>(out[3].t.storage().mutable_data()) + behind;
     if (const int e = vdt_plan_pages(at_or_null<int32_t>(pool.ring), size32(pool.ring.numel(), "pool ring"), at_or_null<int32_t>(pool.span),
                                      at_or_null<int32_t>(pages), width, at_or_null<int32_t>(held), at_or_null<int32_t>(fresh), seqs, page, total,
-                                     out[0].data<int32_t>(block), out[1].data<int32_t>(block), out[2].data<int32_t>(block), out[3].data<int64_t>(block),
-                                     out[4].data<int32_t>(block), block.at(scratch), need, on.handle()))
+                                     at_or_null<int32_t>(out[0].t), at_or_null<int32_t>(out[1].t), at_or_null<int32_t>(out[2].t),
+                                     at_or_null<int64_t>(out[3].t), at_or_null<int32_t>(out[4].t), scratch, need, on.handle()))
         return status_error(e, "vdt_plan_pages");
-    on.result(block.all());
     PyObject* t = PyTuple_New(5);
     for (int i = 0; t && i < 5; ++i) {
-        PyObject* o = out[i].wrap(block);
+        PyObject* o = THPVariable_Wrap(out[i].t);
         if (!o) Py_CLEAR(t);
         else PyTuple_SET_ITEM(t, i, o);
     }
@@ -745,20 +715,12 @@ PyObject* free_pages(PyObject*, PyObject* const* a, Py_ssize_t count) {
     TORCH_CHECK_VALUE(page > 0, "page must be positive");
     const at::Device device = pages.device();
     const OnStream on(a[5], device);
-    Block block;
-    const Ints out(a[6], "out held", at::kInt, seqs, block), span(a[7], "out span", at::kInt, 2, block);
-    block.make(device);
+    const Ints out(a[6], "out held", at::kInt, seqs, device, on), span(a[7], "out span", at::kInt, 2, device, on);
     if (const int e = vdt_free_pages(at_or_null<int32_t>(pool.ring), size32(pool.ring.numel(), "pool ring"), at_or_null<int32_t>(pool.span),
                                      at_or_null<int32_t>(pages), width, at_or_null<int32_t>(held), at_or_null<uint8_t>(done), seqs, page,
-                                     out.data<int32_t>(block), span.data<int32_t>(block), on.handle()))
+                                     at_or_null<int32_t>(out.t), at_or_null<int32_t>(span.t), on.handle()))
         return status_error(e, "vdt_free_pages");
-    on.result(block.all());
-    PyObject* x = out.wrap(block);
-    PyObject* y = x ? span.wrap(block) : nullptr;
-    PyObject* t = y ? PyTuple_Pack(2, x, y) : nullptr;
-    Py_XDECREF(x);
-    Py_XDECREF(y);
-    return t;
+    return pair(out.t, span.t);
     END_HANDLE_TH_ERRORS
 }
 
@@ -799,14 +761,13 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t count) {
     }
     const OnStream on(a[6], x.device());
     if (!even_rows(x)) x = x.contiguous();
-    Block block;
-    const int64_t tokens = block.add(rows, at::kInt), logp = block.add(rows, at::kFloat);
-    block.make(x.device());
+    const Tensor tokens = room({rows}, at::kInt, x.device()), logp = room({rows}, at::kFloat, x.device());
     if (const int e = vdt_sample(x.data_ptr(), type, rows, vocab, x.stride(0), at_or_null<float>(u), temperatures, temperature, top_ks, top_k, top_ps,
-                                 top_p, min_ps, min_p, static_cast<int32_t*>(block.at(tokens)), static_cast<float*>(block.at(logp)), on.handle()))
+                                 top_p, min_ps, min_p, at_or_null<int32_t>(tokens), at_or_null<float>(logp), on.handle()))
         return status_error(e, "vdt_sample");
-    on.result(block.all());
-    return pair(block.part(tokens, {rows}, {1}, at::kInt), block.part(logp, {rows}, {1}, at::kFloat));
+    on.result(tokens);
+    on.result(logp);
+    return pair(tokens, logp);
     END_HANDLE_TH_ERRORS
 }
 
