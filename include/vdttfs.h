@@ -602,7 +602,9 @@ int vdt_add_rms_norm_int8(const void* d_x, int64_t x_stride, const void* d_resid
    free ones, d_ring [ring] with d_span = {place of the first free one, how many}, in
    the order of the sequences, and written into their rows of d_pages [seqs, width].
    span_out = {the first one left, how many}; below zero: that many were lacking,
-   -1 is in the table in their place, and in the slots of their tokens.  Tokens
+   -1 is in the table in their place, and in the slots of their tokens.  A lacking
+   page is not asked for by later steps, whose lengths have gone past it: its tokens
+   stay without one until the sequence is freed and begun again.  Tokens
    past a row's width take no page and have slot -1; rows past the last sequence's
    have position and slot -1.  d_ring and d_new are not changed; kept may be held,
    and span_out span, for a step in place; other buffers must not lie over each other.
@@ -616,7 +618,9 @@ int vdt_plan_pages(const int32_t* d_ring, int ring, const int32_t* d_span, int32
 
 /* The pages of the sequences with done[s] != 0, numbers 0 .. ceil(held[s] / page)
    of their rows that are not negative, go behind the ring's last free one, as
-   far as it has room; held_out is 0 for these sequences and held for the others
+   far as it has room.  A page that stands in two rows (a prefix that sequences
+   share) goes back with each of them: the caller puts -1 in a row that is freed
+   while another still has the page.  held_out is 0 for these sequences and held for the others
    (and may be held), span_out the ring's state after (and may be span). */
 int vdt_free_pages(int32_t* d_ring, int ring, const int32_t* d_span, const int32_t* d_pages, int width,
                    const int32_t* d_held, const uint8_t* d_done, int seqs, int page, int32_t* d_held_out,

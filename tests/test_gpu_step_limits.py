@@ -293,3 +293,30 @@ def test_a_kept_result_holds_its_own_bytes(S):
     for t, most in ((plan.kept, 12), (plan.starts, 16), (plan.span, 8), (plan.positions, 200000)):
         assert t.untyped_storage().nbytes() == most
     assert plan.slots.untyped_storage().nbytes() <= 400000 + 4096
+
+
+# ------------------------------------------------------------- what a page's owner is --
+def test_a_lacking_page_is_not_asked_for_again(S):
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    pool, pages, held = S.PagePool.full(3), torch.full((2, 4), -1, dtype=torch.int32, device="cuda"), ints(0, 0)
+    plan = S.plan_pages(pool, pages, held, ints(32, 32), 16, 64)
+    assert pages.tolist() == [[0, 1, -1, -1], [2, -1, -1, -1]] and plan.span.tolist() == [0, -1]
+    back, span = S.free_pages((pool.ring, plan.span), pages, plan.kept, torch.tensor([True, False]).cuda(), 16)
+    assert back.tolist() == [0, 32] and span.tolist() == [0, 2]
+    plan = S.plan_pages((pool.ring, span), pages, back, ints(0, 1), 16, 1)
+    # sequence 1 goes on in its third page; tokens 16 to 31 stay without one
+    assert pages.tolist()[1] == [2, -1, 0, -1] and plan.slots.tolist() == [0] and plan.span.tolist() == [1, 1]
+    back, span = S.free_pages((pool.ring, plan.span), pages, plan.kept, torch.tensor([False, True]).cuda(), 16)
+    assert back.tolist() == [0, 0] and span.tolist() == [1, 3] and sorted(pool.ring.tolist()) == [0, 1, 2]
+
+
+def test_a_page_of_two_rows_is_taken_out_of_one(S):
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    pages, done = ints(4, 7, 4, 9).view(2, 2), torch.tensor([True, True]).cuda()
+    ring, span = ints(-1, -1, -1, -1, -1), ints(0, 0)
+    _, after = S.free_pages((ring, span), pages, ints(32, 32), done, 16)
+    assert ring.tolist() == [4, 7, 4, 9, -1] and after.tolist() == [0, 4]
+    pages[1, 0] = -1
+    ring.fill_(-1)
+    _, after = S.free_pages((ring, span), pages, ints(32, 32), done, 16)
+    assert ring.tolist() == [4, 7, 9, -1, -1] and after.tolist() == [0, 3]

@@ -230,7 +230,8 @@ def plan_pages(pool, pages, held, new, page, total, out=None, stream=None):
     take, positions what qk_norm_rope takes; slots are page number * page + place.
     Rows past the last sequence's get -1, and so do slots of tokens without a page:
     those past the table's width, and those for which the pool has none (then
-    span[1] is below zero, by as many pages).  ``out``: a PagePlan to write
+    span[1] is below zero, by as many pages; later steps do not ask for these again, so
+    such a sequence is freed and begun anew).  ``out``: a PagePlan to write
     to, any of it None; its kept may be held, its span the pool's.  Nothing is
     copied to the host."""
     return PagePlan._make(_seq.plan_pages(pool, pages, held, new, page, total, stream, *(out or (None,) * 5)))
@@ -238,7 +239,8 @@ def plan_pages(pool, pages, held, new, page, total, out=None, stream=None):
 
 def free_pages(pool, pages, held, done, page, out=None, stream=None):
     """The pages of the sequences with done [seqs] (bool) go behind the pool's last:
-    returns (held, span), 0 tokens held for these.  ``out``: the two to write
+    returns (held, span), 0 tokens held for these.  A page that stands in
+    two rows goes back with each of them.  ``out``: the two to write
     to, which may be held and the pool's span."""
     return _seq.free_pages(pool, pages, held, done, page, stream, *(out or (None, None)))
 
