@@ -193,6 +193,13 @@ __global__ void __launch_bounds__(THREADS < 128 ? 128 : THREADS) k_add_rms_norm(
     }
 }
 
+// The fewest threads that hold a row in one to four vectors each (eight, and more read again, in the
+// longest).  More of them are faster for a few rows and slower for many, fewer the other way round up
+// to a point; the length alone decides.  us for one row and for 16384, bf16 with a residual, codes: 1024
+// columns with 32 threads 3.7 and 25.9, with 128 2.4 and 28.0; 2048 columns with 128 threads
+// 2.9 and 42.4, with 256 2.6 and 56.9, with 32 5.7 and 50.6; 4096 columns with 128 threads 3.9 and 74.0, with
+// 256 3.3 and 83.8; for one row and 8192, 8192 columns with 256 threads 4.8 and 75.6, with 512 4.4 and
+// 108.5, with 128 7.3 and 80.9.
 template <typename T, bool CODES, bool WIDE>
 cudaError_t norm_by_length(const NormParams& p, cudaStream_t s) {
     const int vecs = p.cols / Vec16<T>::N;

@@ -270,7 +270,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_plan_rows(PlanParams p) {
 
 // One CTA: the finished sequences are listed, a warp counts each one's pages, the
 // counts are summed, and the warp that counted them writes them behind the
-// ring's last.
+// ring's last.  Made for the few that end in a step: us, 2 of 48 sequences with 19 pages each 2.8, 6
+// of 200 with 79 3.3; many at once are one SM's latency, 1000 with 128 pages each 59, with 512 179.
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS) k_free(FreeParams p) {
     __shared__ int which[THREADS], tokens[THREADS], counts[THREADS];
