@@ -320,3 +320,24 @@ def test_a_page_of_two_rows_is_taken_out_of_one(S):
     ring.fill_(-1)
     _, after = S.free_pages((ring, span), pages, ints(32, 32), done, 16)
     assert ring.tolist() == [4, 7, 9, -1, -1] and after.tolist() == [0, 3]
+
+
+def test_a_plan_into_buffers_of_the_callers_own(S):
+    """All results given, some of them, none: the same plan, and the given tensors are what comes back."""
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    for seqs, total in ((3, 41), (3, 0), (1500, 1503)):
+        new = torch.full((seqs,), total // seqs, dtype=torch.int32, device="cuda")
+        held = torch.arange(seqs, dtype=torch.int32, device="cuda") % 40
+
+        def go(out):
+            return S.plan_pages(S.PagePool.full(9000), torch.full((seqs, 5), -1, dtype=torch.int32, device="cuda"), held, new, 16, total, out)
+
+        want = go(None)
+        room = [torch.empty_like(t) for t in want]
+        for given in (range(5), (3,), (0, 2, 4), (1,)):
+            out = S.PagePlan._make(room[i] if i in given else None for i in range(5))
+            got = go(out)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(got[i] is room[i] for i in given), (seqs, total, given)
+    with pytest.raises(ValueError):
+        S.plan_pages(S.PagePool.full(4), torch.zeros(2, 3, dtype=torch.int32, device="cuda"), ints(0, 0), ints(1, 1), 16, 2,
+                     S.PagePlan(None, None, None, torch.empty(2, dtype=torch.int32, device="cuda"), None))
